@@ -124,6 +124,7 @@ fhog::Params to_params(const fhog_bwdbwd_args* a) {
   p.causal = a->causal != FHOG_MASK_NONE;
   p.f16 = a->dtype == FHOG_DTYPE_FP16;
   mask_params(a->causal, a->window, a->n_q, a->n_k, &p.mask_off, &p.window);
+  p.sinks = 0;
   p.n_split = 1;
   p.part = nullptr;
   const int order = fhog::tuning().order;
@@ -229,11 +230,35 @@ fhog::AttnParams to_attn_params(const fhog_attn_args* a) {
   p.causal = a->causal != FHOG_MASK_NONE;
   p.f16 = a->dtype == FHOG_DTYPE_FP16;
   mask_params(a->causal, a->window, a->n_q, a->n_k, &p.mask_off, &p.window);
+  p.sinks = 0, p.n_split = 1, p.part = nullptr;
   // as in run_pass: tile-major with a mask, until a slice alone has tiles enough to balance the end of a launch
   const int order = fhog::tuning().order;
   p.tile_major_q = order < 0 ? (p.causal && a->n_q < 16384) : order;
   p.tile_major_k = order < 0 ? (p.causal && a->n_k < 16384) : order;
   return p;
+}
+
+// Sinks of a mask, or the error for a number that is none
+int check_sinks(int64_t sinks) { return sinks < 0 ? fail(FHOG_E_CAUSAL, "sinks must be >= 0 (got %lld)", (long long)sinks) : FHOG_OK; }
+int32_t sinks_of(const fhog_attn_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }
+int32_t sinks_of(const fhog_bwdbwd_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }
+
+// Row sums d of a first backward, rounded up so that what follows stays 16-byte aligned
+size_t row_bytes(const fhog_attn_args* a) { return ((size_t)a->batch * a->n_q * sizeof(float) + 15) & ~(size_t)15; }
+
+size_t attn_sinks_bytes(const fhog_attn_args* a, int64_t sinks, int backward) {
+  const int32_t n = sinks_of(a, sinks);
+  if (backward) return n ? row_bytes(a) + sink_bytes(a->batch, n, a->n_q, a->d) : (size_t)a->batch * a->n_q * sizeof(float);
+  return n ? forward_part_bytes(a->batch, a->n_q, a->d, forward_parts(a->batch, a->n_q, a->n_k, a->d, a->window, n)) : 0;
+}
+
+// A workspace of the entry points with sinks: there, aligned and as large as the call needs
+int check_ws(const void* ws, int64_t have, size_t need) {
+  if (need == 0) return FHOG_OK;
+  if (!ws) return fail(FHOG_E_NULL, "pointer 'ws' is NULL");
+  if (!aligned16(ws)) return fail(FHOG_E_ALIGN, "pointer 'ws' is not 16-byte aligned");
+  if (have < 0 || (size_t)have < need) return fail(FHOG_E_SHAPE, "ws_bytes %lld is below the %zu bytes that this call needs", (long long)have, need);
+  return FHOG_OK;
 }
 
 // Address of `scratch` on the current device, looked up once per device (the first call there) and kept.
@@ -340,6 +365,102 @@ int fhog_attn_bwd(const fhog_attn_args* args, void* hip_stream) {
   return FHOG_OK;
 }
 
+size_t fhog_attn_sinks_workspace_bytes(const fhog_attn_args* args, int64_t sinks, int backward) {
+  fhog_attn_args a;
+  if (!args) return 0;
+  a = *args;
+  if (backward && !a.ws) a.ws = (float*)a.q;   // not there yet: its size is the question
+  if (validate_attn(&a, backward) != FHOG_OK || check_sinks(sinks) != FHOG_OK) return 0;
+  return attn_sinks_bytes(&a, sinks, backward);
+}
+
+int fhog_attn_fwd_sinks(const fhog_attn_args* args, int64_t sinks, void* ws, int64_t ws_bytes, void* hip_stream) {
+  if (const int rc = validate_attn(args, 0)) return rc;
+  if (const int rc = check_sinks(sinks)) return rc;
+  if (const int rc = check_ws(ws, ws_bytes, attn_sinks_bytes(args, sinks, 0))) return rc;
+  const int32_t n = sinks_of(args, sinks);
+  if (n == 0) return fhog_attn_fwd(args, hip_stream);
+  const hipStream_t s = (hipStream_t)hip_stream;
+  fhog::AttnParams p = to_attn_params(args);
+  p.sinks = n;
+  p.n_split = forward_parts(args->batch, args->n_q, args->n_k, args->d, args->window, n);
+  p.part = (float*)ws;
+  const bool bit16 = attn_on_16bit_kernels(args);
+  hipError_t e;
+  if (p.n_split > 1) {
+    e = bit16 ? fhog::launch_small_fwd_parts(p, s) : fhog::launch_attn_split_parts(p, args->dtype, false, s);
+    if (e == hipSuccess) e = fhog::launch_join_forward(p, args->dtype, s);
+  } else if (const int small = bit16 ? small_waves(Small::forward, args) : 0) {
+    e = fhog::launch_small_attn(p, false, small, s);
+  } else {
+    e = bit16 ? fhog::launch_attn_bf16(p, 0, s) : fhog::launch_attn_split(p, args->dtype, false, s);
+  }
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "attention forward: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
+
+int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_bytes, void* hip_stream) {
+  if (const int rc = validate_attn(args, 1)) return rc;
+  if (const int rc = check_sinks(sinks)) return rc;
+  if (const int rc = check_ws(args->ws, ws_bytes, attn_sinks_bytes(args, sinks, 1))) return rc;
+  const int32_t n = sinks_of(args, sinks);
+  if (n == 0) return fhog_attn_bwd(args, hip_stream);
+  const hipStream_t s = (hipStream_t)hip_stream;
+  fhog::AttnParams p = to_attn_params(args);
+  p.sinks = n;
+  hipError_t e;
+  if (!attn_on_16bit_kernels(args)) {
+    e = fhog::launch_attn_split(p, args->dtype, true, s);
+  } else if (const int small = small_waves(Small::backward, args)) {
+    e = fhog::launch_small_attn(p, true, small, s);
+  } else {
+    e = fhog::launch_attn_bf16(p, 1, s);
+    if (e == hipSuccess) e = fhog::launch_attn_bf16(p, 2, s);
+  }
+  if (e == hipSuccess) {
+    p.n_split = sink_parts(args->batch, n, args->n_q);
+    p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
+    e = fhog::launch_sink_keys(p, args->dtype, s);
+  }
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "attention backward: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
+
+size_t fhog_bwdbwd_sinks_workspace_bytes(const fhog_bwdbwd_args* args, int64_t sinks) {
+  if (validate(args) != FHOG_OK || check_sinks(sinks) != FHOG_OK) return 0;
+  const size_t hint = workspace_hint(args, to_params(args), select_impl(args));
+  const int32_t n = sinks_of(args, sinks);
+  const size_t need = n ? stats_bytes(args) + sink_bytes(args->batch, n, args->n_q, args->d) : 0;
+  return need > hint ? need : hint;
+}
+
+int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_stream) {
+  if (const int rc = validate(args)) return rc;
+  if (const int rc = check_sinks(sinks)) return rc;
+  const int32_t n = sinks_of(args, sinks);
+  if (n == 0) return fhog_bwdbwd(args, hip_stream);
+  if (args->schedule != FHOG_SCHEDULE_FUSED_STATS) return fail(FHOG_E_SCHEDULE, "sinks run under schedule %d alone (got %d)", FHOG_SCHEDULE_FUSED_STATS, args->schedule);
+  if (const int rc = check_ws(args->ws, args->ws_bytes, stats_bytes(args) + sink_bytes(args->batch, n, args->n_q, args->d))) return rc;
+  const hipStream_t s = (hipStream_t)hip_stream;
+  const int impl = select_impl(args);
+  fhog::Params p = to_params(args);
+  p.sinks = n;
+  const int small = impl == FHOG_IMPL_BF16 ? small_waves(Small::double_backward, args->batch, args->n_q, args->n_k, args->d, args->causal, args->window) : 0;
+  hipError_t e = hipSuccess;
+  if (small) {
+    e = fhog::launch_small_bwdbwd(p, small, s);
+  } else {
+    if (const int rc = run_pass(args, p, impl, FHOG_PASS_DD_B, s)) return rc;
+    if (const int rc = impl == FHOG_IMPL_BF16 ? run_grads(args, p, FHOG_PASS_DQ_DDO, true, s) : run_pass(args, p, impl, fhog::kPassGrads, s)) return rc;
+  }
+  if (e == hipSuccess) {   // behind the launches whose partial results lay there
+    p.n_split = sink_parts(args->batch, n, args->n_q);
+    p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + stats_bytes(args));
+    e = fhog::launch_sink_keys(p, args->dtype, impl != FHOG_IMPL_BF16, s);
+  }
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
 
 int fhog_abi_version(void) { return FHOG_ABI_VERSION; }
 

@@ -59,13 +59,13 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_bf16(AttnParams p) {
 #pragma unroll
   for (int cb = 0; cb < NC; cb++) acc[0][cb] = f32x16_t{0};
 
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
-  int j_begin, j_end;  // key tiles this workgroup visits
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
+  int j_begin, j_end;  // steps of this workgroup: the key tiles that it visits
   geo.tile_range(q0, WG_ROWS, j_begin, j_end);
   Dma<D> dma;
   dma.init(p.stride_kn, wave, lane);
   const uint32_t ring_lds = lds_addr(smem);
-  dma.template issue_all<2>(ring_lds, TILE, src, (int64_t)j_begin * TS * p.stride_kn, wave, p.n_k - j_begin * TS);
+  dma.template issue_all<2>(ring_lds, TILE, src, geo.offset(j_begin, p.stride_kn), wave, geo.end(j_begin) - geo.at(j_begin));
   dma_wait();
   __syncthreads();
 
@@ -74,14 +74,14 @@ __global__ void __launch_bounds__(256, 2) attn_fwd_bf16(AttnParams p) {
     constexpr int u = decltype(slot)::value;
     if (j + 1 < j_end) {
       const uint32_t dst = ring_lds + (u ^ 1) * STAGE;
-      const int64_t adv = (int64_t)(j + 1) * TS * p.stride_kn;
-      dma.template issue_all<2>(dst, TILE, src, adv, wave, p.n_k - (j + 1) * TS);
+      const int64_t adv = geo.offset(j + 1, p.stride_kn);
+      dma.template issue_all<2>(dst, TILE, src, adv, wave, geo.end(j + 1) - geo.at(j + 1));
     }
-    const int k0 = j * TS;
-    const bool masked = geo.partial(k0, qw);  // wave-uniform: the block holds hidden keys (mask edge or tensor end)
+    const int k0 = geo.at(j);
+    const bool masked = geo.partial(k0, qw, geo.sink(j));  // wave-uniform: the block holds hidden keys (mask edge or tensor end)
     int lo = 0, hi = 0;                       // key k0 + 8g + 4h + e is visible iff lo <= 8g + e <= hi
-    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
-    if (MASK == MASK_NONE || !geo.dead(k0, geo.first_row(qw, p.n_q))) {  // else every key of the tile is hidden from this wave
+    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
+    if (MASK == MASK_NONE || !geo.dead(k0, geo.first_row(qw, p.n_q), geo.sink(j))) {  // else every key of the tile is hidden from this wave
       const char* stage = smem + u * STAGE;
       fwd_block<F16, D>(stage, aoff, troff, Qb, masked, lo, hi, c_scale_log2, m, l, acc);
     }
@@ -153,13 +153,13 @@ __global__ void __launch_bounds__(256, 2) attn_bwd_q_bf16(AttnParams p) {
 #pragma unroll
   for (int cb = 0; cb < NC; cb++) acc[0][cb] = f32x16_t{0};
 
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
-  int j_begin, j_end;  // key tiles this workgroup visits
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
+  int j_begin, j_end;  // steps of this workgroup: the key tiles that it visits
   geo.tile_range(q0, WG_ROWS, j_begin, j_end);
   Dma<D> dma;
   dma.init(p.stride_kn, wave, lane);
   const uint32_t ring_lds = lds_addr(smem);
-  dma.template issue_all<2>(ring_lds, TILE, src, (int64_t)j_begin * TS * p.stride_kn, wave, p.n_k - j_begin * TS);
+  dma.template issue_all<2>(ring_lds, TILE, src, geo.offset(j_begin, p.stride_kn), wave, geo.end(j_begin) - geo.at(j_begin));
   dma_wait();
   __syncthreads();
 
@@ -168,14 +168,14 @@ __global__ void __launch_bounds__(256, 2) attn_bwd_q_bf16(AttnParams p) {
     constexpr int u = decltype(slot)::value;
     if (j + 1 < j_end) {
       const uint32_t dst = ring_lds + (u ^ 1) * STAGE;
-      const int64_t adv = (int64_t)(j + 1) * TS * p.stride_kn;
-      dma.template issue_all<2>(dst, TILE, src, adv, wave, p.n_k - (j + 1) * TS);
+      const int64_t adv = geo.offset(j + 1, p.stride_kn);
+      dma.template issue_all<2>(dst, TILE, src, adv, wave, geo.end(j + 1) - geo.at(j + 1));
     }
-    const int k0 = j * TS;
-    const bool masked = geo.partial(k0, qw);  // wave-uniform: the block holds hidden keys (mask edge or tensor end)
+    const int k0 = geo.at(j);
+    const bool masked = geo.partial(k0, qw, geo.sink(j));  // wave-uniform: the block holds hidden keys (mask edge or tensor end)
     int lo = 0, hi = 0;                       // key k0 + 8g + 4h + e is visible iff lo <= 8g + e <= hi
-    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
-    if (MASK == MASK_NONE || !geo.dead(k0, geo.first_row(qw, p.n_q))) {
+    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
+    if (MASK == MASK_NONE || !geo.dead(k0, geo.first_row(qw, p.n_q), geo.sink(j))) {
       const char* stage = smem + u * STAGE;
       bwd_q_block<F16, D>(stage, aoff, troff, Qb, dOb, masked, lo, hi, c_scale_log2, l_log2, dsum, acc);
     }
@@ -309,8 +309,8 @@ hipError_t launch_attn_d(const AttnParams& p, int which, hipStream_t s) {
     case 0: return launch<attn_fwd_bf16<F16, D, MASK>>(grid_blocks((p.n_q + WG_ROWS - 1) / WG_ROWS, p.batch), 2 * 2 * TILE, s, p);
     case 1: return launch<attn_bwd_q_bf16<F16, D, MASK>>(grid_blocks((p.n_q + WG_ROWS - 1) / WG_ROWS, p.batch), 2 * 2 * TILE, s, p);
     default:
-      if constexpr (D == 64)
-        return launch<attn_bwd_k_bf16<F16, D, MASK>>(grid_blocks((p.n_k + WG_ROWS - 1) / WG_ROWS, p.batch), 2 * (2 * TILE + 2 * TS * 4), s, p);
+      if constexpr (D == 64)   // the rows of the sinks have a launch of their own
+        return launch<attn_bwd_k_bf16<F16, D, MASK == MASK_SINK ? MASK_BAND : MASK>>(grid_blocks((p.n_k + WG_ROWS - 1) / WG_ROWS, p.batch), 2 * (2 * TILE + 2 * TS * 4), s, p);
       else
         return hipErrorInvalidValue;   // d = 128 is dispatched to the producer/consumer kernel before this point
   }
@@ -325,7 +325,8 @@ hipError_t launch_attn_bf16(const AttnParams& p, int which, hipStream_t s) {
   const int mask = mask_mode(p);
 #define FHOG_ATTN(F, DD)                                                            \
   (mask == MASK_NONE ? launch_attn_d<F, DD, MASK_NONE>(p, which, s)                 \
-                     : mask == MASK_CAUSAL ? launch_attn_d<F, DD, MASK_CAUSAL>(p, which, s) : launch_attn_d<F, DD, MASK_BAND>(p, which, s))
+                     : mask == MASK_CAUSAL ? launch_attn_d<F, DD, MASK_CAUSAL>(p, which, s)         \
+                     : mask == MASK_SINK ? launch_attn_d<F, DD, MASK_SINK>(p, which, s) : launch_attn_d<F, DD, MASK_BAND>(p, which, s))
   if (p.f16) return p.d == 128 ? FHOG_ATTN(true, 128) : FHOG_ATTN(true, 64);
   return p.d == 128 ? FHOG_ATTN(false, 128) : FHOG_ATTN(false, 64);
 #undef FHOG_ATTN

@@ -35,7 +35,9 @@ template <int WS, bool TWO>
 constexpr int n_buffers = WS == 1 && !TWO ? 2 : 1;
 
 // OWN_D: dK, dV without the sweep for dQ before it; pairs: as decode_block takes it
-template <typename T, int D, int MODE, int MASK, int WS, bool OWN_D, bool TWO = false>
+// PARTS: the streamed side is dealt out over n_split workgroups, whose partial results are fp32 numbers in p.part: rows and their maximum and sum
+// (PartialRows) of the forward, rows [part][dK | dV][batch * n_k][D] of dK, dV where there is more than one
+template <typename T, int D, int MODE, int MASK, int WS, bool OWN_D, bool TWO = false, bool PARTS = false>
 __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id, bool pairs) {
   constexpr bool KSIDE = MODE == MODE_BWD_K;
   // split_pair: two waves of fp32 tensors on a SIMD run faster without the dot products (dK, dV causal 32 x 2048, d = 64 231 -> 217 us), the VALU-bound ones of
@@ -59,16 +61,19 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
   const int n = lane & 31, h = lane >> 5;
   const int n_sta = KSIDE ? p.n_k : p.n_q, n_str = KSIDE ? p.n_q : p.n_k;
   int bh, tile;
-  if (!decode_block<MASK>((n_sta + ROWS - 1) / ROWS, p.batch, !KSIDE && MASK != MASK_NONE, MASK != MASK_NONE, bh, tile, pairs, id)) return;
+  if (!decode_block<MASK>((n_sta + ROWS - 1) / ROWS, p.batch * (PARTS ? p.n_split : 1), !KSIDE && MASK != MASK_NONE, MASK != MASK_NONE, bh, tile, pairs, id)) return;
+  const int part = PARTS ? bh % p.n_split : 0;
+  if (PARTS) bh /= p.n_split;
   const int64_t qoff = (int64_t)bh * p.stride_qb, koff = (int64_t)bh * p.stride_kb;
   const int64_t sta_ld = KSIDE ? p.stride_kn : p.stride_qn, str_ld = KSIDE ? p.stride_qn : p.stride_kn;
   const int r0 = tile * ROWS, rw = r0 + 32 * group, ri = rw + n;
   const int rr = min(ri, n_sta - 1);         // rows past the end compute on a copy of the last row and store nothing
   const T* const src[2] = {KSIDE ? (const T*)p.q + qoff : (const T*)p.k + koff, KSIDE ? (const T*)p.dO + qoff : (const T*)p.v + koff};
 
-  typename std::conditional<KSIDE, StreamQueries<MASK>, StreamKeys<MASK>>::type geo(p.mask_off, p.window, n_str);
+  typename std::conditional<KSIDE, StreamQueries<MASK>, StreamKeys<MASK>>::type geo(p.mask_off, p.window, n_str, p.sinks);
   int t_begin, t_end;
   geo.tile_range(r0, ROWS, t_begin, t_end);
+  if (PARTS) split_range(part, p.n_split, t_begin, t_end);
 
   const int64_t srow = (int64_t)bh * p.n_q;
   Stage st[WS];
@@ -79,8 +84,8 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
   const auto fetch = [&](int t) {
 #pragma unroll
     for (int g = 0; g < WS; g++) {
-      const int row0 = min((t + g) * TS, n_str - 1);                // a tile past the end is never computed on
-      st[g].fetch(src, str_ld, row0, n_str, tid);
+      const int end = MASK == MASK_SINK ? geo.end(t + g) : n_str, row0 = min(geo.at(t + g), end - 1);   // a tile past the end is never computed on
+      st[g].fetch(src, str_ld, row0, end, tid);
       if (KSIDE && tid < (OWN_D ? 1 : 2) * TS) stat_reg[g] = (tid < TS ? p.lse : p.ws_d)[srow + min(row0 + (tid & 31), p.n_q - 1)];
       if constexpr (KSIDE && OWN_D) {
 #pragma unroll
@@ -171,7 +176,8 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
     asm volatile("" : "+v"(s));   // holds the products in front of the branches that follow: the compiler sinks them to the use of their sum
   };
 
-  const auto block = [&](const char* stage, int s0, auto behind) {
+  // s0: first row of the tile of step t
+  const auto block = [&](const char* stage, int s0, int t, auto behind) {
     const float* stat = reinterpret_cast<const float*>(stage + Stage::BYTES);
     f32x16_t s = {0}, dp = {0};
     if constexpr (MODE == MODE_BWD_Q) {   // u = dP - d comes straight from an accumulator that starts at -d
@@ -208,9 +214,9 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
         }
       }
     }
-    const bool masked = geo.partial(s0, rw);   // wave-uniform: the block holds hidden pairs (mask edge or tensor end)
+    const bool masked = geo.partial(s0, rw, geo.sink(t));   // wave-uniform: the block holds hidden pairs (mask edge or tensor end)
     int lo = 0, hi = 0;
-    if (masked) keep_branch(), geo.limits(s0, ri, h, lo, hi);
+    if (masked) keep_branch(), geo.limits(s0, ri, h, lo, hi, geo.sink(t));
     f32x16_t pv;
     if constexpr (MODE == MODE_FWD) {
 #pragma unroll
@@ -278,16 +284,16 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
   // 264 | 233; two waves 16 x 300 84.3 | 85.2 | 86.3, 4 x 1024 228 | 231 | 229. At d = 32 the test is the faster (bf16 16 x 4096 412 | 420).
   constexpr bool NO_TEST = MASK == MASK_NONE && is_raw<T, D>;
   const auto sweep = [&](auto has_rows) {
-    const auto works = [&](int s0) { return NO_TEST ? decltype(has_rows)::value : !geo.dead(s0, geo.first_row(rw, n_sta)); };
+    const auto works = [&](int s0, int t) { return NO_TEST ? decltype(has_rows)::value : !geo.dead(s0, geo.first_row(rw, n_sta), geo.sink(t)); };
     for (int t = t_begin; t < t_end; t += WS) {
       const int buf = NBUF == 2 ? (t - t_begin) & 1 : 0;
       if constexpr (INTERLEAVED) {
         // The rows of the tile after this one came in during the step before; behind the last tile they are copies of the last row.
         char* const next = smem + (buf ^ 1) * STAGE;
-        const int s0 = t * TS, row0 = min(s0 + 2 * TS, n_str - 1);
-        if (works(s0)) {
-          block(smem + buf * STAGE, s0, [&](int slot, int slots) {
-            st[0].publish_at(next, tid, slot, slots, [&](int i) { st[0].fetch_chunk(i, src, str_ld, row0, n_str, tid); });
+        const int s0 = geo.at(t), end = MASK == MASK_SINK ? geo.end(t + 2) : n_str, row0 = min(MASK == MASK_SINK ? geo.at(t + 2) : s0 + 2 * TS, end - 1);
+        if (works(s0, t)) {
+          block(smem + buf * STAGE, s0, t, [&](int slot, int slots) {
+            st[0].publish_at(next, tid, slot, slots, [&](int i) { st[0].fetch_chunk(i, src, str_ld, row0, end, tid); });
           });
         } else {
           publish(buf ^ 1);
@@ -298,8 +304,8 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
       }
       const bool more = t + WS < t_end;
       if (more) fetch(t + WS);
-      const int s0 = (t + ws) * TS;
-      if ((WS == 1 || t + ws < t_end) && works(s0)) block(smem + (buf * WS + ws) * STAGE, s0, [](int, int) {});
+      const int s0 = geo.at(t + ws);
+      if ((WS == 1 || t + ws < t_end) && works(s0, t + ws)) block(smem + (buf * WS + ws) * STAGE, s0, t + ws, [](int, int) {});
       if (NBUF == 1) __syncthreads();   // the tiles are no longer read
       if (more) publish(NBUF == 2 ? buf ^ 1 : 0);
       __syncthreads();
@@ -347,6 +353,18 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
 
   if constexpr (MODE == MODE_FWD) l += __shfl_xor(l, 32);
   if (ri >= n_sta) return;
+  if constexpr (PARTS && MODE == MODE_FWD) {
+    const PartialRows rows(p);
+    store_rows<float, D>(rows.row(part, row), acc0, 1.f, h);
+    if (h == 0) rows.stats(part)[row] = f32x2_t{m, l};
+    return;
+  }
+  if (PARTS && KSIDE && p.n_split > 1) {
+    float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + ri) * D;
+    store_rows<float, D>(to, acc0, 1.f, h);
+    store_rows<float, D>(to + (int64_t)p.batch * p.n_k * D, acc1, 1.f, h);
+    return;
+  }
   const int64_t out = (KSIDE ? koff : qoff) + (int64_t)ri * sta_ld;
   if constexpr (MODE == MODE_FWD) {
     store_rows<T, D>((T*)p.o + out, acc0, 1.f / l, h);
@@ -359,10 +377,10 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
   }
 }
 
-template <typename T, int D, int MODE, int MASK, int WS, bool TWO>
+template <typename T, int D, int MODE, int MASK, int WS, bool TWO, bool PARTS = false>
 __global__ void __launch_bounds__(256, (min_workgroups<T, D, WS, TWO>)) attn_split(AttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  attn_run<T, D, MODE, MASK, WS, false, TWO>(p, smem, blockIdx.x, MASK != MASK_NONE && WS == 1 && min_workgroups<T, D, WS, TWO> == 2);
+  attn_run<T, D, MODE, MASK, WS, false, TWO, PARTS>(p, smem, blockIdx.x, MASK != MASK_NONE && WS == 1 && min_workgroups<T, D, WS, TWO> == 2);
 }
 
 // dQ (workgroups [0, q_blocks)) and dK, dV (the others; mixed: tile by tile in turn) in one launch; ON_CU: workgroups on a CU
@@ -393,6 +411,17 @@ hipError_t launch_ws(const AttnParams& p, hipStream_t s) {
   const hipError_t e = allow_dynamic_lds<attn_split<T, D, MODE, MASK, WS, TWO>>(smem);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((attn_split<T, D, MODE, MASK, WS, TWO>), dim3(blocks<WS>(MODE == MODE_BWD_K ? p.n_k : p.n_q, p.batch)), dim3(256), smem, s, p);
+  return hipGetLastError();
+}
+
+// Forward (MASK_SINK) or the rows of dK, dV of the sinks (MASK_BAND; p.n_k is their number there, and there is no window), over p.n_split workgroups a tile
+template <typename T, int D, int MODE, int MASK>
+hipError_t launch_parts(const AttnParams& p, hipStream_t s) {
+  constexpr int WS = lds_bytes<T, D, MODE, 4>() <= 160 * 1024 ? 4 : 2, smem = lds_bytes<T, D, MODE, WS>();
+  const hipError_t e = allow_dynamic_lds<attn_split<T, D, MODE, MASK, WS, false, true>>(smem);
+  if (e != hipSuccess) return e;
+  const unsigned grid = blocks<WS>(MODE == MODE_BWD_K ? p.n_k : p.n_q, p.batch * p.n_split);
+  hipLaunchKernelGGL((attn_split<T, D, MODE, MASK, WS, false, true>), dim3(grid), dim3(256), smem, s, p);
   return hipGetLastError();
 }
 
@@ -461,11 +490,30 @@ hipError_t launch_bwd(const AttnParams& p, hipStream_t s) {
 
 template <typename T, int D>
 hipError_t launch_td(const AttnParams& p, bool backward, hipStream_t s) {
+  if (p.sinks > 0) return backward ? launch_bwd<T, D, MASK_SINK>(p, s) : launch_fwd<T, D, MASK_SINK>(p, s);
   if (backward) return p.causal ? launch_bwd<T, D, MASK_BAND>(p, s) : launch_bwd<T, D, MASK_NONE>(p, s);
   return p.causal ? launch_fwd<T, D, MASK_BAND>(p, s) : launch_fwd<T, D, MASK_NONE>(p, s);
 }
 
+template <typename T, int D>
+hipError_t launch_parts_td(const AttnParams& p, bool backward, hipStream_t s) {
+  return backward ? launch_parts<T, D, MODE_BWD_K, MASK_BAND>(p, s) : launch_parts<T, D, MODE_FWD, MASK_SINK>(p, s);
+}
+
 }  // namespace
+
+hipError_t launch_attn_split_parts(const AttnParams& p, int dtype, bool backward, hipStream_t s) {
+  if (dtype == FHOG_DTYPE_FP32) {
+    switch (p.d) {
+      case 32: return launch_parts_td<float, 32>(p, backward, s);
+      case 64: return launch_parts_td<float, 64>(p, backward, s);
+      case 128: return launch_parts_td<float, 128>(p, backward, s);
+      default: return hipErrorInvalidValue;
+    }
+  }
+  if (p.d != 32) return hipErrorInvalidValue;
+  return dtype == FHOG_DTYPE_FP16 ? launch_parts_td<_Float16, 32>(p, backward, s) : launch_parts_td<__bf16, 32>(p, backward, s);
+}
 
 // dtype: FHOG_DTYPE_*. fp32 tensors of every head dim, 16-bit tensors of d = 32.
 hipError_t launch_attn_split(const AttnParams& p, int dtype, bool backward, hipStream_t s) {

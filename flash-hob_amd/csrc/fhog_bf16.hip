@@ -108,8 +108,8 @@ __device__ __forceinline__ void q_sweep_run(const Params& p, char* smem, int bh,
 
   // The first streamed tile is requested before the resident operands: the two round trips to memory overlap instead of
   // following each other (a workgroup that visits four tiles spends most of its time in this prologue).
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
-  int j_begin, j_end;  // key tiles this workgroup visits
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
+  int j_begin, j_end;  // steps of this workgroup: the key tiles that it visits
   geo.tile_range(q0, ROWS, j_begin, j_end);
   if (p.n_split > 1) split_range(split, p.n_split, j_begin, j_end);
   // staging: four waves share the rows of a tile; with eight waves each group of four takes half of the tensors
@@ -128,7 +128,7 @@ __device__ __forceinline__ void q_sweep_run(const Params& p, char* smem, int bh,
   // the ring holds 2 * SUB tiles; tile j lives in slot (j - j_begin) mod (2 * SUB)
   const auto stage_tile = [&](int j) {
     const uint32_t dst = ring_lds + ((j - j_begin) & (2 * SUB - 1)) * STAGE;
-    dma.template issue_all<NLD>(dst, TILE, srcl, (int64_t)j * TS * p.stride_kn, wave & 3, p.n_k - j * TS);
+    dma.template issue_all<NLD>(dst, TILE, srcl, geo.offset(j, p.stride_kn), wave & 3, (MASK == MASK_SINK ? geo.end(j) : p.n_k) - geo.at(j));
   };
 #pragma unroll
   for (int u = 0; u < SUB; u++)
@@ -199,11 +199,11 @@ __device__ __forceinline__ void q_sweep_run(const Params& p, char* smem, int bh,
     for (int u = 0; u < SUB; u++) {
       const int j = jj + u;
       if (SUB > 1 && j >= j_end) continue;
-      const int k0 = j * TS;
-      const bool masked = geo.partial(k0, qw);  // wave-uniform: the block holds hidden keys (mask edge or tensor end)
+      const int k0 = geo.at(j);
+      const bool masked = geo.partial(k0, qw, geo.sink(j));  // wave-uniform: the block holds hidden keys (mask edge or tensor end)
       int lo = 0, hi = 0;                       // key k0 + 8g + 4h + e is visible iff lo <= 8g + e <= hi
-      if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
-      if (MASK == MASK_NONE ? decltype(rows)::value : !geo.dead(k0, geo.first_row(qw, p.n_q))) {  // else every key of the tile is hidden from this wave
+      if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
+      if (MASK == MASK_NONE ? decltype(rows)::value : !geo.dead(k0, geo.first_row(qw, p.n_q), geo.sink(j))) {  // else every key of the tile is hidden from this wave
         const char* stage = smem + (GRP + u) * STAGE;
         q_block<F16, D, PASS>(stage, aoff, troff, Qb, ddQb, dOb, masked, lo, hi, c_scale_log2, l_log2, p.scale, dsum, dd, kc, red, red_dd, red_vdds,
                               red_pu, red_p, acc_dq, acc_ddo);
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(256, 2) dd_sweep64_bf16(Params p) {
   const __bf16* src[NT] = {(const __bf16*)p.k + koff, (const __bf16*)p.ddk + koff};
 
   // the first streamed tile is requested before anything else is loaded: the round trips to memory overlap
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
   int j_begin, j_end;
   geo.tile_range(q0, ROWS, j_begin, j_end);
   Dma<D> dma;
@@ -707,6 +707,22 @@ hipError_t launch_single_d(const Params& p, int pass, hipStream_t s) {
   return e != hipSuccess ? e : hipGetLastError();
 }
 
+// Statistics under a mask with sinks: pass 5, with the choice of launch_single_d
+template <bool F16, int D>
+hipError_t launch_stats_sink(const Params& p, hipStream_t s) {
+  const int tile = TS * 2 * D, slices = p.batch * p.n_split;
+  if constexpr (D == 128) {
+    const unsigned g8 = grid_blocks((p.n_q + 255) / 256, slices);
+    const int b8 = tuning().b8;
+    if (p.n_split == 1 && (b8 < 0 ? g8 >= 512 : b8 == 1)) return launch_sweep<q_sweep_bf16<F16, D, 5, MASK_SINK, 8>>(g8, 2 * 4 * tile, s, p, 512);
+  }
+  const hipError_t e = launch_sweep<q_sweep_bf16<F16, D, 5, MASK_SINK>>(grid_blocks((p.n_q + WG_ROWS - 1) / WG_ROWS, slices), 2 * 4 * tile, s, p);
+  if (e != hipSuccess || p.n_split == 1) return e;
+  const int64_t rows = (int64_t)p.batch * p.n_q;
+  hipLaunchKernelGGL(combine_stats<5>, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
 template <bool F16, int QPASS, int MASK, int SUB>
 hipError_t launch_grads64(const Params& p, bool q_side, bool k_side, hipStream_t s) {
   const int tile = TS * 2 * 64, q_lds = 2 * SUB * 4 * tile, k_lds = 2 * SUB * (3 * tile + 4 * TS * 4);
@@ -748,6 +764,11 @@ hipError_t launch_bf16_pass(const Params& p, int pass, hipStream_t s) {
   if (pass == FHOG_PASS_B_DDO || pass == FHOG_PASS_DD_B_DDO) return launch_bf16_ddo_pass(p, pass, s);
   if (pass != FHOG_PASS_STAGE1 && pass != FHOG_PASS_DD && pass != FHOG_PASS_B && pass != FHOG_PASS_DD_B) return hipErrorInvalidValue;
   const int mask = mask_mode(p);
+  if (mask == MASK_SINK) {
+    if (pass != FHOG_PASS_DD_B) return hipErrorInvalidValue;
+    if (p.f16) return p.d == 128 ? launch_stats_sink<true, 128>(p, s) : launch_stats_sink<true, 64>(p, s);
+    return p.d == 128 ? launch_stats_sink<false, 128>(p, s) : launch_stats_sink<false, 64>(p, s);
+  }
 #define FHOG_SINGLE(F, DD)                                                             \
   (mask == MASK_NONE ? launch_single_d<F, DD, MASK_NONE>(p, pass, s)                   \
                      : mask == MASK_CAUSAL ? launch_single_d<F, DD, MASK_CAUSAL>(p, pass, s) : launch_single_d<F, DD, MASK_BAND>(p, pass, s))
@@ -758,14 +779,15 @@ hipError_t launch_bf16_pass(const Params& p, int pass, hipStream_t s) {
 
 // d = 128: passes 3 and 4 need the producer/consumer split to fit the registers; d = 64: single-role kernels throughout
 hipError_t launch_bf16_grads(const Params& p, int q_pass, bool k_side, hipStream_t s) {
-  if (!bf16_shape_supported(p.n_q, p.n_k, p.d, p.causal)) return hipErrorInvalidValue;
+  if (!bf16_shape_supported(p.n_q, p.n_k, p.d, p.causal) || (p.sinks > 0 && q_pass == FHOG_PASS_DQ)) return hipErrorInvalidValue;
   hipError_t e;
   if (p.d == 128) {
     e = launch_grads_pc(p, q_pass, k_side, s);
   } else {
     const int mask = mask_mode(p);
 #define FHOG_GRADS(F)                                                             \
-  (mask == MASK_NONE ? launch_grads64_f<F, MASK_NONE>(p, q_pass, k_side, s)       \
+  (mask == MASK_SINK ? launch_grads64<F, 3, MASK_SINK, 1>(p, q_pass != 0, k_side, s) \
+   : mask == MASK_NONE ? launch_grads64_f<F, MASK_NONE>(p, q_pass, k_side, s)       \
                      : mask == MASK_CAUSAL ? launch_grads64_f<F, MASK_CAUSAL>(p, q_pass, k_side, s) : launch_grads64_f<F, MASK_BAND>(p, q_pass, k_side, s))
     e = p.f16 ? FHOG_GRADS(true) : FHOG_GRADS(false);
 #undef FHOG_GRADS

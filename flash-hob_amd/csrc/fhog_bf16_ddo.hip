@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) q_sweep_ddo(Params p
                            (const __bf16*)p.ddv + koff};
 
   // the first streamed tile is requested before the resident operands: the two round trips to memory overlap
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
   int j_begin, j_end;  // key tiles this workgroup visits
   geo.tile_range(q0, ROWS, j_begin, j_end);
   // staging: four waves share the rows of a tile; with eight waves each group of four takes two of the four tensors

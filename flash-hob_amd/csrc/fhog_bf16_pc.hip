@@ -169,22 +169,22 @@ __device__ __forceinline__ void consume_q(const Params& p, char* smem, const Str
   dma.init(p.stride_kn, wq, lane);
   const uint32_t ring_lds = lds_addr(smem);
   if (j_begin < j_end)
-    dma.template issue_all<4>(ring_lds, SM::TILE, src, (int64_t)j_begin * TS * p.stride_kn, wq, p.n_k - j_begin * TS);
+    dma.template issue_all<4>(ring_lds, SM::TILE, src, geo.offset(j_begin, p.stride_kn), wq, geo.end(j_begin) - geo.at(j_begin));
   dma_wait();
   __syncthreads();
   int sc = RING - 1, sn = 1;  // ring slots of tile j-1 (read here) and tile j+1 (filled here)
   for (int j = j_begin; j <= j_end; j++) {
     if (j + 1 < j_end) {
       const uint32_t dst = ring_lds + sn * SM::STAGE;
-      const int64_t adv = (int64_t)(j + 1) * TS * p.stride_kn;
-      dma.template issue_all<4>(dst, SM::TILE, src, adv, wq, p.n_k - (j + 1) * TS);
+      const int64_t adv = geo.offset(j + 1, p.stride_kn);
+      dma.template issue_all<4>(dst, SM::TILE, src, adv, wq, geo.end(j + 1) - geo.at(j + 1));
     }
     // block j-1: query block qb of the pair took part iff the tile held a key visible to it
-    const bool act0 = j > j_begin && !geo.dead((j - 1) * TS, geo.first_row(qw0, p.n_q));
+    const bool act0 = j > j_begin && !geo.dead(geo.at(j - 1), geo.first_row(qw0, p.n_q), geo.sink(j - 1));
     // Without a mask block 1 goes along with block 0, past the end of the tensor too (as below under a plain causal one): its operand tiles are not
     // written then, and what is made of them stays in rows that are not stored. Branches around its MFMAs, here and in pass 4, cost every length: double-backward,
     // us, with | without: 4 x 4096 313.0 | 308.8, fp16 1 x 8192 340.6 | 335.8, 64 x 2048 1194.6 | 1190.4; 128 x 400 147.2 | 147.4.
-    const bool act1 = MASK == MASK_NONE ? act0 : j > j_begin && !geo.dead((j - 1) * TS, geo.first_row(qw0 + 32, p.n_q));
+    const bool act1 = MASK == MASK_NONE ? act0 : j > j_begin && !geo.dead(geo.at(j - 1), geo.first_row(qw0 + 32, p.n_q), geo.sink(j - 1));
     const bool act = act0 || act1;
     const char* stage = smem + sc * SM::STAGE;
     const char* sop = sop_pair + ((j - 1) & 1) * SM::SOP_BUF;
@@ -222,7 +222,7 @@ __device__ __forceinline__ void consume_q(const Params& p, char* smem, const Str
           for (int cl = 0; cl < 2; cl++) {
             if (act0) acc[0][2 * cp + cl] = mfma<F16>(a_op[t][0][pr], bop[c][cl][pr], acc[0][2 * cp + cl]);
             // with a plain causal mask a tile that block 0 takes part in is also one for block 1, unless that is past the end of the tensor
-            if (MASK != MASK_BAND || act1) acc[1][2 * cp + cl] = mfma<F16>(a_op[t][1][pr], bop[c][cl][pr], acc[1][2 * cp + cl]);
+            if (!geo.WINDOW || act1) acc[1][2 * cp + cl] = mfma<F16>(a_op[t][1][pr], bop[c][cl][pr], acc[1][2 * cp + cl]);
           }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -285,16 +285,16 @@ __device__ __forceinline__ void consume_dq(const Params& p, char* smem, const St
   dma.init(p.stride_kn, wq, lane);
   const uint32_t ring_lds = lds_addr(smem);
   if (j_begin < j_end)
-    dma.template issue_all<4>(ring_lds, SM::TILE, src, (int64_t)j_begin * TS * p.stride_kn, wq, p.n_k - j_begin * TS);
+    dma.template issue_all<4>(ring_lds, SM::TILE, src, geo.offset(j_begin, p.stride_kn), wq, geo.end(j_begin) - geo.at(j_begin));
   dma_wait();
   __syncthreads();
   int sc = RING - 1, sn = 1;  // ring slots of tile j-1 (read here) and tile j+1 (filled here)
   for (int j = j_begin; j <= j_end; j++) {
     if (j + 1 < j_end) {
       const uint32_t dst = ring_lds + sn * SM::STAGE;
-      dma.template issue_all<4>(dst, SM::TILE, src, (int64_t)(j + 1) * TS * p.stride_kn, wq, p.n_k - (j + 1) * TS);
+      dma.template issue_all<4>(dst, SM::TILE, src, geo.offset(j + 1, p.stride_kn), wq, geo.end(j + 1) - geo.at(j + 1));
     }
-    if (j > j_begin && !geo.dead((j - 1) * TS, geo.first_row(qw0, p.n_q))) {   // block j-1 took part
+    if (j > j_begin && !geo.dead(geo.at(j - 1), geo.first_row(qw0, p.n_q), geo.sink(j - 1))) {   // block j-1 took part
       const char* stage = smem + sc * SM::STAGE;
       const char* sop = sop_wave + ((j - 1) & 1) * SM::SOP_BUF;
       bf16x8_t bop[2][2][2];   // [buffer][column block of the pair][ddK | K]
@@ -353,8 +353,8 @@ __device__ __forceinline__ void q_run_pc(const Params& p, char* smem, int bh, in
   const int n = lane & 31, h = lane >> 5;
   const int q0 = tile * WG_ROWS, qw = q0 + 32 * wq, qi = qw + n;
   const int64_t qoff = (int64_t)bh * p.stride_qb, koff = (int64_t)bh * p.stride_kb;
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
-  int j_begin, j_end;  // key tiles this workgroup visits
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
+  int j_begin, j_end;  // steps of this workgroup: the key tiles that it visits
   geo.tile_range(q0, WG_ROWS, j_begin, j_end);
   if (p.n_split > 1) split_range(split, p.n_split, j_begin, j_end);
   char* sop_base = smem + SM::SOP_BASE + wq * SM::SOP_WAVE;
@@ -372,13 +372,13 @@ __device__ __forceinline__ void q_run_pc(const Params& p, char* smem, int bh, in
     __syncthreads();
     int sp = 0;  // ring slot of tile j
     for (int j = j_begin; j <= j_end; j++) {
-      const int k0 = j * TS;
-      if (j < j_end && !geo.dead(k0, geo.first_row(qw, p.n_q))) {
+      const int k0 = geo.at(j);
+      if (j < j_end && !geo.dead(k0, geo.first_row(qw, p.n_q), geo.sink(j))) {
         const char* stage = smem + sp * SM::STAGE;
         char* sop = sop_base + (j & 1) * SM::SOP_BUF;
-        const bool masked = geo.partial(k0, qw);
+        const bool masked = geo.partial(k0, qw, geo.sink(j));
         int lo = 0, hi = 0;  // key k0 + 8g + 4h + e is visible iff lo <= 8g + e <= hi
-        if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
+        if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
         produce_q<F16, D, false, DQ_ONLY>(stage, sop, Qb, ddQb, dOb, dOb, lane, lo, hi, masked, c_scale_log2, l_log2, p.scale, dsum, dd, b);
       }
       __syncthreads();
@@ -861,7 +861,7 @@ hipError_t launch_attn_bwd_k_pc(const AttnParams& p, hipStream_t s) {
   const int mask = mask_mode(p);
 #define FHOG_BWDK(F)                                                                     \
   (mask == MASK_NONE ? launch_attn_bwd_k_pc_d<F, 128, MASK_NONE>(p, s)                   \
-                     : mask == MASK_CAUSAL ? launch_attn_bwd_k_pc_d<F, 128, MASK_CAUSAL>(p, s) : launch_attn_bwd_k_pc_d<F, 128, MASK_BAND>(p, s))
+                     : mask == MASK_CAUSAL ? launch_attn_bwd_k_pc_d<F, 128, MASK_CAUSAL>(p, s) : /* the sinks' rows have a launch of their own */ launch_attn_bwd_k_pc_d<F, 128, MASK_BAND>(p, s))
   return p.f16 ? FHOG_BWDK(true) : FHOG_BWDK(false);
 #undef FHOG_BWDK
 }
@@ -869,7 +869,7 @@ hipError_t launch_attn_bwd_k_pc(const AttnParams& p, hipStream_t s) {
 hipError_t launch_grads_pc(const Params& p, int q_pass, bool k_side, hipStream_t s) {
   const int mask = mask_mode(p);
 #define FHOG_PC_Q(F, M) (q_pass == FHOG_PASS_DQ ? launch_grads_pc_d<F, 128, M, true>(p, true, k_side, s) : launch_grads_pc_d<F, 128, M, false>(p, q_pass != 0, k_side, s))
-#define FHOG_PC(F) (mask == MASK_NONE ? FHOG_PC_Q(F, MASK_NONE) : mask == MASK_CAUSAL ? FHOG_PC_Q(F, MASK_CAUSAL) : FHOG_PC_Q(F, MASK_BAND))
+#define FHOG_PC(F) (mask == MASK_SINK ? launch_grads_pc_d<F, 128, MASK_SINK, false>(p, q_pass != 0, k_side, s) : mask == MASK_NONE ? FHOG_PC_Q(F, MASK_NONE) : mask == MASK_CAUSAL ? FHOG_PC_Q(F, MASK_CAUSAL) : FHOG_PC_Q(F, MASK_BAND))
   if (p.d != 128) return hipErrorInvalidValue;   // d = 64 runs on the single-role kernels
   return p.f16 ? FHOG_PC(true) : FHOG_PC(false);
 #undef FHOG_PC

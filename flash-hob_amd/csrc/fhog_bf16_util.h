@@ -227,21 +227,42 @@ __device__ __forceinline__ void load_resident(bf16x8_t* dst, const __bf16* base,
 constexpr int MASK_NONE = 0;    // only the tensor ends
 constexpr int MASK_CAUSAL = 1;  // off = 0 and no window, known at compile time (the square causal mask)
 constexpr int MASK_BAND = 2;    // off and win from the arguments
+constexpr int MASK_SINK = 3;    // as MASK_BAND, and the first `sinks` keys stay visible to the queries behind them (j < sinks, j <= i + off)
 // "Streamed" rows come in 32-row tiles starting at t0; "stationary" rows are the 32 rows of a wave starting at r0
 // (or the rows [r0, r0 + nrows) of a workgroup for the tile range).
 //
 // StreamKeys: stationary rows are queries, streamed tiles are keys (statistics sweeps, pass 3, forward, dQ).
+//
+// Steps. A sweep goes over steps [lo, hi) of tile_range; at(j) is the first row of the tile of step j, and rows from end(j) on are not read. Without sinks a
+// step is its tile. With sinks the first steps are visits to the tiles of the sinks (sink(j)) for the keys that lie before a query's window, and the rest
+// is the band, in tiles from its first key on; sinks that some of the queries have in their windows and others before them are visited in both. That way
+// the visible keys of a query are an interval in every step, and the blocks know of nothing but intervals. Keys that no query of the workgroup
+// sees are never read, whatever they hold.
 template <int MASK>
 struct StreamKeys {
+  static constexpr bool WINDOW = MASK == MASK_BAND || MASK == MASK_SINK;
   int off, win, n_k;
-  __device__ __forceinline__ StreamKeys(int off_, int win_, int n_k_)
-      : off(MASK == MASK_BAND ? off_ : 0), win(MASK == MASK_BAND ? win_ : (1 << 28)), n_k(n_k_) {}
-  // tiles [lo, hi) hold a visible key for some query of [r0, r0 + nrows)
-  __device__ __forceinline__ void tile_range(int r0, int nrows, int& lo, int& hi) const {
+  int sinks = 0, visits = 0, first = 0, last = 0;   // MASK_SINK: sink steps of the sweep, and the band's keys [first, last)
+  __device__ __forceinline__ StreamKeys(int off_, int win_, int n_k_, int sinks_ = 0)
+      : off(WINDOW ? off_ : 0), win(WINDOW ? win_ : (1 << 28)), n_k(n_k_), sinks(sinks_) {}
+  // steps [lo, hi) hold a visible key for some query of [r0, r0 + nrows)
+  __device__ __forceinline__ void tile_range(int r0, int nrows, int& lo, int& hi) {
     const int k_tiles = (n_k + TS - 1) / TS;
-    lo = MASK == MASK_BAND ? max(0, r0 + off - win + 1) / TS : 0;
+    lo = WINDOW ? max(0, r0 + off - win + 1) / TS : 0;
     hi = MASK != MASK_NONE ? min(k_tiles, (r0 + nrows - 1 + off) / TS + 1) : k_tiles;
+    if (MASK == MASK_SINK) {
+      visits = (max(0, min(sinks, r0 + nrows - 1 + off - win + 1)) + TS - 1) / TS;   // the last query's window leaves the most sinks before it
+      first = max(0, r0 + off - win + 1), last = min(n_k, r0 + nrows + off);
+      lo = 0, hi = visits + (max(0, last - first) + TS - 1) / TS;
+    }
   }
+  __device__ __forceinline__ bool sink(int j) const { return MASK == MASK_SINK && j < visits; }
+  __device__ __forceinline__ int at(int j) const { return MASK == MASK_SINK && j >= visits ? first + (j - visits) * TS : j * TS; }
+  __device__ __forceinline__ int end(int j) const { return MASK != MASK_SINK ? n_k : j < visits ? sinks : last; }
+  // elements from the first row of the tensor
+  __device__ __forceinline__ int64_t offset(int j, int64_t ld) const { return MASK == MASK_SINK ? at(j) * ld : (int64_t)j * TS * ld; }
+  // sinks before the window of query i: keys [0, before(i)) count in the sink steps
+  __device__ __forceinline__ int before(int i) const { return min(sinks, i + off - win + 1); }
   // For dead(): the first of the 32 rows of a wave or, if all of them lie past the end of their tensor of n rows, one that sees no key. Such a wave
   // computed on copies of the last row, under a causal mask the row with the most keys; now it leaves the SIMD to the others. us, before ->
   // so: fp16 48 x 1537, d = 64, three sweeps, Hessian-vector product 364 -> 350; double-backward bf16 128 x 400 no mask d = 64 87 -> 83, d = 128
@@ -251,49 +272,57 @@ struct StreamKeys {
   // d = 64, no mask, neither | the test | two loops: fp16 1 x 8192 208.3 | 210.7 | 208.9, 4 x 4096 201.6 | 204.3 | 202.3, bf16 2 x 16384 1342 | 1353 | 1344,
   // 128 x 400 88.2 | 82.4 | 83.0).
   __device__ __forceinline__ static int first_row(int r0, int n) { return r0 < n ? r0 : -(1 << 29); }
-  // no key of tile t0 is visible to any query of [r0, r0 + 32)
-  __device__ __forceinline__ bool dead(int t0, int r0) const {
+  // no key of tile t0 is visible to any query of [r0, r0 + 32); s: in a sink step
+  __device__ __forceinline__ bool dead(int t0, int r0, bool s = false) const {
     if (MASK == MASK_NONE) return r0 < 0;
-    return t0 > r0 + 31 + off || (MASK == MASK_BAND && t0 + TS - 1 < r0 + off - win + 1);
+    if (MASK == MASK_SINK && s) return t0 >= before(r0 + 31);
+    return t0 > r0 + 31 + off || (WINDOW && t0 + TS - 1 < r0 + off - win + 1);
   }
   // some key of tile t0 is hidden from some query of [r0, r0 + 32)
-  __device__ __forceinline__ bool partial(int t0, int r0) const {
+  __device__ __forceinline__ bool partial(int t0, int r0, bool s = false) const {
+    if (MASK == MASK_SINK && s) return t0 + TS > before(r0);
     if (t0 + TS > n_k) return true;
     if (MASK == MASK_NONE) return false;
-    return t0 + TS - 1 > r0 + off || (MASK == MASK_BAND && t0 < r0 + 31 + off - win + 1);
+    return t0 + TS - 1 > r0 + off || (WINDOW && t0 < r0 + 31 + off - win + 1);
   }
   // key t0 + 8g + 4h + e is visible to query i iff lo <= 8g + e <= hi
-  __device__ __forceinline__ void limits(int t0, int i, int h, int& lo, int& hi) const {
+  __device__ __forceinline__ void limits(int t0, int i, int h, int& lo, int& hi, bool s = false) const {
     hi = min(MASK != MASK_NONE ? i + off - t0 : TS, n_k - 1 - t0) - 4 * h;
-    lo = MASK == MASK_BAND ? i + off - win + 1 - t0 - 4 * h : -TS;
+    lo = WINDOW ? i + off - win + 1 - t0 - 4 * h : -TS;
+    if (MASK == MASK_SINK && s) hi = before(i) - 1 - t0 - 4 * h, lo = -TS;
   }
 };
-// StreamQueries: stationary rows are keys, streamed tiles are queries (pass 4, dK and dV).
+// StreamQueries: stationary rows are keys, streamed tiles are queries (pass 4, dK and dV). MASK_SINK: the band alone; the rows of the sinks, which the
+// queries behind it see too, are put in their place by a launch of their own (fhog_small.hip, fhog_split.hip, fhog_attn_split.hip).
 template <int MASK>
 struct StreamQueries {
+  static constexpr bool WINDOW = MASK == MASK_BAND || MASK == MASK_SINK;
   int off, win, n_q;
-  __device__ __forceinline__ StreamQueries(int off_, int win_, int n_q_)
-      : off(MASK == MASK_BAND ? off_ : 0), win(MASK == MASK_BAND ? win_ : (1 << 28)), n_q(n_q_) {}
+  __device__ __forceinline__ StreamQueries(int off_, int win_, int n_q_, int = 0)
+      : off(WINDOW ? off_ : 0), win(WINDOW ? win_ : (1 << 28)), n_q(n_q_) {}
+  __device__ __forceinline__ static bool sink(int) { return false; }
+  __device__ __forceinline__ static int at(int j) { return j * TS; }
+  __device__ __forceinline__ int end(int) const { return n_q; }
   __device__ __forceinline__ void tile_range(int r0, int nrows, int& lo, int& hi) const {
     const int q_tiles = (n_q + TS - 1) / TS;
     lo = MASK != MASK_NONE ? max(0, r0 - off) / TS : 0;
-    hi = MASK == MASK_BAND ? (int)min((int64_t)q_tiles, ((int64_t)r0 + nrows - 1 - off + win - 1) / TS + 1) : q_tiles;
+    hi = WINDOW ? (int)min((int64_t)q_tiles, ((int64_t)r0 + nrows - 1 - off + win - 1) / TS + 1) : q_tiles;
     hi = max(hi, lo);
   }
   __device__ __forceinline__ static int first_row(int r0, int n) { return r0 < n ? r0 : 1 << 29; }
-  __device__ __forceinline__ bool dead(int t0, int r0) const {
+  __device__ __forceinline__ bool dead(int t0, int r0, bool = false) const {
     if (MASK == MASK_NONE) return r0 == 1 << 29;
-    return t0 + TS - 1 < r0 - off || (MASK == MASK_BAND && t0 > r0 + 31 - off + win - 1);
+    return t0 + TS - 1 < r0 - off || (WINDOW && t0 > r0 + 31 - off + win - 1);
   }
-  __device__ __forceinline__ bool partial(int t0, int r0) const {
+  __device__ __forceinline__ bool partial(int t0, int r0, bool = false) const {
     if (t0 + TS > n_q) return true;
     if (MASK == MASK_NONE) return false;
-    return t0 < r0 + 31 - off || (MASK == MASK_BAND && t0 + TS - 1 > r0 - off + win - 1);
+    return t0 < r0 + 31 - off || (WINDOW && t0 + TS - 1 > r0 - off + win - 1);
   }
   // query t0 + 8g + 4h + e sees key j iff lo <= 8g + e <= hi
-  __device__ __forceinline__ void limits(int t0, int j, int h, int& lo, int& hi) const {
+  __device__ __forceinline__ void limits(int t0, int j, int h, int& lo, int& hi, bool = false) const {
     lo = MASK != MASK_NONE ? j - off - t0 - 4 * h : -TS;
-    hi = min(MASK == MASK_BAND ? j - off + win - 1 - t0 : TS, n_q - 1 - t0) - 4 * h;
+    hi = min(WINDOW ? j - off + win - 1 - t0 : TS, n_q - 1 - t0) - 4 * h;
   }
 };
 // part `split` of `n` equal parts of the streamed tile range [lo, hi) (the last parts may be empty)
@@ -306,6 +335,7 @@ __device__ __forceinline__ void split_range(int split, int n, int& lo, int& hi) 
 template <typename P>
 inline int mask_mode(const P& p) {
   if (!p.causal) return MASK_NONE;
+  if (p.sinks > 0) return MASK_SINK;
   return (p.mask_off == 0 && p.window >= p.n_q + p.n_k) ? MASK_CAUSAL : MASK_BAND;
 }
 

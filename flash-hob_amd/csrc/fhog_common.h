@@ -55,6 +55,7 @@ struct Params {
   // The same three of the K-tiled side where both share a launch (launch_bf16_grads)
   int32_t n_split_k, tile_major_k;
   float* part_k;
+  int32_t sinks;   // keys [0, sinks) stay visible to the queries whose window lies behind them (0 without a window)
 };
 
 // Launch choices that can be overridden for experiments through the environment variable FHOG_TUNE, a comma-separated
@@ -96,6 +97,10 @@ struct AttnParams {
   int32_t window;
   // Workgroup order within an XCD for the Q-tiled kernels (forward, dQ) and the K-tiled one (dK, dV): see Params
   int32_t tile_major_q, tile_major_k;
+  int32_t sinks;     // see Params
+  // Streamed side over n_split workgroups per stationary tile, fp32 partial results in `part` (the keys of the sinks, forwards of few queries)
+  int32_t n_split;
+  float* part;
 };
 
 // A kernel that uses more than 64 KiB of dynamic LDS needs its limit raised before the first launch. Done once per
@@ -115,6 +120,17 @@ inline hipError_t allow_dynamic_lds(int bytes) {
   return e;
 }
 
+// Partial results of a forward whose streamed keys are dealt out over p.n_split workgroups, in p.part: the rows of O on the row's own maximum
+// [part][batch * n_q][d], then (maximum in log2 units, sum) [part][batch * n_q].
+struct PartialRows {
+  float* base;
+  int64_t rows;
+  int32_t d, n_split;
+  __host__ __device__ explicit PartialRows(const AttnParams& p) : base(p.part), rows((int64_t)p.batch * p.n_q), d(p.d), n_split(p.n_split) {}
+  __device__ float* row(int part, int64_t r) const { return base + (part * rows + r) * d; }
+  __device__ f32x2_t* stats(int part) const { return reinterpret_cast<f32x2_t*>(base + n_split * rows * d) + part * rows; }
+};
+
 constexpr int kPassGrads = -1;   // launch_split_pass: passes 3 and 4 in one launch
 
 // Launchers implemented in the kernel translation units. Each returns hipGetLastError().
@@ -129,6 +145,16 @@ hipError_t launch_attn_split(const AttnParams& p, int dtype, bool backward, hipS
 hipError_t launch_attn_bwd_k_pc(const AttnParams& p, hipStream_t s);                // dK and dV at d = 128 (producer/consumer)
 hipError_t launch_small_bwdbwd(const Params& p, int waves, hipStream_t s);  // default schedule, 16-bit tensors: 4 or 2 waves on 32 rows
 hipError_t launch_small_attn(const AttnParams& p, bool backward, int waves, hipStream_t s);   // first-order passes, likewise
+// Masks with sinks. The rows of dK, dV (dK2, dV2) of the sinks alone: n_k is the number of sinks, mask and window those of bottom-right without one, and the
+// streamed queries are dealt out over n_split workgroups; fhog_sinks.hip adds what they leave in `part`.
+hipError_t launch_small_sink_bwd(const AttnParams& p, hipStream_t s);                          // 16-bit kernels
+hipError_t launch_small_sink_grads(const Params& p, hipStream_t s);
+hipError_t launch_attn_split_parts(const AttnParams& p, int dtype, bool backward, hipStream_t s);   // split products; backward false: as launch_small_fwd_parts
+hipError_t launch_split_sink_grads(const Params& p, int dtype, hipStream_t s);
+hipError_t launch_small_fwd_parts(const AttnParams& p, hipStream_t s);                         // forward, the streamed keys over n_split workgroups
+hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s);                  // O and L from what those leave
+hipError_t launch_sink_keys(const AttnParams& p, int dtype, hipStream_t s);                     // the sinks' rows of dK, dV from start to end
+hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, hipStream_t s);    // ... of dK2, dV2
 hipError_t launch_mfma_rate(float* out, int blocks, int trips, int data_mode, int waves, hipStream_t s);  // measurement aid
 bool bf16_shape_supported(int64_t n_q, int64_t n_k, int64_t d, int causal);
 

@@ -336,6 +336,33 @@ inline int small_waves(Small what, int64_t batch, int64_t n_q, int64_t n_k, int6
 inline int small_waves(Small what, const fhog_attn_args* a) { return small_waves(what, a->batch, a->n_q, a->n_k, a->d, a->causal, a->window); }
 
 
+// ---- masks with sinks ---------------------------------------------------------------------------------------------
+// Sinks that the mask knows: as many as there are keys, none where no query has a key before its window.
+inline int32_t sinks_of(int64_t sinks, int64_t window, int64_t n_k) {   // a window needs a causal mask
+  if (window == 0 || window >= n_k) return 0;
+  return (int32_t)(sinks < n_k ? sinks : n_k);
+}
+// Workgroups that share 32 sinks of a slice, each with a part of the queries: two for every CU, with eight tiles (two of each wave) for each at least.
+inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q) {
+  const int64_t groups = (sinks + 31) / 32 * batch, tiles = (n_q + 31) / 32;
+  int64_t parts = (512 + groups - 1) / groups;
+  if (parts > tiles / 8) parts = tiles / 8;
+  return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+}
+inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d) {
+  const int parts = sink_parts(batch, sinks, n_q);
+  return parts > 1 ? (size_t)parts * 2 * batch * sinks * d * sizeof(float) : 0;
+}
+// Workgroups that share 32 queries of a slice in the forward, each with a part of the keys: 1 where the queries alone give the CUs work.
+inline int forward_parts(int64_t batch, int64_t n_q, int64_t n_k, int64_t d, int64_t window, int64_t sinks) {
+  const int64_t groups = (n_q + 31) / 32 * batch, seen = window + 62 < n_k ? window + 62 : n_k, steps = (seen + 31) / 32 + (sinks + 31) / 32;
+  if (groups >= 192) return 1;
+  int64_t parts = (d == 128 ? 256 : 512) / groups;
+  if (parts > steps / 4) parts = steps / 4;
+  return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+}
+inline size_t forward_part_bytes(int64_t batch, int64_t n_q, int64_t d, int parts) { return parts > 1 ? (size_t)parts * batch * n_q * (d + 2) * sizeof(float) : 0; }
+
 // ---- split products: the query-tiled and the key-tiled sweep of a backward pass (fhog_split.hip, fhog_attn_split.hip) ----------------------
 // In one launch the two fill CUs for each other; each in a launch of its own (0 below) a side that is far shorter, whose few workgroups have a long
 // stream each, gets as many waves on the same rows as it needs by itself. waves_of_side: those, by its 128-row workgroups.

@@ -1,0 +1,129 @@
+// What masks with sinks need beside the sweeps: the rows of dK, dV (dK2, dV2) of the sinks, and the join of forwards whose keys went to several workgroups.
+//
+// A key j < sinks is seen by every query from the diagonal on, n_q - j + ... of them, the other keys by a window's length: as rows of an ordinary
+// workgroup of the key-tiled sweep the sinks would keep it busy n_q / window times as long as the others. The sweep therefore treats them as keys of the band, and
+// a launch behind it computes their rows over ALL their queries and puts them in place: workgroups of 32 sinks, four waves on the same rows, the queries
+// dealt out over `parts` workgroups (sink_parts), whose fp32 sums are added here in a fixed order and rounded once.
+#include "fhog_rules.h"
+#include "fhog_split_util.h"
+
+namespace fhog {
+using namespace splitk;
+namespace {
+
+// Sums of four columns over the parts. Each part is one 16-byte load, `stride` floats from the last; four are under way at a time.
+__device__ __forceinline__ f32x4_t sum_parts(const float* from, int parts, int64_t stride) {
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  int i = 0;
+  for (; i + 4 <= parts; i += 4) {
+    f32x4_t x[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) x[u] = *reinterpret_cast<const f32x4_t*>(from + (i + u) * stride);
+#pragma unroll
+    for (int u = 0; u < 4; u++) sum += x[u];
+  }
+  for (; i < parts; i++) sum += *reinterpret_cast<const f32x4_t*>(from + i * stride);
+  return sum;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* to, f32x4_t x) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4_t*>(to) = x;
+  else *reinterpret_cast<u32x2_t*>(to) = pack4<Terms<T>::F16>(x[0], x[1], x[2], x[3]);
+}
+
+// Rows [part][first | second][batch * sinks][d] -> the first `sinks` rows of two tensors; a thread per four columns of a row of both
+struct SinkRows {
+  const float* part;
+  void *first, *second;
+  int64_t stride_b, stride_n;
+  int32_t parts, batch, sinks, d;
+  float scale;   // of the first tensor
+};
+template <typename T>
+__global__ void __launch_bounds__(256) add_sink_parts(SinkRows a) {
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.batch * a.sinks;
+  const int per_row = a.d / 4;
+  const int64_t row = idx / per_row;
+  const int col = (int)(idx % per_row) * 4;
+  if (row >= rows) return;
+  const float* from = a.part + row * a.d + col;
+  const int64_t to = row / a.sinks * a.stride_b + row % a.sinks * a.stride_n + col;
+  store4((T*)a.first + to, sum_parts(from, a.parts, 2 * rows * a.d) * a.scale);
+  store4((T*)a.second + to, sum_parts(from + rows * a.d, a.parts, 2 * rows * a.d));
+}
+
+hipError_t launch_add(const SinkRows& a, int dtype, hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)a.batch * a.sinks * (a.d / 4) + 255) / 256));
+  switch (dtype) {
+    case FHOG_DTYPE_FP32: hipLaunchKernelGGL(add_sink_parts<float>, grid, dim3(256), 0, s, a); break;
+    case FHOG_DTYPE_FP16: hipLaunchKernelGGL(add_sink_parts<_Float16>, grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(add_sink_parts<__bf16>, grid, dim3(256), 0, s, a);
+  }
+  return hipGetLastError();
+}
+
+// O_i = sum_p 2^(m_p - M) acc_p / l, l = sum_p 2^(m_p - M) l_p, L_i = ln 2 (M + log2 l). A part that saw no key of the row has m = -inf, l = 0 and a row of
+// zeros. A thread per four columns.
+template <typename T>
+__global__ void __launch_bounds__(256) join_forward(AttnParams p) {
+  const PartialRows part(p);
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per_row = p.d / 4;
+  const int64_t row = idx / per_row;
+  const int col = (int)(idx % per_row) * 4;
+  if (row >= part.rows) return;
+  float top = -INFINITY, l = 0.f;
+  for (int i = 0; i < p.n_split; i++) top = fmaxf(top, part.stats(i)[row][0]);
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < p.n_split; i++) {
+    const f32x2_t ml = part.stats(i)[row];
+    const float w = __builtin_amdgcn_exp2f(ml[0] - top);
+    l = __builtin_fmaf(ml[1], w, l);
+    sum += *reinterpret_cast<const f32x4_t*>(part.row(i, row) + col) * w;
+  }
+  const int64_t to = row / p.n_q * p.stride_qb + row % p.n_q * p.stride_qn + col;
+  store4((T*)p.o + to, sum * (1.f / l));
+  if (col == 0) p.lse[row] = (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;   // v_log_f32 is log2
+}
+
+// The problem of the sinks alone: their keys, every query, the mask without its window
+template <typename P>
+P sinks_alone(const P& p) {
+  P a = p;
+  a.n_k = p.sinks;
+  a.window = p.n_q + p.n_k;
+  a.sinks = 0;
+  return a;
+}
+
+}  // namespace
+
+hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)p.batch * p.n_q * (p.d / 4) + 255) / 256));
+  switch (dtype) {
+    case FHOG_DTYPE_FP32: hipLaunchKernelGGL(join_forward<float>, grid, dim3(256), 0, s, p); break;
+    case FHOG_DTYPE_FP16: hipLaunchKernelGGL(join_forward<_Float16>, grid, dim3(256), 0, s, p); break;
+    default: hipLaunchKernelGGL(join_forward<__bf16>, grid, dim3(256), 0, s, p);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_sink_keys(const AttnParams& p, int dtype, hipStream_t s) {
+  AttnParams a = sinks_alone(p);
+  a.tile_major_k = 0;
+  const bool bit16 = dtype != FHOG_DTYPE_FP32 && p.d != 32;
+  const hipError_t e = bit16 ? launch_small_sink_bwd(a, s) : launch_attn_split_parts(a, dtype, true, s);
+  if (e != hipSuccess || a.n_split == 1) return e;
+  return launch_add({a.part, a.dk, a.dv, a.stride_kb, a.stride_kn, a.n_split, a.batch, a.n_k, a.d, a.scale}, dtype, s);
+}
+
+hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, hipStream_t s) {
+  Params a = sinks_alone(p);
+  a.tile_major = a.tile_major_k = 0;
+  const hipError_t e = split_products ? launch_split_sink_grads(a, dtype, s) : launch_small_sink_grads(a, s);
+  if (e != hipSuccess || a.n_split == 1) return e;
+  return launch_add({a.part, a.dk2, a.dv2, a.stride_kb, a.stride_kn, a.n_split, a.batch, a.n_k, a.d, a.scale}, dtype, s);
+}
+
+}  // namespace fhog

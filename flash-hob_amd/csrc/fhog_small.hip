@@ -92,6 +92,15 @@ __device__ __forceinline__ void store_part(uint16_t* row, const f32x4_t (*out)[G
           pack4<F16>(out[cb][g][0] * scale, out[cb][g][1] * scale, out[cb][g][2] * scale, out[cb][g][3] * scale);
 }
 
+// ... as fp32 numbers
+template <int NC, int G>
+__device__ __forceinline__ void store_partial(float* row, const f32x4_t (*out)[G], int ws, int h) {
+#pragma unroll
+  for (int cb = 0; cb < NC; cb++)
+#pragma unroll
+    for (int g = 0; g < G; g++) *reinterpret_cast<f32x4_t*>(row + 32 * cb + 8 * (G * ws + g) + 4 * h) = out[cb][g];
+}
+
 template <int D>
 __device__ __forceinline__ void lane_offsets(int lane, int (&aoff)[D / 16], int (&troff)[D / 32][2]) {
 #pragma unroll
@@ -132,12 +141,12 @@ __global__ void __launch_bounds__(256, 2) small_stats(Params p) {
   const int64_t qoff = (int64_t)bh * p.stride_qb, koff = (int64_t)bh * p.stride_kb, row = (int64_t)bh * p.n_q + qr;
   const __bf16* const src[NT] = {(const __bf16*)p.k + koff, (const __bf16*)p.ddk + koff, (const __bf16*)p.v + koff, (const __bf16*)p.ddv + koff};
 
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
   int j_begin, j_end;
   geo.tile_range(q0, TS, j_begin, j_end);
   Dma<D, 1> dma;
   dma.init(p.stride_kn, 0, lane);
-  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, (int64_t)j * TS * p.stride_kn, 0, p.n_k - j * TS); };
+  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, geo.offset(j, p.stride_kn), 0, geo.end(j) - geo.at(j)); };
   char* const ring = smem + wave * NBUF * STAGE;
   first_tiles<W, NBUF, STAGE>(j_begin + ws, j_end, ring, issue);
 
@@ -156,10 +165,10 @@ __global__ void __launch_bounds__(256, 2) small_stats(Params p) {
   float red[5] = {};   // sum P E, and over keys of P ddS, v ddS, v and P with v = P u
   f32x16_t none[NC];
   own_tiles<W, NBUF, STAGE, NT * Dma<D, 1>::IPT>(j_begin + ws, j_end, ring, issue, [&](const char* stage, int j) {
-    const int k0 = j * TS;
-    const bool masked = geo.partial(k0, q0);
+    const int k0 = geo.at(j);
+    const bool masked = geo.partial(k0, q0, geo.sink(j));
     int lo = 0, hi = 0;
-    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
+    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
     q_block<F16, D, 5>(stage, aoff, troff, Qb, ddQb, dOb, masked, lo, hi, c_scale_log2, l_log2, p.scale, dsum, 0.f, 0.f, red[0], red[1],
                        red[2], red[3], red[4], none, none);
   });
@@ -196,12 +205,12 @@ __device__ __forceinline__ void grads_q(const Params& p, char* smem) {
   const int64_t qoff = (int64_t)bh * p.stride_qb, koff = (int64_t)bh * p.stride_kb, row = (int64_t)bh * p.n_q + qr;
   const __bf16* const src[NT] = {(const __bf16*)p.k + koff, (const __bf16*)p.ddk + koff, (const __bf16*)p.v + koff, (const __bf16*)p.ddv + koff};
 
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
   int j_begin, j_end;
   geo.tile_range(q0, TS, j_begin, j_end);
   Dma<D, 1> dma;
   dma.init(p.stride_kn, 0, lane);
-  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, (int64_t)j * TS * p.stride_kn, 0, p.n_k - j * TS); };
+  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, geo.offset(j, p.stride_kn), 0, geo.end(j) - geo.at(j)); };
   char* const ring = smem + wave * NBUF * STAGE;
   first_tiles<W, NBUF, STAGE>(j_begin + ws, j_end, ring, issue);
 
@@ -220,10 +229,10 @@ __device__ __forceinline__ void grads_q(const Params& p, char* smem) {
   for (int cb = 0; cb < NC; cb++) acc_dq[cb] = f32x16_t{0}, acc_ddo[cb] = f32x16_t{0};
   float none[5] = {};
   own_tiles<W, NBUF, STAGE, NT * Dma<D, 1>::IPT>(j_begin + ws, j_end, ring, issue, [&](const char* stage, int j) {
-    const int k0 = j * TS;
-    const bool masked = geo.partial(k0, q0);
+    const int k0 = geo.at(j);
+    const bool masked = geo.partial(k0, q0, geo.sink(j));
     int lo = 0, hi = 0;
-    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
+    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
     q_block<F16, D, 3>(stage, aoff, troff, Qb, ddQb, dOb, masked, lo, hi, c_scale_log2, l_log2, p.scale, dsum, dd, kc, none[0], none[1],
                        none[2], none[3], none[4], acc_dq, acc_ddo);
   });
@@ -241,11 +250,14 @@ __device__ __forceinline__ void grads_q(const Params& p, char* smem) {
 template <int D>
 constexpr int grads_k_stage = 3 * TS * 2 * D + 4 * TS * 4;   // Q, ddQ, dO tiles and the statistics of their rows
 
-template <bool F16, int D, int MASK, int W>
+// PARTS: the streamed queries are dealt out over n_split workgroups, whose partial results are fp32 rows [part][dK2 | dV2][batch * n_k][D] in p.part
+template <bool F16, int D, int MASK, int W, bool PARTS = false>
 __device__ __forceinline__ void grads_k(const Params& p, char* smem, int id) {
   constexpr int KK = D / 16, NC = D / 32, ROWS = TS * WAVES / W, NT = 3, TILE = TS * 2 * D, STAGE = grads_k_stage<D>, NBUF = n_buffers<D, 4>;
   int bh, tile;
-  if (!decode_block<MASK>((p.n_k + ROWS - 1) / ROWS, p.batch, false, p.tile_major, bh, tile, false, id)) return;
+  if (!decode_block<MASK>((p.n_k + ROWS - 1) / ROWS, p.batch * (PARTS ? p.n_split : 1), false, p.tile_major, bh, tile, false, id)) return;
+  const int part = PARTS ? bh % p.n_split : 0;
+  if (PARTS) bh /= p.n_split;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = wave / W, ws = wave % W;
@@ -257,6 +269,7 @@ __device__ __forceinline__ void grads_k(const Params& p, char* smem, int id) {
   const StreamQueries<MASK> geo(p.mask_off, p.window, p.n_q);
   int t_begin, t_end;
   geo.tile_range(k0, TS, t_begin, t_end);
+  if (PARTS) split_range(part, p.n_split, t_begin, t_end);
   Dma<D, 1> dma;
   dma.init(p.stride_qn, 0, lane);
   const auto issue = [&](int t, uint32_t lds) {
@@ -295,6 +308,12 @@ __device__ __forceinline__ void grads_k(const Params& p, char* smem, int id) {
   f32x4_t out[2 * NC][4 / W];
   add_waves<W>(acc, smem, group, ws, lane, out);
   if (kj >= p.n_k) return;
+  if (PARTS && p.n_split > 1) {
+    float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + kj) * D;
+    store_partial<NC, 4 / W>(to, out, ws, h);
+    store_partial<NC, 4 / W>(to + (int64_t)p.batch * p.n_k * D, out + NC, ws, h);
+    return;
+  }
   store_part<F16, NC, 4 / W>((uint16_t*)p.dk2 + koff + (int64_t)kj * p.stride_kn, out, p.scale, ws, h);
   store_part<F16, NC, 4 / W>((uint16_t*)p.dv2 + koff + (int64_t)kj * p.stride_kn, out + NC, 1.f, ws, h);
 }
@@ -314,12 +333,15 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) small_grads(Params p, in
 template <int D>
 constexpr int fwd_lds = max_of(WAVES * n_buffers<D, 2> * 2 * TS * 2 * D, add_waves_bytes(D / 32) + WAVES * 2 * 64 * 4);
 
-template <bool F16, int D, int MASK, int W>
+// PARTS: the streamed keys are dealt out over n_split workgroups, which leave fp32 rows and their maximum and sum in p.part (PartialRows)
+template <bool F16, int D, int MASK, int W, bool PARTS = false>
 __global__ void __launch_bounds__(256, 2) small_fwd(AttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int KK = D / 16, NC = D / 32, ROWS = TS * WAVES / W, NT = 2, TILE = TS * 2 * D, STAGE = NT * TILE, NBUF = n_buffers<D, NT>;
   int bh, tile;
-  if (!decode_block<MASK>((p.n_q + ROWS - 1) / ROWS, p.batch, MASK != MASK_NONE, MASK != MASK_NONE, bh, tile)) return;
+  if (!decode_block<MASK>((p.n_q + ROWS - 1) / ROWS, p.batch * (PARTS ? p.n_split : 1), MASK != MASK_NONE, MASK != MASK_NONE, bh, tile)) return;
+  const int part = PARTS ? bh % p.n_split : 0;
+  if (PARTS) bh /= p.n_split;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = wave / W, ws = wave % W;   // row group of the wave, and which of its streamed tiles it takes
@@ -327,12 +349,13 @@ __global__ void __launch_bounds__(256, 2) small_fwd(AttnParams p) {
   const int q0 = tile * ROWS + TS * group, qi = q0 + n, qr = min(qi, p.n_q - 1);
   const int64_t qoff = (int64_t)bh * p.stride_qb, koff = (int64_t)bh * p.stride_kb;
   const __bf16* const src[NT] = {(const __bf16*)p.k + koff, (const __bf16*)p.v + koff};
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
   int j_begin, j_end;
   geo.tile_range(q0, TS, j_begin, j_end);
+  if (PARTS) split_range(part, p.n_split, j_begin, j_end);
   Dma<D, 1> dma;
   dma.init(p.stride_kn, 0, lane);
-  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, (int64_t)j * TS * p.stride_kn, 0, p.n_k - j * TS); };
+  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, geo.offset(j, p.stride_kn), 0, geo.end(j) - geo.at(j)); };
   char* const ring = smem + wave * NBUF * STAGE;
   first_tiles<W, NBUF, STAGE>(j_begin + ws, j_end, ring, issue);
   bf16x8_t Qb[KK];
@@ -346,10 +369,10 @@ __global__ void __launch_bounds__(256, 2) small_fwd(AttnParams p) {
 #pragma unroll
   for (int cb = 0; cb < NC; cb++) acc[0][cb] = f32x16_t{0};
   own_tiles<W, NBUF, STAGE, NT * Dma<D, 1>::IPT>(j_begin + ws, j_end, ring, issue, [&](const char* stage, int j) {
-    const int k0 = j * TS;
-    const bool masked = geo.partial(k0, q0);
+    const int k0 = geo.at(j);
+    const bool masked = geo.partial(k0, q0, geo.sink(j));
     int lo = 0, hi = 0;
-    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
+    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
     fwd_block<F16, D>(stage, aoff, troff, Qb, masked, lo, hi, c_scale_log2, m, l, acc);
   });
   __syncthreads();
@@ -372,6 +395,12 @@ __global__ void __launch_bounds__(256, 2) small_fwd(AttnParams p) {
   add_waves<W>(acc[0], smem, group, ws, lane, out);
   l_all += __shfl_xor(l_all, 32);
   if (qi >= p.n_q) return;
+  if (PARTS) {
+    const PartialRows rows(p);
+    store_partial<NC, 4 / W>(rows.row(part, (int64_t)bh * p.n_q + qi), out, ws, h);
+    if (ws == 0 && h == 0) rows.stats(part)[(int64_t)bh * p.n_q + qi] = f32x2_t{m_all, l_all};
+    return;
+  }
   store_part<F16, NC, 4 / W>((uint16_t*)p.o + qoff + (int64_t)qi * p.stride_qn, out, 1.f / l_all, ws, h);
   if (ws == 0 && h == 0) p.lse[(int64_t)bh * p.n_q + qi] = (m_all + __builtin_amdgcn_logf(l_all)) * 0.6931471805599453f;   // v_log_f32 is log2
 }
@@ -389,12 +418,12 @@ __device__ __forceinline__ void bwd_q(const AttnParams& p, char* smem) {
   const int q0 = tile * ROWS + TS * group, qi = q0 + n, qr = min(qi, p.n_q - 1);
   const int64_t qoff = (int64_t)bh * p.stride_qb, koff = (int64_t)bh * p.stride_kb, row = (int64_t)bh * p.n_q + qr;
   const __bf16* const src[NT] = {(const __bf16*)p.k + koff, (const __bf16*)p.v + koff};
-  const StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k);
+  StreamKeys<MASK> geo(p.mask_off, p.window, p.n_k, p.sinks);
   int j_begin, j_end;
   geo.tile_range(q0, TS, j_begin, j_end);
   Dma<D, 1> dma;
   dma.init(p.stride_kn, 0, lane);
-  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, (int64_t)j * TS * p.stride_kn, 0, p.n_k - j * TS); };
+  const auto issue = [&](int j, uint32_t lds) { dma.template issue_all<NT>(lds, TILE, src, geo.offset(j, p.stride_kn), 0, geo.end(j) - geo.at(j)); };
   char* const ring = smem + wave * NBUF * STAGE;
   first_tiles<W, NBUF, STAGE>(j_begin + ws, j_end, ring, issue);
   bf16x8_t Qb[KK], dOb[KK], Ob[KK];
@@ -411,10 +440,10 @@ __device__ __forceinline__ void bwd_q(const AttnParams& p, char* smem) {
 #pragma unroll
   for (int cb = 0; cb < NC; cb++) acc[0][cb] = f32x16_t{0};
   own_tiles<W, NBUF, STAGE, NT * Dma<D, 1>::IPT>(j_begin + ws, j_end, ring, issue, [&](const char* stage, int j) {
-    const int k0 = j * TS;
-    const bool masked = geo.partial(k0, q0);
+    const int k0 = geo.at(j);
+    const bool masked = geo.partial(k0, q0, geo.sink(j));
     int lo = 0, hi = 0;
-    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi);
+    if (masked) keep_branch(), geo.limits(k0, qi, h, lo, hi, geo.sink(j));
     bwd_q_block<F16, D>(stage, aoff, troff, Qb, dOb, masked, lo, hi, c_scale_log2, l_log2, dsum, acc);
   });
   __syncthreads();
@@ -430,11 +459,13 @@ constexpr int bwd_k_stage = 3 * TS * 2 * D + 2 * TS * 4;   // Q, dO, O tiles, L 
 template <int D>
 constexpr int bwd_k_buffers = 2 * WAVES * bwd_k_stage<D> <= 128 * 1024 ? 2 : 1;
 
-template <bool F16, int D, int MASK, int W>
+template <bool F16, int D, int MASK, int W, bool PARTS = false>   // PARTS: as in grads_k
 __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
   constexpr int KK = D / 16, NC = D / 32, ROWS = TS * WAVES / W, NT = 3, TILE = TS * 2 * D, STAGE = bwd_k_stage<D>, NBUF = bwd_k_buffers<D>;
   int bh, tile;
-  if (!decode_block<MASK>((p.n_k + ROWS - 1) / ROWS, p.batch, false, p.tile_major_k != 0, bh, tile, false, id)) return;
+  if (!decode_block<MASK>((p.n_k + ROWS - 1) / ROWS, p.batch * (PARTS ? p.n_split : 1), false, p.tile_major_k != 0, bh, tile, false, id)) return;
+  const int part = PARTS ? bh % p.n_split : 0;
+  if (PARTS) bh /= p.n_split;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = wave / W, ws = wave % W;
@@ -448,6 +479,7 @@ __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
   const StreamQueries<MASK> geo(p.mask_off, p.window, p.n_q);
   int t_begin, t_end;
   geo.tile_range(k0, TS, t_begin, t_end);
+  if (PARTS) split_range(part, p.n_split, t_begin, t_end);
   Dma<D, 1> dma;
   dma.init(p.stride_qn, 0, lane);
   const auto issue = [&](int t, uint32_t lds) {
@@ -486,6 +518,12 @@ __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
   f32x4_t out[2 * NC][4 / W];
   add_waves<W>(all, smem, group, ws, lane, out);
   if (kj >= p.n_k) return;
+  if (PARTS && p.n_split > 1) {
+    float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + kj) * D;
+    store_partial<NC, 4 / W>(to, out, ws, h);
+    store_partial<NC, 4 / W>(to + (int64_t)p.batch * p.n_k * D, out + NC, ws, h);
+    return;
+  }
   store_part<F16, NC, 4 / W>((uint16_t*)p.dk + koff + (int64_t)kj * p.stride_kn, out, p.scale, ws, h);
   store_part<F16, NC, 4 / W>((uint16_t*)p.dv + koff + (int64_t)kj * p.stride_kn, out + NC, 1.f, ws, h);
 }
@@ -498,6 +536,18 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) small_bwd(AttnParams p, 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   if ((int)blockIdx.x < q_blocks) bwd_q<F16, D, MASK, W>(p, smem);
   else bwd_k<F16, D, MASK, W>(p, smem, (int)blockIdx.x - q_blocks);
+}
+
+// The rows of dK, dV (dK2, dV2) of the sinks, over all queries that see them: p.n_k is the number of sinks there, and there is no window
+template <bool F16, int D>
+__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) sink_bwd(AttnParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  bwd_k<F16, D, MASK_BAND, WAVES, true>(p, smem, blockIdx.x);
+}
+template <bool F16, int D>
+__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) sink_grads(Params p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  grads_k<F16, D, MASK_BAND, WAVES, true>(p, smem, blockIdx.x);
 }
 
 template <auto Kernel, typename... Args>
@@ -527,12 +577,20 @@ hipError_t attn_d(const AttnParams& p, bool backward, hipStream_t s) {
   return launch<small_bwd<F16, D, MASK, W>>(gq + gk, bwd_lds<D>, s, p, (int)gq);
 }
 
+template <bool F16, int D>
+hipError_t fwd_parts_d(const AttnParams& p, hipStream_t s) { return launch<small_fwd<F16, D, MASK_SINK, WAVES, true>>(blocks<WAVES>(p.n_q, p.batch * p.n_split), fwd_lds<D>, s, p); }
+template <bool F16, int D>
+hipError_t sink_bwd_d(const AttnParams& p, hipStream_t s) { return launch<sink_bwd<F16, D>>(blocks<WAVES>(p.n_k, p.batch * p.n_split), bwd_lds<D>, s, p); }
+template <bool F16, int D>
+hipError_t sink_grads_d(const Params& p, hipStream_t s) { return launch<sink_grads<F16, D>>(blocks<WAVES>(p.n_k, p.batch * p.n_split), grads_lds<D>, s, p); }
+
 }  // namespace
 
 #define FHOG_SMALL_W(FN, F, DD, M, ...) (waves == 4 ? FN<F, DD, M, 4>(__VA_ARGS__) : FN<F, DD, M, 2>(__VA_ARGS__))
 #define FHOG_SMALL(FN, F, DD, ...)                                          \
   (mask == MASK_NONE ? FHOG_SMALL_W(FN, F, DD, MASK_NONE, __VA_ARGS__)      \
-                     : mask == MASK_CAUSAL ? FHOG_SMALL_W(FN, F, DD, MASK_CAUSAL, __VA_ARGS__) : FHOG_SMALL_W(FN, F, DD, MASK_BAND, __VA_ARGS__))
+                     : mask == MASK_CAUSAL ? FHOG_SMALL_W(FN, F, DD, MASK_CAUSAL, __VA_ARGS__) \
+                     : mask == MASK_SINK ? FHOG_SMALL_W(FN, F, DD, MASK_SINK, __VA_ARGS__) : FHOG_SMALL_W(FN, F, DD, MASK_BAND, __VA_ARGS__))
 
 hipError_t launch_small_bwdbwd(const Params& p, int waves, hipStream_t s) {
   const int mask = mask_mode(p);
@@ -547,5 +605,20 @@ hipError_t launch_small_attn(const AttnParams& p, bool backward, int waves, hipS
 }
 #undef FHOG_SMALL
 #undef FHOG_SMALL_W
+
+hipError_t launch_small_fwd_parts(const AttnParams& p, hipStream_t s) {
+  if (p.f16) return p.d == 128 ? fwd_parts_d<true, 128>(p, s) : fwd_parts_d<true, 64>(p, s);
+  return p.d == 128 ? fwd_parts_d<false, 128>(p, s) : fwd_parts_d<false, 64>(p, s);
+}
+
+hipError_t launch_small_sink_bwd(const AttnParams& p, hipStream_t s) {
+  if (p.f16) return p.d == 128 ? sink_bwd_d<true, 128>(p, s) : sink_bwd_d<true, 64>(p, s);
+  return p.d == 128 ? sink_bwd_d<false, 128>(p, s) : sink_bwd_d<false, 64>(p, s);
+}
+
+hipError_t launch_small_sink_grads(const Params& p, hipStream_t s) {
+  if (p.f16) return p.d == 128 ? sink_grads_d<true, 128>(p, s) : sink_grads_d<true, 64>(p, s);
+  return p.d == 128 ? sink_grads_d<false, 128>(p, s) : sink_grads_d<false, 64>(p, s);
+}
 
 }  // namespace fhog

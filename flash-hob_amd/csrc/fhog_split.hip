@@ -54,7 +54,9 @@ constexpr bool is_direct = WS == 4 && (PASS == 1 || PASS == 2 || PASS == 5);
 
 // PASS 1: d, dd; 2: b; 3: dQ2, ddO; 4: dK2, dV2 (K-tiled); 5: d, dd, b.
 // pairs: as decode_block takes it
-template <typename T, int D, int PASS, int MASK, int WS>
+// PARTS (pass 4): the streamed queries are dealt out over n_split workgroups, whose partial results are fp32 rows [part][dK2 | dV2][batch * n_k][D] in
+// p.part where there is more than one
+template <typename T, int D, int PASS, int MASK, int WS, bool PARTS = false>
 __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, bool pairs) {
   constexpr bool KSIDE = PASS == 4, STATS = PASS == 1 || PASS == 2 || PASS == 5;
   constexpr int NT = PASS == 1 ? 2 : (KSIDE ? 3 : 4);      // streamed tensors: K, ddK, V, ddV | Q, ddQ, dO
@@ -86,7 +88,9 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
   const int n = lane & 31, h = lane >> 5;
   const int n_sta = KSIDE ? p.n_k : p.n_q, n_str = KSIDE ? p.n_q : p.n_k;
   int bh, tile;
-  if (!decode_block<MASK>((n_sta + ROWS - 1) / ROWS, p.batch, !KSIDE && MASK != MASK_NONE, KSIDE ? p.tile_major_k : p.tile_major, bh, tile, pairs, id)) return;
+  if (!decode_block<MASK>((n_sta + ROWS - 1) / ROWS, p.batch * (PARTS ? p.n_split : 1), !KSIDE && MASK != MASK_NONE, KSIDE ? p.tile_major_k : p.tile_major, bh, tile, pairs, id)) return;
+  const int part = PARTS ? bh % p.n_split : 0;
+  if (PARTS) bh /= p.n_split;
   const int64_t qoff = (int64_t)bh * p.stride_qb, koff = (int64_t)bh * p.stride_kb;
   const int64_t sta_ld = KSIDE ? p.stride_kn : p.stride_qn, str_ld = KSIDE ? p.stride_qn : p.stride_kn;
   const int r0 = tile * ROWS, rw = r0 + 32 * group, ri = rw + n;
@@ -99,9 +103,10 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
     if constexpr (NT == 4) src[2] = (const T*)p.v + koff, src[3] = (const T*)p.ddv + koff;
   }
 
-  typename std::conditional<KSIDE, StreamQueries<MASK>, StreamKeys<MASK>>::type geo(p.mask_off, p.window, n_str);
+  typename std::conditional<KSIDE, StreamQueries<MASK>, StreamKeys<MASK>>::type geo(p.mask_off, p.window, n_str, p.sinks);
   int t_begin, t_end;
   geo.tile_range(r0, ROWS, t_begin, t_end);
+  if (PARTS) split_range(part, p.n_split, t_begin, t_end);
 
   const int64_t srow = (int64_t)bh * p.n_q;
   Stage st[WS];
@@ -113,8 +118,9 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
   const auto fetch = [&](int t) {
 #pragma unroll
     for (int g = 0; g < WS; g++) {
-      const int row0 = (t + g) * TS;
-      st[g].fetch(src, str_ld, min(row0, n_str - 1), n_str, tid);   // a tile past the end is never computed on
+      const int row0 = geo.at(t + g);
+      const int end = MASK == MASK_SINK ? geo.end(t + g) : n_str;
+      st[g].fetch(src, str_ld, min(row0, end - 1), end, tid);   // a tile past the end is never computed on
       if constexpr (KSIDE) {
         const int64_t q = srow + min(row0 + (tid & 31), p.n_q - 1);
         stat_reg[g] = stat_src[q], stat_d[g] = p.ws_d[q], stat_dd[g] = p.ws_dd[q];
@@ -187,7 +193,7 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
 
   Chunk<T> ahead[2][NT];           // DIRECT: the next two k-steps of the lane's streamed row
   const auto load_step = [&](int t, int kk) {
-    const int64_t off = (int64_t)min(t * TS + n, n_str - 1) * str_ld + 16 * kk + 8 * h;
+    const int64_t off = (int64_t)min(geo.at(t) + n, (MASK == MASK_SINK ? geo.end(t) : n_str) - 1) * str_ld + 16 * kk + 8 * h;
 #pragma unroll
     for (int x = 0; x < NT; x++) ahead[kk & 1][x] = load_chunk<T>(src[x] + off);
   };
@@ -261,7 +267,8 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
 
   // prefetch: what requests the next tile; called where the registers it lands in are free
   // behind(slot, slots): what is to be done behind MFMA `slot` of the first level (AHEAD)
-  const auto block = [&](const char* stage, int s0, auto prefetch, auto behind) {
+  // s0: first row of the tile of step t
+  const auto block = [&](const char* stage, int s0, int t, auto prefetch, auto behind) {
     const float* stat = reinterpret_cast<const float*>(stage + Stage::BYTES);
     f32x16_t s = {0}, dds = {0}, dp = {0}, e = {0};
     // u = dP - d and E' = E - (dd d + b) come straight from accumulators that start at the row constants
@@ -318,7 +325,7 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
           streamed(NT - 1);
           e = mma1<T>(e, a, r2);                                // ddV dO^T
         }
-        if constexpr (DIRECT) load_step(s0 / TS + (kk + 2 < KK ? 0 : WS), (kk + 2) % KK);   // past the last tile: its last row again
+        if constexpr (DIRECT) load_step((MASK == MASK_SINK ? t : s0 / TS) + (kk + 2 < KK ? 0 : WS), (kk + 2) % KK);   // past the last tile: its last row again
         if constexpr (RAW || DIRECT) __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -332,12 +339,12 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
     }
     if (RAW && MASK != MASK_NONE) {
       int lo, hi;
-      geo.limits(s0, ri, h, lo, hi);
+      geo.limits(s0, ri, h, lo, hi, geo.sink(t));
 #pragma unroll
       for (int r = 0; r < 16; r++) pv[r] = in_limits(r, lo, hi) ? pv[r] : 0.f;
-    } else if (geo.partial(s0, rw)) {   // wave-uniform: the block holds hidden pairs (mask edge or tensor end)
+    } else if (geo.partial(s0, rw, geo.sink(t))) {   // wave-uniform: the block holds hidden pairs (mask edge or tensor end)
       int lo, hi;
-      geo.limits(s0, ri, h, lo, hi);
+      geo.limits(s0, ri, h, lo, hi, geo.sink(t));
       keep_branch();
 #pragma unroll
       for (int r = 0; r < 16; r++) pv[r] = in_limits(r, lo, hi) ? pv[r] : 0.f;
@@ -408,7 +415,7 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
   if constexpr (DIRECT) {
     // the range of 32 rows holds no tile that is dead to the wave
     if (t_begin + ws < t_end) load_step(t_begin + ws, 0), load_step(t_begin + ws, 1);
-    for (int t = t_begin + ws; t < t_end; t += WS) block(smem, t * TS, [] {}, [](int, int) {});
+    for (int t = t_begin + ws; t < t_end; t += WS) block(smem, geo.at(t), t, [] {}, [](int, int) {});
   }
   if (!DIRECT && t_begin < t_end) publish(0);
   if (INTERLEAVED && t_begin < t_end) fetch(t_begin + 1);
@@ -420,17 +427,17 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
   // 3986, 40 x 300 199 | 193, 2000 | 900 rows 1524 | 1459; causal 32 x 2048 2262 | 2156, 48 x 1537 2244 | 2130; window 700 16 x 1000 x 3000 569 | 541.
   constexpr bool NO_TEST = MASK == MASK_NONE && D == 32;
   const auto sweep = [&](auto has_rows) {
-    const auto works = [&](int s0) { return NO_TEST ? decltype(has_rows)::value : !geo.dead(s0, geo.first_row(rw, n_sta)); };
+    const auto works = [&](int s0, int t) { return NO_TEST ? decltype(has_rows)::value : !geo.dead(s0, geo.first_row(rw, n_sta), geo.sink(t)); };
     for (int t = t_begin; !DIRECT && t < t_end; t += WS) {
       const int buf = NBUF == 2 ? (t - t_begin) & 1 : 0;
-      const int s0 = (t + ws) * TS;
+      const int s0 = geo.at(t + ws);
       if constexpr (INTERLEAVED) {
         // The rows of the tile after this one came in during the step before; behind the last tile they are copies of the last row.
         char* const next = smem + (buf ^ 1) * STAGE;
-        const int row0 = min(s0 + 2 * TS, n_str - 1);
-        if (works(s0)) {
-          block(smem + buf * STAGE, s0, [] {}, [&](int slot, int slots) {
-            st[0].publish_at(next, tid, slot, slots, [&](int i) { st[0].fetch_chunk(i, src, str_ld, row0, n_str, tid); });
+        const int end = MASK == MASK_SINK ? geo.end(t + 2) : n_str, row0 = min(MASK == MASK_SINK ? geo.at(t + 2) : s0 + 2 * TS, end - 1);
+        if (works(s0, t)) {
+          block(smem + buf * STAGE, s0, t, [] {}, [&](int slot, int slots) {
+            st[0].publish_at(next, tid, slot, slots, [&](int i) { st[0].fetch_chunk(i, src, str_ld, row0, end, tid); });
           });
         } else {
           publish(buf ^ 1);
@@ -443,8 +450,8 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
           if (more) fetch(t + WS);
         };
         if (!LATE) next();
-        if ((WS == 1 || t + ws < t_end) && works(s0)) {
-          block(smem + (buf * WS + ws) * STAGE, s0, [&]() {
+        if ((WS == 1 || t + ws < t_end) && works(s0, t + ws)) {
+          block(smem + (buf * WS + ws) * STAGE, s0, t + ws, [&]() {
             if (LATE) {
               __builtin_amdgcn_sched_barrier(0);
               next();
@@ -503,6 +510,12 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
     }
   } else {
     if (ri >= n_sta) return;
+    if (PARTS && p.n_split > 1) {
+      float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + ri) * D;
+      store_rows<float, D>(to, acc0, 1.f, h);
+      store_rows<float, D>(to + (int64_t)p.batch * p.n_k * D, acc1, 1.f, h);
+      return;
+    }
     const int64_t out = (KSIDE ? koff : qoff) + (int64_t)ri * sta_ld;
     store_rows<T, D>((T*)(KSIDE ? p.dk2 : p.dq2) + out, acc0, p.scale, h);
     store_rows<T, D>((T*)(KSIDE ? p.dv2 : p.ddo) + out, acc1, 1.f, h);
@@ -539,6 +552,13 @@ constexpr int lds_bytes() {
   constexpr int stages = is_direct<PASS, WS> ? 0 : n_buffers<T, D, WS>(stage) * WS * stage + (is_raw<T, D> && !STATS ? 4 * TS * D * 4 : 0);
   constexpr int xch = WS > 1 ? nw * (WS - 1) * (STATS ? 5 : 2 * D / 32 * 16) * 64 * 4 : 0;
   return stages > xch ? stages : xch;
+}
+
+// The rows of dK2, dV2 of the sinks, over all queries that see them: p.n_k is their number, and there is no window
+template <typename T, int D, int WS>
+__global__ void __launch_bounds__(256, (min_workgroups<D, WS>)) split_sink_grads(Params p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  split_run<T, D, 4, MASK_BAND, WS, true>(p, smem, blockIdx.x, false);
 }
 
 template <typename T, int D, int PASS, int MASK, int WS>
@@ -626,7 +646,17 @@ hipError_t launch_grads(const Params& p, int sides, hipStream_t s) {
 }
 
 template <typename T, int D>
+hipError_t launch_sink_grads(const Params& p, hipStream_t s) {
+  constexpr int WS = lds_bytes<T, D, 4, 4>() <= 160 * 1024 ? 4 : lds_bytes<T, D, 4, 2>() <= 160 * 1024 ? 2 : 1, smem = lds_bytes<T, D, 4, WS>();
+  const hipError_t e = allow_dynamic_lds<split_sink_grads<T, D, WS>>(smem);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((split_sink_grads<T, D, WS>), dim3(blocks<WS>(p.n_k, p.batch * p.n_split)), dim3(256), smem, s, p);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
 hipError_t launch_td(const Params& p, int pass, hipStream_t s) {
+  if (p.sinks > 0) return pass == FHOG_PASS_DD_B ? launch_sweep<T, D, 5, MASK_SINK>(p, s) : pass == kPassGrads ? launch_grads<T, D, MASK_SINK>(p, 3, s) : hipErrorInvalidValue;
 #define FHOG_SPLIT_PASS(N) (p.causal ? launch_sweep<T, D, N, MASK_BAND>(p, s) : launch_sweep<T, D, N, MASK_NONE>(p, s))
   switch (pass) {
     case FHOG_PASS_DD: return FHOG_SPLIT_PASS(1);
@@ -651,6 +681,12 @@ hipError_t launch_t(const Params& p, int pass, hipStream_t s) {
 }
 
 }  // namespace
+
+hipError_t launch_split_sink_grads(const Params& p, int dtype, hipStream_t s) {
+#define FHOG_SINK_GRADS(D) (dtype == FHOG_DTYPE_FP32 ? launch_sink_grads<float, D>(p, s) : dtype == FHOG_DTYPE_FP16 ? launch_sink_grads<_Float16, D>(p, s) : launch_sink_grads<__bf16, D>(p, s))
+  return p.d == 32 ? FHOG_SINK_GRADS(32) : p.d == 64 ? FHOG_SINK_GRADS(64) : p.d == 128 ? FHOG_SINK_GRADS(128) : hipErrorInvalidValue;
+#undef FHOG_SINK_GRADS
+}
 
 hipError_t launch_split_pass(const Params& p, int dtype, int pass, hipStream_t s) {
   if (dtype == FHOG_DTYPE_FP32) return launch_t<float>(p, pass, s);

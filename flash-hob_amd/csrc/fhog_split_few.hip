@@ -54,13 +54,13 @@ __device__ __forceinline__ void run(const Params& p, char* smem, int id) {
   } else {
     src[0] = (const T*)p.k + koff, src[1] = (const T*)p.ddk + koff, src[2] = (const T*)p.v + koff, src[3] = (const T*)p.ddv + koff;
   }
-  typename std::conditional<KSIDE, StreamQueries<MASK>, StreamKeys<MASK>>::type geo(p.mask_off, p.window, n_str);
+  typename std::conditional<KSIDE, StreamQueries<MASK>, StreamKeys<MASK>>::type geo(p.mask_off, p.window, n_str, p.sinks);
   int t_begin, t_end;   // holds no tile that is dead to the rows
   geo.tile_range(rw, 32, t_begin, t_end);
 
   Chunk<T> ahead[2][NT];   // the next two k-steps of the lane's streamed row
   const auto load_step = [&](int t, int kk) {
-    const int64_t off = (int64_t)min(t * TS + n, n_str - 1) * str_ld + 16 * kk + 8 * h;
+    const int64_t off = (int64_t)min(geo.at(t) + n, (MASK == MASK_SINK ? geo.end(t) : n_str) - 1) * str_ld + 16 * kk + 8 * h;
 #pragma unroll
     for (int x = 0; x < NT; x++) ahead[kk & 1][x] = load_chunk<T>(src[x] + off);
   };
@@ -100,7 +100,7 @@ __device__ __forceinline__ void run(const Params& p, char* smem, int id) {
   char* const own = smem + ws * S::BYTES;
   float* const stat = reinterpret_cast<float*>(own + NS * TENSOR);   // L log2(e), -d, dd, -(dd d + b) of the 32 queries
   for (int t = t_begin + ws; t < t_end; t += W) {
-    const int s0 = t * TS;
+    const int s0 = geo.at(t);
     f32x16_t s = {0}, dds = {0}, dp = {0}, e = {0};
     if constexpr (KSIDE) {
       stat[(h ? 2 * TS : 0) + n] = h ? stat_dd : stat_l * kLog2e;
@@ -154,9 +154,9 @@ __device__ __forceinline__ void run(const Params& p, char* smem, int id) {
 #pragma unroll
       for (int i = 0; i < 4; i++) pv[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c_scale_log2, -l4[i]));
     }
-    if (geo.partial(s0, rw)) {   // wave-uniform: the block holds hidden pairs (mask edge or tensor end)
+    if (geo.partial(s0, rw, geo.sink(t))) {   // wave-uniform: the block holds hidden pairs (mask edge or tensor end)
       int lo, hi;
-      geo.limits(s0, ri, h, lo, hi);
+      geo.limits(s0, ri, h, lo, hi, geo.sink(t));
       keep_branch();
 #pragma unroll
       for (int r = 0; r < 16; r++) pv[r] = in_limits(r, lo, hi) ? pv[r] : 0.f;
@@ -232,7 +232,7 @@ hipError_t launch(const Params& p, int sides, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_split_few(const Params& p, int sides, hipStream_t s) {
-#define FHOG_FEW(D) (p.causal ? launch<D, MASK_BAND>(p, sides, s) : launch<D, MASK_NONE>(p, sides, s))
+#define FHOG_FEW(D) (p.sinks > 0 ? launch<D, MASK_SINK>(p, sides, s) : p.causal ? launch<D, MASK_BAND>(p, sides, s) : launch<D, MASK_NONE>(p, sides, s))
   switch (p.d) {
     case 32: return FHOG_FEW(32);
     case 64: return FHOG_FEW(64);

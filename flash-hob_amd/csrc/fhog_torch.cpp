@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <tuple>
@@ -115,11 +116,11 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 
 struct Mask {
   int32_t causal;
-  int64_t window;
+  int64_t window, sinks;
 };
 
 bool mask_applies(const Mask& m, int64_t n_q, int64_t n_k) {
-  if (m.causal < FHOG_MASK_NONE || m.causal > FHOG_MASK_BOTTOM_RIGHT || m.window < 0 || m.window > INT32_MAX) return false;
+  if (m.causal < FHOG_MASK_NONE || m.causal > FHOG_MASK_BOTTOM_RIGHT || m.window < 0 || m.window > INT32_MAX || m.sinks < 0) return false;
   if (m.causal == FHOG_MASK_NONE) return m.window == 0;
   return m.causal == FHOG_MASK_TOP_LEFT ? n_q == n_k : n_k >= n_q;
 }
@@ -148,7 +149,13 @@ Forward forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, double sca
   Tensor lse = at::empty(q_.sizes().slice(0, q_.dim() - 1), q_.options().dtype(at::kFloat));
   a.o = o.data_ptr(), a.lse = (float*)lse.data_ptr();
   if (fhog_attn_validate(&a, 0) != FHOG_OK) return std::nullopt;
-  TORCH_CHECK(fhog_attn_fwd(&a, stream_of(q_)) == FHOG_OK, "fhog_attn_fwd: ", fhog_last_error());
+  if (m.sinks == 0) {
+    TORCH_CHECK(fhog_attn_fwd(&a, stream_of(q_)) == FHOG_OK, "fhog_attn_fwd: ", fhog_last_error());
+  } else {
+    const int64_t bytes = (int64_t)fhog_attn_sinks_workspace_bytes(&a, m.sinks, 0);
+    const Tensor ws = workspace(bytes, q_);
+    TORCH_CHECK(fhog_attn_fwd_sinks(&a, m.sinks, ws.data_ptr(), bytes, stream_of(q_)) == FHOG_OK, "fhog_attn_fwd_sinks: ", fhog_last_error());
+  }
   return std::make_tuple(o, lse);
 }
 
@@ -161,12 +168,17 @@ Backward backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Te
   if (!q.set({&q_, &o_, &do_}, strict) || !k.set({&k_, &v_}, strict) || !attn_args(a, q, k, scale, m)) return std::nullopt;
   if (!L.is_cuda() || L.device() != q_.device() || L.numel() != a.batch * a.n_q) return std::nullopt;
   const c10::DeviceGuard guard(q_.device());
-  const Tensor lse = as_lse(L), ws = workspace(a.batch * a.n_q * 4, q_);
+  const Tensor lse = as_lse(L);
   Tensor dq = q.like(), dk = k.like(), dv = k.like();
-  a.o = q.ptr(1), a.dO = q.ptr(2), a.lse = (float*)lse.data_ptr(), a.ws = (float*)ws.data_ptr();
+  a.o = q.ptr(1), a.dO = q.ptr(2), a.lse = (float*)lse.data_ptr();
   a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv = dv.data_ptr();
+  int64_t bytes = a.batch * a.n_q * 4;
+  if (m.sinks > 0) bytes = std::max(bytes, (int64_t)fhog_attn_sinks_workspace_bytes(&a, m.sinks, 1));
+  const Tensor ws = workspace(bytes, q_);
+  a.ws = (float*)ws.data_ptr();
   if (fhog_attn_validate(&a, 1) != FHOG_OK) return std::nullopt;
-  TORCH_CHECK(fhog_attn_bwd(&a, stream_of(q_)) == FHOG_OK, "fhog_attn_bwd: ", fhog_last_error());
+  const int rc = m.sinks > 0 ? fhog_attn_bwd_sinks(&a, m.sinks, bytes, stream_of(q_)) : fhog_attn_bwd(&a, stream_of(q_));
+  TORCH_CHECK(rc == FHOG_OK, m.sinks > 0 ? "fhog_attn_bwd_sinks: " : "fhog_attn_bwd: ", fhog_last_error());
   return std::make_tuple(dq, dk, dv);
 }
 
@@ -193,12 +205,14 @@ DoubleBackward double_backward(const Tensor& q_, const Tensor& k_, const Tensor&
   a.stride_qb = q.l.sb, a.stride_qn = q.l.sn, a.stride_kb = k.l.sb, a.stride_kn = k.l.sn;
   a.scale = (float)scale, a.causal = m.causal, a.window = m.window, a.impl = impl, a.schedule = schedule;
   a.ws = (float*)q.ptr(0);   // any valid pointer: the hint is computed on the host
-  const size_t hint = fhog_bwdbwd_workspace_hint(&a);
+  if (m.sinks > 0 && schedule != FHOG_SCHEDULE_FUSED_STATS) return std::nullopt;
+  const size_t hint = m.sinks > 0 ? fhog_bwdbwd_sinks_workspace_bytes(&a, m.sinks) : fhog_bwdbwd_workspace_hint(&a);
   if (hint == 0) return std::nullopt;   // not valid
-  const int64_t bytes = split ? (int64_t)hint : 3 * a.batch * a.n_q * 4;
+  const int64_t bytes = split || m.sinks > 0 ? (int64_t)hint : 3 * a.batch * a.n_q * 4;
   const Tensor ws = workspace(bytes, q_);
   a.ws = (float*)ws.data_ptr(), a.ws_bytes = bytes;
-  TORCH_CHECK(fhog_bwdbwd(&a, stream_of(q_)) == FHOG_OK, "fhog_bwdbwd: ", fhog_last_error());
+  const int rc = m.sinks > 0 ? fhog_bwdbwd_sinks(&a, m.sinks, stream_of(q_)) : fhog_bwdbwd(&a, stream_of(q_));
+  TORCH_CHECK(rc == FHOG_OK, m.sinks > 0 ? "fhog_bwdbwd_sinks: " : "fhog_bwdbwd: ", fhog_last_error());
   return std::make_tuple(dq2, dk2, dv2, ddo);
 }
 
@@ -207,21 +221,21 @@ double scale_of(const Tensor& q) { return 1.0 / std::sqrt((double)q.size(-1)); }
 
 struct FirstBackward : torch::autograd::Function<FirstBackward> {
   static tensor_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& grad,
-                             const Tensor& L, int64_t causal, int64_t window, int64_t schedule) {
+                             const Tensor& L, int64_t causal, int64_t window, int64_t schedule, int64_t sinks) {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({q, k, v, o, grad, L});
-    ctx->saved_data["arg"] = std::vector<int64_t>{causal, window, schedule};
-    const auto r = backward_(q, k, v, o, grad, L, causal, window);
+    ctx->saved_data["arg"] = std::vector<int64_t>{causal, window, schedule, sinks};
+    const auto r = backward_(q, k, v, o, grad, L, causal, window, sinks);
     return {std::get<0>(r), std::get<1>(r), std::get<2>(r)};
   }
   static std::tuple<Tensor, Tensor, Tensor> backward_(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& grad,
-                                                      const Tensor& L, int64_t causal, int64_t window) {
-    const auto r = ::backward(unpacked(q), unpacked(k), unpacked(v), unpacked(o), grad, unpacked_lse(L), scale_of(q), Mask{(int32_t)causal, window}, false);
+                                                      const Tensor& L, int64_t causal, int64_t window, int64_t sinks) {
+    const auto r = ::backward(unpacked(q), unpacked(k), unpacked(v), unpacked(o), grad, unpacked_lse(L), scale_of(q), Mask{(int32_t)causal, window, sinks}, false);
     TORCH_CHECK(r, "fhog: first-order backward: ", fhog_last_error());
     return *r;
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list g) {
-    tensor_list out(9);
+    tensor_list out(10);
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
     const auto s = ctx->get_saved_variables();
     const auto arg = ctx->saved_data["arg"].toIntVector();
@@ -231,7 +245,7 @@ struct FirstBackward : torch::autograd::Function<FirstBackward> {
       const at::NoGradGuard no_grad;
       const auto dir = [&](size_t i) { return g[i].defined() ? packed(g[i]) : at::zeros_like(s[i]); };
       const auto r = double_backward(unpacked(s[0]), unpacked(s[1]), unpacked(s[2]), unpacked(s[3]), unpacked(s[4]), dir(0), dir(1), dir(2),
-                                     unpacked_lse(s[5]), scale_of(s[0]), Mask{(int32_t)arg[0], arg[1]}, FHOG_IMPL_AUTO, (int)arg[2], true);
+                                     unpacked_lse(s[5]), scale_of(s[0]), Mask{(int32_t)arg[0], arg[1], arg[3]}, FHOG_IMPL_AUTO, (int)arg[2], true);
       TORCH_CHECK(r, "fhog: double-backward: ", fhog_last_error());
       // O and L are caches of (q, k, v): the four results are already total derivatives
       out[0] = std::get<0>(*r), out[1] = std::get<1>(*r), out[2] = std::get<2>(*r), out[4] = std::get<3>(*r);
@@ -247,29 +261,30 @@ struct FirstBackward : torch::autograd::Function<FirstBackward> {
 };
 
 struct Attention : torch::autograd::Function<Attention> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t causal, int64_t window, int64_t schedule) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t causal, int64_t window, int64_t schedule,
+                        int64_t sinks) {
     // The graph of the first backward reaches this node a second time through the saved O, whose gradient FirstBackward
     // does not have: without work to do, and not to be filled in with zeros
     ctx->set_materialize_grads(false);
-    const auto r = ::forward(q, k, v, scale_of(q), Mask{(int32_t)causal, window});
+    const auto r = ::forward(q, k, v, scale_of(q), Mask{(int32_t)causal, window, sinks});
     TORCH_CHECK(r, "fhog: forward: ", fhog_last_error());
     ctx->save_for_backward({q, k, v, std::get<0>(*r), std::get<1>(*r)});
-    ctx->saved_data["arg"] = std::vector<int64_t>{causal, window, schedule};
+    ctx->saved_data["arg"] = std::vector<int64_t>{causal, window, schedule, sinks};
     return std::get<0>(*r);
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list g) {
-    tensor_list out(6);
+    tensor_list out(7);
     if (!g[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
     const auto arg = ctx->saved_data["arg"].toIntVector();
-    const auto r = FirstBackward::apply(s[0], s[1], s[2], s[3], packed(g[0]), s[4], arg[0], arg[1], arg[2]);
+    const auto r = FirstBackward::apply(s[0], s[1], s[2], s[3], packed(g[0]), s[4], arg[0], arg[1], arg[2], arg[3]);
     out[0] = r[0], out[1] = r[1], out[2] = r[2];
     return out;
   }
 };
 
 // What attention() takes here: what ::forward takes, checked before a node of the graph exists
-std::optional<Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t causal, int64_t window, int64_t schedule) {
+std::optional<Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t causal, int64_t window, int64_t schedule, int64_t sinks) {
   // torch.jit.trace records a Python node as a call of it; of a native one it would record the allocations and miss the launches
   if (at::tracer::impl::is_dispatch_enabled()) return std::nullopt;
   // torch.func transforms: the Python nodes say that they have no rule for them
@@ -287,9 +302,10 @@ std::optional<Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& 
   const int64_t d = q.size(-1), n_q = q.size(-2), n_k = k.size(-2);
   if (dtype_code(q.scalar_type()) < 0 || (d != 32 && d != 64 && d != 128) || v.size(-2) != n_k || q.numel() == 0 || k.numel() == 0 ||
       q.numel() / d >= INT32_MAX || q.numel() / d / n_q > 65535 || n_q > (1 << 24) || n_k > (1 << 24) ||
-      !mask_applies(Mask{(int32_t)causal, window}, n_q, n_k) || schedule < FHOG_SCHEDULE_FOUR_PASS || schedule > FHOG_SCHEDULE_THREE_SWEEP)
+      !mask_applies(Mask{(int32_t)causal, window, sinks}, n_q, n_k) || schedule < FHOG_SCHEDULE_FOUR_PASS || schedule > FHOG_SCHEDULE_THREE_SWEEP ||
+      (sinks > 0 && schedule != FHOG_SCHEDULE_FUSED_STATS))
     return std::nullopt;
-  return Attention::apply(q, k, v, causal, window, schedule);
+  return Attention::apply(q, k, v, causal, window, schedule, sinks);
 }
 
 }  // namespace
@@ -297,19 +313,19 @@ std::optional<Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& 
 PYBIND11_MODULE(_fhog_torch, m) {
   namespace py = pybind11;
   const auto free_lock = py::call_guard<py::gil_scoped_release>();
-  m.def("forward", [](const Tensor& q, const Tensor& k, const Tensor& v, double scale, int causal, int64_t window) {
+  m.def("forward", [](const Tensor& q, const Tensor& k, const Tensor& v, double scale, int causal, int64_t window, int64_t sinks) {
     const at::NoGradGuard no_grad;
-    return forward(q, k, v, scale, Mask{causal, window});
+    return forward(q, k, v, scale, Mask{causal, window, sinks});
   }, free_lock);
   m.def("backward", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& g, const Tensor& L, double scale, int causal,
-                       int64_t window) {
+                       int64_t window, int64_t sinks) {
     const at::NoGradGuard no_grad;
-    return backward(q, k, v, o, g, L, scale, Mask{causal, window}, true);
+    return backward(q, k, v, o, g, L, scale, Mask{causal, window, sinks}, true);
   }, free_lock);
   m.def("double_backward", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& g, const Tensor& ddq, const Tensor& ddk,
-                              const Tensor& ddv, const Tensor& L, double scale, int causal, int64_t window, int impl, int schedule, bool split) {
+                              const Tensor& ddv, const Tensor& L, double scale, int causal, int64_t window, int impl, int schedule, bool split, int64_t sinks) {
     const at::NoGradGuard no_grad;
-    return double_backward(q, k, v, o, g, ddq, ddk, ddv, L, scale, Mask{causal, window}, impl, schedule, split);
+    return double_backward(q, k, v, o, g, ddq, ddk, ddv, L, scale, Mask{causal, window, sinks}, impl, schedule, split);
   }, free_lock);
   m.def("attention", &attention, free_lock);
 }

@@ -100,6 +100,16 @@ def lib() -> ctypes.CDLL:
     L.fhog_attn_fwd.argtypes = [POINTER(AttnArgs), c_void_p]
     L.fhog_attn_bwd.restype = c_int
     L.fhog_attn_bwd.argtypes = [POINTER(AttnArgs), c_void_p]
+    L.fhog_attn_sinks_workspace_bytes.restype = c_size_t
+    L.fhog_attn_sinks_workspace_bytes.argtypes = [POINTER(AttnArgs), c_int64, c_int]
+    L.fhog_attn_fwd_sinks.restype = c_int
+    L.fhog_attn_fwd_sinks.argtypes = [POINTER(AttnArgs), c_int64, c_void_p, c_int64, c_void_p]
+    L.fhog_attn_bwd_sinks.restype = c_int
+    L.fhog_attn_bwd_sinks.argtypes = [POINTER(AttnArgs), c_int64, c_int64, c_void_p]
+    L.fhog_bwdbwd_sinks_workspace_bytes.restype = c_size_t
+    L.fhog_bwdbwd_sinks_workspace_bytes.argtypes = [POINTER(BwdBwdArgs), c_int64]
+    L.fhog_bwdbwd_sinks.restype = c_int
+    L.fhog_bwdbwd_sinks.argtypes = [POINTER(BwdBwdArgs), c_int64, c_void_p]
     L.fhog_probe_mfma_rate.restype = c_int
     L.fhog_probe_mfma_rate.argtypes = [c_void_p, c_int, c_int, c_int, POINTER(ctypes.c_double), c_void_p]
     if L.fhog_attn_args_size() != ctypes.sizeof(AttnArgs):

@@ -30,7 +30,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .bwdbwd import _SCHEDULES, flash_bwdbwd, mask_code, native_mask
+from .bwdbwd import _SCHEDULES, check_sinks, flash_bwdbwd, mask_code, native_mask, native_sinks, sinks_code
 
 _HIP_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 _BLOCK_ELEMS = 1 << 26  # fp32 elements of one materialised (heads, rows, N_K) block (256 MiB)
@@ -45,7 +45,7 @@ def _blocks(batch: int, n_q: int, n_k: int):
             yield slice(b0, min(batch, b0 + heads)), slice(r0, min(n_q, r0 + rows))
 
 
-def _scores(q, k, scale, causal, r0, n_q=None, window=None):
+def _scores(q, k, scale, causal, r0, n_q=None, window=None, sinks=0):
     """fp32 scores of query rows r0.. against all keys, masked entries at -inf."""
     s = torch.matmul(q.float(), k.float().transpose(-1, -2)) * scale
     if causal:
@@ -55,7 +55,7 @@ def _scores(q, k, scale, causal, r0, n_q=None, window=None):
         kj = torch.arange(n_k, device=s.device)[None, :]
         hidden = kj > qi
         if window is not None:
-            hidden = hidden | (qi - kj >= window)
+            hidden = hidden | ((qi - kj >= window) & (kj >= sinks))
         s = s.masked_fill(hidden, float("-inf"))
     return s
 
@@ -91,7 +91,7 @@ def _same_layout(ts) -> bool:
     return all(t.stride() == ts[0].stride() and t.stride(-1) == 1 for t in ts)
 
 
-def _attention_forward_hip(q, k, v, scale, causal, window=None):
+def _attention_forward_hip(q, k, v, scale, causal, window=None, sinks=0):
     """O and L from ``fhog_attn_fwd``; raises _NotCovered when the kernels do not cover the arguments."""
     q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
     if not _same_layout([k, v]):
@@ -104,11 +104,17 @@ def _attention_forward_hip(q, k, v, scale, causal, window=None):
         a.o, a.lse = o.data_ptr(), lse.data_ptr()
         if L_.fhog_attn_validate(ctypes.byref(a), 0) != 0:
             raise _NotCovered(L_.fhog_last_error().decode())
-        _lib.check(L_.fhog_attn_fwd(ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        if sinks:
+            nbytes = L_.fhog_attn_sinks_workspace_bytes(ctypes.byref(a), sinks, 0)
+            ws = torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=q.device)
+            _lib.check(L_.fhog_attn_fwd_sinks(ctypes.byref(a), sinks, ctypes.c_void_p(ws.data_ptr()), nbytes, stream))
+        else:
+            _lib.check(L_.fhog_attn_fwd(ctypes.byref(a), stream))
     return o, lse
 
 
-def _attention_backward_hip(q, k, v, o, do, L, scale, causal, window=None):
+def _attention_backward_hip(q, k, v, o, do, L, scale, causal, window=None, sinks=0):
     ts_q = [t if t.stride(-1) == 1 else t.contiguous() for t in (q, o, do)]
     if not _same_layout(ts_q):
         ts_q = [t.contiguous() for t in ts_q]
@@ -130,12 +136,15 @@ def _attention_backward_hip(q, k, v, o, do, L, scale, causal, window=None):
         dq = torch.empty_strided(q.shape, q.stride(), dtype=q.dtype, device=q.device)
         dk = torch.empty_strided(k.shape, k.stride(), dtype=k.dtype, device=k.device)
         dv = torch.empty_strided(k.shape, k.stride(), dtype=k.dtype, device=k.device)
-        ws = torch.empty(q.shape[0] * q.shape[1], dtype=torch.float32, device=q.device)
         a.o, a.lse, a.dO = o.data_ptr(), lse.data_ptr(), do.data_ptr()
-        a.dq, a.dk, a.dv, a.ws = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr()
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        nbytes = max(q.shape[0] * q.shape[1] * 4, L_.fhog_attn_sinks_workspace_bytes(ctypes.byref(a), sinks, 1) if sinks else 0)
+        ws = torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=q.device)
+        a.ws = ws.data_ptr()
         if L_.fhog_attn_validate(ctypes.byref(a), 1) != 0:
             raise _NotCovered(L_.fhog_last_error().decode())
-        _lib.check(L_.fhog_attn_bwd(ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        _lib.check(L_.fhog_attn_bwd_sinks(ctypes.byref(a), sinks, nbytes, stream) if sinks else L_.fhog_attn_bwd(ctypes.byref(a), stream))
     return dq, dk, dv
 
 
@@ -154,7 +163,7 @@ def _second_path(func: str, entry: str, why: Exception, use_hip: Optional[bool])
 
 
 def attention_forward(q, k, v, scale: Optional[float] = None, causal=False, *, window: Optional[int] = None,
-                      use_hip: Optional[bool] = None):
+                      use_hip: Optional[bool] = None, sinks: int = 0):
     """O (dtype of q) and fp32 L = logsumexp_j(scale q.k_j) for (batch, N, d) tensors.
 
     Takes the place of the reference's forward kernel outputs (``fhog/triton_flash.py:123-133``)
@@ -164,29 +173,33 @@ def attention_forward(q, k, v, scale: Optional[float] = None, causal=False, *, w
     ``use_hip``: None = the HIP kernel; when it refuses the arguments (a non-positive scale with 16-bit tensors, strides
     that are not multiples of 16 bytes, CPU tensors), a ``TorchCompositionWarning`` names the reason and the blocked
     torch composition runs instead. True = the HIP kernel or a ``ValueError``; False = the torch composition.
+
+    ``sinks``: first keys that stay visible behind a sliding window (see :func:`fhog.flash_bwdbwd`). With sinks and few queries (single
+    tokens that continue a long context) the keys are dealt out over the GPU and the parts joined.
     """
     if use_hip is not False and q.is_cuda:
-        res = _lib.torch_ext().forward(q, k, v, float(q.shape[-1] ** -0.5 if scale is None else scale), *native_mask(causal, window))
+        res = _lib.torch_ext().forward(q, k, v, float(q.shape[-1] ** -0.5 if scale is None else scale), *native_mask(causal, window), native_sinks(sinks))
         if res is not None:
             return res
     if q.dim() == 4:
         B, H = q.shape[:2]
         o, L = attention_forward(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), scale, causal, window=window,
-                                 use_hip=use_hip)
+                                 use_hip=use_hip, sinks=sinks)
         return o.view(q.shape), L.view(B, H, -1)
     batch, n_q, d = q.shape
     n_k = k.shape[1]
     mask_code(causal, window, n_q, n_k)  # raises on an inapplicable mask
+    sinks = sinks_code(sinks)
     scale = d ** -0.5 if scale is None else scale
     if use_hip is not False:
         try:
-            return _attention_forward_hip(q, k, v, scale, causal, window)
+            return _attention_forward_hip(q, k, v, scale, causal, window, sinks)
         except _NotCovered as why:
             _second_path("attention_forward", "fhog_attn_fwd", why, use_hip)
     o = torch.empty_like(q)
     L = torch.empty(batch, n_q, dtype=torch.float32, device=q.device)
     for hs, rs in _blocks(batch, n_q, n_k):
-        s = _scores(q[hs, rs], k[hs], scale, causal, rs.start, n_q, window)
+        s = _scores(q[hs, rs], k[hs], scale, causal, rs.start, n_q, window, sinks)
         lse = torch.logsumexp(s, dim=-1)
         p = torch.exp(s - lse[..., None])
         o[hs, rs] = torch.matmul(p, v[hs].float()).to(q.dtype)
@@ -201,18 +214,19 @@ def produce_L(Q, K, is_causal: bool = False):
 
 
 def attention_backward(q, k, v, o, do, L, scale: float, causal, *, window: Optional[int] = None,
-                       use_hip: Optional[bool] = None):
+                       use_hip: Optional[bool] = None, sinks: int = 0):
     """First-order backward (dQ, dK, dV); the arithmetic of ``fhog/triton_flash.py:201-220`` without the
-    (batch, N_Q, N_K) tensors. ``use_hip`` as in :func:`attention_forward`."""
+    (batch, N_Q, N_K) tensors. ``use_hip`` and ``sinks`` as in :func:`attention_forward`."""
     if use_hip is not False and q.is_cuda and q.dim() == 3:
-        res = _lib.torch_ext().backward(q, k, v, o, do, L, float(scale), *native_mask(causal, window))
+        res = _lib.torch_ext().backward(q, k, v, o, do, L, float(scale), *native_mask(causal, window), native_sinks(sinks))
         if res is not None:
             return res
+    sinks = sinks_code(sinks)
     batch, n_q, d = q.shape
     n_k = k.shape[1]
     if use_hip is not False:
         try:
-            return _attention_backward_hip(q, k, v, o, do, L, scale, causal, window)
+            return _attention_backward_hip(q, k, v, o, do, L, scale, causal, window, sinks)
         except _NotCovered as why:
             _second_path("attention_backward", "fhog_attn_bwd", why, use_hip)
     dq = torch.empty_like(q)
@@ -220,7 +234,7 @@ def attention_backward(q, k, v, o, do, L, scale: float, causal, *, window: Optio
     dv = torch.zeros(v.shape, dtype=torch.float32, device=v.device)
     for hs, rs in _blocks(batch, n_q, n_k):
         qf, dof = q[hs, rs].float(), do[hs, rs].float()
-        s = _scores(q[hs, rs], k[hs], scale, causal, rs.start, n_q, window)
+        s = _scores(q[hs, rs], k[hs], scale, causal, rs.start, n_q, window, sinks)
         p = torch.exp(s - L[hs, rs].float()[..., None])
         dsum = (o[hs, rs].float() * dof).sum(-1, keepdim=True)
         dp = torch.matmul(dof, v[hs].float().transpose(-1, -2))
@@ -239,16 +253,17 @@ class AttnBwd(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, q, k, v, o, do, L, scale, causal, window=None, schedule=None):
+    def forward(ctx, q, k, v, o, do, L, scale, causal, window=None, schedule=None, sinks=0):
         ctx.save_for_backward(q, k, v, o, do, L)
         ctx.scale = scale
         ctx.causal = causal
         ctx.window = window
         ctx.schedule = schedule
+        ctx.sinks = sinks
         ctx.set_materialize_grads(False)
         sq = q.shape
         f = (lambda t: t.flatten(0, 1)) if q.dim() == 4 else (lambda t: t)
-        dq, dk, dv = attention_backward(f(q), f(k), f(v), f(o), f(do), f(L), scale, causal, window=window)
+        dq, dk, dv = attention_backward(f(q), f(k), f(v), f(o), f(do), f(L), scale, causal, window=window, sinks=sinks)
         return dq.view(sq), dk.view(k.shape), dv.view(v.shape)
 
     @staticmethod
@@ -256,12 +271,12 @@ class AttnBwd(torch.autograd.Function):
     def backward(ctx, ddq, ddk, ddv):
         q, k, v, o, do, L = ctx.saved_tensors
         if ddq is None and ddk is None and ddv is None:
-            return (None,) * 10
+            return (None,) * 11
         ddq, ddk, ddv = (torch.zeros_like(t) if g is None else g.contiguous() for g, t in ((ddq, q), (ddk, k), (ddv, v)))
         dq2, dk2, dv2, ddo = flash_bwdbwd(q, k, v, o, do, ddq, ddk, ddv, L,
-                                          ctx.scale, causal=ctx.causal, window=ctx.window, schedule=ctx.schedule)
+                                          ctx.scale, causal=ctx.causal, window=ctx.window, schedule=ctx.schedule, sinks=ctx.sinks)
         # O and L are caches of (q, k, v): the four results are already total derivatives.
-        return dq2, dk2, dv2, None, ddo, None, None, None, None, None
+        return dq2, dk2, dv2, None, ddo, None, None, None, None, None, None
 
 
 class FlashAttention(torch.autograd.Function):
@@ -269,13 +284,15 @@ class FlashAttention(torch.autograd.Function):
     ``FlashAttention2`` (``fhog/triton_flash.py:136-198``), twice differentiable."""
 
     @staticmethod
-    def forward(ctx, q, k, v, is_causal=False, window=None, schedule=None):
+    def forward(ctx, q, k, v, is_causal=False, window=None, schedule=None, sinks=0):
+        sinks = check_sinks(sinks, schedule)
         scale = q.shape[-1] ** -0.5
-        o, L = attention_forward(q, k, v, scale, is_causal, window=window)
+        o, L = attention_forward(q, k, v, scale, is_causal, window=window, sinks=sinks)
         ctx.save_for_backward(q, k, v, o, L)
         ctx.is_causal = is_causal
         ctx.window = window
         ctx.schedule = schedule
+        ctx.sinks = sinks
         ctx.scale = scale
         # The graph of the first backward reaches this node a second time through the saved O, whose gradient AttnBwd does
         # not have (O is a cache of q, k, v). Left to fill it in with zeros, autograd would run a whole first backward on
@@ -286,19 +303,20 @@ class FlashAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do):
         if do is None:
-            return (None,) * 6
+            return (None,) * 7
         q, k, v, o, L = ctx.saved_tensors
-        dq, dk, dv = AttnBwd.apply(q, k, v, o, do.contiguous(), L, ctx.scale, ctx.is_causal, ctx.window, ctx.schedule)
-        return dq, dk, dv, None, None, None
+        dq, dk, dv = AttnBwd.apply(q, k, v, o, do.contiguous(), L, ctx.scale, ctx.is_causal, ctx.window, ctx.schedule, ctx.sinks)
+        return dq, dk, dv, None, None, None, None
 
 
-def attention(q, k, v, is_causal=False, window: Optional[int] = None, schedule: Optional[str] = None):
+def attention(q, k, v, is_causal=False, window: Optional[int] = None, schedule: Optional[str] = None, *, sinks: int = 0):
     """Twice-differentiable scaled-dot-product attention (scale = d^-1/2). ``is_causal``: False | True |
     "bottom_right"; ``window``: sliding-window length on top of a causal mask; ``schedule``: pass schedule of the
-    double-backward (see :func:`fhog.flash_bwdbwd`; None = its default, three sweeps with ``dd`` and ``b`` from the first)."""
+    double-backward (see :func:`fhog.flash_bwdbwd`; None = its default, three sweeps with ``dd`` and ``b`` from the first);
+    ``sinks``: first keys that stay visible behind the window (default schedule only)."""
     if q.is_cuda:
         # the same chain as native autograd nodes; declines what the kernels do not cover
-        out = _lib.torch_ext().attention(q, k, v, *native_mask(is_causal, window), _SCHEDULES.get(schedule, -1))
+        out = _lib.torch_ext().attention(q, k, v, *native_mask(is_causal, window), _SCHEDULES.get(schedule, -1), native_sinks(sinks))
         if out is not None:
             return out
-    return FlashAttention.apply(q, k, v, is_causal, window, schedule)
+    return FlashAttention.apply(q, k, v, is_causal, window, schedule, sinks)

@@ -98,14 +98,37 @@ def native_mask(causal, window):
     return code, 0 if window is None else min(int(window), _MAX_WINDOW) if int(window) >= 1 else -1
 
 
-def _workspace(args: "_lib.BwdBwdArgs", device, split: bool) -> torch.Tensor:
+def sinks_code(sinks) -> int:
+    """The number of sinks for the C ABI; raises on what is none."""
+    if isinstance(sinks, bool) or not hasattr(sinks, "__index__") or sinks < 0:
+        raise ValueError(f"sinks must be an integer >= 0, got {sinks!r}")
+    return min(int(sinks), _MAX_WINDOW)
+
+
+def native_sinks(sinks) -> int:
+    """The same for the native host side, which declines what it does not know (-1)."""
+    return min(sinks, _MAX_WINDOW) if type(sinks) is int and sinks >= 0 else -1
+
+
+def check_sinks(sinks, schedule, fused_stats: bool = False) -> int:
+    """:func:`sinks_code`, and that the schedule is the one that knows sinks."""
+    n = sinks_code(sinks)
+    if n and schedule_code(schedule, fused_stats) != _lib.SCHEDULE_FUSED_STATS:
+        raise ValueError(f"sinks run under the default schedule only, not {schedule!r}")
+    return n
+
+
+def _workspace(args: "_lib.BwdBwdArgs", device, split: bool, sinks: int = 0) -> torch.Tensor:
     """Allocate the workspace of a call and enter it into ``args``: the three row statistics ``d | dd | b`` and, with
-    ``split``, room for the partial results of launches that split their streamed side (``fhog_bwdbwd_workspace_hint``)."""
+    ``split`` or sinks, room for the partial results of launches that split their streamed side (``fhog_bwdbwd_workspace_hint``,
+    ``fhog_bwdbwd_sinks_workspace_bytes``)."""
     batch, n_q = args.batch, args.n_q
     nbytes = 3 * batch * n_q * 4
-    if split:
-        args.ws, args.ws_bytes = args.q, 0      # any valid pointer: the hint is computed on the host
-        nbytes = max(nbytes, int(_lib.lib().fhog_bwdbwd_workspace_hint(ctypes.byref(args))))
+    if split or sinks:
+        args.ws, args.ws_bytes = args.q, 0      # any valid pointer: the size is computed on the host
+        L_ = _lib.lib()
+        hint = L_.fhog_bwdbwd_sinks_workspace_bytes(ctypes.byref(args), sinks) if sinks else L_.fhog_bwdbwd_workspace_hint(ctypes.byref(args))
+        nbytes = max(nbytes, int(hint))
     ws = torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device)
     args.ws, args.ws_bytes = ws.data_ptr(), nbytes
     return ws
@@ -146,7 +169,7 @@ def _build_args(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, causal, impl, outs, ws,
 
 def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, window: Optional[int] = None,
                  impl: Optional[str] = None, fused_stats: bool = False, schedule: Optional[str] = None,
-                 return_stats: bool = False, only_pass: Optional[int] = None, split: bool = True):
+                 return_stats: bool = False, only_pass: Optional[int] = None, split: bool = True, sinks: int = 0):
     """Flash Higher-Order-Gradients: VJP of the attention backward pass.
 
     Same positional signature and return order as the reference
@@ -184,7 +207,11 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, windo
         only_pass: run a single pass (0..9, see fhog._lib.PASS_*) instead of the whole chain; for tests and profiling.
         split: allocate the larger workspace that lets launches too small to fill the GPU split their streamed side over
             several workgroups (fp32 partial results, added in a fixed order by a second kernel); False keeps the
-            minimum workspace of three row statistics.
+            minimum workspace of three row statistics (with ``sinks`` the larger one is always there).
+        sinks: number of first keys that stay visible behind a sliding window: with i' as the mask has it, key j is visible to
+            query i iff ``0 <= i' - j < window``, or ``j < sinks`` and ``j <= i'``. ``L`` and ``O`` are those of this mask. More
+            than there are keys means all of them; without a window, sinks change nothing. Default schedule only, and no single
+            passes. (No counterpart in the reference.)
 
     Returns:
         dQ2, dK2, dV2, ddO shaped and typed like Q, K, V, O (+ ``(d, dd, b)`` if ``return_stats``).
@@ -193,7 +220,7 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, windo
         sched = -1 if fused_stats and schedule not in (None, "fused_stats") else _SCHEDULES.get("fused_stats" if fused_stats else schedule, -1)
         try:
             res = _lib.torch_ext().double_backward(Q, K, V, O, dO, ddQ, ddK, ddV, L, float(scale), *native_mask(causal, window),
-                                                   _IMPLS.get(impl, -1), sched, bool(split))
+                                                   _IMPLS.get(impl, -1), sched, bool(split), native_sinks(sinks))
         except TypeError:   # not tensors: named below
             res = None
         if res is not None:
@@ -232,6 +259,9 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, windo
         raise ValueError(f"head dim {d} not supported (32, 64 or 128)")
     mask_code(causal, window, n_q, n_k)  # raises on an inapplicable mask
     sched = schedule_code(schedule, fused_stats)
+    sinks = check_sinks(sinks, schedule, fused_stats)
+    if sinks and only_pass is not None:
+        raise ValueError("single passes do not know sinks")
     if not Q.is_cuda:
         raise ValueError("flash_bwdbwd runs on the GPU only: tensors must be on a ROCm device (there is no CPU path)")
     lse = L.reshape(batch, n_q)
@@ -248,10 +278,12 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, windo
         dv2 = torch.empty_strided(k3.shape, k3.stride(), dtype=Q.dtype, device=Q.device)
         args = _build_args(q3, k3, v3, o3, do3, ddq3, ddk3, ddv3, lse, scale, causal, _IMPLS[impl],
                            (dq2, dk2, dv2, ddo), None, sched, window)
-        ws = _workspace(args, Q.device, split)
+        ws = _workspace(args, Q.device, split, sinks)
         stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
         L_ = _lib.lib()
-        if only_pass is None:
+        if sinks:
+            _lib.check(L_.fhog_bwdbwd_sinks(ctypes.byref(args), sinks, stream))
+        elif only_pass is None:
             _lib.check(L_.fhog_bwdbwd(ctypes.byref(args), stream))
         else:
             _lib.check(L_.fhog_bwdbwd_pass(ctypes.byref(args), int(only_pass), stream))
@@ -272,7 +304,8 @@ class BwdBwdPlan:
     """
 
     def __init__(self, Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, window=None, impl=None,
-                 fused_stats=False, schedule=None, split=True):
+                 fused_stats=False, schedule=None, split=True, sinks=0):
+        self.sinks = check_sinks(sinks, schedule, fused_stats)
         ts = [_flatten(t, "tensor") for t in (Q, K, V, O, dO, ddQ, ddK, ddV)]
         q3, k3, v3, o3, do3, ddq3, ddk3, ddv3 = ts
         q3, o3, do3, ddq3 = _prepare_group([q3, o3, do3, ddq3], "q")
@@ -285,7 +318,7 @@ class BwdBwdPlan:
                           for t in (q3, k3, k3, q3))
         self.args = _build_args(q3, k3, v3, o3, do3, ddq3, ddk3, ddv3, lse, scale, causal, _IMPLS[impl], self.outs, None, schedule_code(schedule, fused_stats), window)
         with torch.cuda.device(Q.device):
-            self.ws_all = _workspace(self.args, Q.device, split)   # d | dd | b, then partial results of split launches
+            self.ws_all = _workspace(self.args, Q.device, split, self.sinks)   # d | dd | b, then partial results of split launches
         self.ws = self.ws_all[:3 * batch * n_q]
         self.lib = _lib.lib()
         _lib.check(self.lib.fhog_validate(ctypes.byref(self.args)))
@@ -295,7 +328,11 @@ class BwdBwdPlan:
         """Enqueue the call. ``static_ws``: through ``fhog_bwdbwd_static_ws``, which keeps the row statistics and partial
         results in the library's own device array instead of this plan's workspace (``self.ws`` is then not written)."""
         s = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream if stream is None else stream)
-        if static_ws:
+        if self.sinks:
+            if static_ws or only_pass is not None:
+                raise ValueError("sinks run as a whole chain in the plan's own workspace")
+            _lib.check(self.lib.fhog_bwdbwd_sinks(ctypes.byref(self.args), self.sinks, s))
+        elif static_ws:
             if only_pass is not None:
                 raise ValueError("static_ws runs the whole chain")
             _lib.check(self.lib.fhog_bwdbwd_static_ws(ctypes.byref(self.args), s))

@@ -257,6 +257,33 @@ int fhog_attn_fwd(const fhog_attn_args* args, void* hip_stream);
    dK and dV, without the (batch, n_q, n_k) tensors: two launches, or one where the call is small. */
 int fhog_attn_bwd(const fhog_attn_args* args, void* hip_stream);
 
+/* ---- sliding window with sinks ---------------------------------------------------------------------------------------
+ * The calls above under a mask that also leaves the first `sinks` keys visible: with i' as for a window W (FHOG_MASK_*), key j is visible to
+ * query i iff 0 <= i' - j < W, or j < sinks and j <= i'. No counterpart in the reference. Every query sees a key. sinks >= 0 (FHOG_E_CAUSAL below);
+ * a number beyond n_k means all keys; without a window, or with one that hides nothing, sinks change nothing. All sums are over the visible
+ * keys: lse, d, dd and b are those of this mask, and dk, dv (dk2, dv2) of a sink come from every query that sees it.
+ * Workspaces belong to one call at a time; nothing in them has to start at any value. Results do not depend on what else runs: partial results are
+ * added in a fixed order. */
+
+/* Bytes of workspace of fhog_attn_fwd_sinks (backward 0; often none) and fhog_attn_bwd_sinks (args->ws need not be set); 0 also if the arguments are not
+   valid. Host-only. */
+size_t fhog_attn_sinks_workspace_bytes(const fhog_attn_args* args, int64_t sinks, int backward);
+
+/* fhog_attn_fwd. ws: 16-byte aligned, fhog_attn_sinks_workspace_bytes(args, sinks, 0) bytes (may be NULL if that is 0): forwards with few
+   queries deal the keys out over several workgroups and join what they leave there. */
+int fhog_attn_fwd_sinks(const fhog_attn_args* args, int64_t sinks, void* ws, int64_t ws_bytes, void* hip_stream);
+
+/* fhog_attn_bwd with args->ws of ws_bytes, at least fhog_attn_sinks_workspace_bytes(args, sinks, 1). */
+int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_bytes, void* hip_stream);
+
+/* Workspace (args->ws, args->ws_bytes) with which fhog_bwdbwd_sinks runs best, as fhog_bwdbwd_workspace_hint tells for fhog_bwdbwd; 0 if the arguments are
+   not valid. Host-only. */
+size_t fhog_bwdbwd_sinks_workspace_bytes(const fhog_bwdbwd_args* args, int64_t sinks);
+
+/* fhog_bwdbwd under FHOG_SCHEDULE_FUSED_STATS (FHOG_E_SCHEDULE under another one, where sinks count). Afterwards d, dd and b are in ws. A workspace below
+   fhog_bwdbwd_sinks_workspace_bytes may be refused (FHOG_E_SHAPE). */
+int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_stream);
+
 /* Measurement aid (no counterpart in the reference): enqueue a loop of bf16 32x32x16 MFMAs on `blocks` workgroups of 8
    waves (one per CU fills the chip), `trips` x 32 MFMAs per wave. data_mode: 0 operands all zero; 1 random operands in
    registers (nothing but MFMAs); 2 random, every A operand read from LDS (one 128-bit read per MFMA, prefetched: the
