@@ -261,6 +261,44 @@ int check_ws(const void* ws, int64_t have, size_t need) {
   return FHOG_OK;
 }
 
+int validate_rotary(const fhog_rotary_args* a) {
+  if (!a) return fail(FHOG_E_NULL, "args is NULL");
+  if (a->dtype != FHOG_DTYPE_BF16 && a->dtype != FHOG_DTYPE_FP16 && a->dtype != FHOG_DTYPE_FP32) return fail(FHOG_E_DTYPE, "unknown dtype %d", a->dtype);
+  if (a->batch < 0 || a->n < 0 || a->heads_q < 1 || a->heads_k < 0)
+    return fail(FHOG_E_SHAPE, "batch, n and heads_k must be >= 0, heads_q >= 1 (got %lld, %lld, %lld, %lld)", (long long)a->batch, (long long)a->n,
+                (long long)a->heads_k, (long long)a->heads_q);
+  if (a->n > INT32_MAX || a->batch > INT32_MAX || a->heads_q > 65535 || a->heads_k > 65535 || a->heads_q + a->heads_k > 65535)
+    return fail(FHOG_E_SHAPE, "more than 2^31 - 1 rows or slices, or 65535 heads of queries and keys, are not supported");
+  if (a->d < 2 || a->d > FHOG_ROTARY_MAX_D || a->d % 2) return fail(FHOG_E_SHAPE, "head dim %lld is not an even number in 2..%d", (long long)a->d, FHOG_ROTARY_MAX_D);
+  if (a->rotary_dim < 2 || a->rotary_dim > a->d || a->rotary_dim % 2)
+    return fail(FHOG_E_SHAPE, "rotary_dim %lld is not an even number in 2..%lld", (long long)a->rotary_dim, (long long)a->d);
+  if (a->n > 0 && a->batch > (int64_t)UINT32_MAX / (a->d / 2) / a->n) return fail(FHOG_E_SHAPE, "batch * n * d / 2 from 2^32 on is not supported");
+  if (a->axes < 1 || a->axes > FHOG_ROTARY_MAX_AXES) return fail(FHOG_E_ROTARY, "axes must be 1..%d (got %d)", FHOG_ROTARY_MAX_AXES, a->axes);
+  int64_t sum = 0;
+  for (int i = 0; i < a->axes; i++) {
+    if (a->sections[i] < 0) return fail(FHOG_E_ROTARY, "section %d is negative", i);
+    sum += a->sections[i];
+  }
+  if (sum != a->rotary_dim / 2) return fail(FHOG_E_ROTARY, "the sections hold %lld frequencies, rotary_dim %lld has %lld", (long long)sum, (long long)a->rotary_dim, (long long)(a->rotary_dim / 2));
+  if (!(a->theta > 0) || !isfinite(a->theta)) return fail(FHOG_E_ROTARY, "theta must be a positive number (got %g)", a->theta);
+  if (a->position_type < FHOG_POSITIONS_INT32 || a->position_type > FHOG_POSITIONS_FP32) return fail(FHOG_E_ROTARY, "unknown type of positions %d", a->position_type);
+  if (a->batch == 0 || a->n == 0) return FHOG_OK;   // nothing is read or written
+  const void* ptrs[] = {a->q, a->q_out, a->positions, a->k, a->k_out};
+  const char* names[] = {"q", "q_out", "positions", "k", "k_out"};
+  const int align = a->dtype == FHOG_DTYPE_FP32 ? 4 : 2;
+  for (int i = 0; i < (a->heads_k > 0 ? 5 : 3); i++) {
+    if (!ptrs[i]) return fail(FHOG_E_NULL, "pointer '%s' is NULL", names[i]);
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) % (i == 2 ? (a->position_type == FHOG_POSITIONS_INT64 ? 8 : 4) : align))
+      return fail(FHOG_E_ALIGN, "pointer '%s' is not aligned to its type", names[i]);
+  }
+  // rows of an output that share an address would be written by several threads
+  const auto packed = [](int64_t size, int64_t stride, int64_t least) { return size == 1 || (stride < 0 ? -stride : stride) >= least; };
+  if (!packed(a->batch, a->stride_qob, a->d) || !packed(a->heads_q, a->stride_qoh, a->d) || !packed(a->n, a->stride_qon, a->d) ||
+      (a->heads_k > 0 && (!packed(a->batch, a->stride_kob, a->d) || !packed(a->heads_k, a->stride_koh, a->d) || !packed(a->n, a->stride_kon, a->d))))
+    return fail(FHOG_E_STRIDE, "rows of an output overlap");
+  return FHOG_OK;
+}
+
 // Address of `scratch` on the current device, looked up once per device (the first call there) and kept.
 constexpr int kMaxDevices = 64;
 std::atomic<void*> g_scratch_ptr[kMaxDevices];
@@ -459,6 +497,18 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
     e = fhog::launch_sink_keys(p, args->dtype, impl != FHOG_IMPL_BF16, s);
   }
   if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
+
+size_t fhog_rotary_args_size(void) { return sizeof(fhog_rotary_args); }
+
+int fhog_rotary_validate(const fhog_rotary_args* args) { return validate_rotary(args); }
+
+int fhog_rotary(const fhog_rotary_args* args, void* hip_stream) {
+  if (const int rc = validate_rotary(args)) return rc;
+  if (args->batch == 0 || args->n == 0) return FHOG_OK;
+  const hipError_t e = fhog::launch_rotary(args, (hipStream_t)hip_stream);
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "rotary positions: HIP error %d (%s)", (int)e, hipGetErrorString(e));
   return FHOG_OK;
 }
 

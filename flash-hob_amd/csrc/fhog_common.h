@@ -155,6 +155,7 @@ hipError_t launch_small_fwd_parts(const AttnParams& p, hipStream_t s);          
 hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s);                  // O and L from what those leave
 hipError_t launch_sink_keys(const AttnParams& p, int dtype, hipStream_t s);                     // the sinks' rows of dK, dV from start to end
 hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, hipStream_t s);    // ... of dK2, dV2
+hipError_t launch_rotary(const fhog_rotary_args* a, hipStream_t s);
 hipError_t launch_mfma_rate(float* out, int blocks, int trips, int data_mode, int waves, hipStream_t s);  // measurement aid
 bool bf16_shape_supported(int64_t n_q, int64_t n_k, int64_t d, int causal);
 

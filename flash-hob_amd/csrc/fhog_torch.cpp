@@ -308,6 +308,126 @@ std::optional<Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& 
   return Attention::apply(q, k, v, causal, window, schedule, sinks);
 }
 
+// ---- rotary positions -----------------------------------------------------------------------------------------------
+// What a call turns by, apart from the positions
+struct Turn {
+  double theta;
+  int64_t rotary_dim;
+  bool interleaved, inverse;
+  std::vector<int64_t> sections;
+};
+
+// positions as (axes, batch, n) strides; false where they are no such thing for a (batch, .., n, d) tensor
+bool positions_of(const Tensor& p, const Tensor& q, size_t axes, fhog_rotary_args& a) {
+  switch (p.scalar_type()) {
+    case at::kInt: a.position_type = FHOG_POSITIONS_INT32; break;
+    case at::kLong: a.position_type = FHOG_POSITIONS_INT64; break;
+    case at::kFloat: a.position_type = FHOG_POSITIONS_FP32; break;
+    default: return false;
+  }
+  if (!p.is_cuda() || p.device() != q.device()) return false;
+  const int64_t lead = axes > 1 ? 1 : 0, dim = p.dim();   // one axis has no dimension of its own
+  if (dim != lead + 1 && dim != lead + 2) return false;
+  if (lead && p.size(0) != (int64_t)axes) return false;
+  if (p.size(dim - 1) != a.n || (dim == lead + 2 && p.size(lead) != a.batch && p.size(lead) != 1)) return false;
+  a.stride_pa = lead ? p.stride(0) : 0;
+  a.stride_pb = dim == lead + 2 && p.size(lead) != 1 ? p.stride(lead) : 0;
+  a.stride_pn = p.stride(dim - 1);
+  a.positions = p.data_ptr();
+  return true;
+}
+
+// The arguments of a call, outputs packed; false where they are not well formed. (batch, N, d) tensors have one head. What is not known yet, the
+// addresses of the outputs, is filled in with those of the inputs.
+bool rotary_args(const Tensor& q, const Tensor& k, const Tensor& positions, const Turn& turn, fhog_rotary_args& a) {
+  const int64_t dim = q.dim();
+  if (!q.is_cuda() || (dim != 3 && dim != 4) || turn.sections.empty() || turn.sections.size() > FHOG_ROTARY_MAX_AXES) return false;
+  if (k.defined() && (!k.is_cuda() || k.device() != q.device() || k.scalar_type() != q.scalar_type() || k.dim() != dim || k.size(0) != q.size(0) ||
+                      k.size(-1) != q.size(-1) || k.size(-2) != q.size(-2)))
+    return false;
+  a = {};
+  a.dtype = dtype_code(q.scalar_type());
+  if (a.dtype < 0) return false;
+  a.batch = q.size(0), a.n = q.size(-2), a.d = q.size(-1), a.rotary_dim = turn.rotary_dim;
+  a.heads_q = dim == 4 ? q.size(1) : 1, a.heads_k = !k.defined() ? 0 : dim == 4 ? k.size(1) : 1;
+  if (k.defined() && a.heads_k == 0) return false;
+  a.theta = turn.theta, a.interleaved = turn.interleaved, a.inverse = turn.inverse, a.axes = (int32_t)turn.sections.size();
+  for (size_t i = 0; i < turn.sections.size(); i++) {
+    if (turn.sections[i] < 0 || turn.sections[i] > FHOG_ROTARY_MAX_D) return false;
+    a.sections[i] = (int32_t)turn.sections[i];
+  }
+  if (!positions_of(positions, q, turn.sections.size(), a)) return false;
+  const auto strides = [&](const Tensor& t, int64_t& b, int64_t& h, int64_t& n) { b = t.stride(0), h = dim == 4 ? t.stride(1) : 0, n = t.stride(dim - 2); };
+  strides(q, a.stride_qb, a.stride_qh, a.stride_qn);
+  a.q = q.data_ptr(), a.q_out = const_cast<void*>(a.q);
+  a.stride_qon = a.d, a.stride_qoh = a.n * a.d, a.stride_qob = a.heads_q * a.stride_qoh;
+  if (k.defined()) {
+    strides(k, a.stride_kb, a.stride_kh, a.stride_kn);
+    a.k = k.data_ptr(), a.k_out = const_cast<void*>(a.k);
+    a.stride_kon = a.d, a.stride_koh = a.n * a.d, a.stride_kob = a.heads_k * a.stride_koh;
+  }
+  return fhog_rotary_validate(&a) == FHOG_OK;
+}
+
+// The turned q and, where k is defined, k, packed; nothing where the arguments are not well formed
+std::optional<tensor_list> rotary_call(const Tensor& q_, const Tensor& k_, const Tensor& positions, const Turn& turn) {
+  fhog_rotary_args a;
+  if (!rotary_args(q_, k_, positions, turn, a)) return std::nullopt;
+  const c10::DeviceGuard guard(q_.device());
+  const auto rows = [](const Tensor& t) { return !t.defined() || t.stride(-1) == 1 ? t : t.contiguous(); };   // channels side by side
+  const Tensor q = rows(q_), k = rows(k_);
+  rotary_args(q, k, positions, turn, a);
+  tensor_list out = {at::empty(q.sizes(), q.options())};
+  a.q_out = out[0].data_ptr();
+  if (k.defined()) out.push_back(at::empty(k.sizes(), k.options())), a.k_out = out[1].data_ptr();
+  TORCH_CHECK(fhog_rotary(&a, stream_of(q)) == FHOG_OK, "fhog_rotary: ", fhog_last_error());
+  return out;
+}
+
+// The rotation of one or two tensors as a node; its gradient is the rotation back, as a node again, so derivatives of every order exist
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+  static tensor_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k, const Tensor& positions, const Turn& turn) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions});
+    ctx->saved_data["sections"] = turn.sections;
+    ctx->saved_data["theta"] = turn.theta;
+    ctx->saved_data["how"] = std::vector<int64_t>{turn.rotary_dim, turn.interleaved, turn.inverse};
+    auto r = rotary_call(q, k ? *k : Tensor(), positions, turn);
+    TORCH_CHECK(r, "fhog: rotary: ", fhog_last_error());
+    return *r;
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+    tensor_list out(4);
+    const auto how = ctx->saved_data["how"].toIntVector();
+    const Turn back{ctx->saved_data["theta"].toDouble(), how[0], how[1] != 0, how[2] == 0, ctx->saved_data["sections"].toIntVector()};
+    const bool both = g.size() == 2 && g[0].defined() && g[1].defined();
+    const size_t one = g[0].defined() ? 0 : 1;
+    if (!both && (one >= g.size() || !g[one].defined())) return out;
+    const Tensor positions = ctx->get_saved_variables()[0];
+    const tensor_list r = both ? RotaryNode::apply(g[0], std::optional<Tensor>(g[1]), positions, back) : RotaryNode::apply(g[one], std::optional<Tensor>(), positions, back);
+    if (both) out[0] = r[0], out[1] = r[1];
+    else out[one] = r[0];
+    return out;
+  }
+};
+
+// What rotary() takes here: what rotary_call takes, checked before a node of the graph exists
+std::optional<tensor_list> rotary(const Tensor& q, const std::optional<Tensor>& k, const Tensor& positions, std::vector<int64_t> sections, double theta,
+                                  int64_t rotary_dim, bool interleaved) {
+  if (at::tracer::impl::is_dispatch_enabled()) return std::nullopt;   // as in attention()
+  if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode)) return std::nullopt;
+  for (const Tensor* t : {&q, k ? &*k : &q, &positions})
+    if (t->unsafeGetTensorImpl()->is_python_dispatch()) return std::nullopt;
+  const Turn turn{theta, rotary_dim, interleaved, false, std::move(sections)};
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k && k->requires_grad()))) {
+    const at::NoGradGuard no_grad;
+    return rotary_call(q, k ? *k : Tensor(), positions, turn);
+  }
+  fhog_rotary_args a;
+  if (positions.requires_grad() || !rotary_args(q, k ? *k : Tensor(), positions, turn, a)) return std::nullopt;
+  return RotaryNode::apply(q, k, positions, turn);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_fhog_torch, m) {
@@ -328,4 +448,5 @@ PYBIND11_MODULE(_fhog_torch, m) {
     return double_backward(q, k, v, o, g, ddq, ddk, ddv, L, scale, Mask{causal, window, sinks}, impl, schedule, split);
   }, free_lock);
   m.def("attention", &attention, free_lock);
+  m.def("rotary", &rotary, free_lock);
 }

@@ -7,12 +7,14 @@ shared object is missing, :func:`lib` raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfhog_hip.so"
 
 DTYPE_BF16, DTYPE_FP32, DTYPE_FP16 = 0, 1, 2
+POSITIONS_INT32, POSITIONS_INT64, POSITIONS_FP32 = 0, 1, 2
+ROTARY_MAX_D, ROTARY_MAX_AXES = 256, 4
 IMPL_AUTO, IMPL_FP32, IMPL_BF16 = 0, 1, 2
 MASK_NONE, MASK_TOP_LEFT, MASK_BOTTOM_RIGHT = 0, 1, 2
 PASS_D, PASS_DD, PASS_B, PASS_DQ_DDO, PASS_DK_DV, PASS_DD_B, PASS_B_DDO, PASS_DQ, PASS_DD_B_DDO, PASS_STAGE1 = range(10)
@@ -23,7 +25,7 @@ STATIC_WS_BYTES = 16 << 20   # of a default build; `lib().fhog_static_ws_bytes()
 ERROR_NAMES = {
     -1: "FHOG_E_NULL", -2: "FHOG_E_SHAPE", -3: "FHOG_E_DTYPE", -4: "FHOG_E_STRIDE", -5: "FHOG_E_ALIGN",
     -6: "FHOG_E_CAUSAL", -7: "FHOG_E_PASS", -8: "FHOG_E_LAUNCH", -9: "FHOG_E_SCALE", -10: "FHOG_E_IMPL",
-    -11: "FHOG_E_SCHEDULE",
+    -11: "FHOG_E_SCHEDULE", -12: "FHOG_E_ROTARY",
 }
 
 
@@ -48,6 +50,19 @@ class AttnArgs(Structure):
         ("batch", c_int64), ("n_q", c_int64), ("n_k", c_int64), ("d", c_int64),
         ("stride_qb", c_int64), ("stride_qn", c_int64), ("stride_kb", c_int64), ("stride_kn", c_int64),
         ("scale", c_float), ("dtype", c_int32), ("causal", c_int32), ("window", c_int32),
+    ]
+
+
+class RotaryArgs(Structure):
+    """Mirror of ``fhog_rotary_args``."""
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p), ("positions", c_void_p),
+        ("batch", c_int64), ("heads_q", c_int64), ("heads_k", c_int64), ("n", c_int64), ("d", c_int64), ("rotary_dim", c_int64),
+        ("stride_qb", c_int64), ("stride_qh", c_int64), ("stride_qn", c_int64), ("stride_kb", c_int64), ("stride_kh", c_int64), ("stride_kn", c_int64),
+        ("stride_qob", c_int64), ("stride_qoh", c_int64), ("stride_qon", c_int64), ("stride_kob", c_int64), ("stride_koh", c_int64),
+        ("stride_kon", c_int64), ("stride_pa", c_int64), ("stride_pb", c_int64), ("stride_pn", c_int64),
+        ("theta", c_double), ("sections", c_int32 * 4), ("axes", c_int32), ("dtype", c_int32), ("position_type", c_int32), ("interleaved", c_int32),
+        ("inverse", c_int32),
     ]
 
 
@@ -110,10 +125,18 @@ def lib() -> ctypes.CDLL:
     L.fhog_bwdbwd_sinks_workspace_bytes.argtypes = [POINTER(BwdBwdArgs), c_int64]
     L.fhog_bwdbwd_sinks.restype = c_int
     L.fhog_bwdbwd_sinks.argtypes = [POINTER(BwdBwdArgs), c_int64, c_void_p]
+    L.fhog_rotary_args_size.restype = c_size_t
+    L.fhog_rotary_args_size.argtypes = []
+    L.fhog_rotary_validate.restype = c_int
+    L.fhog_rotary_validate.argtypes = [POINTER(RotaryArgs)]
+    L.fhog_rotary.restype = c_int
+    L.fhog_rotary.argtypes = [POINTER(RotaryArgs), c_void_p]
     L.fhog_probe_mfma_rate.restype = c_int
     L.fhog_probe_mfma_rate.argtypes = [c_void_p, c_int, c_int, c_int, POINTER(ctypes.c_double), c_void_p]
     if L.fhog_attn_args_size() != ctypes.sizeof(AttnArgs):
         raise RuntimeError("fhog_attn_args layout differs between libfhog_hip.so and the ctypes mirror")
+    if L.fhog_rotary_args_size() != ctypes.sizeof(RotaryArgs):
+        raise RuntimeError("fhog_rotary_args layout differs between libfhog_hip.so and the ctypes mirror")
     if L.fhog_bwdbwd_args_size() != ctypes.sizeof(BwdBwdArgs):
         raise RuntimeError("fhog_bwdbwd_args layout differs between libfhog_hip.so and the ctypes mirror")
     if L.fhog_abi_version() != ABI_VERSION:

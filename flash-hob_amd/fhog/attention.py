@@ -30,6 +30,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .rotary import Rotary
 from .bwdbwd import _SCHEDULES, check_sinks, flash_bwdbwd, mask_code, native_mask, native_sinks, sinks_code
 
 _HIP_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
@@ -309,11 +310,17 @@ class FlashAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
-def attention(q, k, v, is_causal=False, window: Optional[int] = None, schedule: Optional[str] = None, *, sinks: int = 0):
+def attention(q, k, v, is_causal=False, window: Optional[int] = None, schedule: Optional[str] = None, *, sinks: int = 0,
+              rotary: Optional[Rotary] = None):
     """Twice-differentiable scaled-dot-product attention (scale = d^-1/2). ``is_causal``: False | True |
     "bottom_right"; ``window``: sliding-window length on top of a causal mask; ``schedule``: pass schedule of the
     double-backward (see :func:`fhog.flash_bwdbwd`; None = its default, three sweeps with ``dd`` and ``b`` from the first);
-    ``sinks``: first keys that stay visible behind the window (default schedule only)."""
+    ``sinks``: first keys that stay visible behind the window (default schedule only); ``rotary``: rotary positions of the keys, by which q and k are
+    turned first (the queries' positions are those of the last N_Q keys; see :class:`fhog.Rotary`), twice differentiable as well."""
+    if rotary is not None:
+        if not isinstance(rotary, Rotary):
+            raise TypeError(f"rotary must be a fhog.Rotary, got {type(rotary).__name__}")
+        q, k = rotary(q, k)
     if q.is_cuda:
         # the same chain as native autograd nodes; declines what the kernels do not cover
         out = _lib.torch_ext().attention(q, k, v, *native_mask(is_causal, window), _SCHEDULES.get(schedule, -1), native_sinks(sinks))

@@ -48,7 +48,8 @@ extern "C" {
 #define FHOG_E_LAUNCH (-8)    /* HIP reported an error at launch */
 #define FHOG_E_SCALE (-9)     /* scale is not finite (fhog_attn_fwd / fhog_attn_bwd: not finite or not positive) */
 #define FHOG_E_IMPL (-10)     /* unknown kernel family (fhog_bwdbwd_args.impl) */
-#define FHOG_E_SCHEDULE (-11) /* unknown pass schedule (fhog_bwdbwd_args.schedule) */
+#define FHOG_E_SCHEDULE (-11) /* unknown pass schedule (fhog_bwdbwd_args.schedule), or one that does not know sinks */
+#define FHOG_E_ROTARY (-12)   /* axes, sections, base or type of the positions (fhog_rotary_args) */
 
 /* pass ids for fhog_bwdbwd_pass */
 #define FHOG_PASS_D 0      /* d_i  = sum_c O_ic dO_ic                         (fhog/triton_bwdbwd.py:580)     */
@@ -283,6 +284,48 @@ size_t fhog_bwdbwd_sinks_workspace_bytes(const fhog_bwdbwd_args* args, int64_t s
 /* fhog_bwdbwd under FHOG_SCHEDULE_FUSED_STATS (FHOG_E_SCHEDULE under another one, where sinks count). Afterwards d, dd and b are in ws. A workspace below
    fhog_bwdbwd_sinks_workspace_bytes may be refused (FHOG_E_SHAPE). */
 int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_stream);
+
+/* ---- rotary positions ------------------------------------------------------------------------------------------------
+ * Queries and keys with their pairs of channels turned by angles that grow with the token's position, before attention. No counterpart in the reference.
+ * With rd = rotary_dim and f = 0 .. rd / 2 - 1: angle = p[axis(f)] * theta^(-2 f / rd), (u, w) -> (u cos - w sin, w cos + u sin) on the channels
+ * (f, f + rd / 2), or (2 f, 2 f + 1) where `interleaved`; channels rd .. d - 1 are copied. The first sections[0] frequencies belong to axis 0, the next
+ * sections[1] to axis 1, and so on (text has one axis; time, height and width of images and video are three). `inverse` turns the other way: the
+ * gradient of the call is the call on the gradient with `inverse` flipped, and so are the derivatives beyond it.
+ * Angles are formed in 64 bits: exact to 5e-16 * |p| turns, sines and cosines to 1e-7. A position that is no number makes NaN of its token's rows.
+ * Queries and keys may have different numbers of heads; heads_k = 0 leaves the keys out. Strides are in elements and may be 0 or negative on the
+ * inputs; the last dimension is contiguous. Outputs may be the inputs (same pointers and strides), else must not overlap with them. Rows that lie on
+ * multiples of 16 bytes, with d and rd multiples of 32 bytes, go 16 bytes at a time, others pair by pair. */
+#define FHOG_ROTARY_MAX_D 256
+#define FHOG_ROTARY_MAX_AXES 4
+#define FHOG_POSITIONS_INT32 0
+#define FHOG_POSITIONS_INT64 1
+#define FHOG_POSITIONS_FP32 2
+typedef struct fhog_rotary_args {
+  const void* q;         /* (batch, heads_q, n, d) */
+  const void* k;         /* (batch, heads_k, n, d); not looked at if heads_k is 0 */
+  void* q_out;
+  void* k_out;
+  const void* positions; /* (axes, batch, n) */
+  int64_t batch, heads_q, heads_k, n, d, rotary_dim;
+  int64_t stride_qb, stride_qh, stride_qn, stride_kb, stride_kh, stride_kn;
+  int64_t stride_qob, stride_qoh, stride_qon, stride_kob, stride_koh, stride_kon;
+  int64_t stride_pa, stride_pb, stride_pn;
+  double theta;
+  int32_t sections[FHOG_ROTARY_MAX_AXES]; /* frequencies of each axis, rotary_dim / 2 in all */
+  int32_t axes;
+  int32_t dtype;         /* FHOG_DTYPE_* */
+  int32_t position_type; /* FHOG_POSITIONS_* */
+  int32_t interleaved;
+  int32_t inverse;
+} fhog_rotary_args;
+
+size_t fhog_rotary_args_size(void);
+
+/* Host-only: FHOG_OK if fhog_rotary takes these arguments, else the FHOG_E_* code that it would return. */
+int fhog_rotary_validate(const fhog_rotary_args* args);
+
+/* One launch; none where batch or n is 0. */
+int fhog_rotary(const fhog_rotary_args* args, void* hip_stream);
 
 /* Measurement aid (no counterpart in the reference): enqueue a loop of bf16 32x32x16 MFMAs on `blocks` workgroups of 8
    waves (one per CU fills the chip), `trips` x 32 MFMAs per wave. data_mode: 0 operands all zero; 1 random operands in
