@@ -243,13 +243,17 @@ int check_sinks(int64_t sinks) { return sinks < 0 ? fail(FHOG_E_CAUSAL, "sinks m
 int32_t sinks_of(const fhog_attn_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }
 int32_t sinks_of(const fhog_bwdbwd_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }
 
+int forward_parts(const fhog_attn_args* a, int32_t sinks) {
+  return fhog::rules::forward_parts(a->batch, a->n_q, a->n_k, a->d, a->window, sinks, a->dtype == FHOG_DTYPE_FP32 ? 4 : 2);
+}
+
 // Row sums d of a first backward, rounded up so that what follows stays 16-byte aligned
 size_t row_bytes(const fhog_attn_args* a) { return ((size_t)a->batch * a->n_q * sizeof(float) + 15) & ~(size_t)15; }
 
 size_t attn_sinks_bytes(const fhog_attn_args* a, int64_t sinks, int backward) {
   const int32_t n = sinks_of(a, sinks);
   if (backward) return n ? row_bytes(a) + sink_bytes(a->batch, n, a->n_q, a->d) : (size_t)a->batch * a->n_q * sizeof(float);
-  return n ? forward_part_bytes(a->batch, a->n_q, a->d, forward_parts(a->batch, a->n_q, a->n_k, a->d, a->window, n)) : 0;
+  return n ? forward_part_bytes(a->batch, a->n_q, a->d, forward_parts(a, n)) : 0;
 }
 
 // A workspace of the entry points with sinks: there, aligned and as large as the call needs
@@ -421,13 +425,13 @@ int fhog_attn_fwd_sinks(const fhog_attn_args* args, int64_t sinks, void* ws, int
   const hipStream_t s = (hipStream_t)hip_stream;
   fhog::AttnParams p = to_attn_params(args);
   p.sinks = n;
-  p.n_split = forward_parts(args->batch, args->n_q, args->n_k, args->d, args->window, n);
-  p.part = (float*)ws;
+  const int parts = forward_parts(args, n);
   const bool bit16 = attn_on_16bit_kernels(args);
   hipError_t e;
-  if (p.n_split > 1) {
+  if (parts > 0) {
+    p.n_split = parts, p.part = (float*)ws;
     e = bit16 ? fhog::launch_small_fwd_parts(p, s) : fhog::launch_attn_split_parts(p, args->dtype, false, s);
-    if (e == hipSuccess) e = fhog::launch_join_forward(p, args->dtype, s);
+    if (e == hipSuccess && parts > 1) e = fhog::launch_join_forward(p, args->dtype, s);
   } else if (const int small = bit16 ? small_waves(Small::forward, args) : 0) {
     e = fhog::launch_small_attn(p, false, small, s);
   } else {

@@ -35,8 +35,8 @@ template <int WS, bool TWO>
 constexpr int n_buffers = WS == 1 && !TWO ? 2 : 1;
 
 // OWN_D: dK, dV without the sweep for dQ before it; pairs: as decode_block takes it
-// PARTS: the streamed side is dealt out over n_split workgroups, whose partial results are fp32 numbers in p.part: rows and their maximum and sum
-// (PartialRows) of the forward, rows [part][dK | dV][batch * n_k][D] of dK, dV where there is more than one
+// PARTS: the streamed side is dealt out over n_split workgroups, whose partial results are fp32 numbers in p.part where there are several: rows and their
+// maximum and sum (PartialRows) of the forward, rows [part][dK | dV][batch * n_k][D] of dK, dV
 template <typename T, int D, int MODE, int MASK, int WS, bool OWN_D, bool TWO = false, bool PARTS = false>
 __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id, bool pairs) {
   constexpr bool KSIDE = MODE == MODE_BWD_K;
@@ -353,7 +353,7 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
 
   if constexpr (MODE == MODE_FWD) l += __shfl_xor(l, 32);
   if (ri >= n_sta) return;
-  if constexpr (PARTS && MODE == MODE_FWD) {
+  if (PARTS && MODE == MODE_FWD && p.n_split > 1) {
     const PartialRows rows(p);
     store_rows<float, D>(rows.row(part, row), acc0, 1.f, h);
     if (h == 0) rows.stats(part)[row] = f32x2_t{m, l};

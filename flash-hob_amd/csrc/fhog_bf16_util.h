@@ -251,6 +251,8 @@ struct StreamKeys {
     lo = WINDOW ? max(0, r0 + off - win + 1) / TS : 0;
     hi = MASK != MASK_NONE ? min(k_tiles, (r0 + nrows - 1 + off) / TS + 1) : k_tiles;
     if (MASK == MASK_SINK) {
+      // the tile of a workgroup comes out of divisions, which are vector instructions: back to a scalar, or all that follows takes registers of the lanes
+      r0 = __builtin_amdgcn_readfirstlane(r0);
       visits = (max(0, min(sinks, r0 + nrows - 1 + off - win + 1)) + TS - 1) / TS;   // the last query's window leaves the most sinks before it
       first = max(0, r0 + off - win + 1), last = min(n_k, r0 + nrows + off);
       lo = 0, hi = visits + (max(0, last - first) + TS - 1) / TS;
@@ -275,7 +277,8 @@ struct StreamKeys {
   // no key of tile t0 is visible to any query of [r0, r0 + 32); s: in a sink step
   __device__ __forceinline__ bool dead(int t0, int r0, bool s = false) const {
     if (MASK == MASK_NONE) return r0 < 0;
-    if (MASK == MASK_SINK && s) return t0 >= before(r0 + 31);
+    // without branches: two of them cost passes 3 and 4 of fp32 tensors at d = 128 another 252 bytes of a lane in scratch memory
+    if (MASK == MASK_SINK) return (s & (t0 >= before(r0 + 31))) | (!s & ((t0 > r0 + 31 + off) | (t0 + TS - 1 < r0 + off - win + 1)));
     return t0 > r0 + 31 + off || (WINDOW && t0 + TS - 1 < r0 + off - win + 1);
   }
   // some key of tile t0 is hidden from some query of [r0, r0 + 32)
@@ -287,9 +290,14 @@ struct StreamKeys {
   }
   // key t0 + 8g + 4h + e is visible to query i iff lo <= 8g + e <= hi
   __device__ __forceinline__ void limits(int t0, int i, int h, int& lo, int& hi, bool s = false) const {
+    if (MASK == MASK_SINK) {   // what depends on s is the same for the wave: chosen between scalars, without a register of the lane
+      const int start = i + off - win + 1 - 4 * h;
+      hi = min(start + (s ? -1 - t0 : win - 1 - t0), (s ? sinks : n_k) - 1 - t0 - 4 * h);
+      lo = start - (s ? 1 << 29 : t0);
+      return;
+    }
     hi = min(MASK != MASK_NONE ? i + off - t0 : TS, n_k - 1 - t0) - 4 * h;
     lo = WINDOW ? i + off - win + 1 - t0 - 4 * h : -TS;
-    if (MASK == MASK_SINK && s) hi = before(i) - 1 - t0 - 4 * h, lo = -TS;
   }
 };
 // StreamQueries: stationary rows are keys, streamed tiles are queries (pass 4, dK and dV). MASK_SINK: the band alone; the rows of the sinks, which the

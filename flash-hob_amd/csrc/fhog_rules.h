@@ -342,24 +342,53 @@ inline int32_t sinks_of(int64_t sinks, int64_t window, int64_t n_k) {   // a win
   if (window == 0 || window >= n_k) return 0;
   return (int32_t)(sinks < n_k ? sinks : n_k);
 }
-// Workgroups that share 32 sinks of a slice, each with a part of the queries: two for every CU, with eight tiles (two of each wave) for each at least.
+// Workgroups that share 32 sinks of a slice, each with a part of the queries: one for every CU, with four tiles (one of each wave) for each at least.
+// First | second backward, us, 512 workgroups of eight tiles -> 256 of four: bf16 32 x 4096, d = 128, window 1024, 4 sinks 290 | 678 -> 282 | 675; fp32 16 x 1024, d = 64,
+// window 256, 33 sinks 64.9 | 153 -> 61.7 | 149; 8 x 4096, d = 128 448 | 1401 -> 440 | 1357; 1024 of four 296 | 686, 61.7 | 148, 440 | 1358.
 inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q) {
   const int64_t groups = (sinks + 31) / 32 * batch, tiles = (n_q + 31) / 32;
-  int64_t parts = (512 + groups - 1) / groups;
-  if (parts > tiles / 8) parts = tiles / 8;
+  int64_t parts = (256 + groups - 1) / groups;
+  if (parts > tiles / 4) parts = tiles / 4;
   return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
 }
 inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d) {
   const int parts = sink_parts(batch, sinks, n_q);
   return parts > 1 ? (size_t)parts * 2 * batch * sinks * d * sizeof(float) : 0;
 }
-// Workgroups that share 32 queries of a slice in the forward, each with a part of the keys: 1 where the queries alone give the CUs work.
-inline int forward_parts(int64_t batch, int64_t n_q, int64_t n_k, int64_t d, int64_t window, int64_t sinks) {
-  const int64_t groups = (n_q + 31) / 32 * batch, seen = window + 62 < n_k ? window + 62 : n_k, steps = (seen + 31) / 32 + (sinks + 31) / 32;
-  if (groups >= 192) return 1;
-  int64_t parts = (d == 128 ? 256 : 512) / groups;
-  if (parts > steps / 4) parts = steps / 4;
-  return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+// Forwards of up to 32 queries under a mask with sinks: workgroups that share the queries of a slice, each with a part of the keys, or 0 for the kernels of longer ones. What
+// a number of parts costs is reckoned up, in us: rounds of the workgroups, each with something to start and to end (fixed) and its waves' tiles one after the
+// other (slower where two workgroups share a CU), no less than the bytes at 5.5 TB/s; several parts have their join. One query, 4 sinks, us, one part -> several:
+//   bf16 d = 128  16 slices, window 512 9.2 -> 9.6, 1024 13.2 -> 10.5, 4096 36.9 -> 13.8; 64, 4096 35.2 -> 27.3; 160, 4096 82 -> 62 (3 parts)
+//   bf16 d = 64   16, 512 7.7 -> 8.1, 2048 15.7 -> 9.5; 96, 1024 10.5 -> 10.1, 4096 29.4 -> 22.0; 160, 2048 17.8 -> 17.1
+//   fp32 d = 64   16, 256 14.3 -> 13.3, 4096 109 -> 22; 128, 1024 58 -> 26; d = 128 16, 1024 75.7 -> 21.5; bf16 d = 32 64, 4096 66.7 -> 15.3
+// 70 such shapes take 0.97 times as long as with the best of five fixed rules for each. More slices than the GPU holds workgroups: the kernels of longer ones, which share
+// the tiles of 128 rows (fp32 d = 64 512 slices, window 2048 119 against 133, bf16 d = 128 512, 4096 175 against 176), except at d = 32 (1000, 1024 33 -> 26).
+struct FewQueries {
+  double fixed, tile, join;
+  int waves, slots;   // waves on the rows; workgroups that the GPU holds at a time
+};
+inline FewQueries few_queries(int64_t d, int bytes) {
+  if (bytes == 2 && d == 128) return {4, 1.05, 4.2, 4, 256};
+  if (bytes == 2 && d == 64) return {3.6, 0.66, 4, 4, 512};
+  if (d == 32) return {bytes == 2 ? 4. : 5., bytes == 2 ? 0.95 : 1.6, 4, 4, 512};
+  return d == 64 ? FewQueries{6.5, 2.95, 3.5, 4, 256} : FewQueries{9, 4.1, 3.5, 2, 256};
+}
+inline int forward_parts(int64_t batch, int64_t n_q, int64_t n_k, int64_t d, int64_t window, int64_t sinks, int bytes) {
+  const FewQueries c = few_queries(d, bytes);
+  if (n_q > 32 || (d != 32 && batch > c.slots)) return 0;
+  const int64_t seen = window + n_q - 1 < n_k ? window + n_q - 1 : n_k, steps = (seen + 31) / 32 + (sinks + 31) / 32;
+  const double memory = (double)batch * (double)(seen + sinks) * (double)(2 * d * bytes) / 5.5e6;
+  int best = 1;
+  double best_cost = 0;
+  for (int parts = 1; parts <= 64 && parts * c.waves < steps + c.waves; parts++) {
+    const int64_t of_a_part = (steps + parts - 1) / parts;
+    const double tile = c.tile * (batch * parts > 256 && c.slots > 256 ? 1.6 : 1);
+    double cost = (double)((batch * parts + c.slots - 1) / c.slots) * (c.fixed + tile * (double)((of_a_part + c.waves - 1) / c.waves));
+    if (cost < memory) cost = memory;
+    if (parts > 1) cost += c.join + 0.05 * parts;
+    if (parts == 1 || cost < best_cost) best = parts, best_cost = cost;
+  }
+  return best;
 }
 inline size_t forward_part_bytes(int64_t batch, int64_t n_q, int64_t d, int parts) { return parts > 1 ? (size_t)parts * batch * n_q * (d + 2) * sizeof(float) : 0; }
 

@@ -11,18 +11,25 @@ namespace fhog {
 using namespace splitk;
 namespace {
 
-// Sums of four columns over the parts. Each part is one 16-byte load, `stride` floats from the last; four are under way at a time.
-__device__ __forceinline__ f32x4_t sum_parts(const float* from, int parts, int64_t stride) {
+constexpr int kLanes = 8;   // lanes that share the parts of four columns
+
+// Sums of four columns over the parts: lane i adds parts i, i + 8, .., four loads at a time, and the lanes' sums are added pairwise, which gives all of them
+// the same bits. Up to 32 parts are one round trip to memory (one thread to all the parts of four columns took 5.0 us for 16 parts, two trips of four lanes 4.2).
+__device__ __forceinline__ f32x4_t sum_parts(const float* from, int parts, int64_t stride, int lane) {
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-  int i = 0;
-  for (; i + 4 <= parts; i += 4) {
+  for (int i = lane; i < parts; i += 4 * kLanes) {
     f32x4_t x[4];
 #pragma unroll
-    for (int u = 0; u < 4; u++) x[u] = *reinterpret_cast<const f32x4_t*>(from + (i + u) * stride);
-#pragma unroll
-    for (int u = 0; u < 4; u++) sum += x[u];
+    for (int u = 0; u < 4; u++) {
+      x[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (i + u * kLanes < parts) x[u] = *reinterpret_cast<const f32x4_t*>(from + (i + u * kLanes) * stride);
+    }
+    sum += (x[0] + x[1]) + (x[2] + x[3]);
   }
-  for (; i < parts; i++) sum += *reinterpret_cast<const f32x4_t*>(from + i * stride);
+#pragma unroll
+  for (int m = 1; m < kLanes; m *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] += __shfl_xor(sum[e], m);
   return sum;
 }
 
@@ -32,7 +39,7 @@ __device__ __forceinline__ void store4(T* to, f32x4_t x) {
   else *reinterpret_cast<u32x2_t*>(to) = pack4<Terms<T>::F16>(x[0], x[1], x[2], x[3]);
 }
 
-// Rows [part][first | second][batch * sinks][d] -> the first `sinks` rows of two tensors; a thread per four columns of a row of both
+// Rows [part][first | second][batch * sinks][d] -> the first `sinks` rows of two tensors; kLanes threads to four columns of a row of one
 struct SinkRows {
   const float* part;
   void *first, *second;
@@ -42,19 +49,18 @@ struct SinkRows {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) add_sink_parts(SinkRows a) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.batch * a.sinks;
-  const int per_row = a.d / 4;
-  const int64_t row = idx / per_row;
+  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes, rows = (int64_t)a.batch * a.sinks;
+  const int per_row = a.d / 4, lane = threadIdx.x % kLanes;
+  const int64_t row = idx / per_row % rows;
   const int col = (int)(idx % per_row) * 4;
-  if (row >= rows) return;
-  const float* from = a.part + row * a.d + col;
-  const int64_t to = row / a.sinks * a.stride_b + row % a.sinks * a.stride_n + col;
-  store4((T*)a.first + to, sum_parts(from, a.parts, 2 * rows * a.d) * a.scale);
-  store4((T*)a.second + to, sum_parts(from + rows * a.d, a.parts, 2 * rows * a.d));
+  const bool second = idx >= rows * per_row;
+  if (idx >= 2 * rows * per_row) return;   // kLanes at a time
+  const f32x4_t sum = sum_parts(a.part + ((second ? rows : 0) + row) * a.d + col, a.parts, 2 * rows * a.d, lane);
+  if (lane == 0) store4((T*)(second ? a.second : a.first) + row / a.sinks * a.stride_b + row % a.sinks * a.stride_n + col, sum * (second ? 1.f : a.scale));
 }
 
 hipError_t launch_add(const SinkRows& a, int dtype, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.batch * a.sinks * (a.d / 4) + 255) / 256));
+  const dim3 grid((unsigned)(((int64_t)a.batch * a.sinks * (a.d / 4) * 2 * kLanes + 255) / 256));
   switch (dtype) {
     case FHOG_DTYPE_FP32: hipLaunchKernelGGL(add_sink_parts<float>, grid, dim3(256), 0, s, a); break;
     case FHOG_DTYPE_FP16: hipLaunchKernelGGL(add_sink_parts<_Float16>, grid, dim3(256), 0, s, a); break;
@@ -64,27 +70,49 @@ hipError_t launch_add(const SinkRows& a, int dtype, hipStream_t s) {
 }
 
 // O_i = sum_p 2^(m_p - M) acc_p / l, l = sum_p 2^(m_p - M) l_p, L_i = ln 2 (M + log2 l). A part that saw no key of the row has m = -inf, l = 0 and a row of
-// zeros. A thread per four columns.
+// zeros. kLanes threads to four columns of a row: lane i takes parts i, i + 8, .. and up to two of them, 16 parts in all, wait for no more than one round trip.
 template <typename T>
 __global__ void __launch_bounds__(256) join_forward(AttnParams p) {
   const PartialRows part(p);
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per_row = p.d / 4;
+  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
+  const int per_row = p.d / 4, lane = threadIdx.x % kLanes;
   const int64_t row = idx / per_row;
   const int col = (int)(idx % per_row) * 4;
-  if (row >= part.rows) return;
+  if (row >= part.rows) return;   // kLanes at a time
   float top = -INFINITY, l = 0.f;
-  for (int i = 0; i < p.n_split; i++) top = fmaxf(top, part.stats(i)[row][0]);
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < p.n_split; i++) {
-    const f32x2_t ml = part.stats(i)[row];
-    const float w = __builtin_amdgcn_exp2f(ml[0] - top);
-    l = __builtin_fmaf(ml[1], w, l);
-    sum += *reinterpret_cast<const f32x4_t*>(part.row(i, row) + col) * w;
+  for (int i = lane; i < p.n_split; i += 2 * kLanes) {   // on the maximum so far
+    f32x2_t ml[2];
+    f32x4_t x[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      ml[u] = f32x2_t{-INFINITY, 0.f}, x[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (i + u * kLanes < p.n_split) ml[u] = part.stats(i + u * kLanes)[row], x[u] = *reinterpret_cast<const f32x4_t*>(part.row(i + u * kLanes, row) + col);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const float more = fmaxf(top, ml[u][0]), ref = more == -INFINITY ? 0.f : more;
+      const float old = __builtin_amdgcn_exp2f(top - ref), w = __builtin_amdgcn_exp2f(ml[u][0] - ref);
+      l = __builtin_fmaf(l, old, ml[u][1] * w);
+      sum = sum * old + x[u] * w;
+      top = more;
+    }
   }
+  float all = top;
+#pragma unroll
+  for (int m = 1; m < kLanes; m *= 2) all = fmaxf(all, __shfl_xor(all, m));
+  const float mine = __builtin_amdgcn_exp2f(top - (all == -INFINITY ? 0.f : all));
+  l *= mine, sum *= mine;
+#pragma unroll
+  for (int m = 1; m < kLanes; m *= 2) {
+    l += __shfl_xor(l, m);
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] += __shfl_xor(sum[e], m);
+  }
+  if (lane != 0) return;
   const int64_t to = row / p.n_q * p.stride_qb + row % p.n_q * p.stride_qn + col;
   store4((T*)p.o + to, sum * (1.f / l));
-  if (col == 0) p.lse[row] = (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;   // v_log_f32 is log2
+  if (col == 0) p.lse[row] = (all + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;   // v_log_f32 is log2
 }
 
 // The problem of the sinks alone: their keys, every query, the mask without its window
@@ -100,7 +128,7 @@ P sinks_alone(const P& p) {
 }  // namespace
 
 hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)p.batch * p.n_q * (p.d / 4) + 255) / 256));
+  const dim3 grid((unsigned)(((int64_t)p.batch * p.n_q * (p.d / 4) * kLanes + 255) / 256));
   switch (dtype) {
     case FHOG_DTYPE_FP32: hipLaunchKernelGGL(join_forward<float>, grid, dim3(256), 0, s, p); break;
     case FHOG_DTYPE_FP16: hipLaunchKernelGGL(join_forward<_Float16>, grid, dim3(256), 0, s, p); break;

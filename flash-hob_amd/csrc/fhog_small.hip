@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) small_grads(Params p, in
 template <int D>
 constexpr int fwd_lds = max_of(WAVES * n_buffers<D, 2> * 2 * TS * 2 * D, add_waves_bytes(D / 32) + WAVES * 2 * 64 * 4);
 
-// PARTS: the streamed keys are dealt out over n_split workgroups, which leave fp32 rows and their maximum and sum in p.part (PartialRows)
+// PARTS: the streamed keys are dealt out over n_split workgroups, which leave fp32 rows and their maximum and sum in p.part (PartialRows) where there are several
 template <bool F16, int D, int MASK, int W, bool PARTS = false>
 __global__ void __launch_bounds__(256, 2) small_fwd(AttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(256, 2) small_fwd(AttnParams p) {
   add_waves<W>(acc[0], smem, group, ws, lane, out);
   l_all += __shfl_xor(l_all, 32);
   if (qi >= p.n_q) return;
-  if (PARTS) {
+  if (PARTS && p.n_split > 1) {
     const PartialRows rows(p);
     store_partial<NC, 4 / W>(rows.row(part, (int64_t)bh * p.n_q + qi), out, ws, h);
     if (ws == 0 && h == 0) rows.stats(part)[(int64_t)bh * p.n_q + qi] = f32x2_t{m_all, l_all};
@@ -454,14 +454,17 @@ __device__ __forceinline__ void bwd_q(const AttnParams& p, char* smem) {
   if (ws == 0 && h == 0) p.ws_d[row] = dsum;
 }
 
-template <int D>
-constexpr int bwd_k_stage = 3 * TS * 2 * D + 2 * TS * 4;   // Q, dO, O tiles, L log2(e) and d of their rows
-template <int D>
-constexpr int bwd_k_buffers = 2 * WAVES * bwd_k_stage<D> <= 128 * 1024 ? 2 : 1;
+// Q, dO and, without a sweep for dQ before it (OWN_D), O tiles; L log2(e) and d of their rows
+template <int D, bool OWN_D>
+constexpr int bwd_k_stage = (OWN_D ? 3 : 2) * TS * 2 * D + 2 * TS * 4;
+template <int D, bool OWN_D>
+constexpr int bwd_k_buffers = 2 * WAVES * bwd_k_stage<D, OWN_D> <= (OWN_D ? 128 : 160) * 1024 ? 2 : 1;
 
-template <bool F16, int D, int MASK, int W, bool PARTS = false>   // PARTS: as in grads_k
+template <bool F16, int D, int MASK, int W, bool PARTS = false>   // PARTS: as in grads_k, behind a sweep for dQ
 __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
-  constexpr int KK = D / 16, NC = D / 32, ROWS = TS * WAVES / W, NT = 3, TILE = TS * 2 * D, STAGE = bwd_k_stage<D>, NBUF = bwd_k_buffers<D>;
+  constexpr int KK = D / 16, NC = D / 32, ROWS = TS * WAVES / W, TILE = TS * 2 * D;
+  constexpr bool OWN_D = !PARTS;
+  constexpr int NT = OWN_D ? 3 : 2, STAGE = bwd_k_stage<D, OWN_D>, NBUF = bwd_k_buffers<D, OWN_D>;
   int bh, tile;
   if (!decode_block<MASK>((p.n_k + ROWS - 1) / ROWS, p.batch * (PARTS ? p.n_split : 1), false, p.tile_major_k != 0, bh, tile, false, id)) return;
   const int part = PARTS ? bh % p.n_split : 0;
@@ -485,8 +488,8 @@ __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
   const auto issue = [&](int t, uint32_t lds) {
     const int64_t adv = (int64_t)t * TS * p.stride_qn;
     dma.template issue_all<2>(lds, TILE, src, adv, 0, p.n_q - t * TS);
-    dma.template issue_all<1>(lds + O, TILE, src_o, adv, 0, p.n_q - t * TS);
-    stage_words(lds + STAT, p.lse + srow + min(t * TS + n, p.n_q - 1));
+    if (OWN_D) dma.template issue_all<1>(lds + O, TILE, src_o, adv, 0, p.n_q - t * TS);
+    stage_words(lds + STAT, (OWN_D || !h ? p.lse : p.ws_d) + srow + min(t * TS + n, p.n_q - 1));
   };
   char* const ring = smem + wave * NBUF * STAGE;
   first_tiles<W, NBUF, STAGE>(t_begin + ws, t_end, ring, issue);
@@ -502,13 +505,17 @@ __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
   for (int cb = 0; cb < NC; cb++) acc[0][cb] = f32x16_t{0}, acc[1][cb] = f32x16_t{0};
   own_tiles<W, NBUF, STAGE, NT * Dma<D, 1>::IPT + 1>(t_begin + ws, t_end, ring, issue, [&](char* stage, int t) {
     float* const stat = reinterpret_cast<float*>(stage + STAT);
-    bf16x8_t Ob[KK], dOb[KK];
+    if constexpr (OWN_D) {
+      bf16x8_t Ob[KK], dOb[KK];
 #pragma unroll
-    for (int kk = 0; kk < KK; kk++) Ob[kk] = lds_read128(stage + O, aoff[kk]), dOb[kk] = lds_read128(stage + TILE, aoff[kk]);
-    float d = half_row_dot<F16, D>(Ob, dOb);
-    d += __shfl_xor(d, 32);
-    const float l = stat[n];
-    stat[h * TS + n] = h ? d : l * kLog2e;
+      for (int kk = 0; kk < KK; kk++) Ob[kk] = lds_read128(stage + O, aoff[kk]), dOb[kk] = lds_read128(stage + TILE, aoff[kk]);
+      float d = half_row_dot<F16, D>(Ob, dOb);
+      d += __shfl_xor(d, 32);
+      const float l = stat[n];
+      stat[h * TS + n] = h ? d : l * kLog2e;
+    } else if (!h) {
+      stat[n] *= kLog2e;
+    }
     bwd_k_block<F16, D>(geo, stage, aoff, troff, Kb, Vb, t * TS, k0, kj, h, c_scale_log2, acc);
   });
   __syncthreads();
@@ -529,7 +536,10 @@ __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
 }
 
 template <int D>
-constexpr int bwd_lds = max_of(max_of(WAVES * n_buffers<D, 2> * 2 * TS * 2 * D, WAVES * bwd_k_buffers<D> * bwd_k_stage<D>), add_waves_bytes(2 * D / 32));
+constexpr int bwd_lds = max_of(max_of(WAVES * n_buffers<D, 2> * 2 * TS * 2 * D, WAVES * bwd_k_buffers<D, true> * bwd_k_stage<D, true>), add_waves_bytes(2 * D / 32));
+
+template <int D>
+constexpr int sink_bwd_lds = max_of(WAVES * bwd_k_buffers<D, false> * bwd_k_stage<D, false>, add_waves_bytes(2 * D / 32));
 
 template <bool F16, int D, int MASK, int W>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) small_bwd(AttnParams p, int q_blocks) {
@@ -580,7 +590,7 @@ hipError_t attn_d(const AttnParams& p, bool backward, hipStream_t s) {
 template <bool F16, int D>
 hipError_t fwd_parts_d(const AttnParams& p, hipStream_t s) { return launch<small_fwd<F16, D, MASK_SINK, WAVES, true>>(blocks<WAVES>(p.n_q, p.batch * p.n_split), fwd_lds<D>, s, p); }
 template <bool F16, int D>
-hipError_t sink_bwd_d(const AttnParams& p, hipStream_t s) { return launch<sink_bwd<F16, D>>(blocks<WAVES>(p.n_k, p.batch * p.n_split), bwd_lds<D>, s, p); }
+hipError_t sink_bwd_d(const AttnParams& p, hipStream_t s) { return launch<sink_bwd<F16, D>>(blocks<WAVES>(p.n_k, p.batch * p.n_split), sink_bwd_lds<D>, s, p); }
 template <bool F16, int D>
 hipError_t sink_grads_d(const Params& p, hipStream_t s) { return launch<sink_grads<F16, D>>(blocks<WAVES>(p.n_k, p.batch * p.n_split), grads_lds<D>, s, p); }
 
