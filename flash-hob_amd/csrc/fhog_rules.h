@@ -355,13 +355,16 @@ inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d) {
   const int parts = sink_parts(batch, sinks, n_q);
   return parts > 1 ? (size_t)parts * 2 * batch * sinks * d * sizeof(float) : 0;
 }
-// Forwards of up to 32 queries under a mask with sinks: workgroups that share the queries of a slice, each with a part of the keys, or 0 for the kernels of longer ones. What
+// Forwards of few queries under a mask with sinks: workgroups that share 32 queries of a slice, each with a part of the keys, or 0 for the kernels of longer ones. What
 // a number of parts costs is reckoned up, in us: rounds of the workgroups, each with something to start and to end (fixed) and its waves' tiles one after the
-// other (slower where two workgroups share a CU), no less than the bytes at 5.5 TB/s; several parts have their join. One query, 4 sinks, us, one part -> several:
+// other (slower where two workgroups share a CU), no less than the bytes at 5.5 TB/s; several parts have their join, with the bytes of partial
+// results written and read. One query, 4 sinks, us, one part -> several:
 //   bf16 d = 128  16 slices, window 512 9.2 -> 9.6, 1024 13.2 -> 10.5, 4096 36.9 -> 13.8; 64, 4096 35.2 -> 27.3; 160, 4096 82 -> 62 (3 parts)
 //   bf16 d = 64   16, 512 7.7 -> 8.1, 2048 15.7 -> 9.5; 96, 1024 10.5 -> 10.1, 4096 29.4 -> 22.0; 160, 2048 17.8 -> 17.1
 //   fp32 d = 64   16, 256 14.3 -> 13.3, 4096 109 -> 22; 128, 1024 58 -> 26; d = 128 16, 1024 75.7 -> 21.5; bf16 d = 32 64, 4096 66.7 -> 15.3
-// 70 such shapes take 0.97 times as long as with the best of five fixed rules for each. More slices than the GPU holds workgroups: the kernels of longer ones, which share
+// More queries, the kernels of longer ones -> this rule: 1 x 512 | 9000, d = 128, window 4096 35 -> 14; 2 x 1000 | 9000, d = 64, 4096 25.6 -> 15.6; 8 x 128 | 5000, d = 128,
+// 2048 21.0 -> 14; fp32 2 x 64 | 9000, d = 128, 4096 279 -> 20; not 16 x 100 | 5000, d = 128, 1024 13.7, 16 x 256, 2048 22.
+// 70 of the shapes with one query take 0.97 times as long as with the best of five fixed rules for each. More slices than the GPU holds workgroups: the kernels of longer ones, which share
 // the tiles of 128 rows (fp32 d = 64 512 slices, window 2048 119 against 133, bf16 d = 128 512, 4096 175 against 176), except at d = 32 (1000, 1024 33 -> 26).
 struct FewQueries {
   double fixed, tile, join;
@@ -375,20 +378,21 @@ inline FewQueries few_queries(int64_t d, int bytes) {
 }
 inline int forward_parts(int64_t batch, int64_t n_q, int64_t n_k, int64_t d, int64_t window, int64_t sinks, int bytes) {
   const FewQueries c = few_queries(d, bytes);
-  if (n_q > 32 || (d != 32 && batch > c.slots)) return 0;
-  const int64_t seen = window + n_q - 1 < n_k ? window + n_q - 1 : n_k, steps = (seen + 31) / 32 + (sinks + 31) / 32;
-  const double memory = (double)batch * (double)(seen + sinks) * (double)(2 * d * bytes) / 5.5e6;
+  const int64_t groups = (n_q + 31) / 32 * batch, rows = n_q < 32 ? n_q : 32;
+  if (groups > c.slots && (n_q > 32 || d != 32)) return 0;
+  const int64_t seen = window + rows - 1 < n_k ? window + rows - 1 : n_k, steps = (seen + 31) / 32 + (sinks + 31) / 32;
+  const double memory = (double)batch * (double)((window + n_q - 1 < n_k ? window + n_q - 1 : n_k) + sinks) * (double)(2 * d * bytes) / 5.5e6;
   int best = 1;
   double best_cost = 0;
-  for (int parts = 1; parts <= 64 && parts * c.waves < steps + c.waves; parts++) {
+  for (int parts = 1; parts <= 64 && parts * c.waves < steps + c.waves && (parts == 1 || groups * parts <= 512); parts++) {
     const int64_t of_a_part = (steps + parts - 1) / parts;
-    const double tile = c.tile * (batch * parts > 256 && c.slots > 256 ? 1.6 : 1);
-    double cost = (double)((batch * parts + c.slots - 1) / c.slots) * (c.fixed + tile * (double)((of_a_part + c.waves - 1) / c.waves));
+    const double tile = c.tile * (groups * parts > 256 && c.slots > 256 ? 1.6 : 1);
+    double cost = (double)((groups * parts + c.slots - 1) / c.slots) * (c.fixed + tile * (double)((of_a_part + c.waves - 1) / c.waves));
     if (cost < memory) cost = memory;
-    if (parts > 1) cost += c.join + 0.05 * parts;
+    if (parts > 1) cost += c.join + 0.05 * parts + (double)parts * (double)(batch * n_q * d * 8) / 2e6;
     if (parts == 1 || cost < best_cost) best = parts, best_cost = cost;
   }
-  return best;
+  return best == 1 && n_q > 32 ? 0 : best;
 }
 inline size_t forward_part_bytes(int64_t batch, int64_t n_q, int64_t d, int parts) { return parts > 1 ? (size_t)parts * batch * n_q * (d + 2) * sizeof(float) : 0; }
 

@@ -13,21 +13,23 @@ namespace {
 
 constexpr int kLanes = 8;   // lanes that share the parts of four columns
 
-// Sums of four columns over the parts: lane i adds parts i, i + 8, .., four loads at a time, and the lanes' sums are added pairwise, which gives all of them
-// the same bits. Up to 32 parts are one round trip to memory (one thread to all the parts of four columns took 5.0 us for 16 parts, two trips of four lanes 4.2).
+// Sums of four columns over the parts: lane i of LANES adds parts i, i + LANES, .., four loads at a time, and the lanes' sums are added pairwise, which gives all of
+// them the same bits. With eight lanes up to 32 parts are one round trip to memory (one thread to all the parts of four columns took 5.0 us for 16
+// parts, four lanes 4.2, eight 2.5); up to four parts are that for one lane, and eight lanes take 7.8 us for two parts of 4800 rows of 64.
+template <int LANES>
 __device__ __forceinline__ f32x4_t sum_parts(const float* from, int parts, int64_t stride, int lane) {
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-  for (int i = lane; i < parts; i += 4 * kLanes) {
+  for (int i = lane; i < parts; i += 4 * LANES) {
     f32x4_t x[4];
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       x[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      if (i + u * kLanes < parts) x[u] = *reinterpret_cast<const f32x4_t*>(from + (i + u * kLanes) * stride);
+      if (i + u * LANES < parts) x[u] = *reinterpret_cast<const f32x4_t*>(from + (i + u * LANES) * stride);
     }
     sum += (x[0] + x[1]) + (x[2] + x[3]);
   }
 #pragma unroll
-  for (int m = 1; m < kLanes; m *= 2)
+  for (int m = 1; m < LANES; m *= 2)
 #pragma unroll
     for (int e = 0; e < 4; e++) sum[e] += __shfl_xor(sum[e], m);
   return sum;
@@ -39,7 +41,7 @@ __device__ __forceinline__ void store4(T* to, f32x4_t x) {
   else *reinterpret_cast<u32x2_t*>(to) = pack4<Terms<T>::F16>(x[0], x[1], x[2], x[3]);
 }
 
-// Rows [part][first | second][batch * sinks][d] -> the first `sinks` rows of two tensors; kLanes threads to four columns of a row of one
+// Rows [part][first | second][batch * sinks][d] -> the first `sinks` rows of two tensors; LANES threads to four columns of a row of one
 struct SinkRows {
   const float* part;
   void *first, *second;
@@ -47,26 +49,28 @@ struct SinkRows {
   int32_t parts, batch, sinks, d;
   float scale;   // of the first tensor
 };
-template <typename T>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) add_sink_parts(SinkRows a) {
-  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes, rows = (int64_t)a.batch * a.sinks;
-  const int per_row = a.d / 4, lane = threadIdx.x % kLanes;
-  const int64_t row = idx / per_row % rows;
-  const int col = (int)(idx % per_row) * 4;
+  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES, rows = (int64_t)a.batch * a.sinks;
+  const int per_row = a.d / 4, lane = threadIdx.x % LANES;
+  if (idx >= 2 * rows * per_row) return;   // LANES at a time
   const bool second = idx >= rows * per_row;
-  if (idx >= 2 * rows * per_row) return;   // kLanes at a time
-  const f32x4_t sum = sum_parts(a.part + ((second ? rows : 0) + row) * a.d + col, a.parts, 2 * rows * a.d, lane);
+  const int64_t row = idx / per_row - (second ? rows : 0);
+  const int col = (int)(idx % per_row) * 4;
+  const f32x4_t sum = sum_parts<LANES>(a.part + ((second ? rows : 0) + row) * a.d + col, a.parts, 2 * rows * a.d, lane);
   if (lane == 0) store4((T*)(second ? a.second : a.first) + row / a.sinks * a.stride_b + row % a.sinks * a.stride_n + col, sum * (second ? 1.f : a.scale));
 }
 
-hipError_t launch_add(const SinkRows& a, int dtype, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.batch * a.sinks * (a.d / 4) * 2 * kLanes + 255) / 256));
-  switch (dtype) {
-    case FHOG_DTYPE_FP32: hipLaunchKernelGGL(add_sink_parts<float>, grid, dim3(256), 0, s, a); break;
-    case FHOG_DTYPE_FP16: hipLaunchKernelGGL(add_sink_parts<_Float16>, grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL(add_sink_parts<__bf16>, grid, dim3(256), 0, s, a);
-  }
+template <typename T>
+hipError_t launch_add_t(const SinkRows& a, hipStream_t s) {
+  const int64_t columns = (int64_t)a.batch * a.sinks * (a.d / 4) * 2;   // fours of them
+  if (a.parts <= 4) hipLaunchKernelGGL((add_sink_parts<T, 1>), dim3((unsigned)((columns + 255) / 256)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((add_sink_parts<T, kLanes>), dim3((unsigned)((columns * kLanes + 255) / 256)), dim3(256), 0, s, a);
   return hipGetLastError();
+}
+
+hipError_t launch_add(const SinkRows& a, int dtype, hipStream_t s) {
+  return dtype == FHOG_DTYPE_FP32 ? launch_add_t<float>(a, s) : dtype == FHOG_DTYPE_FP16 ? launch_add_t<_Float16>(a, s) : launch_add_t<__bf16>(a, s);
 }
 
 // O_i = sum_p 2^(m_p - M) acc_p / l, l = sum_p 2^(m_p - M) l_p, L_i = ln 2 (M + log2 l). A part that saw no key of the row has m = -inf, l = 0 and a row of

@@ -61,7 +61,9 @@ def test_all_orders_against_the_formulas(shape, causal, window, sinks, d, dtype)
 
 # launches large enough for the kernels with 128 and 256 rows to a workgroup, and those that split their streamed side
 LARGE = [((40, 900, 900), True, 150, 5), ((33, 1024, 1024), True, 300, 70), ((104, 1100, 1100), True, 64, 4), ((24, 1000, 1700), "bottom_right", 500, 33),
-         ((1, 3000, 3000), True, 1500, 70), ((2, 2500, 4000), "bottom_right", 2000, 4)]
+         ((1, 3000, 3000), True, 1500, 70), ((2, 2500, 4000), "bottom_right", 2000, 4), ((6, 1537, 1537), True, 400, 100),
+         ((1, 100, 5000), "bottom_right", 4096, 4), ((2, 70, 3000), "bottom_right", 2500, 33), ((3, 1, 9000), "bottom_right", 8192, 64),
+         ((300, 2, 500), "bottom_right", 300, 4)]
 
 
 @pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 128), (torch.float32, 32), (torch.float32, 64),
@@ -115,6 +117,41 @@ def test_autograd_chains_agree_and_match(n_q, n_k, causal, dtype, d):
     p = fhog.BwdBwdPlan(q, k, v, o, do, ddq, ddk, ddv, L, d ** -0.5, causal=causal, window=20, sinks=6)
     for a, b in zip(p.run(), native[4:]):
         assert torch.equal(a, b.flatten(0, 1))
+
+
+@pytest.mark.parametrize("shape, causal, window, sinks", [((2, 333, 333), True, 64, 33), ((40, 900, 900), True, 150, 5), ((1, 64, 900), "bottom_right", 300, 4)])
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 64), (torch.float16, 128)])
+def test_split_products_of_16_bit_tensors(shape, causal, window, sinks, dtype, d):
+    """impl="fp32": the double-backward of bf16 and fp16 tensors on the kernels of fp32 accuracy, beside what the 16-bit ones give."""
+    import fhog
+    batch, n_q, n_k = shape
+    q, k, v, do, ddq, ddk, ddv = x = _inputs(batch, n_q, n_k, d, dtype, 31)
+    o, L = fhog.attention_forward(q, k, v, None, causal, window=window, sinks=sinks)
+    args = (q, k, v, o, do, ddq, ddk, ddv, L, d ** -0.5)
+    kw = dict(causal=causal, window=window, sinks=sinks)
+    got, stats = fhog.flash_bwdbwd(*args, impl="fp32", **kw), fhog.flash_bwdbwd(*args, impl="bf16", return_stats=True, **kw)[4]
+    ref = attention_with_bounds(*(t[:2] for t in x), d ** -0.5, visible(n_q, n_k, causal, window, sinks, "cuda"))
+    for name, t in zip(("dq2", "dk2", "dv2", "ddo"), got):
+        assert_within(t[:2], ref[name], name)
+    assert all(torch.isfinite(t).all() and t.shape == L.shape for t in stats)
+    d_row = (o.double() * do.double()).sum(-1)
+    assert (stats[0].double() - d_row).abs().max() <= 2.0 ** -24 * (d + 64) * (o.double().abs() * do.double().abs()).sum(-1).max()
+
+
+def test_what_the_kernels_refuse_goes_to_the_composition_with_the_same_mask():
+    import warnings
+
+    import fhog
+    q, k, v, do = _inputs(2, 50, 50, 64, torch.bfloat16, 33)[:4]
+    seen = visible(50, 50, True, 9, 4, "cuda")
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        o, L = fhog.attention_forward(q, k, v, -0.125, True, window=9, sinks=4)
+    s = (q.double() @ k.double().mT * -0.125).masked_fill(~seen, float("-inf"))
+    assert (L.double() - torch.logsumexp(s, -1)).abs().max() < 1e-5
+    assert (o.double() - torch.softmax(s, -1) @ v.double()).abs().max() <= 2.0 ** -8 * v.double().abs().max()
+    with pytest.raises(ValueError, match="positive"):
+        fhog.attention_forward(q, k, v, -0.125, True, window=9, sinks=4, use_hip=True)
 
 
 def test_gradients_against_differences():
