@@ -124,7 +124,7 @@ fhog::Params to_params(const fhog_bwdbwd_args* a) {
   p.causal = a->causal != FHOG_MASK_NONE;
   p.f16 = a->dtype == FHOG_DTYPE_FP16;
   mask_params(a->causal, a->window, a->n_q, a->n_k, &p.mask_off, &p.window);
-  p.sinks = 0;
+  p.sinks = 0, p.n_split_s = 1, p.part_s = nullptr;
   p.n_split = 1;
   p.part = nullptr;
   const int order = fhog::tuning().order;
@@ -450,6 +450,9 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
   const hipStream_t s = (hipStream_t)hip_stream;
   fhog::AttnParams p = to_attn_params(args);
   p.sinks = n;
+  const int parts = sink_parts(args->batch, n, args->n_q);
+  float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
+  bool swept = false;
   hipError_t e;
   if (!attn_on_16bit_kernels(args)) {
     e = fhog::launch_attn_split(p, args->dtype, true, s);
@@ -457,12 +460,12 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
     e = fhog::launch_small_attn(p, true, small, s);
   } else {
     e = fhog::launch_attn_bf16(p, 1, s);
+    if ((swept = fhog::rules::sinks_ride(args->d, parts))) p.n_split = parts, p.part = part;
     if (e == hipSuccess) e = fhog::launch_attn_bf16(p, 2, s);
   }
   if (e == hipSuccess) {
-    p.n_split = sink_parts(args->batch, n, args->n_q);
-    p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
-    e = fhog::launch_sink_keys(p, args->dtype, s);
+    p.n_split = parts, p.part = part;
+    e = fhog::launch_sink_keys(p, args->dtype, swept, s);
   }
   if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "attention backward: HIP error %d (%s)", (int)e, hipGetErrorString(e));
   return FHOG_OK;
@@ -472,8 +475,7 @@ size_t fhog_bwdbwd_sinks_workspace_bytes(const fhog_bwdbwd_args* args, int64_t s
   if (validate(args) != FHOG_OK || check_sinks(sinks) != FHOG_OK) return 0;
   const size_t hint = workspace_hint(args, to_params(args), select_impl(args));
   const int32_t n = sinks_of(args, sinks);
-  const size_t need = n ? stats_bytes(args) + sink_bytes(args->batch, n, args->n_q, args->d) : 0;
-  return need > hint ? need : hint;
+  return n ? ((hint + 15) & ~(size_t)15) + sink_bytes(args->batch, n, args->n_q, args->d) : hint;
 }
 
 int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_stream) {
@@ -482,24 +484,27 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
   const int32_t n = sinks_of(args, sinks);
   if (n == 0) return fhog_bwdbwd(args, hip_stream);
   if (args->schedule != FHOG_SCHEDULE_FUSED_STATS) return fail(FHOG_E_SCHEDULE, "sinks run under schedule %d alone (got %d)", FHOG_SCHEDULE_FUSED_STATS, args->schedule);
-  if (const int rc = check_ws(args->ws, args->ws_bytes, stats_bytes(args) + sink_bytes(args->batch, n, args->n_q, args->d))) return rc;
+  const size_t of_sinks = sink_bytes(args->batch, n, args->n_q, args->d);
+  if (const int rc = check_ws(args->ws, args->ws_bytes, stats_bytes(args) + of_sinks)) return rc;
   const hipStream_t s = (hipStream_t)hip_stream;
   const int impl = select_impl(args);
-  fhog::Params p = to_params(args);
-  p.sinks = n;
+  fhog_bwdbwd_args a = *args;   // the sweeps have what lies before the partial results of the sinks, which are a multiple of 16 bytes
+  a.ws_bytes = (args->ws_bytes & ~(int64_t)15) - (int64_t)of_sinks;
+  fhog::Params p = to_params(&a);
+  p.sinks = n, p.n_split_s = sink_parts(a.batch, n, a.n_q);
+  float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + a.ws_bytes);
   const int small = impl == FHOG_IMPL_BF16 ? small_waves(Small::double_backward, args->batch, args->n_q, args->n_k, args->d, args->causal, args->window) : 0;
+  bool swept = false;
   hipError_t e = hipSuccess;
   if (small) {
     e = fhog::launch_small_bwdbwd(p, small, s);
   } else {
-    if (const int rc = run_pass(args, p, impl, FHOG_PASS_DD_B, s)) return rc;
-    if (const int rc = impl == FHOG_IMPL_BF16 ? run_grads(args, p, FHOG_PASS_DQ_DDO, true, s) : run_pass(args, p, impl, fhog::kPassGrads, s)) return rc;
+    if (const int rc = run_pass(&a, p, impl, FHOG_PASS_DD_B, s)) return rc;
+    if ((swept = impl == FHOG_IMPL_BF16 && fhog::rules::sinks_ride(a.d, p.n_split_s))) p.part_s = part;
+    if (const int rc = impl == FHOG_IMPL_BF16 ? run_grads(&a, p, FHOG_PASS_DQ_DDO, true, s) : run_pass(&a, p, impl, fhog::kPassGrads, s)) return rc;
   }
-  if (e == hipSuccess) {   // behind the launches whose partial results lay there
-    p.n_split = sink_parts(args->batch, n, args->n_q);
-    p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + stats_bytes(args));
-    e = fhog::launch_sink_keys(p, args->dtype, impl != FHOG_IMPL_BF16, s);
-  }
+  p.part_s = part;
+  if (e == hipSuccess) e = fhog::launch_sink_keys(p, args->dtype, impl != FHOG_IMPL_BF16, swept, s);
   if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "HIP error %d (%s)", (int)e, hipGetErrorString(e));
   return FHOG_OK;
 }

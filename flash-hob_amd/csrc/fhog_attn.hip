@@ -18,7 +18,7 @@
 // of the cycles and the VALU 48 %, and taking out the exponentials, the LDS reads or half of the staging moves the time by less
 // than 5 %. Issuing the first level of a tile beside the second level of the tile before, each behind the other's
 // elementwise work, measured equal (d = 64: +-3 %, d = 128: 2 % slower); fewer VALU instructions per block is what paid.
-#include "fhog_bf16_blocks.h"
+#include "fhog_small.h"
 
 namespace fhog {
 using namespace bf16k;
@@ -198,9 +198,17 @@ __global__ void __launch_bounds__(256, 2) attn_bwd_q_bf16(AttnParams p) {
 }
 
 // ---- backward, K-tiled: dK, dV (d = 64; at d = 128 attn_bwd_k_pc of fhog_bf16_pc.hip) ---------------------------------
-template <bool F16, int D, int MASK>
+// RIDERS: behind those workgroups come the ones that sum up the rows of the sinks over n_split parts of the queries (fhog_sinks.hip)
+template <bool F16, int D, int MASK, bool RIDERS = false>
 __global__ void __launch_bounds__(256, 2) attn_bwd_k_bf16(AttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  if constexpr (RIDERS) {
+    const int id = (int)blockIdx.x - (int)gridDim.x + (int)grid_blocks((p.sinks + TS - 1) / TS, p.batch * p.n_split);
+    if (id >= 0) {
+      sinks_alone(p);
+      return smallk::bwd_k<F16, D, MASK_BAND, smallk::WAVES, true>(p, smem, id);
+    }
+  }
   constexpr int KK = D / 16, NC = D / 32, TILE = TS * 2 * D;
   constexpr int STAT = 2 * TS * 4;         // L log2(e) and d of the 32 staged queries
   constexpr int STAGE = 2 * TILE + STAT;   // Q tile, dO tile, statistics
@@ -309,7 +317,14 @@ hipError_t launch_attn_d(const AttnParams& p, int which, hipStream_t s) {
     case 0: return launch<attn_fwd_bf16<F16, D, MASK>>(grid_blocks((p.n_q + WG_ROWS - 1) / WG_ROWS, p.batch), 2 * 2 * TILE, s, p);
     case 1: return launch<attn_bwd_q_bf16<F16, D, MASK>>(grid_blocks((p.n_q + WG_ROWS - 1) / WG_ROWS, p.batch), 2 * 2 * TILE, s, p);
     default:
-      if constexpr (D == 64)   // the rows of the sinks have a launch of their own
+      if constexpr (D == 64 && MASK == MASK_SINK) {
+        if (p.part) {   // sinks_ride
+          const unsigned blocks = grid_blocks((p.n_k + WG_ROWS - 1) / WG_ROWS, p.batch), more = grid_blocks((p.sinks + TS - 1) / TS, p.batch * p.n_split);
+          constexpr int lds = smallk::sink_bwd_lds<D> > 2 * (2 * TILE + 2 * TS * 4) ? smallk::sink_bwd_lds<D> : 2 * (2 * TILE + 2 * TS * 4);
+          return launch<attn_bwd_k_bf16<F16, D, MASK_BAND, true>>(blocks + more, lds, s, p);
+        }
+      }
+      if constexpr (D == 64)
         return launch<attn_bwd_k_bf16<F16, D, MASK == MASK_SINK ? MASK_BAND : MASK>>(grid_blocks((p.n_k + WG_ROWS - 1) / WG_ROWS, p.batch), 2 * (2 * TILE + 2 * TS * 4), s, p);
       else
         return hipErrorInvalidValue;   // d = 128 is dispatched to the producer/consumer kernel before this point

@@ -27,7 +27,7 @@
 
 #include <type_traits>
 
-#include "fhog_bf16_blocks.h"
+#include "fhog_small.h"
 #include "fhog_rules.h"
 
 namespace fhog {
@@ -619,13 +619,22 @@ __device__ __forceinline__ void k_sweep_run(const Params& p, char* smem, int bh,
 }
 
 // Passes 3 or 7 (workgroups [0, q_blocks)) and 4 (the others) in one launch at d = 64: given the row statistics neither needs the
-// other. Either side may be empty.
-template <bool F16, int D, int QPASS, int MASK, int SUB>
+// other. Either side may be empty. RIDERS: behind both come the workgroups that sum up the rows of the sinks (fhog_sinks.hip); their rings have one
+// stage (51 KB), so that two workgroups stay on a CU.
+template <bool F16, int D, int QPASS, int MASK, int SUB, bool RIDERS = false>
 __global__ void __launch_bounds__(256, 2) grads_bf16(Params p, int q_blocks, bool mixed) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int riders = RIDERS ? (int)grid_blocks((p.sinks + TS - 1) / TS, p.batch * p.n_split_s) : 0;
+  if constexpr (RIDERS) {
+    const int first = (int)gridDim.x - riders;
+    if ((int)blockIdx.x >= first) {
+      sinks_alone(p);
+      return smallk::grads_k<F16, D, MASK_BAND, smallk::WAVES, true, 1>(p, smem, (int)blockIdx.x - first);
+    }
+  }
   int bh, tile, split = 0, id = blockIdx.x;
   const bool pairs = MASK != MASK_NONE && !mixed;   // workgroups that join others of their own sweep on a CU
-  if (first_of_two(q_blocks, (int)gridDim.x - q_blocks, mixed, MASK != MASK_NONE, id)) {
+  if (first_of_two(q_blocks, (int)gridDim.x - riders - q_blocks, mixed, MASK != MASK_NONE, id)) {
     if (!decode_block<MASK>((p.n_q + WG_ROWS - 1) / WG_ROWS, p.batch * p.n_split, MASK != MASK_NONE, p.tile_major, bh, tile, pairs, id)) return;
     if (p.n_split > 1) split = bh % p.n_split, bh /= p.n_split;
     RowChain unused;
@@ -728,6 +737,18 @@ hipError_t launch_grads64(const Params& p, bool q_side, bool k_side, hipStream_t
   const int tile = TS * 2 * 64, q_lds = 2 * SUB * 4 * tile, k_lds = 2 * SUB * (3 * tile + 4 * TS * 4);
   const unsigned gq = q_side ? grid_blocks((p.n_q + WG_ROWS - 1) / WG_ROWS, p.batch * p.n_split) : 0;
   const unsigned gk = k_side ? grid_blocks((p.n_k + WG_ROWS - 1) / WG_ROWS, p.batch * p.n_split_k) : 0;
+  if constexpr (MASK == MASK_SINK) {
+    if (p.part_s) {   // sinks_ride
+      const unsigned gs = grid_blocks((p.sinks + TS - 1) / TS, p.batch * p.n_split_s);
+      int lds = smallk::WAVES * smallk::grads_k_stage<64>;
+      lds = lds > smallk::add_waves_bytes(4) ? lds : smallk::add_waves_bytes(4);
+      lds = lds > q_lds ? lds : q_lds, lds = lds > k_lds ? lds : k_lds;
+      const hipError_t e = allow_dynamic_lds<grads_bf16<F16, 64, QPASS, MASK, SUB, true>>(lds);
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL((grads_bf16<F16, 64, QPASS, MASK, SUB, true>), dim3(gq + gk + gs), dim3(256), lds, s, p, (int)gq, rules::mixed_order(p, gq, gk));
+      return hipGetLastError();
+    }
+  }
   const hipError_t e = allow_dynamic_lds<grads_bf16<F16, 64, QPASS, MASK, SUB>>(q_lds > k_lds ? q_lds : k_lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((grads_bf16<F16, 64, QPASS, MASK, SUB>), dim3(gq + gk), dim3(256), q_lds > k_lds ? q_lds : k_lds, s, p, (int)gq, rules::mixed_order(p, gq, gk));

@@ -366,7 +366,7 @@ __device__ __forceinline__ bool in_limits(int r, int lo, int hi) {  // r: regist
 // 16384 rows or more, stretches -> every eighth tile, causal: double-backward d = 128 2 x 30280 6443 -> 4087, 1 x 31258 3829 -> 2400, fp32 d = 64
 // 1 x 17018 5495 -> 3487; first backward d = 64 1 x 29336 1401 -> 765, d = 128 3 x 22609 2106 -> 1304; windows of 1 to 9 % of the rows within 2 %.
 // number of workgroups to launch for n_tiles tiles per slice
-__host__ __forceinline__ unsigned grid_blocks(int n_tiles, int batch) { return (unsigned)(((int64_t)n_tiles * batch + 7) / 8 * 8); }
+__host__ __device__ __forceinline__ unsigned grid_blocks(int n_tiles, int batch) { return (unsigned)(((int64_t)n_tiles * batch + 7) / 8 * 8); }
 // Returns false when the id falls beyond the last tile.
 // tile_major: the slices that share an XCD advance through their tiles together (ids enumerate tile 0 of every
 // slice, then tile 1 of every slice, ...) instead of one slice after the other. With a mask the work of a tile grows

@@ -56,6 +56,9 @@ struct Params {
   int32_t n_split_k, tile_major_k;
   float* part_k;
   int32_t sinks;   // keys [0, sinks) stay visible to the queries whose window lies behind them (0 without a window)
+  // The sinks' rows of dK2, dV2: workgroups that share 32 of them, and their partial results
+  int32_t n_split_s;
+  float* part_s;
 };
 
 // Launch choices that can be overridden for experiments through the environment variable FHOG_TUNE, a comma-separated
@@ -98,10 +101,17 @@ struct AttnParams {
   // Workgroup order within an XCD for the Q-tiled kernels (forward, dQ) and the K-tiled one (dK, dV): see Params
   int32_t tile_major_q, tile_major_k;
   int32_t sinks;     // see Params
-  // Streamed side over n_split workgroups per stationary tile, fp32 partial results in `part` (the keys of the sinks, forwards of few queries)
+  // Streamed side over n_split workgroups per stationary tile, fp32 partial results in `part` (the sinks' rows of dK, dV; forwards of few queries)
   int32_t n_split;
   float* part;
 };
+
+// The problem of the rows of the sinks: their keys, every query, the mask without its window
+__host__ __device__ inline void sinks_alone(AttnParams& p) { p.window = p.n_q + p.n_k, p.n_k = p.sinks, p.sinks = 0, p.tile_major_k = 0; }
+__host__ __device__ inline void sinks_alone(Params& p) {
+  p.window = p.n_q + p.n_k, p.n_k = p.sinks, p.sinks = 0, p.tile_major = p.tile_major_k = 0;
+  p.n_split = p.n_split_s, p.part = p.part_s;
+}
 
 // A kernel that uses more than 64 KiB of dynamic LDS needs its limit raised before the first launch. Done once per
 // kernel and device (not per launch: the call takes a lock in the runtime and must not run under stream capture, so
@@ -153,8 +163,9 @@ hipError_t launch_attn_split_parts(const AttnParams& p, int dtype, bool backward
 hipError_t launch_split_sink_grads(const Params& p, int dtype, hipStream_t s);
 hipError_t launch_small_fwd_parts(const AttnParams& p, hipStream_t s);                         // forward, the streamed keys over n_split workgroups
 hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s);                  // O and L from what those leave
-hipError_t launch_sink_keys(const AttnParams& p, int dtype, hipStream_t s);                     // the sinks' rows of dK, dV from start to end
-hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, hipStream_t s);    // ... of dK2, dV2
+// The sinks' rows of dK, dV and of dK2, dV2; swept: a launch before this one (launch_attn_bf16, launch_bf16_grads) left their partial results
+hipError_t launch_sink_keys(const AttnParams& p, int dtype, bool swept, hipStream_t s);
+hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, bool swept, hipStream_t s);
 hipError_t launch_rotary(const fhog_rotary_args* a, hipStream_t s);
 hipError_t launch_mfma_rate(float* out, int blocks, int trips, int data_mode, int waves, hipStream_t s);  // measurement aid
 bool bf16_shape_supported(int64_t n_q, int64_t n_k, int64_t d, int causal);

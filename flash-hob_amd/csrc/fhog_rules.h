@@ -351,6 +351,11 @@ inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q) {
   if (parts > tiles / 4) parts = tiles / 4;
   return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
 }
+// Whether those workgroups come at the end of the launch of the key-tiled sweep of the 16-bit kernels with 128 rows, where they fill the CUs that its last ones leave idle: at
+// d = 64, where two workgroups of either fit a CU. First backward, double-backward in a launch of their own and here: fp16 48 x 1537, 100 sinks 77, 158 us
+// and 68, 144; bf16 64 x 2048, 4 sinks 105, 225 and 99, 222. At d = 128 the sweep is one of producers and consumers, whose workgroups have a CU to
+// themselves. With one part the rows are stored directly, which has to follow the sweep.
+inline bool sinks_ride(int64_t d, int parts) { return d == 64 && parts > 1; }
 inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d) {
   const int parts = sink_parts(batch, sinks, n_q);
   return parts > 1 ? (size_t)parts * 2 * batch * sinks * d * sizeof(float) : 0;

@@ -3,7 +3,8 @@
 // A key j < sinks is seen by every query from the diagonal on, n_q - j + ... of them, the other keys by a window's length: as rows of an ordinary
 // workgroup of the key-tiled sweep the sinks would keep it busy n_q / window times as long as the others. The sweep therefore treats them as keys of the band, and
 // a launch behind it computes their rows over ALL their queries and puts them in place: workgroups of 32 sinks, four waves on the same rows, the queries
-// dealt out over `parts` workgroups (sink_parts), whose fp32 sums are added here in a fixed order and rounded once.
+// dealt out over `parts` workgroups (sink_parts), whose fp32 sums are added here in a fixed order and rounded once. At d = 64 those workgroups come
+// last in the launch of the key-tiled sweep itself (sinks_ride).
 #include "fhog_rules.h"
 #include "fhog_split_util.h"
 
@@ -119,16 +120,6 @@ __global__ void __launch_bounds__(256) join_forward(AttnParams p) {
   if (col == 0) p.lse[row] = (all + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;   // v_log_f32 is log2
 }
 
-// The problem of the sinks alone: their keys, every query, the mask without its window
-template <typename P>
-P sinks_alone(const P& p) {
-  P a = p;
-  a.n_k = p.sinks;
-  a.window = p.n_q + p.n_k;
-  a.sinks = 0;
-  return a;
-}
-
 }  // namespace
 
 hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s) {
@@ -141,19 +132,19 @@ hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_sink_keys(const AttnParams& p, int dtype, hipStream_t s) {
-  AttnParams a = sinks_alone(p);
-  a.tile_major_k = 0;
+hipError_t launch_sink_keys(const AttnParams& p, int dtype, bool swept, hipStream_t s) {
+  AttnParams a = p;
+  sinks_alone(a);
   const bool bit16 = dtype != FHOG_DTYPE_FP32 && p.d != 32;
-  const hipError_t e = bit16 ? launch_small_sink_bwd(a, s) : launch_attn_split_parts(a, dtype, true, s);
+  const hipError_t e = swept ? hipSuccess : bit16 ? launch_small_sink_bwd(a, s) : launch_attn_split_parts(a, dtype, true, s);
   if (e != hipSuccess || a.n_split == 1) return e;
   return launch_add({a.part, a.dk, a.dv, a.stride_kb, a.stride_kn, a.n_split, a.batch, a.n_k, a.d, a.scale}, dtype, s);
 }
 
-hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, hipStream_t s) {
-  Params a = sinks_alone(p);
-  a.tile_major = a.tile_major_k = 0;
-  const hipError_t e = split_products ? launch_split_sink_grads(a, dtype, s) : launch_small_sink_grads(a, s);
+hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, bool swept, hipStream_t s) {
+  Params a = p;
+  sinks_alone(a);
+  const hipError_t e = swept ? hipSuccess : split_products ? launch_split_sink_grads(a, dtype, s) : launch_small_sink_grads(a, s);
   if (e != hipSuccess || a.n_split == 1) return e;
   return launch_add({a.part, a.dk2, a.dv2, a.stride_kb, a.stride_kn, a.n_split, a.batch, a.n_k, a.d, a.scale}, dtype, s);
 }

@@ -66,7 +66,7 @@ LARGE = [((40, 900, 900), True, 150, 5), ((33, 1024, 1024), True, 300, 70), ((10
          ((300, 2, 500), "bottom_right", 300, 4)]
 
 
-@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 128), (torch.float32, 32), (torch.float32, 64),
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 64), (torch.float16, 128), (torch.float32, 32), (torch.float32, 64),
                                       (torch.float32, 128), (torch.bfloat16, 32)])
 @pytest.mark.parametrize("shape, causal, window, sinks", LARGE)
 def test_large_launches_against_the_formulas(shape, causal, window, sinks, d, dtype):
