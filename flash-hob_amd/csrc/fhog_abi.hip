@@ -239,12 +239,13 @@ fhog::AttnParams to_attn_params(const fhog_attn_args* a) {
 }
 
 // Sinks of a mask, or the error for a number that is none
+int dtype_bytes(int dtype) { return dtype == FHOG_DTYPE_FP32 ? 4 : 2; }
 int check_sinks(int64_t sinks) { return sinks < 0 ? fail(FHOG_E_CAUSAL, "sinks must be >= 0 (got %lld)", (long long)sinks) : FHOG_OK; }
 int32_t sinks_of(const fhog_attn_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }
 int32_t sinks_of(const fhog_bwdbwd_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }
 
 int forward_parts(const fhog_attn_args* a, int32_t sinks) {
-  return fhog::rules::forward_parts(a->batch, a->n_q, a->n_k, a->d, a->window, sinks, a->dtype == FHOG_DTYPE_FP32 ? 4 : 2);
+  return fhog::rules::forward_parts(a->batch, a->n_q, a->n_k, a->d, a->window, sinks, dtype_bytes(a->dtype));
 }
 
 // Row sums d of a first backward, rounded up so that what follows stays 16-byte aligned
@@ -452,15 +453,18 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
   p.sinks = n;
   const int parts = sink_parts(args->batch, n, args->n_q);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
-  bool swept = false;
+  const bool bit16 = attn_on_16bit_kernels(args);
+  bool swept = fhog::rules::sinks_ride(p, parts, dtype_bytes(args->dtype), !bit16);
   hipError_t e;
-  if (!attn_on_16bit_kernels(args)) {
+  if (!bit16) {
+    if (swept) p.n_split = parts, p.part = part;
     e = fhog::launch_attn_split(p, args->dtype, true, s);
   } else if (const int small = small_waves(Small::backward, args)) {
+    swept = false;
     e = fhog::launch_small_attn(p, true, small, s);
   } else {
     e = fhog::launch_attn_bf16(p, 1, s);
-    if ((swept = fhog::rules::sinks_ride(args->d, parts))) p.n_split = parts, p.part = part;
+    if (swept) p.n_split = parts, p.part = part;
     if (e == hipSuccess) e = fhog::launch_attn_bf16(p, 2, s);
   }
   if (e == hipSuccess) {
@@ -494,13 +498,13 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
   p.sinks = n, p.n_split_s = sink_parts(a.batch, n, a.n_q);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + a.ws_bytes);
   const int small = impl == FHOG_IMPL_BF16 ? small_waves(Small::double_backward, args->batch, args->n_q, args->n_k, args->d, args->causal, args->window) : 0;
-  bool swept = false;
+  const bool swept = !small && fhog::rules::sinks_ride(p, dtype_bytes(a.dtype), impl != FHOG_IMPL_BF16);
   hipError_t e = hipSuccess;
   if (small) {
     e = fhog::launch_small_bwdbwd(p, small, s);
   } else {
     if (const int rc = run_pass(&a, p, impl, FHOG_PASS_DD_B, s)) return rc;
-    if ((swept = impl == FHOG_IMPL_BF16 && fhog::rules::sinks_ride(a.d, p.n_split_s))) p.part_s = part;
+    if (swept) p.part_s = part;
     if (const int rc = impl == FHOG_IMPL_BF16 ? run_grads(&a, p, FHOG_PASS_DQ_DDO, true, s) : run_pass(&a, p, impl, fhog::kPassGrads, s)) return rc;
   }
   p.part_s = part;

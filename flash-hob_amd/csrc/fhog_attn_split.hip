@@ -383,16 +383,6 @@ __global__ void __launch_bounds__(256, (min_workgroups<T, D, WS, TWO>)) attn_spl
   attn_run<T, D, MODE, MASK, WS, false, TWO, PARTS>(p, smem, blockIdx.x, MASK != MASK_NONE && WS == 1 && min_workgroups<T, D, WS, TWO> == 2);
 }
 
-// dQ (workgroups [0, q_blocks)) and dK, dV (the others; mixed: tile by tile in turn) in one launch; ON_CU: workgroups on a CU
-template <typename T, int D, int MASK, int WS, int ON_CU>
-__global__ void __launch_bounds__(256, ON_CU) attn_split_bwd(AttnParams p, int q_blocks, bool mixed) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr bool joins = MASK != MASK_NONE && WS == 1 && ON_CU == 2;   // workgroups of a masked launch that share a CU
-  int id = blockIdx.x;
-  if (first_of_two(q_blocks, (int)gridDim.x - q_blocks, mixed, joins, id)) attn_run<T, D, MODE_BWD_Q, MASK, WS, false>(p, smem, id, joins && !mixed);
-  else attn_run<T, D, MODE_BWD_K, MASK, WS, true>(p, smem, id, joins && !mixed);
-}
-
 template <typename T, int D, int MODE, int WS, bool TWO = false>
 constexpr int lds_bytes() {
   constexpr bool KSIDE = MODE == MODE_BWD_K;
@@ -402,7 +392,31 @@ constexpr int lds_bytes() {
 }
 
 template <int WS>
-unsigned blocks(int rows, int batch) { return grid_blocks((rows + 128 / WS - 1) / (128 / WS), batch); }
+__host__ __device__ unsigned blocks(int rows, int batch) { return grid_blocks((rows + 128 / WS - 1) / (128 / WS), batch); }
+
+// Waves on the same 32 rows where several workgroups share the streamed side: as many as fit the LDS, with ON_CU workgroups on a CU
+template <typename T, int D, int MODE, int ON_CU = 1>
+constexpr int part_waves = ON_CU * lds_bytes<T, D, MODE, 4>() <= 160 * 1024 ? 4 : 2;
+
+// dQ (workgroups [0, q_blocks)) and dK, dV (the others; mixed: tile by tile in turn) in one launch; ON_CU: workgroups on a CU.
+// MASK_SINK: behind both come the workgroups that sum up the rows of the sinks (fhog_sinks.hip), where rules::sinks_ride says so.
+template <typename T, int D, int MASK, int WS, int ON_CU>
+__global__ void __launch_bounds__(256, ON_CU) attn_split_bwd(AttnParams p, int q_blocks, bool mixed) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr bool joins = MASK != MASK_NONE && WS == 1 && ON_CU == 2;   // workgroups of a masked launch that share a CU
+  int id = blockIdx.x, riders = 0;
+  if constexpr (MASK == MASK_SINK) {
+    constexpr int W = part_waves<T, D, MODE_BWD_K, ON_CU>;
+    riders = p.part ? (int)blocks<W>(p.sinks, p.batch * p.n_split) : 0;
+    const int first = (int)gridDim.x - riders;
+    if (id >= first) {
+      sinks_alone(p);
+      return attn_run<T, D, MODE_BWD_K, MASK_BAND, W, true, false, true>(p, smem, id - first, false);
+    }
+  }
+  if (first_of_two(q_blocks, (int)gridDim.x - riders - q_blocks, mixed, joins, id)) attn_run<T, D, MODE_BWD_Q, MASK, WS, false>(p, smem, id, joins && !mixed);
+  else attn_run<T, D, MODE_BWD_K, MASK, WS, true>(p, smem, id, joins && !mixed);
+}
 
 template <typename T, int D, int MODE, int MASK, int WS, bool TWO = false>
 hipError_t launch_ws(const AttnParams& p, hipStream_t s) {
@@ -417,7 +431,7 @@ hipError_t launch_ws(const AttnParams& p, hipStream_t s) {
 // Forward (MASK_SINK) or the rows of dK, dV of the sinks (MASK_BAND; p.n_k is their number there, and there is no window), over p.n_split workgroups a tile
 template <typename T, int D, int MODE, int MASK>
 hipError_t launch_parts(const AttnParams& p, hipStream_t s) {
-  constexpr int WS = lds_bytes<T, D, MODE, 4>() <= 160 * 1024 ? 4 : 2, smem = lds_bytes<T, D, MODE, WS>();
+  constexpr int WS = part_waves<T, D, MODE>, smem = lds_bytes<T, D, MODE, WS>();
   const hipError_t e = allow_dynamic_lds<attn_split<T, D, MODE, MASK, WS, false, true>>(smem);
   if (e != hipSuccess) return e;
   const unsigned grid = blocks<WS>(MODE == MODE_BWD_K ? p.n_k : p.n_q, p.batch * p.n_split);
@@ -427,12 +441,14 @@ hipError_t launch_parts(const AttnParams& p, hipStream_t s) {
 
 template <typename T, int D, int MASK, int WS, int ON_CU = min_workgroups<T, D, WS, false>>
 hipError_t launch_bwd_ws(const AttnParams& p, hipStream_t s, bool mixed = false) {
-  constexpr int lq = lds_bytes<T, D, MODE_BWD_Q, WS>(), lk = lds_bytes<T, D, MODE_BWD_K, WS>(), smem = lq > lk ? lq : lk;
+  constexpr int lq = lds_bytes<T, D, MODE_BWD_Q, WS>(), lk = lds_bytes<T, D, MODE_BWD_K, WS>(), own = lq > lk ? lq : lk;
+  constexpr int W = part_waves<T, D, MODE_BWD_K, ON_CU>, riders = MASK == MASK_SINK ? lds_bytes<T, D, MODE_BWD_K, W>() : 0, smem = own > riders ? own : riders;
   static_assert(smem <= 160 * 1024, "stages and exchange buffer have to fit the LDS");
   const hipError_t e = allow_dynamic_lds<attn_split_bwd<T, D, MASK, WS, ON_CU>>(smem);
   if (e != hipSuccess) return e;
   const unsigned gq = blocks<WS>(p.n_q, p.batch), gk = blocks<WS>(p.n_k, p.batch);
-  hipLaunchKernelGGL((attn_split_bwd<T, D, MASK, WS, ON_CU>), dim3(gq + gk), dim3(256), smem, s, p, (int)gq, mixed);
+  const unsigned gs = MASK == MASK_SINK && p.part ? blocks<W>(p.sinks, p.batch * p.n_split) : 0;
+  hipLaunchKernelGGL((attn_split_bwd<T, D, MASK, WS, ON_CU>), dim3(gq + gk + gs), dim3(256), smem, s, p, (int)gq, mixed);
   return hipGetLastError();
 }
 

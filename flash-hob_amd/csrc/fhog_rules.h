@@ -351,11 +351,6 @@ inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q) {
   if (parts > tiles / 4) parts = tiles / 4;
   return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
 }
-// Whether those workgroups come at the end of the launch of the key-tiled sweep of the 16-bit kernels with 128 rows, where they fill the CUs that its last ones leave idle: at
-// d = 64, where two workgroups of either fit a CU. First backward, double-backward in a launch of their own and here: fp16 48 x 1537, 100 sinks 77, 158 us
-// and 68, 144; bf16 64 x 2048, 4 sinks 105, 225 and 99, 222. At d = 128 the sweep is one of producers and consumers, whose workgroups have a CU to
-// themselves. With one part the rows are stored directly, which has to follow the sweep.
-inline bool sinks_ride(int64_t d, int parts) { return d == 64 && parts > 1; }
 inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d) {
   const int parts = sink_parts(batch, sinks, n_q);
   return parts > 1 ? (size_t)parts * 2 * batch * sinks * d * sizeof(float) : 0;
@@ -553,6 +548,18 @@ inline int split_bwd_waves(const AttnParams& p, int bytes) {
                              : waves == 2 ? 2 * n_q >= 3 * n_k && n_q - n_k >= 250
                                           : (2 * n_q >= 5 * n_k && n_q - n_k >= 250) || (groups >= 1000 && 4 * n_q >= 5 * n_k);
   return long_key_side ? 0 : waves;
+}
+
+// Whether the workgroups that sum up the rows of the sinks come at the end of the launch of the key-tiled sweep, where they fill the CUs that its last ones leave idle,
+// and not in a launch of their own. On the 16-bit kernels with 128 rows: at d = 64, where two workgroups of either fit a CU; at d = 128 the sweep is one of producers and
+// consumers, whose workgroups have a CU to themselves. Of split products: where one launch holds both sides. With one part the rows are stored directly, which
+// has to follow the sweep. First backward, double-backward, us, in a launch of their own and here: fp16 48 x 1537, d = 64, 100 sinks 77, 158 and 68, 144; bf16
+// 64 x 2048, d = 64, 4 sinks 105, 225 and 99, 222; bf16 16 x 512, d = 32, one sink 15.3, 24.4 and 11.2, 22; fp32 8 x 4096, d = 128, 4 sinks 439, 1192 and 411, 1176.
+inline bool sinks_ride(const AttnParams& p, int parts, int bytes, bool split_products) {
+  return parts > 1 && (split_products ? split_bwd_waves(p, bytes) != 0 : p.d == 64);
+}
+inline bool sinks_ride(const Params& p, int bytes, bool split_products) {
+  return p.n_split_s > 1 && (split_products ? !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0 : p.d == 64);
 }
 
 }  // namespace rules

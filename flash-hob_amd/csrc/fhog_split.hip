@@ -535,15 +535,6 @@ __global__ void __launch_bounds__(256, (min_workgroups<D, WS>)) split_sweep(Para
   split_run<T, D, PASS, MASK, WS>(p, smem, blockIdx.x, joins<D, MASK, WS>);
 }
 
-// Passes 3 (workgroups [0, q_blocks)) and 4 (the others; mixed: tile by tile in turn) in one launch: given the row statistics neither needs the other.
-template <typename T, int D, int MASK, int WS3, int WS4>
-__global__ void __launch_bounds__(256, (min_workgroups<D, (WS3 > WS4 ? WS3 : WS4)>)) split_grads(Params p, int q_blocks, bool mixed) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  int id = blockIdx.x;
-  if (first_of_two(q_blocks, (int)gridDim.x - q_blocks, mixed, joins<D, MASK, WS3>, id)) split_run<T, D, 3, MASK, WS3>(p, smem, id, joins<D, MASK, WS3> && !mixed);
-  else split_run<T, D, 4, MASK, WS4>(p, smem, id, joins<D, MASK, WS4> && !mixed);
-}
-
 template <typename T, int D, int PASS, int WS>
 constexpr int lds_bytes() {
   constexpr bool KSIDE = PASS == 4, STATS = PASS == 1 || PASS == 2 || PASS == 5;
@@ -552,6 +543,32 @@ constexpr int lds_bytes() {
   constexpr int stages = is_direct<PASS, WS> ? 0 : n_buffers<T, D, WS>(stage) * WS * stage + (is_raw<T, D> && !STATS ? 4 * TS * D * 4 : 0);
   constexpr int xch = WS > 1 ? nw * (WS - 1) * (STATS ? 5 : 2 * D / 32 * 16) * 64 * 4 : 0;
   return stages > xch ? stages : xch;
+}
+
+template <int WS>
+__host__ __device__ unsigned blocks(int rows, int batch) { return grid_blocks((rows + 128 / WS - 1) / (128 / WS), batch); }
+
+// Waves on the same 32 rows of the sinks: as many as fit the LDS
+template <typename T, int D>
+constexpr int sink_waves = lds_bytes<T, D, 4, 4>() <= 160 * 1024 ? 4 : lds_bytes<T, D, 4, 2>() <= 160 * 1024 ? 2 : 1;
+
+// Passes 3 (workgroups [0, q_blocks)) and 4 (the others; mixed: tile by tile in turn) in one launch: given the row statistics neither needs the other. MASK_SINK: behind
+// both come the workgroups that sum up the rows of the sinks (fhog_sinks.hip), where rules::sinks_ride says so.
+template <typename T, int D, int MASK, int WS3, int WS4>
+__global__ void __launch_bounds__(256, (min_workgroups<D, (WS3 > WS4 ? WS3 : WS4)>)) split_grads(Params p, int q_blocks, bool mixed) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  int id = blockIdx.x, riders = 0;
+  if constexpr (MASK == MASK_SINK) {
+    constexpr int WS = sink_waves<T, D>;
+    riders = p.part_s ? (int)blocks<WS>(p.sinks, p.batch * p.n_split_s) : 0;
+    const int first = (int)gridDim.x - riders;
+    if (id >= first) {
+      sinks_alone(p);
+      return split_run<T, D, 4, MASK_BAND, WS, true>(p, smem, id - first, false);
+    }
+  }
+  if (first_of_two(q_blocks, (int)gridDim.x - riders - q_blocks, mixed, joins<D, MASK, WS3>, id)) split_run<T, D, 3, MASK, WS3>(p, smem, id, joins<D, MASK, WS3> && !mixed);
+  else split_run<T, D, 4, MASK, WS4>(p, smem, id, joins<D, MASK, WS4> && !mixed);
 }
 
 // The rows of dK2, dV2 of the sinks, over all queries that see them: p.n_k is their number, and there is no window
@@ -596,20 +613,19 @@ hipError_t launch_sweep(const Params& p, hipStream_t s) {
   return launch_ws<T, D, PASS, MASK, 1>(p, s);
 }
 
-template <int WS>
-unsigned blocks(int rows, int batch) { return grid_blocks((rows + 128 / WS - 1) / (128 / WS), batch); }
-
 // At most MOST waves on the same rows, as many as let either pass fit the LDS. sides: 1 pass 3, 2 pass 4, 3 both
 template <typename T, int D, int MASK, int MOST>
 hipError_t launch_grads_most(const Params& p, int sides, hipStream_t s) {
   constexpr int ws3 = MOST >= 4 && lds_bytes<T, D, 3, 4>() <= 160 * 1024 ? 4 : MOST >= 2 && lds_bytes<T, D, 3, 2>() <= 160 * 1024 ? 2 : 1;
   constexpr int ws4 = MOST >= 4 && lds_bytes<T, D, 4, 4>() <= 160 * 1024 ? 4 : MOST >= 2 && lds_bytes<T, D, 4, 2>() <= 160 * 1024 ? 2 : 1;
-  constexpr int l3 = lds_bytes<T, D, 3, ws3>(), l4 = lds_bytes<T, D, 4, ws4>(), smem = l3 > l4 ? l3 : l4;
+  constexpr int l3 = lds_bytes<T, D, 3, ws3>(), l4 = lds_bytes<T, D, 4, ws4>(), own = l3 > l4 ? l3 : l4;
+  constexpr int riders = MASK == MASK_SINK ? lds_bytes<T, D, 4, sink_waves<T, D>>() : 0, smem = own > riders ? own : riders;
   static_assert(smem <= 160 * 1024, "stages and exchange buffer have to fit the LDS");
   const hipError_t e = allow_dynamic_lds<split_grads<T, D, MASK, ws3, ws4>>(smem);
   if (e != hipSuccess) return e;
   const unsigned gq = sides & 1 ? blocks<ws3>(p.n_q, p.batch) : 0, gk = sides & 2 ? blocks<ws4>(p.n_k, p.batch) : 0;
-  hipLaunchKernelGGL((split_grads<T, D, MASK, ws3, ws4>), dim3(gq + gk), dim3(256), smem, s, p, (int)gq, ws3 == 1 && ws4 == 1 && rules::split_in_turn(p, gq, gk));
+  const unsigned gs = MASK == MASK_SINK && p.part_s ? blocks<sink_waves<T, D>>(p.sinks, p.batch * p.n_split_s) : 0;
+  hipLaunchKernelGGL((split_grads<T, D, MASK, ws3, ws4>), dim3(gq + gk + gs), dim3(256), smem, s, p, (int)gq, ws3 == 1 && ws4 == 1 && rules::split_in_turn(p, gq, gk));
   return hipGetLastError();
 }
 
@@ -647,7 +663,7 @@ hipError_t launch_grads(const Params& p, int sides, hipStream_t s) {
 
 template <typename T, int D>
 hipError_t launch_sink_grads(const Params& p, hipStream_t s) {
-  constexpr int WS = lds_bytes<T, D, 4, 4>() <= 160 * 1024 ? 4 : lds_bytes<T, D, 4, 2>() <= 160 * 1024 ? 2 : 1, smem = lds_bytes<T, D, 4, WS>();
+  constexpr int WS = sink_waves<T, D>, smem = lds_bytes<T, D, 4, WS>();
   const hipError_t e = allow_dynamic_lds<split_sink_grads<T, D, WS>>(smem);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((split_sink_grads<T, D, WS>), dim3(blocks<WS>(p.n_k, p.batch * p.n_split)), dim3(256), smem, s, p);
