@@ -454,19 +454,13 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
   const int parts = sink_parts(args->batch, n, args->n_q);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
   const bool bit16 = attn_on_16bit_kernels(args);
-  bool swept = fhog::rules::sinks_ride(p, parts, dtype_bytes(args->dtype), !bit16);
-  hipError_t e;
-  if (!bit16) {
-    if (swept) p.n_split = parts, p.part = part;
-    e = fhog::launch_attn_split(p, args->dtype, true, s);
-  } else if (const int small = small_waves(Small::backward, args)) {
-    swept = false;
-    e = fhog::launch_small_attn(p, true, small, s);
-  } else {
-    e = fhog::launch_attn_bf16(p, 1, s);
-    if (swept) p.n_split = parts, p.part = part;
-    if (e == hipSuccess) e = fhog::launch_attn_bf16(p, 2, s);
-  }
+  const int small = bit16 ? small_waves(Small::backward, args) : 0;
+  const bool swept = fhog::rules::sinks_ride(p, parts, dtype_bytes(args->dtype), bit16, small);
+  hipError_t e = hipSuccess;
+  if (bit16 && !small) e = fhog::launch_attn_bf16(p, 1, s);
+  if (swept) p.n_split = parts, p.part = part;
+  if (e == hipSuccess)
+    e = !bit16 ? fhog::launch_attn_split(p, args->dtype, true, s) : small ? fhog::launch_small_attn(p, true, small, s) : fhog::launch_attn_bf16(p, 2, s);
   if (e == hipSuccess) {
     p.n_split = parts, p.part = part;
     e = fhog::launch_sink_keys(p, args->dtype, swept, s);
@@ -498,13 +492,13 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
   p.sinks = n, p.n_split_s = sink_parts(a.batch, n, a.n_q);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + a.ws_bytes);
   const int small = impl == FHOG_IMPL_BF16 ? small_waves(Small::double_backward, args->batch, args->n_q, args->n_k, args->d, args->causal, args->window) : 0;
-  const bool swept = !small && fhog::rules::sinks_ride(p, dtype_bytes(a.dtype), impl != FHOG_IMPL_BF16);
+  const bool swept = fhog::rules::sinks_ride(p, dtype_bytes(a.dtype), impl == FHOG_IMPL_BF16, small);
+  if (swept) p.part_s = part;
   hipError_t e = hipSuccess;
   if (small) {
     e = fhog::launch_small_bwdbwd(p, small, s);
   } else {
     if (const int rc = run_pass(&a, p, impl, FHOG_PASS_DD_B, s)) return rc;
-    if (swept) p.part_s = part;
     if (const int rc = impl == FHOG_IMPL_BF16 ? run_grads(&a, p, FHOG_PASS_DQ_DDO, true, s) : run_pass(&a, p, impl, fhog::kPassGrads, s)) return rc;
   }
   p.part_s = part;

@@ -203,10 +203,10 @@ template <bool F16, int D, int MASK, bool RIDERS = false>
 __global__ void __launch_bounds__(256, 2) attn_bwd_k_bf16(AttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   if constexpr (RIDERS) {
-    const int id = (int)blockIdx.x - (int)gridDim.x + (int)grid_blocks((p.sinks + TS - 1) / TS, p.batch * p.n_split);
+    const int id = smallk::sink_workgroup(p.sinks, p.batch * p.n_split);
     if (id >= 0) {
       sinks_alone(p);
-      return smallk::bwd_k<F16, D, MASK_BAND, smallk::WAVES, true>(p, smem, id);
+      return smallk::bwd_k<F16, D, MASK_BAND, smallk::WAVES, true, false>(p, smem, id);
     }
   }
   constexpr int KK = D / 16, NC = D / 32, TILE = TS * 2 * D;

@@ -551,15 +551,16 @@ inline int split_bwd_waves(const AttnParams& p, int bytes) {
 }
 
 // Whether the workgroups that sum up the rows of the sinks come at the end of the launch of the key-tiled sweep, where they fill the CUs that its last ones leave idle,
-// and not in a launch of their own. On the 16-bit kernels with 128 rows: at d = 64, where two workgroups of either fit a CU; at d = 128 the sweep is one of producers and
+// and not in a launch of their own. In small launches of the 16-bit kernels: always. On those with 128 rows: at d = 64, where two workgroups of either fit a CU; at d = 128 the sweep is one of producers and
 // consumers, whose workgroups have a CU to themselves. Of split products: where one launch holds both sides. With one part the rows are stored directly, which
 // has to follow the sweep. First backward, double-backward, us, in a launch of their own and here: fp16 48 x 1537, d = 64, 100 sinks 77, 158 and 68, 144; bf16
-// 64 x 2048, d = 64, 4 sinks 105, 225 and 99, 222; bf16 16 x 512, d = 32, one sink 15.3, 24.4 and 11.2, 22; fp32 8 x 4096, d = 128, 4 sinks 439, 1192 and 411, 1176.
-inline bool sinks_ride(const AttnParams& p, int parts, int bytes, bool split_products) {
-  return parts > 1 && (split_products ? split_bwd_waves(p, bytes) != 0 : p.d == 64);
+// 64 x 2048, d = 64, 4 sinks 105, 225 and 99, 222; bf16 16 x 512, d = 32, one sink 15.3, 24.4 and 11.2, 22; small: 2 x 1000,
+// d = 64, 4 sinks 17.0, 26.9 and 11.6, 21.0, 8 x 1024, d = 128 32.7, 54.3 and 29.9, 48.5; fp32 8 x 4096, d = 128, 4 sinks 439, 1192 and 411, 1176.
+inline bool sinks_ride(const AttnParams& p, int parts, int bytes, bool bit16, int small) {
+  return parts > 1 && (bit16 ? small || p.d == 64 : split_bwd_waves(p, bytes) != 0);
 }
-inline bool sinks_ride(const Params& p, int bytes, bool split_products) {
-  return p.n_split_s > 1 && (split_products ? !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0 : p.d == 64);
+inline bool sinks_ride(const Params& p, int bytes, bool bit16, int small) {
+  return p.n_split_s > 1 && (bit16 ? small || p.d == 64 : !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0);
 }
 
 }  // namespace rules

@@ -191,10 +191,9 @@ constexpr int bwd_k_stage = (OWN_D ? 3 : 2) * TS * 2 * D + 2 * TS * 4;
 template <int D, bool OWN_D>
 constexpr int bwd_k_buffers = 2 * WAVES * bwd_k_stage<D, OWN_D> <= (OWN_D ? 128 : 160) * 1024 ? 2 : 1;
 
-template <bool F16, int D, int MASK, int W, bool PARTS = false>   // PARTS: as in grads_k, behind a sweep for dQ
+template <bool F16, int D, int MASK, int W, bool PARTS = false, bool OWN_D = true>   // PARTS: as in grads_k; without OWN_D behind a sweep for dQ
 __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
   constexpr int KK = D / 16, NC = D / 32, ROWS = TS * WAVES / W, TILE = TS * 2 * D;
-  constexpr bool OWN_D = !PARTS;
   constexpr int NT = OWN_D ? 3 : 2, STAGE = bwd_k_stage<D, OWN_D>, NBUF = bwd_k_buffers<D, OWN_D>;
   int bh, tile;
   if (!decode_block<MASK>((p.n_k + ROWS - 1) / ROWS, p.batch * (PARTS ? p.n_split : 1), false, p.tile_major_k != 0, bh, tile, false, id)) return;
@@ -268,6 +267,9 @@ __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
 
 template <int D>
 constexpr int sink_bwd_lds = max_of(WAVES * bwd_k_buffers<D, false> * bwd_k_stage<D, false>, add_waves_bytes(2 * D / 32));
+
+// Of the workgroups that sum up the rows of the sinks, the last ones of a launch (none without sinks): this one's number among them, negative for the others
+__device__ __forceinline__ int sink_workgroup(int sinks, int slices) { return (int)blockIdx.x - (int)gridDim.x + (int)grid_blocks((sinks + TS - 1) / TS, slices); }
 
 }  // namespace smallk
 }  // namespace fhog

@@ -147,9 +147,17 @@ __device__ __forceinline__ void grads_q(const Params& p, char* smem) {
 template <int D>
 constexpr int grads_lds = max_of(WAVES * n_buffers<D, 4> * max_of(4 * TS * 2 * D, grads_k_stage<D>), add_waves_bytes(2 * D / 32));
 
+// MASK_SINK, small_bwd too: behind both come the workgroups that sum up the rows of the sinks (fhog_sinks.hip)
 template <bool F16, int D, int MASK, int W>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) small_grads(Params p, int q_blocks) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  if constexpr (MASK == MASK_SINK) {
+    const int id = sink_workgroup(p.part_s ? p.sinks : 0, p.batch * p.n_split_s);
+    if (id >= 0) {
+      sinks_alone(p);
+      return grads_k<F16, D, MASK_BAND, WAVES, true>(p, smem, id);
+    }
+  }
   if ((int)blockIdx.x < q_blocks) grads_q<F16, D, MASK, W>(p, smem);
   else grads_k<F16, D, MASK, W>(p, smem, (int)blockIdx.x - q_blocks);
 }
@@ -285,6 +293,13 @@ constexpr int bwd_lds = max_of(max_of(WAVES * n_buffers<D, 2> * 2 * TS * 2 * D, 
 template <bool F16, int D, int MASK, int W>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) small_bwd(AttnParams p, int q_blocks) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  if constexpr (MASK == MASK_SINK) {
+    const int id = sink_workgroup(p.part ? p.sinks : 0, p.batch * p.n_split);
+    if (id >= 0) {
+      sinks_alone(p);
+      return bwd_k<F16, D, MASK_BAND, WAVES, true>(p, smem, id);
+    }
+  }
   if ((int)blockIdx.x < q_blocks) bwd_q<F16, D, MASK, W>(p, smem);
   else bwd_k<F16, D, MASK, W>(p, smem, (int)blockIdx.x - q_blocks);
 }
@@ -293,7 +308,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) small_bwd(AttnParams p, 
 template <bool F16, int D>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) sink_bwd(AttnParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  bwd_k<F16, D, MASK_BAND, WAVES, true>(p, smem, blockIdx.x);
+  bwd_k<F16, D, MASK_BAND, WAVES, true, false>(p, smem, blockIdx.x);
 }
 template <bool F16, int D>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) sink_grads(Params p) {
@@ -315,17 +330,17 @@ unsigned blocks(int rows, int batch) { return grid_blocks((rows + TS * WAVES / W
 template <bool F16, int D, int MASK, int W>
 hipError_t bwdbwd_d(const Params& p, hipStream_t s) {
   static_assert(stats_lds<D> <= 160 * 1024 && grads_lds<D> <= 160 * 1024, "the stages of four waves have to fit the LDS");
-  const unsigned gq = blocks<W>(p.n_q, p.batch), gk = blocks<W>(p.n_k, p.batch);
+  const unsigned gq = blocks<W>(p.n_q, p.batch), gk = blocks<W>(p.n_k, p.batch), gs = MASK == MASK_SINK && p.part_s ? blocks<WAVES>(p.sinks, p.batch * p.n_split_s) : 0;
   const hipError_t e = launch<small_stats<F16, D, MASK, W>>(gq, stats_lds<D>, s, p);
-  return e != hipSuccess ? e : launch<small_grads<F16, D, MASK, W>>(gq + gk, grads_lds<D>, s, p, (int)gq);
+  return e != hipSuccess ? e : launch<small_grads<F16, D, MASK, W>>(gq + gk + gs, grads_lds<D>, s, p, (int)gq);
 }
 
 template <bool F16, int D, int MASK, int W>
 hipError_t attn_d(const AttnParams& p, bool backward, hipStream_t s) {
   static_assert(fwd_lds<D> <= 160 * 1024 && bwd_lds<D> <= 160 * 1024, "the stages of four waves have to fit the LDS");
-  const unsigned gq = blocks<W>(p.n_q, p.batch), gk = blocks<W>(p.n_k, p.batch);
+  const unsigned gq = blocks<W>(p.n_q, p.batch), gk = blocks<W>(p.n_k, p.batch), gs = MASK == MASK_SINK && p.part ? blocks<WAVES>(p.sinks, p.batch * p.n_split) : 0;
   if (!backward) return launch<small_fwd<F16, D, MASK, W>>(gq, fwd_lds<D>, s, p);
-  return launch<small_bwd<F16, D, MASK, W>>(gq + gk, bwd_lds<D>, s, p, (int)gq);
+  return launch<small_bwd<F16, D, MASK, W>>(gq + gk + gs, bwd_lds<D>, s, p, (int)gq);
 }
 
 template <bool F16, int D>
