@@ -253,7 +253,7 @@ size_t row_bytes(const fhog_attn_args* a) { return ((size_t)a->batch * a->n_q * 
 
 size_t attn_sinks_bytes(const fhog_attn_args* a, int64_t sinks, int backward) {
   const int32_t n = sinks_of(a, sinks);
-  if (backward) return n ? row_bytes(a) + sink_bytes(a->batch, n, a->n_q, a->d) : (size_t)a->batch * a->n_q * sizeof(float);
+  if (backward) return n ? row_bytes(a) + sink_bytes(a->batch, n, a->n_q, a->d, dtype_bytes(a->dtype), false) : (size_t)a->batch * a->n_q * sizeof(float);
   return n ? forward_part_bytes(a->batch, a->n_q, a->d, forward_parts(a, n)) : 0;
 }
 
@@ -451,18 +451,18 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
   const hipStream_t s = (hipStream_t)hip_stream;
   fhog::AttnParams p = to_attn_params(args);
   p.sinks = n;
-  const int parts = sink_parts(args->batch, n, args->n_q);
+  const int parts = sink_parts(args->batch, n, args->n_q, args->d, dtype_bytes(args->dtype), false);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
   const bool bit16 = attn_on_16bit_kernels(args);
   const int small = bit16 ? small_waves(Small::backward, args) : 0;
-  const bool swept = fhog::rules::sinks_ride(p, parts, dtype_bytes(args->dtype), bit16, small);
+  const bool swept = fhog::rules::sinks_ride(p, dtype_bytes(args->dtype), bit16, small);
   hipError_t e = hipSuccess;
   if (bit16 && !small) e = fhog::launch_attn_bf16(p, 1, s);
   if (swept) p.n_split = parts, p.part = part;
   if (e == hipSuccess)
     e = !bit16 ? fhog::launch_attn_split(p, args->dtype, true, s) : small ? fhog::launch_small_attn(p, true, small, s) : fhog::launch_attn_bf16(p, 2, s);
   if (e == hipSuccess) {
-    p.n_split = parts, p.part = part;
+    p.n_split = parts, p.part = swept || parts > 1 ? part : nullptr;
     e = fhog::launch_sink_keys(p, args->dtype, swept, s);
   }
   if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "attention backward: HIP error %d (%s)", (int)e, hipGetErrorString(e));
@@ -473,7 +473,7 @@ size_t fhog_bwdbwd_sinks_workspace_bytes(const fhog_bwdbwd_args* args, int64_t s
   if (validate(args) != FHOG_OK || check_sinks(sinks) != FHOG_OK) return 0;
   const size_t hint = workspace_hint(args, to_params(args), select_impl(args));
   const int32_t n = sinks_of(args, sinks);
-  return n ? ((hint + 15) & ~(size_t)15) + sink_bytes(args->batch, n, args->n_q, args->d) : hint;
+  return n ? ((hint + 15) & ~(size_t)15) + sink_bytes(args->batch, n, args->n_q, args->d, dtype_bytes(args->dtype), true) : hint;
 }
 
 int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_stream) {
@@ -482,14 +482,14 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
   const int32_t n = sinks_of(args, sinks);
   if (n == 0) return fhog_bwdbwd(args, hip_stream);
   if (args->schedule != FHOG_SCHEDULE_FUSED_STATS) return fail(FHOG_E_SCHEDULE, "sinks run under schedule %d alone (got %d)", FHOG_SCHEDULE_FUSED_STATS, args->schedule);
-  const size_t of_sinks = sink_bytes(args->batch, n, args->n_q, args->d);
+  const size_t of_sinks = sink_bytes(args->batch, n, args->n_q, args->d, dtype_bytes(args->dtype), true);
   if (const int rc = check_ws(args->ws, args->ws_bytes, stats_bytes(args) + of_sinks)) return rc;
   const hipStream_t s = (hipStream_t)hip_stream;
   const int impl = select_impl(args);
   fhog_bwdbwd_args a = *args;   // the sweeps have what lies before the partial results of the sinks, which are a multiple of 16 bytes
   a.ws_bytes = (args->ws_bytes & ~(int64_t)15) - (int64_t)of_sinks;
   fhog::Params p = to_params(&a);
-  p.sinks = n, p.n_split_s = sink_parts(a.batch, n, a.n_q);
+  p.sinks = n, p.n_split_s = sink_parts(a.batch, n, a.n_q, a.d, dtype_bytes(a.dtype), true);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + a.ws_bytes);
   const int small = impl == FHOG_IMPL_BF16 ? small_waves(Small::double_backward, args->batch, args->n_q, args->n_k, args->d, args->causal, args->window) : 0;
   const bool swept = fhog::rules::sinks_ride(p, dtype_bytes(a.dtype), impl == FHOG_IMPL_BF16, small);
@@ -501,7 +501,7 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
     if (const int rc = run_pass(&a, p, impl, FHOG_PASS_DD_B, s)) return rc;
     if (const int rc = impl == FHOG_IMPL_BF16 ? run_grads(&a, p, FHOG_PASS_DQ_DDO, true, s) : run_pass(&a, p, impl, fhog::kPassGrads, s)) return rc;
   }
-  p.part_s = part;
+  p.part_s = swept || p.n_split_s > 1 ? part : nullptr;
   if (e == hipSuccess) e = fhog::launch_sink_keys(p, args->dtype, impl != FHOG_IMPL_BF16, swept, s);
   if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "HIP error %d (%s)", (int)e, hipGetErrorString(e));
   return FHOG_OK;

@@ -359,7 +359,7 @@ __device__ __forceinline__ void attn_run(const AttnParams& p, char* smem, int id
     if (h == 0) rows.stats(part)[row] = f32x2_t{m, l};
     return;
   }
-  if (PARTS && KSIDE && p.n_split > 1) {
+  if (PARTS && KSIDE && p.part) {
     float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + ri) * D;
     store_rows<float, D>(to, acc0, 1.f, h);
     store_rows<float, D>(to + (int64_t)p.batch * p.n_k * D, acc1, 1.f, h);

@@ -342,18 +342,20 @@ inline int32_t sinks_of(int64_t sinks, int64_t window, int64_t n_k) {   // a win
   if (window == 0 || window >= n_k) return 0;
   return (int32_t)(sinks < n_k ? sinks : n_k);
 }
-// Workgroups that share 32 sinks of a slice, each with a part of the queries: one for every CU, with four tiles (one of each wave) for each at least.
+// Workgroups that share 32 sinks of a slice, each with a part of the queries: one for every CU, with a tile for each of its waves at least.
 // First | second backward, us, 512 workgroups of eight tiles -> 256 of four: bf16 32 x 4096, d = 128, window 1024, 4 sinks 290 | 678 -> 282 | 675; fp32 16 x 1024, d = 64,
 // window 256, 33 sinks 64.9 | 153 -> 61.7 | 149; 8 x 4096, d = 128 448 | 1401 -> 440 | 1357; 1024 of four 296 | 686, 61.7 | 148, 440 | 1358.
-inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q) {
-  const int64_t groups = (sinks + 31) / 32 * batch, tiles = (n_q + 31) / 32;
+// Single precision of d = 128 with four tiles at least -> one for each of its two | one waves: 1 x 1000, window 100 41.2 | 123 -> 41.5 | 89.
+inline int64_t sink_groups(int64_t batch, int64_t sinks) { return (sinks + 31) / 32 * batch; }
+inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q, int64_t d, int bytes, bool second) {
+  const int64_t groups = sink_groups(batch, sinks), tiles = (n_q + 31) / 32, waves = bytes * d < 512 ? 4 : second ? 1 : 2;   // on the same rows
   int64_t parts = (256 + groups - 1) / groups;
-  if (parts > tiles / 4) parts = tiles / 4;
+  if (parts > tiles / waves) parts = tiles / waves;
   return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
 }
-inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d) {
-  const int parts = sink_parts(batch, sinks, n_q);
-  return parts > 1 ? (size_t)parts * 2 * batch * sinks * d * sizeof(float) : 0;
+// Partial results; more groups than CUs store their rows directly
+inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d, int bytes, bool second) {
+  return sink_groups(batch, sinks) <= 256 ? (size_t)sink_parts(batch, sinks, n_q, d, bytes, second) * 2 * batch * sinks * d * sizeof(float) : 0;
 }
 // Forwards of few queries under a mask with sinks: workgroups that share 32 queries of a slice, each with a part of the keys, or 0 for the kernels of longer ones. What
 // a number of parts costs is reckoned up, in us: rounds of the workgroups, each with something to start and to end (fixed) and its waves' tiles one after the
@@ -552,15 +554,16 @@ inline int split_bwd_waves(const AttnParams& p, int bytes) {
 
 // Whether the workgroups that sum up the rows of the sinks come at the end of the launch of the key-tiled sweep, where they fill the CUs that its last ones leave idle,
 // and not in a launch of their own. In small launches of the 16-bit kernels: always. On those with 128 rows: at d = 64, where two workgroups of either fit a CU; at d = 128 the sweep is one of producers and
-// consumers, whose workgroups have a CU to themselves. Of split products: where one launch holds both sides. With one part the rows are stored directly, which
-// has to follow the sweep. First backward, double-backward, us, in a launch of their own and here: fp16 48 x 1537, d = 64, 100 sinks 77, 158 and 68, 144; bf16
+// consumers, whose workgroups have a CU to themselves. Of split products: where one launch holds both sides. More groups than CUs fill the GPU by themselves, and store their rows
+// directly, which has to follow the sweep. First backward, double-backward, us, in a launch of their own and here: fp16 48 x 1537, d = 64, 100 sinks 77, 158 and 68, 144; bf16
 // 64 x 2048, d = 64, 4 sinks 105, 225 and 99, 222; bf16 16 x 512, d = 32, one sink 15.3, 24.4 and 11.2, 22; small: 2 x 1000,
-// d = 64, 4 sinks 17.0, 26.9 and 11.6, 21.0, 8 x 1024, d = 128 32.7, 54.3 and 29.9, 48.5; fp32 8 x 4096, d = 128, 4 sinks 439, 1192 and 411, 1176.
-inline bool sinks_ride(const AttnParams& p, int parts, int bytes, bool bit16, int small) {
-  return parts > 1 && (bit16 ? small || p.d == 64 : split_bwd_waves(p, bytes) != 0);
+// d = 64, 4 sinks 17.0, 26.9 and 11.6, 21.0, 8 x 1024, d = 128 32.7, 54.3 and 29.9, 48.5; one part: 30 x 75 x 115, fp32, d = 64 21.5, 46.9
+// and 13.9, 33.5, 8 x 36 x 79, fp16, d = 64 11.4, 19.3 and 11.2, 16.2; fp32 8 x 4096, d = 128, 4 sinks 439, 1192 and 411, 1176.
+inline bool sinks_ride(const AttnParams& p, int bytes, bool bit16, int small) {
+  return sink_groups(p.batch, p.sinks) <= 256 && (bit16 ? small || p.d == 64 : split_bwd_waves(p, bytes) != 0);
 }
 inline bool sinks_ride(const Params& p, int bytes, bool bit16, int small) {
-  return p.n_split_s > 1 && (bit16 ? small || p.d == 64 : !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0);
+  return sink_groups(p.batch, p.sinks) <= 256 && (bit16 ? small || p.d == 64 : !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0);
 }
 
 }  // namespace rules

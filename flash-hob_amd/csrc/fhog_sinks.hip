@@ -137,7 +137,7 @@ hipError_t launch_sink_keys(const AttnParams& p, int dtype, bool swept, hipStrea
   sinks_alone(a);
   const bool bit16 = dtype != FHOG_DTYPE_FP32 && p.d != 32;
   const hipError_t e = swept ? hipSuccess : bit16 ? launch_small_sink_bwd(a, s) : launch_attn_split_parts(a, dtype, true, s);
-  if (e != hipSuccess || a.n_split == 1) return e;
+  if (e != hipSuccess || !a.part) return e;
   return launch_add({a.part, a.dk, a.dv, a.stride_kb, a.stride_kn, a.n_split, a.batch, a.n_k, a.d, a.scale}, dtype, s);
 }
 
@@ -145,7 +145,7 @@ hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, boo
   Params a = p;
   sinks_alone(a);
   const hipError_t e = swept ? hipSuccess : split_products ? launch_split_sink_grads(a, dtype, s) : launch_small_sink_grads(a, s);
-  if (e != hipSuccess || a.n_split == 1) return e;
+  if (e != hipSuccess || !a.part) return e;
   return launch_add({a.part, a.dk2, a.dv2, a.stride_kb, a.stride_kn, a.n_split, a.batch, a.n_k, a.d, a.scale}, dtype, s);
 }
 

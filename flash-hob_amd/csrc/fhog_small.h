@@ -174,7 +174,7 @@ __device__ __forceinline__ void grads_k(const Params& p, char* smem, int id) {
   f32x4_t out[2 * NC][4 / W];
   add_waves<W>(acc, smem, group, ws, lane, out);
   if (kj >= p.n_k) return;
-  if (PARTS && p.n_split > 1) {
+  if (PARTS && p.part) {
     float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + kj) * D;
     store_partial<NC, 4 / W>(to, out, ws, h);
     store_partial<NC, 4 / W>(to + (int64_t)p.batch * p.n_k * D, out + NC, ws, h);
@@ -255,7 +255,7 @@ __device__ __forceinline__ void bwd_k(const AttnParams& p, char* smem, int id) {
   f32x4_t out[2 * NC][4 / W];
   add_waves<W>(all, smem, group, ws, lane, out);
   if (kj >= p.n_k) return;
-  if (PARTS && p.n_split > 1) {
+  if (PARTS && p.part) {
     float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + kj) * D;
     store_partial<NC, 4 / W>(to, out, ws, h);
     store_partial<NC, 4 / W>(to + (int64_t)p.batch * p.n_k * D, out + NC, ws, h);

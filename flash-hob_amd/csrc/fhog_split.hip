@@ -510,7 +510,7 @@ __device__ __forceinline__ void split_run(const Params& p, char* smem, int id, b
     }
   } else {
     if (ri >= n_sta) return;
-    if (PARTS && p.n_split > 1) {
+    if (PARTS && p.part) {
       float* const to = p.part + ((int64_t)part * 2 * p.batch * p.n_k + (int64_t)bh * p.n_k + ri) * D;
       store_rows<float, D>(to, acc0, 1.f, h);
       store_rows<float, D>(to + (int64_t)p.batch * p.n_k * D, acc1, 1.f, h);
