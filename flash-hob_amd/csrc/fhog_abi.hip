@@ -433,7 +433,7 @@ int fhog_attn_fwd_sinks(const fhog_attn_args* args, int64_t sinks, void* ws, int
     p.n_split = parts, p.part = (float*)ws;
     e = bit16 ? fhog::launch_small_fwd_parts(p, s) : fhog::launch_attn_split_parts(p, args->dtype, false, s);
     if (e == hipSuccess && parts > 1) e = fhog::launch_join_forward(p, args->dtype, s);
-  } else if (const int small = bit16 ? small_waves(Small::forward, args) : 0) {
+  } else if (const int small = bit16 ? sink_small_waves(Small::forward, args) : 0) {
     e = fhog::launch_small_attn(p, false, small, s);
   } else {
     e = bit16 ? fhog::launch_attn_bf16(p, 0, s) : fhog::launch_attn_split(p, args->dtype, false, s);
@@ -454,7 +454,7 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
   const int parts = sink_parts(args->batch, n, args->n_q, args->d, dtype_bytes(args->dtype), false);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
   const bool bit16 = attn_on_16bit_kernels(args);
-  const int small = bit16 ? small_waves(Small::backward, args) : 0;
+  const int small = bit16 ? sink_small_waves(Small::backward, args) : 0;
   const bool swept = fhog::rules::sinks_ride(p, dtype_bytes(args->dtype), bit16, small);
   hipError_t e = hipSuccess;
   if (bit16 && !small) e = fhog::launch_attn_bf16(p, 1, s);
@@ -491,7 +491,7 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
   fhog::Params p = to_params(&a);
   p.sinks = n, p.n_split_s = sink_parts(a.batch, n, a.n_q, a.d, dtype_bytes(a.dtype), true);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + a.ws_bytes);
-  const int small = impl == FHOG_IMPL_BF16 ? small_waves(Small::double_backward, args->batch, args->n_q, args->n_k, args->d, args->causal, args->window) : 0;
+  const int small = impl == FHOG_IMPL_BF16 ? sink_small_waves(Small::double_backward, args) : 0;
   const bool swept = fhog::rules::sinks_ride(p, dtype_bytes(a.dtype), impl == FHOG_IMPL_BF16, small);
   if (swept) p.part_s = part;
   hipError_t e = hipSuccess;

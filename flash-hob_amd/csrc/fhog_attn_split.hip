@@ -452,10 +452,22 @@ hipError_t launch_bwd_ws(const AttnParams& p, hipStream_t s, bool mixed = false)
   return hipGetLastError();
 }
 
+template <typename T, int D, int MODE, int MASK>
+hipError_t launch_side(const AttnParams& p, int waves, hipStream_t s) {
+  if constexpr (lds_bytes<T, D, MODE, 4>() <= 160 * 1024) {
+    if (waves == 4) return launch_ws<T, D, MODE, MASK, 4>(p, s);
+  }
+  return waves >= 2 ? launch_ws<T, D, MODE, MASK, 2>(p, s) : launch_ws<T, D, MODE, MASK, 1>(p, s);
+}
+
 // As in fhog_split.hip: four waves on 128 rows when that fills the GPU, two or four on the same 32 rows when it does not.
 template <typename T, int D, int MASK>
 hipError_t launch_fwd(const AttnParams& p, hipStream_t s) {
   const int64_t groups = (int64_t)(p.n_q + 127) / 128 * p.batch;
+  if constexpr (MASK == MASK_SINK) {
+    const int waves = p.n_k > 2 * TS ? rules::sink_forward_waves(groups, D, sizeof(T), p.window) : 0;
+    if (waves > 1) return launch_side<T, D, MODE_FWD, MASK>(p, waves, s);
+  }
   if constexpr (lds_bytes<T, D, MODE_FWD, 4>() <= 160 * 1024) {
     if (groups < 64 && p.n_k > 2 * TS) return launch_ws<T, D, MODE_FWD, MASK, 4>(p, s);
   }
@@ -464,14 +476,6 @@ hipError_t launch_fwd(const AttnParams& p, hipStream_t s) {
     if (rules::two_forwards_on_a_cu(groups, MASK != MASK_NONE)) return launch_ws<T, D, MODE_FWD, MASK, 1, true>(p, s);
   }
   return launch_ws<T, D, MODE_FWD, MASK, 1>(p, s);
-}
-
-template <typename T, int D, int MODE, int MASK>
-hipError_t launch_side(const AttnParams& p, int waves, hipStream_t s) {
-  if constexpr (lds_bytes<T, D, MODE, 4>() <= 160 * 1024) {
-    if (waves == 4) return launch_ws<T, D, MODE, MASK, 4>(p, s);
-  }
-  return waves >= 2 ? launch_ws<T, D, MODE, MASK, 2>(p, s) : launch_ws<T, D, MODE, MASK, 1>(p, s);
 }
 
 // dQ and dK, dV side by side fill CUs for each other, as passes 3 and 4 do in fhog_split.hip, and the rule for waves on the same rows is of

@@ -342,6 +342,50 @@ inline int32_t sinks_of(int64_t sinks, int64_t window, int64_t n_k) {   // a win
   if (window == 0 || window >= n_k) return 0;
   return (int32_t)(sinks < n_k ? sinks : n_k);
 }
+// small_waves under such a mask, whose windows are short: 2 waves on the same rows for more launches. us, by the rule above -> here, bf16, 4 sinks:
+//   forward         d = 64: 24 x 1024, window 256 15.2 -> 10.7, 8 x 4096, 1024 30.0 -> 21.5, 40 x 400, 50 10.4 -> 7.5; as good from 400 groups on. d = 128: 4 x 4096, 1024 27.4 -> 22.9
+//   first backward  8 x 1024, 256 d = 64 19.5 -> 16.2, d = 128 30.6 -> 23.4; 4 x 2048, 1024 (left at 4) 26.3, with 2 28.0; d = 64: 10 x 2048, 512 43.9 -> 38.1, 16 x 1000 x 3001, 700
+//                   55 -> 45, 32 x 1024, 256 (left) 35.7, 41.0; d = 128: 60 x 300, 20 37.0 -> 32.2, 5 x 4096, 64 (left) 39.4, 44.3
+//   second          8 x 1024, 256 d = 64 32.7 -> 30.1, d = 128 49.4 -> 46.1; d = 128: 12 x 1024, 64 52.7 -> 43.7, 20 x 1024, 128 87.5 -> 78.4, 5 x 4096, 512 (left) 135, 155
+inline int sink_small_waves(Small what, int64_t batch, int64_t n_q, int64_t n_k, int64_t d, int32_t causal, int64_t window) {
+  const int64_t g_q = (n_q + 127) / 128 * batch, g_k = (n_k + 127) / 128 * batch, groups = g_q + g_k, least = g_q < g_k ? g_q : g_k;
+  const int64_t tiles = (window + 63 + 31) / 32;
+  if (tuning().small < 0) {
+    if (what == Small::forward) {
+      if (n_k > 64 && (d == 64 ? g_q > 128 && g_q < 400 : g_q > 64 && g_q <= 128)) return 2;
+    } else if (what == Small::backward) {
+      if (groups <= 128) return tiles <= 24 ? 2 : 4;
+      if (d == 64 ? groups <= 400 || (least <= 128 && groups <= 512) : groups <= 360 && tiles <= 3) return 2;
+    } else {
+      if (groups <= 128 && tiles <= 12) return 2;
+      if (d == 128 && (groups <= 200 ? tiles <= 10 : groups <= 384 && tiles <= 6)) return 2;
+    }
+  }
+  return small_waves(what, batch, n_q, n_k, d, causal, window);
+}
+template <typename Args>
+int sink_small_waves(Small what, const Args* a) { return sink_small_waves(what, a->batch, a->n_q, a->n_k, a->d, a->causal, a->window); }
+// Waves on the same 32 rows in the split products' forwards and statistics sweeps under such a mask, at so many groups of 128 rows; 0: by the rule for other masks
+// (16-bit tensors of d = 64, 128, which were not measured). A workgroup streams a short window, so that several waves to a row tile fill the CUs for longer. us, by that
+// rule -> here, window 256:
+//   forward      fp32 d = 64 16 x 1024 28.7 -> 19.2, 32 x 1024 27.6 -> 26.3, 64 x 1024 (left at 1) 41.6, with 2 43.5; d = 32 24 x 1024 20.6 -> 15.9, 96 x 1024 36.9 -> 34.6, 128 x 1024 (left)
+//                39.6, 41.2; d = 128 16 x 1024 53.1 -> 33.2, 24 x 1024 (left) 51.0, 63.2; bf16 d = 32 32 x 1024 14.9 -> 10.1, 96 x 1024 23.6 -> 17.8, 256 x 1024 40.4 -> 39.1
+//   double-backward with the sweep  fp32 d = 64 16 x 1024 148 -> 133, 24 x 1024 (left) 180, 195; d = 32 16 x 1024 90 -> 79, 32 x 1024 (left) 102, 106; d = 128
+//                16 x 1024 321 -> 287, 32 x 1024 (left) 478, 496; bf16 d = 32 16 x 1024 50 -> 42, 32 x 1024 52 -> 47, 64 x 1024 (left) 82.9, 84.5
+// Windows of a tile or so keep four waves of an fp32 row tile less busy than two: forward d = 32 100 x 100, window 10 6.8, with 4 8.3.
+inline int sink_forward_waves(int64_t groups, int d, int bytes, int64_t window) {
+  if (bytes == 2) return d != 32 ? 0 : groups <= 384 ? 4 : 2;
+  if (window <= 32) return 0;
+  if (d == 32) return groups <= 192 ? 4 : groups < 1024 ? 2 : 1;
+  if (d == 64) return groups <= 64 ? 4 : groups <= 256 ? 2 : 1;
+  return groups <= 128 ? 2 : 1;
+}
+inline int sink_sweep_waves(int64_t groups, int d, int bytes, int64_t window) {
+  if (bytes == 2) return d != 32 ? 0 : groups <= 384 ? 4 : 1;
+  if (window <= 32) return 0;
+  if (d == 64) return groups <= 64 ? 4 : groups <= 128 ? 2 : 1;
+  return groups < (d == 32 ? 192 : 256) ? 4 : 1;
+}
 // Workgroups that share 32 sinks of a slice, each with a part of the queries: one for every CU, with a tile for each of its waves at least.
 // First | second backward, us, 512 workgroups of eight tiles -> 256 of four: bf16 32 x 4096, d = 128, window 1024, 4 sinks 290 | 678 -> 282 | 675; fp32 16 x 1024, d = 64,
 // window 256, 33 sinks 64.9 | 153 -> 61.7 | 149; 8 x 4096, d = 128 448 | 1401 -> 440 | 1357; 1024 of four 296 | 686, 61.7 | 148, 440 | 1358.

@@ -604,6 +604,14 @@ template <typename T, int D, int PASS, int MASK>
 hipError_t launch_sweep(const Params& p, hipStream_t s) {
   const int64_t groups = (int64_t)(p.n_q + 127) / 128 * p.batch;
   const bool triangle = MASK != MASK_NONE && p.mask_off == 0 && p.window >= p.n_k;
+  if constexpr (MASK == MASK_SINK) {
+    const int waves = p.n_k > 2 * TS ? rules::sink_sweep_waves(groups, D, sizeof(T), p.window) : 0;
+    if (waves == 4) return launch_ws<T, D, PASS, MASK, 4>(p, s);
+    if constexpr (lds_bytes<T, D, PASS, 2>() <= 160 * 1024) {
+      if (waves == 2) return launch_ws<T, D, PASS, MASK, 2>(p, s);
+    }
+    if (waves) return launch_ws<T, D, PASS, MASK, 1>(p, s);
+  }
   constexpr bool splits_dear = sizeof(T) == 4 && D < 128;
   const int64_t line = triangle ? (splits_dear ? 160 : 256) : splits_dear ? 64 : 128;
   if (groups < line && p.n_k > 2 * TS) return launch_ws<T, D, PASS, MASK, 4>(p, s);
