@@ -238,8 +238,8 @@ fhog::AttnParams to_attn_params(const fhog_attn_args* a) {
   return p;
 }
 
-// Sinks of a mask, or the error for a number that is none
 int dtype_bytes(int dtype) { return dtype == FHOG_DTYPE_FP32 ? 4 : 2; }
+// Sinks of a mask, or the error for a number that is none
 int check_sinks(int64_t sinks) { return sinks < 0 ? fail(FHOG_E_CAUSAL, "sinks must be >= 0 (got %lld)", (long long)sinks) : FHOG_OK; }
 int32_t sinks_of(const fhog_attn_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }
 int32_t sinks_of(const fhog_bwdbwd_args* a, int64_t sinks) { return fhog::rules::sinks_of(sinks, a->window, a->n_k); }

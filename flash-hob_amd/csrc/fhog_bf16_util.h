@@ -301,7 +301,7 @@ struct StreamKeys {
   }
 };
 // StreamQueries: stationary rows are keys, streamed tiles are queries (pass 4, dK and dV). MASK_SINK: the band alone; the rows of the sinks, which the
-// queries behind it see too, are put in their place by a launch of their own (fhog_small.hip, fhog_split.hip, fhog_attn_split.hip).
+// queries behind it see too, are put in their place afterwards (fhog_sinks.hip).
 template <int MASK>
 struct StreamQueries {
   static constexpr bool WINDOW = MASK == MASK_BAND || MASK == MASK_SINK;

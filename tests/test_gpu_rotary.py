@@ -239,6 +239,17 @@ def test_rotary_and_attention_differentiated_twice(n_q, n_k, causal, window, sin
         assert normalised_max_error(a, b) <= gate, name
 
 
+def test_offsets_beyond_32_bits():
+    """Rows far apart in a tensor of more than 2^31 elements."""
+    import fhog
+    n, d, ld = 17000, 64, 1 << 17
+    assert n * ld > 2 ** 31
+    far = torch.zeros(1, n, ld, dtype=torch.bfloat16, device="cuda")[:, :, :d]
+    far.copy_(torch.randn(1, n, d, device="cuda"))
+    pos = torch.arange(n, device="cuda")
+    assert torch.equal(fhog.rotary(far, None, pos), fhog.rotary(far.contiguous(), None, pos))
+
+
 def test_other_streams_and_captured_graphs():
     """Rotary and attention, first backward included, on a side stream and captured: every replay has the bits of the eager call, on new
     inputs and positions too, while an eager graph of the same leaves lives."""

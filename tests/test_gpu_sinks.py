@@ -63,7 +63,8 @@ def test_all_orders_against_the_formulas(shape, causal, window, sinks, d, dtype)
 LARGE = [((40, 900, 900), True, 150, 5), ((33, 1024, 1024), True, 300, 70), ((104, 1100, 1100), True, 64, 4), ((24, 1000, 1700), "bottom_right", 500, 33),
          ((1, 3000, 3000), True, 1500, 70), ((2, 2500, 4000), "bottom_right", 2000, 4), ((6, 1537, 1537), True, 400, 100),
          ((1, 100, 5000), "bottom_right", 4096, 4), ((2, 70, 3000), "bottom_right", 2500, 33), ((3, 1, 9000), "bottom_right", 8192, 64),
-         ((300, 2, 500), "bottom_right", 300, 4)]
+         ((300, 2, 500), "bottom_right", 300, 4), ((300, 130, 200), "bottom_right", 50, 40), ((270, 260, 260), True, 31, 3),
+         ((20, 75, 115), "bottom_right", 19, 1)]
 
 
 @pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 64), (torch.float16, 128), (torch.float32, 32), (torch.float32, 64),
@@ -247,6 +248,59 @@ def test_padded_rows_and_what_lies_between_them(dtype, d):
         assert torch.equal(t[:, :n, :d], ref[name]), name
     for name, (t, n) in room.items():
         assert (t[:, n:] == 7).all() and (t[:, :, d:] == 7).all(), name
+
+
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 128), (torch.float32, 64)])
+def test_offsets_beyond_32_bits(dtype, d):
+    """Three queries behind a cache of more than 2^31 elements: the few keys that they see, and zeros in the gradients of the others."""
+    n_q, n_k, window, sinks, ld = 3, 1 << 24, 1000, 5, 132
+    assert n_k * ld > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(41)
+    near = torch.cat([torch.arange(sinks), torch.arange(n_k - window - n_q + 1, n_k)]).cuda()
+    rows = lambda n: torch.randn(1, n, d, generator=g, device="cuda").to(dtype)   # noqa: E731
+    q, do, ddq = rows(n_q), rows(n_q), rows(n_q)
+    small = [rows(len(near)) for _ in range(4)]
+    wide = ld if dtype == torch.float32 else ld + 4   # rows of a multiple of 16 bytes
+    big = []
+    for t in small:
+        c = torch.zeros(1, n_k, wide, dtype=dtype, device="cuda")[:, :, :d]
+        c[:, near] = t
+        big.append(c)
+    k, v, ddk, ddv = big
+    got = _all_orders((q, k, v, do, ddq, ddk, ddv), d ** -0.5, "bottom_right", window, sinks)
+    at = torch.arange(n_k - n_q, n_k, device="cuda")[:, None]
+    seen = (near[None] <= at) & ((at - near[None] < window) | (near[None] < sinks))
+    k, v, ddk, ddv = small
+    ref = attention_with_bounds(q, k, v, do, ddq, ddk, ddv, d ** -0.5, seen)
+    for name, t in got.items():
+        if name in ("dk", "dv", "dk2", "dv2"):
+            assert not t[:, sinks:n_k - window - n_q + 1].any(), name
+            t = t[:, near]
+        assert_within(t, ref[name], name)
+
+
+def test_two_streams_at_a_time():
+    """The same calls on two streams, nothing waited for in between: either has its own workspaces and its own results."""
+    sizes = [(torch.bfloat16, 64, (40, 300, 300), 50, 4), (torch.float32, 128, (2, 5, 3000), 2500, 33), (torch.bfloat16, 128, (8, 900, 900), 100, 40)]
+    runs = []
+    for i, (dtype, d, (batch, n_q, n_k), window, sinks) in enumerate(sizes):
+        x = [_inputs(batch, n_q, n_k, d, dtype, 60 + 2 * i + j) for j in (0, 1)]
+        runs.append([(lambda t=t, d=d, w=window, s=sinks: _all_orders(t, d ** -0.5, "bottom_right", w, s)) for t in x])
+    want = [[f() for f in pair] for pair in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for pair in runs:
+            got.append([])
+            for stream, f in zip(streams, pair):
+                with torch.cuda.stream(stream):
+                    got[-1].append(f())
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            for x, y in zip(a, b):
+                for name in x:
+                    assert torch.equal(x[name], y[name]), name
 
 
 def test_other_streams_and_captured_graphs():
