@@ -419,7 +419,10 @@ std::optional<tensor_list> rotary(const Tensor& q, const std::optional<Tensor>& 
   for (const Tensor* t : {&q, k ? &*k : &q, &positions})
     if (t->unsafeGetTensorImpl()->is_python_dispatch()) return std::nullopt;
   const Turn turn{theta, rotary_dim, interleaved, false, std::move(sections)};
-  if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k && k->requires_grad()))) {
+  // Who asks for a derivative, backwards or forwards, gets the node, which refuses what it does not have, a tangent: dual tensors require no gradient
+  bool dual = false;
+  for (const Tensor* t : {&q, k ? &*k : &q, &positions}) dual = dual || t->_fw_grad(0).defined();
+  if (!dual && (!at::GradMode::is_enabled() || !(q.requires_grad() || (k && k->requires_grad())))) {
     const at::NoGradGuard no_grad;
     return rotary_call(q, k ? *k : Tensor(), positions, turn);
   }

@@ -296,3 +296,27 @@ def test_other_streams_and_captured_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(captured, want)), rep
+
+
+def test_forward_mode_and_transforms_are_refused_by_name():
+    """Dual tensors and torch.func transforms, alone and in front of attention: refused, never a result without its derivative."""
+    import fhog
+    import torch.autograd.forward_ad as fwAD
+    q, k, v = (torch.randn(2, 3, 40, 64, device="cuda") for _ in range(3))
+    p, one = torch.arange(40, device="cuda").float(), torch.ones_like(q)
+    turn = fhog.Rotary(p)
+    leaf = k.clone().requires_grad_(True)
+    with fwAD.dual_level():
+        dq, dk, dp = fwAD.make_dual(q, one), fwAD.make_dual(k, one), fwAD.make_dual(p, torch.ones_like(p))
+        for f in (lambda: fhog.rotary(dq, k, p), lambda: fhog.rotary(q, dk, p), lambda: fhog.rotary(dq, None, p), lambda: fhog.rotary(q, k, dp),
+                  lambda: fhog.rotary(dq, leaf, p), lambda: fhog.rotary(q, leaf, dp), lambda: fhog.attention(dq, k, v, True, rotary=turn),
+                  lambda: fhog.attention(q, dk, v, True, 9, sinks=2, rotary=turn), lambda: fhog.attention(q[:, :, :7], dk, v, "bottom_right", rotary=turn)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="(?i)forward AD|jvp"):
+                    f()
+        assert fwAD.unpack_dual(fhog.rotary(q, k, p)[0]).tangent is None
+    for f in (lambda: torch.func.grad(lambda a: fhog.rotary(a, k, p)[0].sum())(q), lambda: torch.func.vmap(lambda a: fhog.rotary(a, k, p))(q[None]),
+              lambda: torch.func.jvp(lambda a: fhog.rotary(a, k, p), (q,), (one,)), lambda: torch.func.grad(lambda a: (fhog.rotary(q, None, p) * a).sum())(q),
+              lambda: torch.func.grad(lambda a: fhog.attention(a, k, v, True, rotary=turn).sum())(q)):
+        with pytest.raises(RuntimeError, match="setup_context"):
+            f()
