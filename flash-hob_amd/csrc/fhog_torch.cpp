@@ -419,15 +419,17 @@ std::optional<tensor_list> rotary(const Tensor& q, const std::optional<Tensor>& 
   for (const Tensor* t : {&q, k ? &*k : &q, &positions})
     if (t->unsafeGetTensorImpl()->is_python_dispatch()) return std::nullopt;
   const Turn turn{theta, rotary_dim, interleaved, false, std::move(sections)};
-  // Who asks for a derivative, backwards or forwards, gets the node, which refuses what it does not have, a tangent: dual tensors require no gradient
-  bool dual = false;
-  for (const Tensor* t : {&q, k ? &*k : &q, &positions}) dual = dual || t->_fw_grad(0).defined();
-  if (!dual && (!at::GradMode::is_enabled() || !(q.requires_grad() || (k && k->requires_grad())))) {
+  // Who asks for a derivative, backwards or forwards, gets the node, which refuses what it does not have: a tangent (dual tensors require no gradient)
+  // and, by the caller, a gradient of the positions
+  bool reverse = false, dual = false;
+  for (const Tensor* t : {&q, k ? &*k : &q, &positions}) reverse = reverse || t->requires_grad(), dual = dual || t->_fw_grad(0).defined();
+  reverse = reverse && at::GradMode::is_enabled();
+  if (!reverse && !dual) {
     const at::NoGradGuard no_grad;
     return rotary_call(q, k ? *k : Tensor(), positions, turn);
   }
   fhog_rotary_args a;
-  if (positions.requires_grad() || !rotary_args(q, k ? *k : Tensor(), positions, turn, a)) return std::nullopt;
+  if ((reverse && positions.requires_grad()) || !rotary_args(q, k ? *k : Tensor(), positions, turn, a)) return std::nullopt;
   return RotaryNode::apply(q, k, positions, turn);
 }
 

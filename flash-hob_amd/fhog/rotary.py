@@ -49,7 +49,7 @@ def _check(q, k, positions, sections, theta, rotary_dim) -> Tuple[int, ...]:
         raise ValueError(f"theta must be a positive number, got {theta!r}")
     if positions.dtype not in _POSITIONS:
         raise TypeError(f"positions have dtype {positions.dtype}; expected torch.int32, torch.int64 or torch.float32")
-    if positions.requires_grad:
+    if positions.requires_grad and torch.is_grad_enabled():
         raise ValueError("positions are constants: no gradient is formed for them")
     axes, n, batch = len(sections), q.shape[-2], q.shape[0]
     lead = () if axes == 1 else (axes,)

@@ -320,3 +320,16 @@ def test_forward_mode_and_transforms_are_refused_by_name():
               lambda: torch.func.grad(lambda a: fhog.attention(a, k, v, True, rotary=turn).sum())(q)):
         with pytest.raises(RuntimeError, match="setup_context"):
             f()
+
+
+def test_positions_have_no_gradient():
+    """Positions that ask for one are refused, whether queries or keys ask or not; where nobody records, they are numbers like others."""
+    import fhog
+    q = torch.randn(2, 3, 40, 64, device="cuda")
+    p = torch.arange(40, device="cuda").float().requires_grad_(True)
+    for leaf in (q, q.clone().requires_grad_(True)):
+        for f in (lambda: fhog.rotary(leaf, None, p), lambda: fhog.rotary(q, leaf, p), lambda: fhog.attention(leaf, q, q, True, rotary=fhog.Rotary(p))):
+            with pytest.raises(ValueError, match="constants"):
+                f()
+    with torch.no_grad():
+        assert torch.equal(fhog.rotary(q, None, p), fhog.rotary(q, None, p.detach()))
