@@ -18,6 +18,11 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torc
 _POSITIONS = {torch.int32: _lib.POSITIONS_INT32, torch.int64: _lib.POSITIONS_INT64, torch.float32: _lib.POSITIONS_FP32}
 
 
+def _sizes(t) -> Tuple[int, ...]:
+    """The shape in numbers; under torch.jit.trace ``t.shape`` holds tensors."""
+    return tuple(int(n) for n in t.shape)
+
+
 def _check(q, k, positions, sections, theta, rotary_dim) -> Tuple[int, ...]:
     """Raises on what the kernel does not take, the messages name the argument; returns the frequencies of each axis."""
     for name, t in (("q", q), ("positions", positions)) + ((("k", k),) if k is not None else ()):
@@ -25,17 +30,18 @@ def _check(q, k, positions, sections, theta, rotary_dim) -> Tuple[int, ...]:
             raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if q.dim() not in (3, 4):
         raise ValueError(f"q: expected a 3-D (batch, N, d) or 4-D (B, H, N, d) tensor, got shape {tuple(q.shape)}")
+    size_q, size_k, size_p = _sizes(q), None if k is None else _sizes(k), _sizes(positions)
     if q.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {q.dtype}; expected torch.bfloat16, torch.float16 or torch.float32")
     if k is not None:
         if k.dtype != q.dtype:
             raise TypeError(f"k has dtype {k.dtype}, expected {q.dtype} like q")
-        if k.dim() != q.dim() or k.shape[0] != q.shape[0] or k.shape[-2:] != q.shape[-2:]:
-            raise ValueError(f"k has shape {tuple(k.shape)}: apart from the number of heads it has to be {tuple(q.shape)} like q")
-    heads = q.shape[1] if q.dim() == 4 else 1, 1 if k is None else k.shape[1] if k.dim() == 4 else 1
+        if k.dim() != q.dim() or size_k[0] != size_q[0] or size_k[-2:] != size_q[-2:]:
+            raise ValueError(f"k has shape {size_k}: apart from the number of heads it has to be {size_q} like q")
+    heads = size_q[1] if q.dim() == 4 else 1, 1 if k is None else size_k[1] if k.dim() == 4 else 1
     if min(heads) < 1 or sum(heads) > 65535:
         raise ValueError(f"{heads[0]} and {heads[1]} heads: expected 1 or more, and 65535 or fewer in all")
-    d = q.shape[-1]
+    d = size_q[-1]
     if d < 2 or d > _lib.ROTARY_MAX_D or d % 2:
         raise ValueError(f"head dim {d} not supported (an even number in 2..{_lib.ROTARY_MAX_D})")
     if isinstance(rotary_dim, bool) or not isinstance(rotary_dim, int) or rotary_dim < 2 or rotary_dim > d or rotary_dim % 2:
@@ -51,10 +57,10 @@ def _check(q, k, positions, sections, theta, rotary_dim) -> Tuple[int, ...]:
         raise TypeError(f"positions have dtype {positions.dtype}; expected torch.int32, torch.int64 or torch.float32")
     if positions.requires_grad and torch.is_grad_enabled():
         raise ValueError("positions are constants: no gradient is formed for them")
-    axes, n, batch = len(sections), q.shape[-2], q.shape[0]
+    axes, n, batch = len(sections), size_q[-2], size_q[0]
     lead = () if axes == 1 else (axes,)
-    if tuple(positions.shape) not in {lead + (n,), lead + (batch, n), lead + (1, n)}:
-        raise ValueError(f"positions have shape {tuple(positions.shape)}, expected {lead + (n,)} or {lead + (batch, n)}")
+    if size_p not in {lead + (n,), lead + (batch, n), lead + (1, n)}:
+        raise ValueError(f"positions have shape {size_p}, expected {lead + (n,)} or {lead + (batch, n)}")
     for name, t in (("q", q), ("k", k), ("positions", positions)):
         if t is not None and (not t.is_cuda or t.device != q.device):
             raise ValueError(f"{name} is on {t.device}: rotary runs on the GPU only, on one device (there is no CPU path)")
@@ -71,12 +77,12 @@ def _turn(q, k, positions, sections, theta, rotary_dim, interleaved, inverse):
             continue
         setattr(a, x, t.data_ptr())
         setattr(a, x + "_out", out.data_ptr())
-        setattr(a, "heads_" + x, t.shape[1] if t.dim() == 4 else 1)
+        setattr(a, "heads_" + x, int(t.shape[1]) if t.dim() == 4 else 1)
         for s, of in ((f"stride_{x}", t), (f"stride_{x}o", out)):
             setattr(a, s + "b", of.stride(0))
             setattr(a, s + "h", of.stride(1) if t.dim() == 4 else 0)
             setattr(a, s + "n", of.stride(-2))
-    a.batch, a.n, a.d, a.rotary_dim = q.shape[0], q.shape[-2], q.shape[-1], rotary_dim
+    a.batch, a.n, a.d, a.rotary_dim = int(q.shape[0]), int(q.shape[-2]), int(q.shape[-1]), rotary_dim
     a.positions, a.position_type = positions.data_ptr(), _POSITIONS[positions.dtype]
     lead = 1 if len(sections) > 1 else 0
     a.stride_pa = positions.stride(0) if lead else 0
@@ -131,7 +137,7 @@ def rotary(q, k, positions, *, sections: Optional[Sequence[int]] = None, theta: 
     """
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
-    rotary_dim = (q.shape[-1] if q.dim() else 0) if rotary_dim is None else rotary_dim
+    rotary_dim = (int(q.shape[-1]) if q.dim() else 0) if rotary_dim is None else rotary_dim
     try:
         res = _lib.torch_ext().rotary(q, k, positions, [rotary_dim // 2] if sections is None else sections, theta, rotary_dim, bool(interleaved))
     except TypeError:   # not tensors or numbers: named below

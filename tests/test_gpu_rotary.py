@@ -333,3 +333,29 @@ def test_positions_have_no_gradient():
                 f()
     with torch.no_grad():
         assert torch.equal(fhog.rotary(q, None, p), fhog.rotary(q, None, p.detach()))
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("how", [dict(), dict(rotary_dim=32, sections=(6, 10), interleaved=True)])
+def test_traced_module_computes_on_new_inputs(how, requires_grad):
+    """torch.jit.trace: the rotation of queries and keys, of queries alone and in front of attention, on new inputs and positions and, where
+    the inputs ask for it, differentiated."""
+    import fhog
+    g = torch.Generator(device="cuda").manual_seed(31)
+    axes = len(how.get("sections", (0,)))
+    mk = lambda h: torch.randn(2, h, 33, 64, generator=g, device="cuda").requires_grad_(requires_grad)   # noqa: E731
+    lead = () if axes == 1 else (axes,)
+    pos = lambda: torch.randint(0, 900, (*lead, 2, 33), generator=g, device="cuda")                      # noqa: E731
+    fs = (lambda q, k, p: fhog.rotary(q, k, p, **how), lambda q, k, p: (fhog.rotary(q, None, p, **how), k * 2),
+          lambda q, k, p: (fhog.attention(q, k, k, True, 9, sinks=2, rotary=fhog.Rotary(p, **how)), k * 2),
+          lambda q, k, p: (fhog.attention(q[:, :, 20:], k, k, "bottom_right", rotary=fhog.Rotary(p, **how)), k * 2))
+    for f, heads in zip(fs, (1, 1, 3, 3)):
+        traced = torch.jit.trace(f, (mk(3), mk(heads), pos()), check_trace=False)
+        q, k, p = mk(3), mk(heads), pos()
+        got, want = traced(q, k, p), f(q, k, p)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b) and a.requires_grad == requires_grad
+        if requires_grad:
+            w = [torch.randn(t.shape, generator=g, device="cuda") for t in want]
+            for a, b in zip(torch.autograd.grad(got, (q, k), w), torch.autograd.grad(want, (q, k), w)):
+                assert torch.equal(a, b)
