@@ -38,6 +38,10 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
+// False where the storage holds no memory: fake tensors, and storages that were resized to nothing. A view of one that starts behind its first
+// element has an address all the same, and it is no one's.
+bool in_memory(const Tensor& t) { return !t.has_storage() || t.numel() == 0 || t.storage().data() != nullptr; }
+
 // (batch, N, d) or (B, H, N, d) as the library sees it: batch = B * H slices sb elements apart, rows sn elements apart
 struct Layout {
   int64_t batch = 0, n = 0, d = 0, sb = 0, sn = 0;
@@ -341,6 +345,7 @@ bool positions_of(const Tensor& p, const Tensor& q, size_t axes, fhog_rotary_arg
 // addresses of the outputs, is filled in with those of the inputs.
 bool rotary_args(const Tensor& q, const Tensor& k, const Tensor& positions, const Turn& turn, fhog_rotary_args& a) {
   const int64_t dim = q.dim();
+  if (!in_memory(q) || !in_memory(positions) || (k.defined() && !in_memory(k))) return false;
   if (!q.is_cuda() || (dim != 3 && dim != 4) || turn.sections.empty() || turn.sections.size() > FHOG_ROTARY_MAX_AXES) return false;
   if (k.defined() && (!k.is_cuda() || k.device() != q.device() || k.scalar_type() != q.scalar_type() || k.dim() != dim || k.size(0) != q.size(0) ||
                       k.size(-1) != q.size(-1) || k.size(-2) != q.size(-2)))
@@ -452,6 +457,7 @@ PYBIND11_MODULE(_fhog_torch, m) {
     const at::NoGradGuard no_grad;
     return double_backward(q, k, v, o, g, ddq, ddk, ddv, L, scale, Mask{causal, window, sinks}, impl, schedule, split);
   }, free_lock);
+  m.def("in_memory", &in_memory, free_lock);
   m.def("attention", &attention, free_lock);
   m.def("rotary", &rotary, free_lock);
 }

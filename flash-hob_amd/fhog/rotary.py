@@ -11,6 +11,7 @@ from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
 
 from . import _lib
 
@@ -64,11 +65,20 @@ def _check(q, k, positions, sections, theta, rotary_dim) -> Tuple[int, ...]:
     for name, t in (("q", q), ("k", k), ("positions", positions)):
         if t is not None and (not t.is_cuda or t.device != q.device):
             raise ValueError(f"{name} is on {t.device}: rotary runs on the GPU only, on one device (there is no CPU path)")
+    fake = isinstance(q, FakeTensor)
+    if k is not None and isinstance(k, FakeTensor) != fake:
+        raise ValueError("one of q and k is a fake tensor, the other is not")
+    if not fake:
+        for name, t in (("q", q), ("k", k), ("positions", positions)):
+            if t is not None and not _lib.torch_ext().in_memory(t):
+                raise ValueError(f"{name} holds no memory (a fake tensor beside real ones, or a storage that was resized to nothing)")
     return sections
 
 
 def _turn(q, k, positions, sections, theta, rotary_dim, interleaved, inverse):
-    """The kernel through the C ABI, on arguments that :func:`_check` let pass."""
+    """The kernel through the C ABI, on arguments that :func:`_check` let pass; of fake tensors the shapes, without a launch."""
+    if isinstance(q, FakeTensor):
+        return [None if t is None else t.new_empty(t.shape) for t in (q, k)]
     a = _lib.RotaryArgs()
     q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (q, k))
     outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]

@@ -359,3 +359,26 @@ def test_traced_module_computes_on_new_inputs(how, requires_grad):
             w = [torch.randn(t.shape, generator=g, device="cuda") for t in want]
             for a, b in zip(torch.autograd.grad(got, (q, k), w), torch.autograd.grad(want, (q, k), w)):
                 assert torch.equal(a, b)
+
+
+def test_tensors_without_memory_are_not_launched_on():
+    """Fake tensors and views of them: shapes, first and second derivatives included. Storages that were resized to nothing: refused."""
+    import fhog
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    real = torch.randn(2, 3, 40, 64, device="cuda", dtype=torch.bfloat16)
+    p, mode = torch.arange(40, device="cuda"), FakeTensorMode()
+    with mode:
+        q, pos = mode.from_tensor(real), mode.from_tensor(p)
+    leaf, grad = q[:, :, 1:].detach().requires_grad_(True), q[:, :, 1:].detach().requires_grad_(True)
+    y = fhog.rotary(leaf, leaf, pos[1:])
+    first = torch.autograd.grad(y[0], leaf, grad, create_graph=True)[0]
+    second = torch.autograd.grad(first.float().sum(), grad)[0]
+    for t in (*y, first, second):
+        assert isinstance(t, FakeTensor) and t.shape == leaf.shape and t.dtype == leaf.dtype and t.device == leaf.device
+    gone = real.clone()
+    views = gone, gone[:, :, 1:]
+    gone.untyped_storage().resize_(0)
+    for f in (lambda: fhog.rotary(views[0], None, p), lambda: fhog.rotary(views[1], None, p[1:]), lambda: fhog.rotary(real[:, :, 1:], views[1], p[1:]),
+              lambda: fhog.rotary(views[1].detach().requires_grad_(True), None, p[1:]), lambda: fhog.rotary(real[:, :, 1:], None, pos[1:])):
+        with pytest.raises(ValueError, match="no memory"):
+            f()

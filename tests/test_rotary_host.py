@@ -90,3 +90,43 @@ def test_refusals_of_the_python_entry_points():
         fhog.attention(q, q, q, rotary=p)
     with pytest.raises(ValueError, match="queries"):
         fhog.Rotary(p)(q, k[:, :, :5])
+
+
+def test_fake_tensors_propagate_shapes_without_a_launch():
+    """Tensors without memory, views of them that start behind their first element too (those have an address, which is no one's), inside their
+    mode and outside: shapes and types of such, and nothing is launched; a mixture with real tensors is refused."""
+    import fhog
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    mode = FakeTensorMode()
+    with mode:
+        q, k = torch.empty(2, 4, 10, 16, device="cuda", dtype=torch.bfloat16), torch.empty(2, 1, 10, 16, device="cuda", dtype=torch.bfloat16)
+        p, p2 = torch.empty(10, device="cuda", dtype=torch.int64), torch.empty(2, 2, 10, device="cuda", dtype=torch.int64)
+
+    def everything():
+        for a, b, pos, how in ((q, k, p, {}), (q[:, :, 1:], k[:, :, 1:], p[1:], {}), (q, None, p2, dict(sections=(3, 5))), (q[1:], k[1:], p2[0, 1:], {}),
+                               (q[:, 0], k[:, 0], p, dict(rotary_dim=8, interleaved=True))):
+            y = fhog.rotary(a, b, pos, **how)
+            for t, like in zip(y if b is not None else (y,), (a, b)):
+                assert isinstance(t, FakeTensor) and t.shape == like.shape and t.dtype == like.dtype and t.device == like.device and t.is_contiguous()
+        with pytest.raises(ValueError, match="positions have shape"):
+            fhog.rotary(q, k, p[1:])
+
+    everything()
+    with mode:
+        everything()
+    with pytest.raises(ValueError, match="fake|no memory|on cpu"):
+        fhog.rotary(q, torch.zeros(2, 1, 10, 16, dtype=torch.bfloat16), p)
+
+
+def test_what_holds_memory():
+    from fhog import _lib
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    there = _lib.torch_ext().in_memory
+    x, y = torch.zeros(10), torch.zeros(10)
+    gone = y[2:]
+    y.untyped_storage().resize_(0)
+    with FakeTensorMode():
+        fake = torch.empty(10, device="cuda")
+        views = fake, fake[2:]
+    assert there(x) and there(x[2:]) and there(x[:0]) and there(torch.empty(0))
+    assert gone.data_ptr() and not any(there(t) for t in (y, gone, *views, torch.empty(3, device="meta")))
