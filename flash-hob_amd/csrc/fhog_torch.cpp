@@ -76,7 +76,7 @@ struct Group {
   bool set(const std::array<const Tensor*, N>& in, bool strict) {
     bool same = true;
     for (size_t i = 0; i < N; i++) {
-      if (!in[i]->defined() || !in[i]->is_cuda() || in[i]->scalar_type() != in[0]->scalar_type() || in[i]->device() != in[0]->device())
+      if (!in[i]->defined() || !in_memory(*in[i]) || !in[i]->is_cuda() || in[i]->scalar_type() != in[0]->scalar_type() || in[i]->device() != in[0]->device())
         return false;
       t[i] = *in[i];
       Layout x = layout_of(t[i]);
@@ -170,7 +170,7 @@ Backward backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Te
   Group<2> k;
   fhog_attn_args a;
   if (!q.set({&q_, &o_, &do_}, strict) || !k.set({&k_, &v_}, strict) || !attn_args(a, q, k, scale, m)) return std::nullopt;
-  if (!L.is_cuda() || L.device() != q_.device() || L.numel() != a.batch * a.n_q) return std::nullopt;
+  if (!in_memory(L) || !L.is_cuda() || L.device() != q_.device() || L.numel() != a.batch * a.n_q) return std::nullopt;
   const c10::DeviceGuard guard(q_.device());
   const Tensor lse = as_lse(L);
   Tensor dq = q.like(), dk = k.like(), dv = k.like();
@@ -193,7 +193,7 @@ DoubleBackward double_backward(const Tensor& q_, const Tensor& k_, const Tensor&
   Group<4> q, k;
   if (!q.set({&q_, &o_, &do_, &ddq_}, false) || !k.set({&k_, &v_, &ddk_, &ddv_}, false)) return std::nullopt;
   if (k.l.batch != q.l.batch || k.l.d != q.l.d || k_.scalar_type() != q_.scalar_type() || k_.device() != q_.device() ||
-      !mask_applies(m, q.l.n, k.l.n) || !L.is_cuda() || L.device() != q_.device() || L.numel() != q.l.batch * q.l.n)
+      !mask_applies(m, q.l.n, k.l.n) || !in_memory(L) || !L.is_cuda() || L.device() != q_.device() || L.numel() != q.l.batch * q.l.n)
     return std::nullopt;
   fhog_bwdbwd_args a = {};
   a.dtype = dtype_code(q_.scalar_type());
@@ -295,8 +295,7 @@ std::optional<Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& 
   if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode)) return std::nullopt;
   for (const Tensor* t : {&q, &k, &v}) {
     const int64_t dim = t->dim();
-    // tensors that dispatch to Python (fake ones among them) have no memory to launch on
-    if (t->unsafeGetTensorImpl()->is_python_dispatch()) return std::nullopt;
+    if (t->unsafeGetTensorImpl()->is_python_dispatch() || !in_memory(*t)) return std::nullopt;
     if (!t->is_cuda() || t->device() != q.device() || t->scalar_type() != q.scalar_type() || (dim != 3 && dim != 4) || dim != q.dim()) return std::nullopt;
     for (int64_t i = 0; i < dim; i++)
       if (i != dim - 2 && t->size(i) != q.size(i)) return std::nullopt;

@@ -161,6 +161,13 @@ def torch_ext():
     return _TORCH_EXT
 
 
+def check_memory(**tensors) -> None:
+    """Raise on a tensor on a GPU whose storage holds no memory. A view of one that starts behind its first element has an address all the same."""
+    for name, t in tensors.items():
+        if t is not None and t.is_cuda and not torch_ext().in_memory(t):
+            raise ValueError(f"{name} holds no memory (a fake tensor, or a storage that was resized to nothing)")
+
+
 def check(rc: int) -> None:
     if rc != 0:
         raise FhogError(rc, lib().fhog_last_error().decode())

@@ -28,6 +28,7 @@ from typing import Optional, Tuple
 import ctypes
 
 import torch
+from torch._subclasses.fake_tensor import FakeTensor
 
 from . import _lib
 from .rotary import Rotary
@@ -66,6 +67,14 @@ class _NotCovered(Exception):
     """The HIP first-order kernels do not take these arguments; the message says why."""
 
 
+def _check_memory(**tensors) -> None:
+    """Before anything is read: _NotCovered for fake tensors, whose shapes the torch composition propagates, an error for other tensors without memory."""
+    for name, t in tensors.items():
+        if isinstance(t, FakeTensor):
+            raise _NotCovered(f"{name} is a fake tensor")
+    _lib.check_memory(**tensors)
+
+
 def _hip_args(q, k, v, scale, causal, window=None) -> _lib.AttnArgs:
     """Arguments for the HIP first-order kernels; raises _NotCovered when they do not cover these tensors."""
     if not q.is_cuda:
@@ -94,6 +103,7 @@ def _same_layout(ts) -> bool:
 
 def _attention_forward_hip(q, k, v, scale, causal, window=None, sinks=0):
     """O and L from ``fhog_attn_fwd``; raises _NotCovered when the kernels do not cover the arguments."""
+    _check_memory(q=q, k=k, v=v)
     q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
     if not _same_layout([k, v]):
         k, v = k.contiguous(), v.contiguous()
@@ -116,6 +126,7 @@ def _attention_forward_hip(q, k, v, scale, causal, window=None, sinks=0):
 
 
 def _attention_backward_hip(q, k, v, o, do, L, scale, causal, window=None, sinks=0):
+    _check_memory(q=q, k=k, v=v, o=o, do=do, L=L)
     ts_q = [t if t.stride(-1) == 1 else t.contiguous() for t in (q, o, do)]
     if not _same_layout(ts_q):
         ts_q = [t.contiguous() for t in ts_q]
@@ -198,7 +209,7 @@ def attention_forward(q, k, v, scale: Optional[float] = None, causal=False, *, w
         except _NotCovered as why:
             _second_path("attention_forward", "fhog_attn_fwd", why, use_hip)
     o = torch.empty_like(q)
-    L = torch.empty(batch, n_q, dtype=torch.float32, device=q.device)
+    L = q.new_empty((batch, n_q), dtype=torch.float32)
     for hs, rs in _blocks(batch, n_q, n_k):
         s = _scores(q[hs, rs], k[hs], scale, causal, rs.start, n_q, window, sinks)
         lse = torch.logsumexp(s, dim=-1)
@@ -231,8 +242,7 @@ def attention_backward(q, k, v, o, do, L, scale: float, causal, *, window: Optio
         except _NotCovered as why:
             _second_path("attention_backward", "fhog_attn_bwd", why, use_hip)
     dq = torch.empty_like(q)
-    dk = torch.zeros(k.shape, dtype=torch.float32, device=k.device)
-    dv = torch.zeros(v.shape, dtype=torch.float32, device=v.device)
+    dk, dv = (t.new_zeros(t.shape, dtype=torch.float32) for t in (k, v))
     for hs, rs in _blocks(batch, n_q, n_k):
         qf, dof = q[hs, rs].float(), do[hs, rs].float()
         s = _scores(q[hs, rs], k[hs], scale, causal, rs.start, n_q, window, sinks)

@@ -239,6 +239,7 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, windo
             raise TypeError(f"{n} has dtype {t.dtype}, expected {Q.dtype} like Q")
         if t.device != Q.device:
             raise ValueError(f"{n} is on {t.device}, expected {Q.device} like Q")
+    _lib.check_memory(**tensors, L=L)
     if impl not in _IMPLS:
         raise ValueError(f"impl must be one of {sorted(k for k in _IMPLS if k)} or None, got {impl!r}")
     out_shape_q, out_shape_k = Q.shape, K.shape
@@ -306,6 +307,7 @@ class BwdBwdPlan:
     def __init__(self, Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, causal=False, window=None, impl=None,
                  fused_stats=False, schedule=None, split=True, sinks=0):
         self.sinks = check_sinks(sinks, schedule, fused_stats)
+        _lib.check_memory(Q=Q, K=K, V=V, O=O, dO=dO, ddQ=ddQ, ddK=ddK, ddV=ddV, L=L)
         ts = [_flatten(t, "tensor") for t in (Q, K, V, O, dO, ddQ, ddK, ddV)]
         q3, k3, v3, o3, do3, ddq3, ddk3, ddv3 = ts
         q3, o3, do3, ddq3 = _prepare_group([q3, o3, do3, ddq3], "q")

@@ -69,9 +69,7 @@ def _check(q, k, positions, sections, theta, rotary_dim) -> Tuple[int, ...]:
     if k is not None and isinstance(k, FakeTensor) != fake:
         raise ValueError("one of q and k is a fake tensor, the other is not")
     if not fake:
-        for name, t in (("q", q), ("k", k), ("positions", positions)):
-            if t is not None and not _lib.torch_ext().in_memory(t):
-                raise ValueError(f"{name} holds no memory (a fake tensor beside real ones, or a storage that was resized to nothing)")
+        _lib.check_memory(q=q, k=k, positions=positions)
     return sections
 
 

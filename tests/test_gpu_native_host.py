@@ -209,3 +209,20 @@ def test_tensors_elsewhere_or_of_other_shapes_are_refused():
             f()
     with pytest.raises(TypeError):
         fhog.BwdBwdPlan(x, x, x, x, x, x.half(), x, x, L, 0.125)
+
+
+def test_storages_that_were_resized_to_nothing_are_refused():
+    """Their views have addresses still; every entry point names them before anything is read."""
+    import fhog
+    x, L = torch.zeros(2, 41, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(2, 40, device="cuda")
+    y, M = x.clone(), L.clone()
+    gone, x = y[:, 1:], x[:, 1:]
+    for t in (y, M):
+        t.untyped_storage().resize_(0)
+    for f in (lambda: fhog.attention(gone, x, x), lambda: fhog.attention(x, gone, x), lambda: fhog.attention(x.detach().requires_grad_(True), x, gone),
+              lambda: fhog.FlashAttention.apply(gone, x, x), lambda: fhog.attention_forward(x, x, gone, None, True, window=9, sinks=3),
+              lambda: fhog.attention_backward(x, x, x, x, gone, L, 0.125, False), lambda: fhog.attention_backward(x, x, x, x, x, M, 0.125, False),
+              lambda: fhog.flash_bwdbwd(x, x, x, gone, x, x, x, x, L, 0.125), lambda: fhog.flash_bwdbwd(x, x, x, x, x, x, gone, x, L, 0.125),
+              lambda: fhog.flash_bwdbwd(x, x, x, x, x, x, x, x, M, 0.125), lambda: fhog.BwdBwdPlan(x, x, x, x, x, x, x, gone, L, 0.125)):
+        with pytest.raises(ValueError, match="no memory"):
+            f()
