@@ -6,6 +6,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "fhog_common.h"
@@ -266,6 +267,23 @@ int check_ws(const void* ws, int64_t have, size_t need) {
   return FHOG_OK;
 }
 
+// Whether the rows of a (batch, heads, n, d) output lie apart: from the shortest stride up, each has to pass what lies below it
+bool rows_apart(int64_t batch, int64_t heads, int64_t n, int64_t d, int64_t stride_b, int64_t stride_h, int64_t stride_n) {
+  struct Dim {
+    int64_t size;
+    __int128 stride;
+  } dims[] = {{batch, stride_b}, {heads, stride_h}, {n, stride_n}};
+  for (Dim& x : dims) x.stride = x.size == 1 ? 0 : x.stride < 0 ? -x.stride : x.stride;   // a dimension of one is never stepped along
+  std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  __int128 extent = d;
+  for (const Dim& x : dims) {
+    if (x.size == 1) continue;
+    if (x.stride < extent) return false;
+    extent += (x.size - 1) * x.stride;
+  }
+  return true;
+}
+
 int validate_rotary(const fhog_rotary_args* a) {
   if (!a) return fail(FHOG_E_NULL, "args is NULL");
   if (a->dtype != FHOG_DTYPE_BF16 && a->dtype != FHOG_DTYPE_FP16 && a->dtype != FHOG_DTYPE_FP32) return fail(FHOG_E_DTYPE, "unknown dtype %d", a->dtype);
@@ -296,10 +314,9 @@ int validate_rotary(const fhog_rotary_args* a) {
     if (reinterpret_cast<uintptr_t>(ptrs[i]) % (i == 2 ? (a->position_type == FHOG_POSITIONS_INT64 ? 8 : 4) : align))
       return fail(FHOG_E_ALIGN, "pointer '%s' is not aligned to its type", names[i]);
   }
-  // rows of an output that share an address would be written by several threads
-  const auto packed = [](int64_t size, int64_t stride, int64_t least) { return size == 1 || (stride < 0 ? -stride : stride) >= least; };
-  if (!packed(a->batch, a->stride_qob, a->d) || !packed(a->heads_q, a->stride_qoh, a->d) || !packed(a->n, a->stride_qon, a->d) ||
-      (a->heads_k > 0 && (!packed(a->batch, a->stride_kob, a->d) || !packed(a->heads_k, a->stride_koh, a->d) || !packed(a->n, a->stride_kon, a->d))))
+  // rows that share an address would be written by several threads
+  if (!rows_apart(a->batch, a->heads_q, a->n, a->d, a->stride_qob, a->stride_qoh, a->stride_qon) ||
+      (a->heads_k > 0 && (a->q_out == a->k_out || !rows_apart(a->batch, a->heads_k, a->n, a->d, a->stride_kob, a->stride_koh, a->stride_kon))))
     return fail(FHOG_E_STRIDE, "rows of an output overlap");
   return FHOG_OK;
 }

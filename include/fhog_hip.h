@@ -293,7 +293,9 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
  * gradient of the call is the call on the gradient with `inverse` flipped, and so are the derivatives beyond it.
  * Angles are formed in 64 bits: exact to 5e-16 * |p| turns, sines and cosines to 1e-7. A position that is no number makes NaN of its token's rows.
  * Queries and keys may have different numbers of heads; heads_k = 0 leaves the keys out. Strides are in elements and may be 0 or negative on the
- * inputs; the last dimension is contiguous. Outputs may be the inputs (same pointers and strides), else must not overlap with them. Rows that lie on
+ * inputs; the last dimension is contiguous. Rows of an output lie apart (FHOG_E_STRIDE): from the shortest stride of its dimensions up, each passes what lies
+ * below it. Outputs may be the inputs (same pointers and strides), else must not overlap with them, and q_out and k_out must not overlap with one
+ * another, though their rows may lie between each other's; neither is checked, but for one address given as both outputs (FHOG_E_STRIDE). Rows that lie on
  * multiples of 16 bytes, with d and rd multiples of 32 bytes, go 16 bytes at a time, others pair by pair. */
 #define FHOG_ROTARY_MAX_D 256
 #define FHOG_ROTARY_MAX_AXES 4

@@ -130,3 +130,18 @@ def test_what_holds_memory():
         views = fake, fake[2:]
     assert there(x) and there(x[2:]) and there(x[:0]) and there(torch.empty(0))
     assert gone.data_ptr() and not any(there(t) for t in (y, gone, *views, torch.empty(3, device="meta")))
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(stride_qoh=64, stride_qon=64), -4),                                    # (h, t) and (h + 1, t - 1) are one row
+    (dict(stride_koh=6400, stride_kob=6400), -4), (dict(stride_qoh=128, stride_qon=64), -4), (dict(stride_qon=-64, stride_qoh=6336), -4),
+    (dict(stride_qon=100, stride_qoh=9999), -4), (dict(q_out=0x40000, k_out=0x40000), -4), (dict(q_out=0x40000, k_out=0x40000, heads_k=0), 0),
+    (dict(stride_qon=-64, stride_qoh=-6400), 0), (dict(stride_qon=256, stride_qoh=64), 0),                             # backwards; a token's heads together
+    (dict(stride_qon=400, stride_qoh=64, stride_kon=400, stride_koh=64, stride_kob=40000, stride_qob=40000, k_out=0x30200), 0),   # one row for both
+    (dict(stride_qon=64, stride_qoh=25600, stride_qob=6400), 0), (dict(stride_qoh=0, heads_q=1), 0), (dict(stride_qon=0, n=1), 0),
+    (dict(stride_qob=2 ** 63 - 1, stride_qoh=2 ** 63 - 1), -4), (dict(stride_qob=-2 ** 63), 0)])
+def test_outputs_that_overlap(L, change, code):
+    a = _args(**change)
+    assert L.fhog_rotary_validate(ctypes.byref(a)) == code
+    if code:
+        assert "overlap" in L.fhog_last_error().decode() and L.fhog_rotary(ctypes.byref(a), None) == code
