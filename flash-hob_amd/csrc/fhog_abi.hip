@@ -295,7 +295,8 @@ int validate_rotary(const fhog_rotary_args* a) {
   if (a->d < 2 || a->d > FHOG_ROTARY_MAX_D || a->d % 2) return fail(FHOG_E_SHAPE, "head dim %lld is not an even number in 2..%d", (long long)a->d, FHOG_ROTARY_MAX_D);
   if (a->rotary_dim < 2 || a->rotary_dim > a->d || a->rotary_dim % 2)
     return fail(FHOG_E_SHAPE, "rotary_dim %lld is not an even number in 2..%lld", (long long)a->rotary_dim, (long long)a->d);
-  if (a->n > 0 && a->batch > (int64_t)UINT32_MAX / (a->d / 2) / a->n) return fail(FHOG_E_SHAPE, "batch * n * d / 2 from 2^32 on is not supported");
+  // a thread for each, in whole workgroups: a launch has fewer than 2^32
+  if (a->n > 0 && a->batch > ((int64_t)UINT32_MAX - 255) / (a->d / 2) / a->n) return fail(FHOG_E_SHAPE, "batch * n * d / 2 above 2^32 - 256 is not supported");
   if (a->axes < 1 || a->axes > FHOG_ROTARY_MAX_AXES) return fail(FHOG_E_ROTARY, "axes must be 1..%d (got %d)", FHOG_ROTARY_MAX_AXES, a->axes);
   int64_t sum = 0;
   for (int i = 0; i < a->axes; i++) {

@@ -145,3 +145,13 @@ def test_outputs_that_overlap(L, change, code):
     assert L.fhog_rotary_validate(ctypes.byref(a)) == code
     if code:
         assert "overlap" in L.fhog_last_error().decode() and L.fhog_rotary(ctypes.byref(a), None) == code
+
+
+def test_no_more_threads_than_a_launch_may_have(L):
+    """A thread for every pair of a token, in whole workgroups of 256, has to stay below 2^32."""
+    dims = dict(d=2, rotary_dim=2, sections=(1, 0), axes=1, heads_q=1, heads_k=0, stride_qn=2, stride_qon=2)
+    for batch, n, code in ((65535, 65537, -2), (2 ** 8, 2 ** 24 - 1, 0), (2 ** 8, 2 ** 24, -2), (1, 2 ** 31 - 1, 0), (255, 16843009, -2), (65536, 65535, 0)):
+        a = _args(batch=batch, n=n, stride_qob=2 * n, stride_qb=2 * n, **dims)
+        assert L.fhog_rotary_validate(ctypes.byref(a)) == code, (batch, n)
+        assert code == 0 or "2^32" in L.fhog_last_error().decode()
+        assert (code == 0) == (-(-batch * n // 256) * 256 < 2 ** 32)
