@@ -5,9 +5,10 @@
 // on the pair (f, f + rotary_dim / 2), or (2 f, 2 f + 1) interleaved; the channels from rotary_dim on pass. The rotation is linear and orthogonal: its adjoint, and with
 // it every derivative, is the rotation by the negative angle (inverse).
 //
-// A far position turns the first frequencies millions of times, so the number of turns is formed in 64 bits: p (theta^(-2f/rd) / 2 pi), less the nearest quarter, is
-// right to 2^-52 p of a turn; what is left, an eighth of a turn at most either way, goes through the sine's and cosine's own power series in single precision
-// (terms up to x^9 and x^8: the first ones left out are 2e-9 and 3e-8 at pi / 4).
+// A far position turns the first frequencies millions of times, so the number of turns is formed in 64 bits: p (theta^(-2f/rd) / 2 pi) is right to
+// (6 + |ln theta|) 2^-53 of itself (the position, 1 / 2 pi, two products and the power, a step of 2^-52, are rounded, and so is its exponent, which ln theta multiplies),
+// with theta >= 1 an angle to 2^-50 p at most. The nearest quarter is taken off exactly, and what is left, an eighth of a turn at most either way, goes through the sine's and cosine's own power series in single precision
+// (terms up to x^9 and x^8: the first ones left out are 2e-9 and 3e-8 at pi / 4; with the roundings 6e-8 and 9.3e-8 off at most, over four million angles).
 //
 // What bounds it: memory, every channel in and out once. A thread owns V pairs of one token (two loads and two stores of 16 bytes) and keeps their sines and cosines in
 // registers while it goes through the heads, of queries and keys alike; nothing is shared, so there is neither LDS nor a barrier.

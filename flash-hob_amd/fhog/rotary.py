@@ -137,10 +137,10 @@ def rotary(q, k, positions, *, sections: Optional[Sequence[int]] = None, theta: 
     Args:
         q, k: (batch, N, d) or (B, H, N, d), bf16, fp16 or fp32, on a ROCm device; the numbers of heads may differ. d even, at most 256. Any strides.
         positions: int32, int64 or fp32, (N,) or (batch, N); with two or more ``sections`` (axes, N) or (axes, batch, N). Angles are formed in
-            64 bits, right for positions up to 2^31 to 1e-6.
+            64 bits, right to (6 + abs(ln(theta))) 2^-53 of their size (theta >= 1: to 2^-50 of the position, 2e-6 at 2^31).
         sections: how many of the rd / 2 frequencies belong to each axis, in their order (1 to 4 axes; for images and video: time, height,
             width). None: one axis.
-        theta: base of the frequencies.
+        theta: base of the frequencies, any positive number; below 1 they grow, and the error of the angles with them.
         rotary_dim: channels that are turned, the first ones; the others pass. None: all of them.
     """
     if not isinstance(q, torch.Tensor):

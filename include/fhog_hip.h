@@ -291,7 +291,8 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
  * (f, f + rd / 2), or (2 f, 2 f + 1) where `interleaved`; channels rd .. d - 1 are copied. The first sections[0] frequencies belong to axis 0, the next
  * sections[1] to axis 1, and so on (text has one axis; time, height and width of images and video are three). `inverse` turns the other way: the
  * gradient of the call is the call on the gradient with `inverse` flipped, and so are the derivatives beyond it.
- * Angles are formed in 64 bits: exact to 5e-16 * |p| turns, sines and cosines to 1e-7. A position that is no number makes NaN of its token's rows.
+ * Angles are formed in 64 bits: right to (6 + |ln theta|) 2^-53 of their size (theta >= 1: to 2^-50 |p|, 2e-6 at 2^31; below 1 they grow to almost p / theta),
+ * sines and cosines of what is left of a turn to 1e-7. A position that is no number makes NaN of its token's rows.
  * Queries and keys may have different numbers of heads; heads_k = 0 leaves the keys out. Strides are in elements and may be 0 or negative on the
  * inputs; the last dimension is contiguous. Rows of an output lie apart (FHOG_E_STRIDE): from the shortest stride of its dimensions up, each passes what lies
  * below it. Outputs may be the inputs (same pointers and strides), else must not overlap with them, and q_out and k_out must not overlap with one

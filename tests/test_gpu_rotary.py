@@ -382,3 +382,17 @@ def test_tensors_without_memory_are_not_launched_on():
               lambda: fhog.rotary(views[1].detach().requires_grad_(True), None, p[1:]), lambda: fhog.rotary(real[:, :, 1:], None, pos[1:])):
         with pytest.raises(ValueError, match="no memory"):
             f()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("theta, rotary_dim, top", [(0.25, 64, 2 ** 31 - 1), (1.0, 64, 2 ** 31 - 1), (1e-3, 40, 10 ** 6), (1e-6, 64, 10 ** 7), (3.0, 36, 2 ** 31 - 1)])
+def test_small_bases(theta, rotary_dim, top, dtype):
+    """Frequencies that grow: angles up to top / theta, which the kernel and the definition each have right to (6 + |ln theta|) 2^-53 of themselves."""
+    import fhog
+    g = torch.Generator(device="cuda").manual_seed(41)
+    q, k = (torch.randn(2, h, 51, 64, generator=g, device="cuda").to(dtype) for h in (3, 1))
+    positions = torch.randint(-top, top, (2, 51), generator=g, device="cuda")
+    largest = top * max(1.0, theta ** (2 / rotary_dim - 1))
+    as_position = 2 * (6 + abs(math.log(theta))) * 2.0 ** -53 * largest / (2 * math.pi * 2.0 ** -51)   # what _assert_close makes an angle's error of
+    for y, x in zip(fhog.rotary(q, k, positions, theta=theta, rotary_dim=rotary_dim), (q, k)):
+        _assert_close(y, _definition(x, positions[None], (rotary_dim // 2,), theta, False, rotary_dim), as_position)
