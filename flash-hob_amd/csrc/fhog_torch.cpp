@@ -38,7 +38,7 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
-// False where the storage holds no memory: fake tensors, and storages that were resized to nothing. A view of one that starts behind its first
+// False where the storage holds no memory: fake tensors and wrappers of other tensors, and storages that were resized to nothing. A view of one that starts behind its first
 // element has an address all the same, and it is no one's.
 bool in_memory(const Tensor& t) { return !t.has_storage() || t.numel() == 0 || t.storage().data() != nullptr; }
 
@@ -457,6 +457,7 @@ PYBIND11_MODULE(_fhog_torch, m) {
     return double_backward(q, k, v, o, g, ddq, ddk, ddv, L, scale, Mask{causal, window, sinks}, impl, schedule, split);
   }, free_lock);
   m.def("in_memory", &in_memory, free_lock);
+  m.def("dispatches_to_python", [](const Tensor& t) { return t.unsafeGetTensorImpl()->is_python_dispatch(); }, free_lock);
   m.def("attention", &attention, free_lock);
   m.def("rotary", &rotary, free_lock);
 }

@@ -28,7 +28,6 @@ from typing import Optional, Tuple
 import ctypes
 
 import torch
-from torch._subclasses.fake_tensor import FakeTensor
 
 from . import _lib
 from .rotary import Rotary
@@ -68,10 +67,10 @@ class _NotCovered(Exception):
 
 
 def _check_memory(**tensors) -> None:
-    """Before anything is read: _NotCovered for fake tensors, whose shapes the torch composition propagates, an error for other tensors without memory."""
+    """Before anything is read: _NotCovered for fake tensors and wrappers, which the torch composition dispatches, an error for other tensors without memory."""
     for name, t in tensors.items():
-        if isinstance(t, FakeTensor):
-            raise _NotCovered(f"{name} is a fake tensor")
+        if t.is_cuda and not _lib.torch_ext().in_memory(t) and _lib.torch_ext().dispatches_to_python(t):
+            raise _NotCovered(f"{name} is a fake tensor or a wrapper of others, and holds no memory itself")
     _lib.check_memory(**tensors)
 
 

@@ -226,3 +226,32 @@ def test_storages_that_were_resized_to_nothing_are_refused():
               lambda: fhog.flash_bwdbwd(x, x, x, x, x, x, x, x, M, 0.125), lambda: fhog.BwdBwdPlan(x, x, x, x, x, x, x, gone, L, 0.125)):
         with pytest.raises(ValueError, match="no memory"):
             f()
+
+
+def test_wrappers_without_memory_of_their_own_run_the_composition():
+    """A tensor subclass that holds another tensor and dispatches to Python: the first-order calls compute on what it holds, views of it too."""
+    import fhog
+    from fhog.attention import TorchCompositionWarning
+    from torch.utils._pytree import tree_map
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            w = torch.Tensor._make_wrapper_subclass(cls, inner.shape, strides=inner.stride(), storage_offset=inner.storage_offset(), dtype=inner.dtype, device=inner.device)
+            w.inner = inner
+            return w
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            open_ = lambda t: t.inner if isinstance(t, cls) else t                           # noqa: E731
+            out = func(*tree_map(open_, args), **tree_map(open_, kwargs or {}))
+            return tree_map(lambda t: cls(t) if isinstance(t, torch.Tensor) else t, out)
+
+    g = torch.Generator(device="cuda").manual_seed(77)
+    q, k, v, do = (torch.randn(2, 41, 64, generator=g, device="cuda")[:, 1:] for _ in range(4))
+    want = fhog.attention_forward(q, k, v, None, True, window=9, sinks=2, use_hip=False)
+    with pytest.warns(TorchCompositionWarning, match="wrapper"):
+        got = fhog.attention_forward(*(Wrapper(t) for t in (q, k, v)), None, True, window=9, sinks=2)
+        grads = fhog.attention_backward(*(Wrapper(t) for t in (q, k, v, want[0], do, want[1])), 0.125, True, window=9, sinks=2)
+    for a, b in zip((*got, *grads), (*want, *fhog.attention_backward(q, k, v, want[0], do, want[1], 0.125, True, window=9, sinks=2, use_hip=False))):
+        assert isinstance(a, Wrapper) and torch.equal(a.inner, b)
