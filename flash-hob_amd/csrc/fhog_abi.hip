@@ -254,11 +254,7 @@ size_t row_bytes(const fhog_attn_args* a) { return ((size_t)a->batch * a->n_q * 
 
 size_t attn_sinks_bytes(const fhog_attn_args* a, int64_t sinks, int backward) {
   const int32_t n = sinks_of(a, sinks);
-  if (backward) {
-    fhog::AttnParams p = to_attn_params(a);
-    p.sinks = n;
-    return n ? row_bytes(a) + sink_bytes(p, dtype_bytes(a->dtype), attn_on_16bit_kernels(a)) : (size_t)a->batch * a->n_q * sizeof(float);
-  }
+  if (backward) return n ? row_bytes(a) + sink_bytes(a->batch, n, a->n_q, a->d, dtype_bytes(a->dtype), false) : (size_t)a->batch * a->n_q * sizeof(float);
   return n ? forward_part_bytes(a->batch, a->n_q, a->d, forward_parts(a, n)) : 0;
 }
 
@@ -473,9 +469,9 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
   const hipStream_t s = (hipStream_t)hip_stream;
   fhog::AttnParams p = to_attn_params(args);
   p.sinks = n;
+  const int parts = sink_parts(args->batch, n, args->n_q, args->d, dtype_bytes(args->dtype), false);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(args->ws) + row_bytes(args));
   const bool bit16 = attn_on_16bit_kernels(args);
-  const int parts = sink_parts(p, dtype_bytes(args->dtype), bit16);
   const int small = bit16 ? sink_small_waves(Small::backward, args) : 0;
   const bool swept = fhog::rules::sinks_ride(p, dtype_bytes(args->dtype), bit16, small);
   hipError_t e = hipSuccess;
@@ -493,11 +489,9 @@ int fhog_attn_bwd_sinks(const fhog_attn_args* args, int64_t sinks, int64_t ws_by
 
 size_t fhog_bwdbwd_sinks_workspace_bytes(const fhog_bwdbwd_args* args, int64_t sinks) {
   if (validate(args) != FHOG_OK || check_sinks(sinks) != FHOG_OK) return 0;
-  fhog::Params p = to_params(args);
-  const int impl = select_impl(args);
-  const size_t hint = workspace_hint(args, p, impl);
-  p.sinks = sinks_of(args, sinks);
-  return p.sinks ? ((hint + 15) & ~(size_t)15) + sink_bytes(p, dtype_bytes(args->dtype), impl == FHOG_IMPL_BF16) : hint;
+  const size_t hint = workspace_hint(args, to_params(args), select_impl(args));
+  const int32_t n = sinks_of(args, sinks);
+  return n ? ((hint + 15) & ~(size_t)15) + sink_bytes(args->batch, n, args->n_q, args->d, dtype_bytes(args->dtype), true) : hint;
 }
 
 int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_stream) {
@@ -506,14 +500,14 @@ int fhog_bwdbwd_sinks(const fhog_bwdbwd_args* args, int64_t sinks, void* hip_str
   const int32_t n = sinks_of(args, sinks);
   if (n == 0) return fhog_bwdbwd(args, hip_stream);
   if (args->schedule != FHOG_SCHEDULE_FUSED_STATS) return fail(FHOG_E_SCHEDULE, "sinks run under schedule %d alone (got %d)", FHOG_SCHEDULE_FUSED_STATS, args->schedule);
+  const size_t of_sinks = sink_bytes(args->batch, n, args->n_q, args->d, dtype_bytes(args->dtype), true);
+  if (const int rc = check_ws(args->ws, args->ws_bytes, stats_bytes(args) + of_sinks)) return rc;
   const hipStream_t s = (hipStream_t)hip_stream;
   const int impl = select_impl(args);
-  fhog::Params p = to_params(args);
-  p.sinks = n, p.n_split_s = sink_parts(p, dtype_bytes(args->dtype), impl == FHOG_IMPL_BF16);
-  const size_t of_sinks = sink_bytes(p, dtype_bytes(args->dtype), impl == FHOG_IMPL_BF16);
-  if (const int rc = check_ws(args->ws, args->ws_bytes, stats_bytes(args) + of_sinks)) return rc;
   fhog_bwdbwd_args a = *args;   // the sweeps have what lies before the partial results of the sinks, which are a multiple of 16 bytes
   a.ws_bytes = (args->ws_bytes & ~(int64_t)15) - (int64_t)of_sinks;
+  fhog::Params p = to_params(&a);
+  p.sinks = n, p.n_split_s = sink_parts(a.batch, n, a.n_q, a.d, dtype_bytes(a.dtype), true);
   float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.ws) + a.ws_bytes);
   const int small = impl == FHOG_IMPL_BF16 ? sink_small_waves(Small::double_backward, args) : 0;
   const bool swept = fhog::rules::sinks_ride(p, dtype_bytes(a.dtype), impl == FHOG_IMPL_BF16, small);

@@ -394,9 +394,9 @@ constexpr int lds_bytes() {
 template <int WS>
 __host__ __device__ unsigned blocks(int rows, int batch) { return grid_blocks((rows + 128 / WS - 1) / (128 / WS), batch); }
 
-// Waves on the same 32 rows where several workgroups share the streamed side, with ON_CU workgroups on a CU: as many as fit the LDS
+// Waves on the same 32 rows where several workgroups share the streamed side: as many as fit the LDS, with ON_CU workgroups on a CU
 template <typename T, int D, int MODE, int ON_CU = 1>
-constexpr int part_waves = MODE == MODE_BWD_K ? rules::split_sink_waves(D, sizeof(T), false, ON_CU) : lds_bytes<T, D, MODE, 4>() <= 160 * 1024 ? 4 : 2;
+constexpr int part_waves = ON_CU * lds_bytes<T, D, MODE, 4>() <= 160 * 1024 ? 4 : 2;
 
 // dQ (workgroups [0, q_blocks)) and dK, dV (the others; mixed: tile by tile in turn) in one launch; ON_CU: workgroups on a CU.
 // MASK_SINK: behind both come the workgroups that sum up the rows of the sinks (fhog_sinks.hip), where rules::sinks_ride says so.
@@ -432,7 +432,6 @@ hipError_t launch_ws(const AttnParams& p, hipStream_t s) {
 template <typename T, int D, int MODE, int MASK>
 hipError_t launch_parts(const AttnParams& p, hipStream_t s) {
   constexpr int WS = part_waves<T, D, MODE>, smem = lds_bytes<T, D, MODE, WS>();
-  static_assert(smem <= 160 * 1024, "stages and exchange buffer have to fit the LDS");
   const hipError_t e = allow_dynamic_lds<attn_split<T, D, MODE, MASK, WS, false, true>>(smem);
   if (e != hipSuccess) return e;
   const unsigned grid = blocks<WS>(MODE == MODE_BWD_K ? p.n_k : p.n_q, p.batch * p.n_split);
@@ -444,7 +443,7 @@ template <typename T, int D, int MASK, int WS, int ON_CU = min_workgroups<T, D, 
 hipError_t launch_bwd_ws(const AttnParams& p, hipStream_t s, bool mixed = false) {
   constexpr int lq = lds_bytes<T, D, MODE_BWD_Q, WS>(), lk = lds_bytes<T, D, MODE_BWD_K, WS>(), own = lq > lk ? lq : lk;
   constexpr int W = part_waves<T, D, MODE_BWD_K, ON_CU>, riders = MASK == MASK_SINK ? lds_bytes<T, D, MODE_BWD_K, W>() : 0, smem = own > riders ? own : riders;
-  static_assert(smem <= 160 * 1024 && ON_CU * riders <= 160 * 1024, "stages and exchange buffer have to fit the LDS");
+  static_assert(smem <= 160 * 1024, "stages and exchange buffer have to fit the LDS");
   const hipError_t e = allow_dynamic_lds<attn_split_bwd<T, D, MASK, WS, ON_CU>>(smem);
   if (e != hipSuccess) return e;
   const unsigned gq = blocks<WS>(p.n_q, p.batch), gk = blocks<WS>(p.n_k, p.batch);

@@ -386,6 +386,21 @@ inline int sink_sweep_waves(int64_t groups, int d, int bytes, int64_t window) {
   if (d == 64) return groups <= 64 ? 4 : groups <= 128 ? 2 : 1;
   return groups < (d == 32 ? 192 : 256) ? 4 : 1;
 }
+// Workgroups that share 32 sinks of a slice, each with a part of the queries: one for every CU, with a tile for each of its waves at least.
+// First | second backward, us, 512 workgroups of eight tiles -> 256 of four: bf16 32 x 4096, d = 128, window 1024, 4 sinks 290 | 678 -> 282 | 675; fp32 16 x 1024, d = 64,
+// window 256, 33 sinks 64.9 | 153 -> 61.7 | 149; 8 x 4096, d = 128 448 | 1401 -> 440 | 1357; 1024 of four 296 | 686, 61.7 | 148, 440 | 1358.
+// Single precision of d = 128 with four tiles at least -> one for each of its two | one waves: 1 x 1000, window 100 41.2 | 123 -> 41.5 | 89.
+inline int64_t sink_groups(int64_t batch, int64_t sinks) { return (sinks + 31) / 32 * batch; }
+inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q, int64_t d, int bytes, bool second) {
+  const int64_t groups = sink_groups(batch, sinks), tiles = (n_q + 31) / 32, waves = bytes * d < 512 ? 4 : second ? 1 : 2;   // on the same rows
+  int64_t parts = (256 + groups - 1) / groups;
+  if (parts > tiles / waves) parts = tiles / waves;
+  return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+}
+// Partial results; more groups than CUs store their rows directly
+inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d, int bytes, bool second) {
+  return sink_groups(batch, sinks) <= 256 ? (size_t)sink_parts(batch, sinks, n_q, d, bytes, second) * 2 * batch * sinks * d * sizeof(float) : 0;
+}
 // Forwards of few queries under a mask with sinks: workgroups that share 32 queries of a slice, each with a part of the keys, or 0 for the kernels of longer ones. What
 // a number of parts costs is reckoned up, in us: rounds of the workgroups, each with something to start and to end (fixed) and its waves' tiles one after the
 // other (slower where two workgroups share a CU), no less than the bytes at 5.5 TB/s; several parts have their join, with the bytes of partial
@@ -581,44 +596,6 @@ inline int split_bwd_waves(const AttnParams& p, int bytes) {
   return long_key_side ? 0 : waves;
 }
 
-// ---- the rows of the sinks ----------------------------------------------------------------------------------------------------
-// Waves of a workgroup on the same sinks, of which it has 128 / waves: four on the 16-bit kernels, on split products as many as leave LDS for their tiles' terms. Those have
-// 128 bytes a row or less: four; 256 (fp32 d = 64, 16-bit tensors of d = 128): four in a first backward with a CU to itself (100 KB), two in others; 512 (fp32 d = 128): two in a
-// first backward, one in a second. At d = 64 four waves of fp32 tensors would fit a double-backward (149 KB), with 61 registers too many in the launch of both sweeps;
-// 16 x 1024, window 256, us, with four -> two: 33 sinks 147 -> 138, 4 sinks 128 -> 127.
-constexpr int split_sink_waves(int d, int bytes, bool second, int on_cu) {
-  return bytes * d <= 128 ? 4 : bytes * d >= 512 ? (second ? 1 : 2) : second || on_cu > 1 ? 2 : 4;
-}
-inline int sink_waves(const Params& p, int bytes, bool bit16) { return bit16 ? 4 : split_sink_waves(p.d, bytes, true, 1); }
-inline int sink_waves(const AttnParams& p, int bytes, bool bit16) {
-  if (bit16) return 4;
-  const bool shared = bytes == 4 && p.d == 64 && split_bwd_waves(p, bytes) == 1 && bwd_company(p) != Company::none;   // they ride where a CU has two workgroups
-  return split_sink_waves(p.d, bytes, false, shared ? 2 : 1);
-}
-// Workgroups that share the rows of a group of sinks, each with a part of the queries: one for every CU, with a tile for each of its waves at least.
-// First | second backward, us, 512 workgroups of eight tiles -> 256 of four: bf16 32 x 4096, d = 128, window 1024, 4 sinks 290 | 678 -> 282 | 675; fp32 16 x 1024, d = 64,
-// window 256, 33 sinks 64.9 | 153 -> 61.7 | 149; 8 x 4096, d = 128 448 | 1401 -> 440 | 1357; 1024 of four 296 | 686, 61.7 | 148, 440 | 1358.
-// Single precision of d = 128 with four tiles at least -> one for each of its two | one waves: 1 x 1000, window 100 41.2 | 123 -> 41.5 | 89. Every group counted as one of 32 sinks,
-// which leaves launches of 64 and 128 to a group with a half or a quarter of the workgroups -> as here, 100 sinks, fp32 d = 128: 64 x 1024, window 256 450 | 1196 -> 414 | 1034,
-// 32 x 2048, 512 606 | 1630 -> 566 | 1468, 100 x 512, 64 280 | 745 -> 301 | 636; d = 64: 100 x 512 117 | 284 -> 117 | 268, 64 x 1024 162 | 466 -> 162 | 448.
-template <typename P>
-int64_t sink_groups(const P& p, int bytes, bool bit16) {
-  const int rows = 128 / sink_waves(p, bytes, bit16);
-  return ((int64_t)p.sinks + rows - 1) / rows * p.batch;
-}
-template <typename P>
-int sink_parts(const P& p, int bytes, bool bit16) {
-  const int64_t groups = sink_groups(p, bytes, bit16), most = (p.n_q + 31) / 32 / sink_waves(p, bytes, bit16);
-  int64_t parts = (256 + groups - 1) / groups;
-  if (parts > most) parts = most;
-  return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
-}
-// Partial results; more groups than CUs store their rows directly
-template <typename P>
-size_t sink_bytes(const P& p, int bytes, bool bit16) {
-  return sink_groups(p, bytes, bit16) <= 256 ? (size_t)sink_parts(p, bytes, bit16) * 2 * p.batch * p.sinks * p.d * sizeof(float) : 0;
-}
-
 // Whether the workgroups that sum up the rows of the sinks come at the end of the launch of the key-tiled sweep, where they fill the CUs that its last ones leave idle,
 // and not in a launch of their own. In small launches of the 16-bit kernels: always. On those with 128 rows: at d = 64, where two workgroups of either fit a CU; at d = 128 the sweep is one of producers and
 // consumers, whose workgroups have a CU to themselves. Of split products: where one launch holds both sides. More groups than CUs fill the GPU by themselves, and store their rows
@@ -627,10 +604,10 @@ size_t sink_bytes(const P& p, int bytes, bool bit16) {
 // d = 64, 4 sinks 17.0, 26.9 and 11.6, 21.0, 8 x 1024, d = 128 32.7, 54.3 and 29.9, 48.5; one part: 30 x 75 x 115, fp32, d = 64 21.5, 46.9
 // and 13.9, 33.5, 8 x 36 x 79, fp16, d = 64 11.4, 19.3 and 11.2, 16.2; fp32 8 x 4096, d = 128, 4 sinks 439, 1192 and 411, 1176.
 inline bool sinks_ride(const AttnParams& p, int bytes, bool bit16, int small) {
-  return sink_groups(p, bytes, bit16) <= 256 && (bit16 ? small || p.d == 64 : split_bwd_waves(p, bytes) != 0);
+  return sink_groups(p.batch, p.sinks) <= 256 && (bit16 ? small || p.d == 64 : split_bwd_waves(p, bytes) != 0);
 }
 inline bool sinks_ride(const Params& p, int bytes, bool bit16, int small) {
-  return sink_groups(p, bytes, bit16) <= 256 && (bit16 ? small || p.d == 64 : !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0);
+  return sink_groups(p.batch, p.sinks) <= 256 && (bit16 ? small || p.d == 64 : !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0);
 }
 
 }  // namespace rules

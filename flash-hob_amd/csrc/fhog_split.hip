@@ -548,9 +548,10 @@ constexpr int lds_bytes() {
 template <int WS>
 __host__ __device__ unsigned blocks(int rows, int batch) { return grid_blocks((rows + 128 / WS - 1) / (128 / WS), batch); }
 
-// Waves on the same 32 rows of the sinks
+// Waves on the same 32 rows of the sinks: as many as fit the LDS, four where that leaves room for another workgroup. At d = 64 four of fp32 tensors take 149 KB and, in the launch of
+// both sweeps, 61 registers too many; double-backward 16 x 1024, window 256, us, with four -> two: 33 sinks 147 -> 138, 4 sinks 128 -> 127.
 template <typename T, int D>
-constexpr int sink_waves = rules::split_sink_waves(D, sizeof(T), true, 1);
+constexpr int sink_waves = 2 * lds_bytes<T, D, 4, 4>() <= 160 * 1024 ? 4 : lds_bytes<T, D, 4, 2>() <= 160 * 1024 ? 2 : 1;
 
 // Passes 3 (workgroups [0, q_blocks)) and 4 (the others; mixed: tile by tile in turn) in one launch: given the row statistics neither needs the other. MASK_SINK: behind
 // both come the workgroups that sum up the rows of the sinks (fhog_sinks.hip), where rules::sinks_ride says so.
@@ -672,7 +673,6 @@ hipError_t launch_grads(const Params& p, int sides, hipStream_t s) {
 template <typename T, int D>
 hipError_t launch_sink_grads(const Params& p, hipStream_t s) {
   constexpr int WS = sink_waves<T, D>, smem = lds_bytes<T, D, 4, WS>();
-  static_assert(smem <= 160 * 1024, "stages and exchange buffer have to fit the LDS");
   const hipError_t e = allow_dynamic_lds<split_sink_grads<T, D, WS>>(smem);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((split_sink_grads<T, D, WS>), dim3(blocks<WS>(p.n_k, p.batch * p.n_split)), dim3(256), smem, s, p);
