@@ -386,20 +386,30 @@ inline int sink_sweep_waves(int64_t groups, int d, int bytes, int64_t window) {
   if (d == 64) return groups <= 64 ? 4 : groups <= 128 ? 2 : 1;
   return groups < (d == 32 ? 192 : 256) ? 4 : 1;
 }
-// Workgroups that share 32 sinks of a slice, each with a part of the queries: one for every CU, with a tile for each of its waves at least.
+// Workgroups that share a group of sinks of a slice, each with a part of the queries: one for every CU, with four tiles at least, fp32 d = 128 one for each wave.
 // First | second backward, us, 512 workgroups of eight tiles -> 256 of four: bf16 32 x 4096, d = 128, window 1024, 4 sinks 290 | 678 -> 282 | 675; fp32 16 x 1024, d = 64,
 // window 256, 33 sinks 64.9 | 153 -> 61.7 | 149; 8 x 4096, d = 128 448 | 1401 -> 440 | 1357; 1024 of four 296 | 686, 61.7 | 148, 440 | 1358.
 // Single precision of d = 128 with four tiles at least -> one for each of its two | one waves: 1 x 1000, window 100 41.2 | 123 -> 41.5 | 89.
-inline int64_t sink_groups(int64_t batch, int64_t sinks) { return (sinks + 31) / 32 * batch; }
+// A group is counted as one of 32 sinks, what a workgroup of four waves on the same rows covers. On split products two waves cover 64 (fp32 d = 64 in a double-backward and where two workgroups
+// share a CU, d = 128 in a first backward, 16-bit tensors of d = 128 in a double-backward), so that more than 32 sinks have down to half the workgroups; counted as groups of 64 they gain in some launches
+// and lose in others. 32 -> 64, us: first backward d = 128 64 x 1024, window 256, 100 sinks 450 -> 414, but 20 x 512, 64, 100 72 -> 91, 90 x 1024, 256, 40 535 -> 573; double-backward d = 64
+// 40 x 512, 64, 200 170 -> 150, but 40 x 300, 64, 70 82 -> 93. In a double-backward of fp32 tensors of d = 128 a workgroup has one wave to 32 sinks and 128 in all, and is counted so: 32 -> 128,
+// 16 x 1024, window 256, 33 | 200 sinks 278 | 375 -> 273 | 365, 40 x 512, 64, 40 | 100 | 200 245 | 312 | 467 -> 254 | 283 | 322, 40 x 1024, 256, 200 1089 -> 801, 64 x 1024, 256, 100 1196 -> 1034,
+// 120 x 512, 64, 100 801 -> 735; at most 1.09 times as long (70 x 300, 64, 70 sinks 265 -> 289).
+constexpr int sink_rows(int64_t d, int bytes, bool second) { return second && bytes * d >= 512 ? 128 : 32; }
+inline int64_t sink_groups(int64_t batch, int64_t sinks, int64_t d, int bytes, bool second) {
+  const int rows = sink_rows(d, bytes, second);
+  return (sinks + rows - 1) / rows * batch;
+}
 inline int sink_parts(int64_t batch, int64_t sinks, int64_t n_q, int64_t d, int bytes, bool second) {
-  const int64_t groups = sink_groups(batch, sinks), tiles = (n_q + 31) / 32, waves = bytes * d < 512 ? 4 : second ? 1 : 2;   // on the same rows
+  const int64_t groups = sink_groups(batch, sinks, d, bytes, second), tiles = (n_q + 31) / 32, least = bytes * d < 512 ? 4 : second ? 1 : 2;
   int64_t parts = (256 + groups - 1) / groups;
-  if (parts > tiles / waves) parts = tiles / waves;
+  if (parts > tiles / least) parts = tiles / least;
   return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
 }
 // Partial results; more groups than CUs store their rows directly
 inline size_t sink_bytes(int64_t batch, int64_t sinks, int64_t n_q, int64_t d, int bytes, bool second) {
-  return sink_groups(batch, sinks) <= 256 ? (size_t)sink_parts(batch, sinks, n_q, d, bytes, second) * 2 * batch * sinks * d * sizeof(float) : 0;
+  return sink_groups(batch, sinks, d, bytes, second) <= 256 ? (size_t)sink_parts(batch, sinks, n_q, d, bytes, second) * 2 * batch * sinks * d * sizeof(float) : 0;
 }
 // Forwards of few queries under a mask with sinks: workgroups that share 32 queries of a slice, each with a part of the keys, or 0 for the kernels of longer ones. What
 // a number of parts costs is reckoned up, in us: rounds of the workgroups, each with something to start and to end (fixed) and its waves' tiles one after the
@@ -604,10 +614,10 @@ inline int split_bwd_waves(const AttnParams& p, int bytes) {
 // d = 64, 4 sinks 17.0, 26.9 and 11.6, 21.0, 8 x 1024, d = 128 32.7, 54.3 and 29.9, 48.5; one part: 30 x 75 x 115, fp32, d = 64 21.5, 46.9
 // and 13.9, 33.5, 8 x 36 x 79, fp16, d = 64 11.4, 19.3 and 11.2, 16.2; fp32 8 x 4096, d = 128, 4 sinks 439, 1192 and 411, 1176.
 inline bool sinks_ride(const AttnParams& p, int bytes, bool bit16, int small) {
-  return sink_groups(p.batch, p.sinks) <= 256 && (bit16 ? small || p.d == 64 : split_bwd_waves(p, bytes) != 0);
+  return sink_groups(p.batch, p.sinks, p.d, bytes, false) <= 256 && (bit16 ? small || p.d == 64 : split_bwd_waves(p, bytes) != 0);
 }
 inline bool sinks_ride(const Params& p, int bytes, bool bit16, int small) {
-  return sink_groups(p.batch, p.sinks) <= 256 && (bit16 ? small || p.d == 64 : !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0);
+  return sink_groups(p.batch, p.sinks, p.d, bytes, true) <= 256 && (bit16 ? small || p.d == 64 : !few_rows(p, bytes) && split_grads_waves(p, bytes) != 0);
 }
 
 }  // namespace rules

@@ -2,8 +2,8 @@
 //
 // A key j < sinks is seen by every query from the diagonal on, n_q - j + ... of them, the other keys by a window's length: as rows of an ordinary
 // workgroup of the key-tiled sweep the sinks would keep it busy n_q / window times as long as the others. The sweep therefore treats them as keys of the band, and
-// a launch behind it computes their rows over ALL their queries and puts them in place: workgroups of 32 sinks, four waves on the same rows, the queries
-// dealt out over `parts` workgroups (sink_parts), whose fp32 sums are added here in a fixed order and rounded once. Where they can, those workgroups
+// a launch behind it computes their rows over ALL their queries and puts them in place: workgroups of 32 sinks with four waves on the same rows (of split
+// products also 64 with two and 128 with one, as their terms fit the LDS), the queries dealt out over `parts` workgroups (rules::sink_parts), whose fp32 sums are added here in a fixed order and rounded once. Where they can, those workgroups
 // come last in the launch of the key-tiled sweep itself (rules::sinks_ride).
 #include "fhog_rules.h"
 #include "fhog_split_util.h"

@@ -552,6 +552,7 @@ __host__ __device__ unsigned blocks(int rows, int batch) { return grid_blocks((r
 // both sweeps, 61 registers too many; double-backward 16 x 1024, window 256, us, with four -> two: 33 sinks 147 -> 138, 4 sinks 128 -> 127.
 template <typename T, int D>
 constexpr int sink_waves = 2 * lds_bytes<T, D, 4, 4>() <= 160 * 1024 ? 4 : lds_bytes<T, D, 4, 2>() <= 160 * 1024 ? 2 : 1;
+static_assert(128 / sink_waves<float, 128> == rules::sink_rows(128, 4, true), "the rule for parts counts what a workgroup covers");
 
 // Passes 3 (workgroups [0, q_blocks)) and 4 (the others; mixed: tile by tile in turn) in one launch: given the row statistics neither needs the other. MASK_SINK: behind
 // both come the workgroups that sum up the rows of the sinks (fhog_sinks.hip), where rules::sinks_ride says so.

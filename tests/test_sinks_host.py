@@ -133,3 +133,20 @@ def test_refusals_of_the_python_entry_points():
         with pytest.raises(ValueError, match="sinks"):
             check_sinks(2, schedule)
     assert check_sinks(2, "fused_stats") == check_sinks(2, None) == check_sinks(2, None, True) == 2
+
+
+@pytest.mark.parametrize("dtype, d, impl, second, rows", [(0, 64, 0, False, 32), (0, 128, 0, True, 32), (2, 64, 1, True, 32), (0, 128, 1, True, 32), (0, 32, 0, False, 32), (2, 32, 0, True, 32),
+                                                          (1, 32, 0, True, 32), (1, 64, 0, False, 32), (1, 64, 0, True, 32), (1, 128, 0, False, 32), (1, 128, 0, True, 128)])
+@pytest.mark.parametrize("batch, sinks", [(16, 4), (16, 33), (16, 100), (3, 200), (200, 100), (250, 20), (300, 5)])
+def test_parts_by_the_groups_of_sinks(L, batch, sinks, dtype, d, impl, second, rows):
+    """The queries of the sinks are dealt out so that there is a workgroup for every one of 256 CUs, by groups of 32 sinks and, where one wave sums up 32 of the 128 that a
+    workgroup covers (double-backward, fp32, d = 128), by groups of 128; with more groups than CUs there are no partial results. Read off the
+    workspaces: [part][2][batch][sinks][d] floats."""
+    n = 4096
+    dims = dict(batch=batch, n_q=n, n_k=n, d=d, stride_qn=d, stride_kn=d, stride_qb=n * d, stride_kb=n * d, causal=1, window=1024, dtype=dtype)
+    a = _bwdbwd(impl=impl, **dims) if second else _attn(**dims)
+    got = L.fhog_bwdbwd_sinks_workspace_bytes(ctypes.byref(a), sinks) if second else L.fhog_attn_sinks_workspace_bytes(ctypes.byref(a), sinks, 1)
+    other = (L.fhog_bwdbwd_workspace_hint(ctypes.byref(a)) + 15) // 16 * 16 if second else batch * n * 4
+    groups = batch * -(-sinks // rows)
+    parts = 0 if groups > 256 else -(-256 // groups)
+    assert got - other == parts * 2 * batch * sinks * d * 4
