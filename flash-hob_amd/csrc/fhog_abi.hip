@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <utility>
 
 #include "fhog_common.h"
 #include "fhog_rules.h"
@@ -322,6 +323,135 @@ int validate_rotary(const fhog_rotary_args* a) {
   return FHOG_OK;
 }
 
+bool dtype_known(int dtype) { return dtype == FHOG_DTYPE_BF16 || dtype == FHOG_DTYPE_FP32 || dtype == FHOG_DTYPE_FP16; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+constexpr int64_t kMaxEntries = (int64_t)1 << 30;   // of a sequence
+constexpr int64_t kMaxIndex = (int64_t)INT32_MAX - 255;
+
+// Strides of rows that are read 16 bytes at a time; dimensions of one are never stepped along
+int check_strides(const char* name, int dtype, const int64_t (&size)[3], const int64_t (&stride)[3]) {
+  const int64_t vec = 16 / dtype_bytes(dtype);
+  for (int i = 0; i < 3; i++)
+    if (size[i] > 1 && stride[i] % vec) return fail(FHOG_E_STRIDE, "strides of '%s' must be multiples of %lld elements (16 bytes)", name, (long long)vec);
+  return FHOG_OK;
+}
+int check_pointer(const char* name, const void* p, bool wide) {
+  if (!p) return fail(FHOG_E_NULL, "pointer '%s' is NULL", name);
+  if (wide ? !aligned16(p) : !aligned4(p)) return fail(FHOG_E_ALIGN, "pointer '%s' is not %s-byte aligned", name, wide ? "16" : "4");
+  return FHOG_OK;
+}
+
+int validate_cache(const fhog_paged_cache& c, bool written) {
+  if (!dtype_known(c.dtype)) return fail(FHOG_E_DTYPE, "unknown dtype %d", c.dtype);
+  if (c.d != 32 && c.d != 64 && c.d != 128) return fail(FHOG_E_SHAPE, "head dim %lld not in {32, 64, 128}", (long long)c.d);
+  if (c.batch < 0 || c.heads_k < 1 || c.batch > 65535 || c.heads_k > 65535 || c.batch * c.heads_k > 65535)
+    return fail(FHOG_E_SHAPE, "%lld sequences of %lld heads of keys: expected 1 head or more, and 65535 or fewer of all sequences together", (long long)c.batch, (long long)c.heads_k);
+  if (c.pages < 1 || c.pages > INT32_MAX) return fail(FHOG_E_PAGED, "%lld pages: expected 1 to 2^31 - 1", (long long)c.pages);
+  if (c.page < 1 || c.table_width < 1 || c.page > kMaxEntries || c.table_width > kMaxEntries / c.page)
+    return fail(FHOG_E_PAGED, "pages of %lld entries, %lld to a sequence: expected 1 or more of each, and 2^30 entries or fewer of a sequence", (long long)c.page, (long long)c.table_width);
+  if (const int rc = check_strides("keys", c.dtype, {c.pages, c.heads_k, c.page}, {c.stride_p, c.stride_h, c.stride_n})) return rc;
+  if (c.page > 1 && (c.stride_n < c.d || c.stride_n > kMaxRowStride)) return fail(FHOG_E_STRIDE, "entries of a page have to lie d to 2^24 elements apart (got %lld)", (long long)c.stride_n);
+  if (!rows_apart(c.pages, c.heads_k, c.page, c.d, c.stride_p, c.stride_h, c.stride_n)) return fail(FHOG_E_STRIDE, "entries of the pages overlap");
+  if (c.batch == 0) return FHOG_OK;
+  for (const auto& x : {std::make_pair("keys", c.keys), std::make_pair("values", c.values)})
+    if (const int rc = check_pointer(x.first, x.second, true)) return rc;
+  if (const int rc = check_pointer("table", c.table, false)) return rc;
+  if (const int rc = check_pointer("lengths", c.lengths, false)) return rc;
+  if (written && c.keys == c.values) return fail(FHOG_E_PAGED, "keys and values lie in the same place");
+  return FHOG_OK;
+}
+
+int validate_append(const fhog_paged_append_args* a) {
+  if (!a) return fail(FHOG_E_NULL, "args is NULL");
+  const fhog_paged_cache& c = a->cache;
+  if (const int rc = validate_cache(c, true)) return rc;
+  if (a->n < 0 || a->n > kMaxEntries) return fail(FHOG_E_SHAPE, "n must be 0 to 2^30 (got %lld)", (long long)a->n);
+  if (c.batch == 0 || a->n == 0) return FHOG_OK;
+  if (a->n > kMaxIndex / (c.d * dtype_bytes(c.dtype) / 16) / (c.batch * c.heads_k)) return fail(FHOG_E_SHAPE, "more than 2^31 - 256 pieces of 16 bytes are not supported");
+  if (const int rc = check_strides("k", c.dtype, {c.batch, c.heads_k, a->n}, {a->stride_kb, a->stride_kh, a->stride_kn})) return rc;
+  if (const int rc = check_strides("v", c.dtype, {c.batch, c.heads_k, a->n}, {a->stride_vb, a->stride_vh, a->stride_vn})) return rc;
+  if (const int rc = check_pointer("k", a->k, true)) return rc;
+  if (const int rc = check_pointer("v", a->v, true)) return rc;
+  return a->counts ? check_pointer("counts", a->counts, false) : FHOG_OK;
+}
+
+int validate_paged_attn(const fhog_paged_attn_args* a) {
+  if (!a) return fail(FHOG_E_NULL, "args is NULL");
+  const fhog_paged_cache& c = a->cache;
+  if (const int rc = validate_cache(c, false)) return rc;
+  if (a->heads_q < 1 || a->heads_q > 65535 || a->heads_q % c.heads_k || c.batch * a->heads_q > INT32_MAX / 128)
+    return fail(FHOG_E_SHAPE, "%lld heads of queries and %lld of keys: expected a multiple, 65535 or fewer, and 2^24 - 1 or fewer of all sequences together", (long long)a->heads_q,
+                (long long)c.heads_k);
+  if (!isfinite(a->scale)) return fail(FHOG_E_SCALE, "scale is not finite");
+  if (a->window < 0) return fail(FHOG_E_CAUSAL, "window must be >= 0");
+  if (const int rc = check_sinks(a->sinks)) return rc;
+  const int64_t capacity = c.page * c.table_width;
+  if (c.batch * c.heads_k * ((capacity + 1023) / 1024) > kMaxIndex / 2) return fail(FHOG_E_SHAPE, "more than 2^40 entries of all sequences together are not supported");
+  if (c.batch == 0) return FHOG_OK;
+  if (const int rc = check_strides("q", c.dtype, {c.batch, a->heads_q, 1}, {a->stride_qb, a->stride_qh, 0})) return rc;
+  if (const int rc = check_strides("o", c.dtype, {c.batch, a->heads_q, 1}, {a->stride_ob, a->stride_oh, 0})) return rc;
+  if (!rows_apart(c.batch, a->heads_q, 1, c.d, a->stride_ob, a->stride_oh, 0)) return fail(FHOG_E_STRIDE, "rows of an output overlap");
+  if (const int rc = check_pointer("q", a->q, true)) return rc;
+  if (const int rc = check_pointer("o", a->o, true)) return rc;
+  if (const int rc = check_pointer("lse", a->lse, false)) return rc;
+  if (!a->weights_in != !a->weights_out) return fail(FHOG_E_NULL, "one of weights_in and weights_out is NULL");
+  if (!a->weights_out) return FHOG_OK;
+  if (const int rc = check_pointer("weights_in", a->weights_in, false)) return rc;
+  if (const int rc = check_pointer("weights_out", a->weights_out, false)) return rc;
+  if (!rows_apart(c.batch, c.heads_k, 1, capacity, a->stride_wob, a->stride_woh, 0)) return fail(FHOG_E_STRIDE, "rows of an output overlap");
+  return FHOG_OK;
+}
+
+int validate_key_weights(const fhog_key_weights_args* a) {
+  if (!a) return fail(FHOG_E_NULL, "args is NULL");
+  if (!dtype_known(a->dtype)) return fail(FHOG_E_DTYPE, "unknown dtype %d", a->dtype);
+  if (a->d != 32 && a->d != 64 && a->d != 128) return fail(FHOG_E_SHAPE, "head dim %lld not in {32, 64, 128}", (long long)a->d);
+  if (a->batch < 0 || a->batch > 65535 || a->heads_k < 1 || a->heads_k > 65535 || a->heads_q < 1 || a->heads_q > 65535 || a->heads_q % a->heads_k)
+    return fail(FHOG_E_SHAPE, "%lld sequences, %lld heads of queries and %lld of keys: expected 65535 or fewer, the heads a multiple", (long long)a->batch, (long long)a->heads_q,
+                (long long)a->heads_k);
+  if (a->n_q < 1 || a->n_k < 1 || a->n_q > (1 << 24) || a->n_k > (1 << 24)) return fail(FHOG_E_SHAPE, "n_q/n_k out of range");
+  if ((a->n_q + 63) / 64 * (a->heads_q / a->heads_k) > kMaxIndex / 2) return fail(FHOG_E_SHAPE, "more than 2^36 queries to a head of keys are not supported");
+  if (const int rc = check_mask(a->causal, a->window, a->n_q, a->n_k)) return rc;
+  if (const int rc = check_sinks(a->sinks)) return rc;
+  if (!isfinite(a->scale)) return fail(FHOG_E_SCALE, "scale is not finite");
+  if (a->lengths && a->causal == FHOG_MASK_NONE) return fail(FHOG_E_CAUSAL, "lengths need a causal mask, under which padding comes last");
+  if (a->batch == 0) return FHOG_OK;
+  if (const int rc = check_strides("q", a->dtype, {a->batch, a->heads_q, a->n_q}, {a->stride_qb, a->stride_qh, a->stride_qn})) return rc;
+  if (const int rc = check_strides("k", a->dtype, {a->batch, a->heads_k, a->n_k}, {a->stride_kb, a->stride_kh, a->stride_kn})) return rc;
+  if ((a->n_q > 1 && (a->stride_qn < 0 || a->stride_qn > kMaxRowStride)) || (a->n_k > 1 && (a->stride_kn < 0 || a->stride_kn > kMaxRowStride)))
+    return fail(FHOG_E_STRIDE, "row stride outside 0..2^24 elements");
+  if (const int rc = check_pointer("q", a->q, true)) return rc;
+  if (const int rc = check_pointer("k", a->k, true)) return rc;
+  if (const int rc = check_pointer("lse", a->lse, false)) return rc;
+  if (const int rc = check_pointer("out", a->out, false)) return rc;
+  if (a->lengths)
+    if (const int rc = check_pointer("lengths", a->lengths, false)) return rc;
+  if (!rows_apart(a->batch, a->heads_k, 1, a->n_k, a->stride_ob, a->stride_oh, 0)) return fail(FHOG_E_STRIDE, "rows of an output overlap");
+  return FHOG_OK;
+}
+
+int validate_evict(const fhog_paged_evict_args* a) {
+  if (!a) return fail(FHOG_E_NULL, "args is NULL");
+  const fhog_paged_cache& c = a->cache;
+  if (const int rc = validate_cache(c, true)) return rc;
+  if (a->budget < 1 || a->budget > kMaxEntries) return fail(FHOG_E_PAGED, "budget must be 1 to 2^30 (got %lld)", (long long)a->budget);
+  if (a->sinks < 0 || a->recent < 0 || a->sinks > a->budget || a->recent > a->budget - a->sinks)
+    return fail(FHOG_E_PAGED, "sinks (%lld) and recent (%lld) must be >= 0 and within the budget (%lld) together", (long long)a->sinks, (long long)a->recent, (long long)a->budget);
+  const int64_t capacity = c.page * c.table_width, rows = std::min(a->budget, capacity);
+  if (a->into_width < 1 || a->into_width > kMaxEntries / c.page || a->into_width * c.page < rows)
+    return fail(FHOG_E_PAGED, "'into' has %lld pages of %lld entries: expected room for %lld", (long long)a->into_width, (long long)c.page, (long long)rows);
+  if (rows * (c.d * dtype_bytes(c.dtype) / 16) > kMaxIndex) return fail(FHOG_E_SHAPE, "more than 2^31 - 256 pieces of 16 bytes to a head are not supported");
+  if (c.batch == 0) return FHOG_OK;
+  const void* ptrs[] = {a->weights, a->into, a->lengths_out, a->kept, a->weights_out};
+  const char* names[] = {"weights", "into", "lengths_out", "kept", "weights_out"};
+  for (int i = 0; i < 5; i++)
+    if (const int rc = check_pointer(names[i], ptrs[i], false)) return rc;
+  if (a->weights == a->weights_out) return fail(FHOG_E_PAGED, "weights_out is the array 'weights'");
+  if (a->into == c.table) return fail(FHOG_E_PAGED, "'into' is the table of the cache: entries would be written over others that are still to be read");
+  if (a->lengths_out == c.lengths) return fail(FHOG_E_PAGED, "lengths_out are the lengths of the cache, which are still being read");
+  return FHOG_OK;
+}
+
 // Address of `scratch` on the current device, looked up once per device (the first call there) and kept.
 constexpr int kMaxDevices = 64;
 std::atomic<void*> g_scratch_ptr[kMaxDevices];
@@ -534,6 +664,60 @@ int fhog_rotary(const fhog_rotary_args* args, void* hip_stream) {
   if (args->batch == 0 || args->n == 0) return FHOG_OK;
   const hipError_t e = fhog::launch_rotary(args, (hipStream_t)hip_stream);
   if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "rotary positions: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
+
+size_t fhog_paged_append_args_size(void) { return sizeof(fhog_paged_append_args); }
+
+int fhog_paged_append_validate(const fhog_paged_append_args* args) { return validate_append(args); }
+
+int fhog_paged_append(const fhog_paged_append_args* args, void* hip_stream) {
+  if (const int rc = validate_append(args)) return rc;
+  if (args->cache.batch == 0 || args->n == 0) return FHOG_OK;
+  const hipError_t e = fhog::launch_paged_append(args, (hipStream_t)hip_stream);
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "paged append: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
+
+size_t fhog_paged_attn_args_size(void) { return sizeof(fhog_paged_attn_args); }
+
+int fhog_paged_attn_validate(const fhog_paged_attn_args* args) { return validate_paged_attn(args); }
+
+size_t fhog_paged_attn_workspace_bytes(const fhog_paged_attn_args* args) { return validate_paged_attn(args) == FHOG_OK && args->cache.batch ? fhog::paged_attn_bytes(args) : 0; }
+
+int fhog_paged_attn(const fhog_paged_attn_args* args, void* hip_stream) {
+  if (const int rc = validate_paged_attn(args)) return rc;
+  if (args->cache.batch == 0) return FHOG_OK;
+  if (const int rc = check_ws(args->ws, args->ws_bytes, fhog::paged_attn_bytes(args))) return rc;
+  const hipError_t e = fhog::launch_paged_attn(args, (hipStream_t)hip_stream);
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "paged attention: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
+
+size_t fhog_key_weights_args_size(void) { return sizeof(fhog_key_weights_args); }
+
+int fhog_key_weights_validate(const fhog_key_weights_args* args) { return validate_key_weights(args); }
+
+size_t fhog_key_weights_workspace_bytes(const fhog_key_weights_args* args) { return validate_key_weights(args) == FHOG_OK && args->batch ? fhog::key_weights_bytes(args) : 0; }
+
+int fhog_key_weights(const fhog_key_weights_args* args, void* hip_stream) {
+  if (const int rc = validate_key_weights(args)) return rc;
+  if (args->batch == 0) return FHOG_OK;
+  if (const int rc = check_ws(args->ws, args->ws_bytes, fhog::key_weights_bytes(args))) return rc;
+  const hipError_t e = fhog::launch_key_weights(args, (hipStream_t)hip_stream);
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "weights of keys: HIP error %d (%s)", (int)e, hipGetErrorString(e));
+  return FHOG_OK;
+}
+
+size_t fhog_paged_evict_args_size(void) { return sizeof(fhog_paged_evict_args); }
+
+int fhog_paged_evict_validate(const fhog_paged_evict_args* args) { return validate_evict(args); }
+
+int fhog_paged_evict(const fhog_paged_evict_args* args, void* hip_stream) {
+  if (const int rc = validate_evict(args)) return rc;
+  if (args->cache.batch == 0) return FHOG_OK;
+  const hipError_t e = fhog::launch_paged_evict(args, (hipStream_t)hip_stream);
+  if (e != hipSuccess) return fail(FHOG_E_LAUNCH, "paged eviction: HIP error %d (%s)", (int)e, hipGetErrorString(e));
   return FHOG_OK;
 }
 

@@ -167,6 +167,13 @@ hipError_t launch_join_forward(const AttnParams& p, int dtype, hipStream_t s);  
 hipError_t launch_sink_keys(const AttnParams& p, int dtype, bool swept, hipStream_t s);
 hipError_t launch_sink_keys(const Params& p, int dtype, bool split_products, bool swept, hipStream_t s);
 hipError_t launch_rotary(const fhog_rotary_args* a, hipStream_t s);
+// A cache in pages (fhog_paged.hip, fhog_paged_attn.hip) and the weights of a prompt's keys (fhog_key_weights.hip); workspaces in bytes
+hipError_t launch_paged_append(const fhog_paged_append_args* a, hipStream_t s);
+hipError_t launch_paged_evict(const fhog_paged_evict_args* a, hipStream_t s);
+hipError_t launch_paged_attn(const fhog_paged_attn_args* a, hipStream_t s);
+size_t paged_attn_bytes(const fhog_paged_attn_args* a);
+hipError_t launch_key_weights(const fhog_key_weights_args* a, hipStream_t s);
+size_t key_weights_bytes(const fhog_key_weights_args* a);
 hipError_t launch_mfma_rate(float* out, int blocks, int trips, int data_mode, int waves, hipStream_t s);  // measurement aid
 bool bf16_shape_supported(int64_t n_q, int64_t n_k, int64_t d, int causal);
 

@@ -1,0 +1,62 @@
+// What the kernels on a cache in pages share: where an entry lies, and which tiles of its entries a token sees.
+#pragma once
+#include "fhog_common.h"
+
+namespace fhog {
+namespace paged {
+
+// j / page for 0 <= j < 2^31 without a division: with s = ceil(log2 page) and M = floor(2^(31 + s) / page) + 1 the error M page - 2^(31 + s) is at most page <= 2^s, and
+// j times it below 2^(31 + s)
+struct Divisor {
+  uint32_t by = 1, mul = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t page) : by(page) {
+    while (((uint64_t)1 << shift) < page) shift++;
+    mul = (uint32_t)(((uint64_t)1 << (31 + shift)) / page + 1);
+  }
+  __host__ __device__ __forceinline__ uint32_t operator()(uint32_t j) const { return (uint32_t)(((uint64_t)(2 * j) * mul) >> 32) >> shift; }
+};
+
+struct Cache {
+  char* keys;
+  char* values;
+  const int32_t* table;
+  const int32_t* lengths;
+  int64_t stride_p, stride_h, stride_n;   // in bytes
+  int64_t stride_tb;
+  Divisor page;
+  int32_t pages, width, capacity, heads_k, batch;
+  // entries of sequence b
+  __device__ __forceinline__ int length(int b) const { return max(0, min(lengths[b], capacity)); }
+};
+
+inline Cache cache_of(const fhog_paged_cache& c) {
+  const int es = c.dtype == FHOG_DTYPE_FP32 ? 4 : 2;
+  Cache r;
+  r.keys = (char*)c.keys, r.values = (char*)c.values, r.table = c.table, r.lengths = c.lengths;
+  r.stride_p = c.stride_p * es, r.stride_h = c.stride_h * es, r.stride_n = c.stride_n * es, r.stride_tb = c.stride_tb;
+  r.page = Divisor((uint32_t)c.page);
+  r.pages = (int32_t)c.pages, r.width = (int32_t)c.table_width, r.capacity = (int32_t)(c.table_width * c.page), r.heads_k = (int32_t)c.heads_k, r.batch = (int32_t)c.batch;
+  return r;
+}
+
+// The tiles of T entries of which a token sees some, in a row: those of the sinks that lie before its window, then the window's
+template <int T>
+struct Seen {
+  int n, lo, sinks;     // entry j is seen iff j < n and (j >= lo or j < sinks)
+  int first, skip, tiles;
+  __device__ __forceinline__ Seen(int n_, int window, int sinks_) : n(n_) {
+    lo = window > 0 ? max(0, n - window) : 0;
+    sinks = min(sinks_, lo);
+    const int all = (n + T - 1) / T;
+    first = (sinks + T - 1) / T;
+    skip = max(first, lo / T) - first;      // tiles between the two
+    tiles = all - skip;
+  }
+  __device__ __forceinline__ int at(int i) const { return (i < first ? i : i + skip) * T; }
+  __device__ __forceinline__ bool sees(int j) const { return j < n && (j >= lo || j < sinks); }
+  __device__ __forceinline__ bool whole(int j0) const { return j0 + T <= n && (j0 >= lo || j0 + T <= sinks); }
+};
+
+}  // namespace paged
+}  // namespace fhog

@@ -1,0 +1,201 @@
+// New entries into a cache in pages, and the eviction of the entries of the least weight (include/fhog_hip.h).
+//
+// Both move rows: nothing is computed on them, and what bounds them is memory, every row in and out once, 16 bytes to a lane.
+#include "fhog_paged.h"
+
+namespace fhog {
+namespace {
+
+using namespace paged;
+constexpr int kThreads = 256;
+
+struct Append {
+  Cache c;
+  const char* k;
+  const char* v;
+  const int32_t* counts;
+  int64_t kb, kh, kn, vb, vh, vn;   // strides in bytes
+  Divisor chunks, tokens, heads;    // of a row; n; heads of keys
+  uint32_t total;
+};
+
+// A thread has one chunk of a key and of its value: (sequence, head, token, chunk), the last one fastest
+__global__ void __launch_bounds__(kThreads) append_entries(Append a) {
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  if (id >= a.total) return;
+  uint32_t rest = a.chunks(id);
+  const uint32_t chunk = id - rest * a.chunks.by;
+  uint32_t row = a.tokens(rest);
+  const int t = (int)(rest - row * a.tokens.by);
+  const uint32_t b = a.heads(row), h = row - b * a.heads.by;
+  const int n = a.c.length(b), count = min(a.counts ? max(0, a.counts[b]) : (int)a.tokens.by, min((int)a.tokens.by, n));
+  if (t >= count) return;
+  const u32x4_t k = *reinterpret_cast<const u32x4_t*>(a.k + b * a.kb + h * a.kh + t * a.kn + chunk * 16);
+  const u32x4_t v = *reinterpret_cast<const u32x4_t*>(a.v + b * a.vb + h * a.vh + t * a.vn + chunk * 16);
+  const uint32_t j = n - count + t, at = a.c.page(j);
+  const int32_t page = a.c.table[b * a.c.stride_tb + at];
+  if ((uint32_t)page >= (uint32_t)a.c.pages) return;
+  const int64_t to = page * a.c.stride_p + h * a.c.stride_h + (j - at * a.c.page.by) * a.c.stride_n + chunk * 16;
+  *reinterpret_cast<u32x4_t*>(a.c.keys + to) = k;
+  *reinterpret_cast<u32x4_t*>(a.c.values + to) = v;
+}
+
+// ---- eviction ---------------------------------------------------------------------------------------------------------
+struct Evict {
+  Cache c;
+  const float* weights;
+  const int32_t* into;
+  int32_t* lengths_out;
+  int32_t* kept;
+  float* weights_out;
+  int64_t wb, wh, ib;
+  int64_t budget;
+  int32_t rows;             // rows that may stay: min(budget, capacity)
+  int32_t sinks, recent, into_width;
+  Divisor chunks;           // of a row
+};
+
+constexpr int kSelect = 1024, kWaves = kSelect / 64;
+
+// A number for each entry that grows with the order in which entries stay: what is protected first, then by weight, NaN last
+__device__ __forceinline__ uint32_t rank_of(float w, int j, int n, const Evict& e) {
+  if (j < e.sinks || j >= n - e.recent) return 0xffffffffu;
+  if (w != w) return 0;
+  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.f);   // -0 becomes 0
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Which entries of one sequence and head of keys stay. The rank of the last one that does is found digit by digit, eight bits at a time from the top: a histogram
+// of the digit over the entries whose higher digits are those found so far, and the digit at which the sum from above reaches what is still to be
+// found. Then the entries that stay are counted wave by wave, each wave a stretch of its own, and written to the places that the counts give.
+__global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
+  __shared__ uint32_t histogram[256];
+  __shared__ uint32_t found[2];               // digits so far; how many of the entries of that rank stay
+  __shared__ int counts[2][kWaves];           // entries of a wave's stretch above the rank, and of the rank itself
+  const int b = blockIdx.x / e.c.heads_k, h = blockIdx.x - b * e.c.heads_k, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = e.c.length(b), m = (int)min((int64_t)n, e.budget);
+  const float* const w = e.weights + b * e.wb + h * e.wh;
+  int32_t* const kept = e.kept + (int64_t)blockIdx.x * e.budget;
+  float* const out = e.weights_out + (int64_t)blockIdx.x * e.c.capacity;
+  if (h == 0 && tid == 0) e.lengths_out[b] = m;
+  for (int64_t i = m + tid; i < e.budget; i += kSelect) kept[i] = -1;
+  for (int i = m + tid; i < e.c.capacity; i += kSelect) out[i] = 0.f;
+  uint32_t rank = 0;
+  int ties = n;
+  if (m < n) {
+    uint32_t above = 0;
+    int need = m;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) histogram[tid] = 0;
+      __syncthreads();
+      for (int j0 = wave * 64; j0 < n; j0 += kSelect) {
+        const int j = j0 + lane;
+        const uint32_t r = j < n ? rank_of(w[j], j, n, e) : 0;
+        const bool in = j < n && (shift == 24 || r >> (shift + 8) == above);
+        const uint32_t digit = r >> shift & 255;
+        const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+        if (who == 0) continue;
+        // one addition where all lanes have the same digit, as they do where many weights are equal
+        const uint32_t one = __builtin_amdgcn_readlane(digit, __builtin_ctzll(who));
+        if (__builtin_amdgcn_ballot_w64(in && digit != one) == 0) {
+          if (lane == 0) atomicAdd(&histogram[one], (uint32_t)__builtin_popcountll(who));
+        } else if (in) {
+          atomicAdd(&histogram[digit], 1u);
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {
+        // lane l has the digits 4 l .. 4 l + 3; sum of the digits from there up
+        uint32_t c[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum += c[i] = histogram[4 * lane + i];
+        uint32_t up = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const uint32_t other = __shfl_down(up, d);
+          up += lane + d < 64 ? other : 0;
+        }
+        uint32_t over = up - sum;   // entries of higher digits than this lane's
+        if (over < (uint32_t)need && up >= (uint32_t)need) {   // one lane alone
+          int i = 3;
+          while (over + c[i] < (uint32_t)need) over += c[i], i--;
+          found[0] = above << 8 | (4 * lane + i), found[1] = need - over;
+        }
+      }
+      __syncthreads();
+      above = found[0], need = (int)found[1];
+    }
+    rank = above, ties = need;
+  }
+  const int stretch = ((n + kWaves - 1) / kWaves + 63) & ~63, begin = min(n, wave * stretch), end = min(n, begin + stretch);
+  int over = 0, same = 0;
+  for (int j0 = begin; j0 < end; j0 += 64) {
+    const int j = j0 + lane;
+    const uint32_t r = j < end ? rank_of(w[j], j, n, e) : 0;
+    over += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j < end && r > rank));
+    same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j < end && r == rank));
+  }
+  if (lane == 0) counts[0][wave] = over, counts[1][wave] = same;
+  __syncthreads();
+  over = same = 0;
+  for (int i = 0; i < wave; i++) over += counts[0][i], same += counts[1][i];
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  for (int j0 = begin; j0 < end; j0 += 64) {
+    const int j = j0 + lane;
+    const float x = j < end ? w[j] : 0.f;
+    const uint32_t r = j < end ? rank_of(x, j, n, e) : 0;
+    const uint64_t o = __builtin_amdgcn_ballot_w64(j < end && r > rank), s = __builtin_amdgcn_ballot_w64(j < end && r == rank);
+    const int same_before = same + __builtin_popcountll(s & below), at = over + __builtin_popcountll(o & below) + min(same_before, ties);
+    if (j < end && (r > rank || (r == rank && same_before < ties))) kept[at] = j, out[at] = x;
+    over += __builtin_popcountll(o), same += __builtin_popcountll(s);
+  }
+}
+
+// The rows that stay, to their new places: a thread has one chunk of a key and of its value
+__global__ void __launch_bounds__(kThreads) move_entries(Evict e) {
+  const int b = blockIdx.y / e.c.heads_k, h = blockIdx.y - b * e.c.heads_k;
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x, i = e.chunks(id), chunk = id - i * e.chunks.by;
+  if (i >= (uint32_t)min(e.c.length(b), e.rows)) return;
+  const uint32_t j = e.kept[(int64_t)blockIdx.y * e.budget + i], at = e.c.page(j), to = e.c.page(i);
+  const int32_t from_page = e.c.table[b * e.c.stride_tb + at], to_page = e.into[b * e.ib + to];
+  if ((uint32_t)from_page >= (uint32_t)e.c.pages || (uint32_t)to_page >= (uint32_t)e.c.pages) return;
+  const int64_t inside = h * e.c.stride_h + chunk * 16;
+  const int64_t src = from_page * e.c.stride_p + (j - at * e.c.page.by) * e.c.stride_n + inside, dst = to_page * e.c.stride_p + (i - to * e.c.page.by) * e.c.stride_n + inside;
+  const u32x4_t k = *reinterpret_cast<const u32x4_t*>(e.c.keys + src), v = *reinterpret_cast<const u32x4_t*>(e.c.values + src);
+  *reinterpret_cast<u32x4_t*>(e.c.keys + dst) = k;
+  *reinterpret_cast<u32x4_t*>(e.c.values + dst) = v;
+}
+
+uint32_t row_chunks(const fhog_paged_cache& c) { return (uint32_t)(c.d * (c.dtype == FHOG_DTYPE_FP32 ? 4 : 2) / 16); }
+
+}  // namespace
+
+hipError_t launch_paged_append(const fhog_paged_append_args* a, hipStream_t s) {
+  Append p;
+  const int es = a->cache.dtype == FHOG_DTYPE_FP32 ? 4 : 2;
+  p.c = cache_of(a->cache), p.k = (const char*)a->k, p.v = (const char*)a->v, p.counts = a->counts;
+  p.kb = a->stride_kb * es, p.kh = a->stride_kh * es, p.kn = a->stride_kn * es, p.vb = a->stride_vb * es, p.vh = a->stride_vh * es, p.vn = a->stride_vn * es;
+  p.chunks = Divisor(row_chunks(a->cache)), p.tokens = Divisor((uint32_t)a->n), p.heads = Divisor((uint32_t)a->cache.heads_k);
+  p.total = (uint32_t)(a->cache.batch * a->cache.heads_k * a->n * p.chunks.by);
+  hipLaunchKernelGGL(append_entries, dim3((p.total + kThreads - 1) / kThreads), dim3(kThreads), 0, s, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_evict(const fhog_paged_evict_args* a, hipStream_t s) {
+  Evict e;
+  e.c = cache_of(a->cache), e.weights = a->weights, e.into = a->into, e.lengths_out = a->lengths_out, e.kept = a->kept, e.weights_out = a->weights_out;
+  e.wb = a->stride_wb, e.wh = a->stride_wh, e.ib = a->stride_ib, e.budget = a->budget;
+  e.rows = (int32_t)(a->budget < e.c.capacity ? a->budget : e.c.capacity);
+  // beyond the capacity all entries are protected either way
+  e.sinks = (int32_t)(a->sinks < e.c.capacity ? a->sinks : e.c.capacity), e.recent = (int32_t)(a->recent < e.c.capacity ? a->recent : e.c.capacity);
+  e.into_width = (int32_t)a->into_width, e.chunks = Divisor(row_chunks(a->cache));
+  const unsigned slices = (unsigned)(a->cache.batch * a->cache.heads_k);
+  hipLaunchKernelGGL(select_entries, dim3(slices), dim3(kSelect), 0, s, e);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || e.rows == 0) return err;
+  hipLaunchKernelGGL(move_entries, dim3((unsigned)(((int64_t)e.rows * e.chunks.by + kThreads - 1) / kThreads), slices), dim3(kThreads), 0, s, e);
+  return hipGetLastError();
+}
+
+}  // namespace fhog

@@ -1,0 +1,466 @@
+// Attention of one new token of each sequence over a cache in pages.
+//
+//   s_hj = scale q_h . k_gj, L_h = ln sum_j exp s_hj, O_h = sum_j exp(s_hj - L_h) v_gj;   W'_gj = W_gj + sum_(h of g) exp(s_hj - L_h)
+//
+// over the entries j that the token sees; g: the head of keys that head h of queries belongs to.
+//
+// What bounds it: memory, every key and value once (4 flop to a byte with one head of queries to one of keys, 64 with 16). So nothing goes through LDS: a wave takes
+// tiles of its own, keys and values straight into the registers that the matrix instructions read, and the waves meet only at the end.
+//
+// A tile is 32 entries (16 of fp32). The heads of queries of a head of keys are the columns, up to 16 of them; more take workgroups of their own. S^T = K Q^T
+// with 16x16 products: lane l has row l % 16 of K, 16 bytes at a time, and gets column l % 16 of S^T, entries 4 (l / 16) + 0..3 of each 16. These are, with
+// the entries counted in that order, the B operand of O^T = V^T P^T as they lie. Its A operand wants a channel to a lane and entries along it. A lane
+// therefore loads the entries of its own group (l / 16), channels c (l % 16) .. + c - 1 with c = d / 16, which fills a row of a page with 16 lanes, and turns the
+// 8 x c block that it has in its own registers: product i of c takes channel c m + i as its row m, so the results of a lane are c consecutive channels.
+#include <algorithm>
+
+#include "fhog_paged.h"
+
+namespace fhog {
+namespace {
+
+using namespace paged;
+constexpr int kThreads = 256, kWaves = 4, kColumns = 16;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Token {
+  Cache c;
+  const char* q;
+  char* o;
+  float* lse;
+  const float* weights_in;
+  float* weights_out;
+  int64_t qb, qh, ob, oh;          // in bytes
+  int64_t wib, wih, wob, woh;
+  int32_t heads_q, group, columns; // group: heads of queries of a head of keys; columns: workgroups that they take
+  int32_t window, sinks;
+  int32_t splits, least;           // workgroups to a sequence and head of keys, at most; tiles to one of them, at least
+  float scale_log2;
+  float* part;                     // [split][batch * heads_q][d]
+  f32x2_t* stats;                  // [split][batch * heads_q]: maximum in log2 units, sum
+  float* scores;                   // [batch * heads_q][row]: scores in log2 units of the entries that are seen
+  int64_t row;
+};
+
+// Parts into which the tiles of a sequence go: as many as leave each `least`, the same number in every kernel
+__device__ __forceinline__ int parts_of(int tiles, const Token& t) { return min(t.splits, (tiles + t.least - 1) / t.least); }
+
+template <int DT>
+struct Type;   // by FHOG_DTYPE_*
+template <>
+struct Type<FHOG_DTYPE_BF16> {
+  typedef __bf16 T;
+};
+template <>
+struct Type<FHOG_DTYPE_FP16> {
+  typedef _Float16 T;
+};
+template <>
+struct Type<FHOG_DTYPE_FP32> {
+  typedef float T;
+};
+
+template <int BYTES>
+struct Words {
+  typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4)));
+};
+template <>
+struct Words<4> {
+  typedef uint32_t type;
+};
+template <int W>
+__device__ __forceinline__ uint32_t word(const typename Words<4 * W>::type& v, int i) {
+  if constexpr (W == 1) return v;
+  else return v[i];
+}
+
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
+template <int DT>
+__device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
+  if constexpr (DT == FHOG_DTYPE_FP16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// The bits of a vector's element as a number; handed over by value: of an element itself __builtin_bit_cast takes the vector's first
+__device__ __forceinline__ float number(uint32_t bits) { return __builtin_bit_cast(float, bits); }
+template <int DT>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  typedef typename Type<DT>::T T;
+  typedef T pair __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, pair{(T)lo, (T)hi});
+}
+
+// PAGES16: pages of a multiple of 16 entries, so that 16 in a row share one. WEIGHTS: scores are kept.
+template <int DT, int D, bool PAGES16, bool WEIGHTS>
+__global__ void __launch_bounds__(kThreads) attend(Token t) {
+  constexpr bool WIDE = DT == FHOG_DTYPE_FP32;
+  typedef typename Type<DT>::T T;
+  constexpr int TILE = WIDE ? 16 : 32, SUB = TILE / 16;   // entries of a tile; 16 at a time
+  constexpr int STEPS = D * (int)sizeof(T) / 64;          // 16-byte pieces of a row that a lane has (four lanes to a row)
+  constexpr int C = D / 16;                               // channels of a lane in V and O
+  constexpr int VB = C * sizeof(T), VW = VB >= 16 ? 4 : VB / 4, VN = VB >= 16 ? VB / 16 : 1;   // bytes of them, words of a load, loads
+  typedef typename Words<4 * VW>::type VWord;
+  __shared__ float tops[kWaves][kColumns], sums[kWaves][kColumns];
+  __shared__ float rows[kWaves][kColumns][D + 4];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, quarter = lane >> 4;
+  const int split = blockIdx.x, b = blockIdx.z, g = blockIdx.y / t.columns, first_head = (blockIdx.y - g * t.columns) * kColumns;
+  const int heads = min(kColumns, t.group - first_head);
+  const int64_t row0 = (int64_t)b * t.heads_q + g * t.group + first_head;   // of (batch * heads_q)
+  const Seen<TILE> seen(t.c.length(b), t.window, t.sinks);
+  const int parts = parts_of(seen.tiles, t);
+  if (split >= max(parts, 1)) return;
+
+  u32x4_t q[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; s++) {
+    q[s] = u32x4_t{0, 0, 0, 0};
+    if (m < heads) q[s] = *reinterpret_cast<const u32x4_t*>(t.q + b * t.qb + (int64_t)(g * t.group + first_head + m) * t.qh + s * 64 + quarter * 16);
+  }
+  float top = -INFINITY, sum = 0.f;   // of column m; the sum is this lane's share
+  f32x4_t acc[C];
+#pragma unroll
+  for (int i = 0; i < C; i++) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const int begin = parts ? (int)((int64_t)seen.tiles * split / parts) : 0, end = parts ? (int)((int64_t)seen.tiles * (split + 1) / parts) : 0;
+  const int32_t* const table = t.c.table + b * t.c.stride_tb;
+  const char* const keys = t.c.keys + (int64_t)g * t.c.stride_h;
+  const char* const values = t.c.values + (int64_t)g * t.c.stride_h;
+  // a lane's bytes from the first of 16 entries that lie in a row
+  const uint32_t stride = (uint32_t)t.c.stride_n, key_off = m * stride + quarter * 16;
+  uint32_t value_off[4];
+#pragma unroll
+  for (int x = 0; x < 4; x++) value_off[x] = (4 * quarter + x) * stride + m * VB;
+  for (int i = begin + wave; i < end; i += kWaves) {
+    const int j0 = seen.at(i);
+    u32x4_t k[SUB][STEPS];
+    VWord v[SUB][4][VN];
+    bool there[SUB][4];                 // whether the entries of this lane's values are there; `hidden`: some of the tile's are not, the same for the wave
+    bool hidden = !seen.whole(j0);
+    if constexpr (PAGES16) {
+      int64_t base[SUB];                // of 16 entries, from the pool's head g
+      bool found[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; u++) {
+        const uint32_t j = j0 + 16 * u, p = __builtin_amdgcn_readfirstlane(t.c.page(j));
+        int32_t page = -1;
+        if ((int)j < seen.n) page = table[p];
+        page = __builtin_amdgcn_readfirstlane(page);
+        found[u] = (uint32_t)page < (uint32_t)t.c.pages;
+        hidden = hidden || !found[u];
+        base[u] = page * t.c.stride_p + (j - p * t.c.page.by) * t.c.stride_n;
+      }
+      const auto read = [&](auto sees) {
+#pragma unroll
+        for (int u = 0; u < SUB; u++) {
+          const bool ok = sees(u, m);
+#pragma unroll
+          for (int s = 0; s < STEPS; s++) k[u][s] = ok ? *reinterpret_cast<const u32x4_t*>(keys + base[u] + key_off + s * 64) : u32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; u++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            there[u][x] = sees(u, 4 * quarter + x);
+#pragma unroll
+            for (int y = 0; y < VN; y++) v[u][x][y] = there[u][x] ? *reinterpret_cast<const VWord*>(values + base[u] + value_off[x] + y * 16) : VWord(0u);
+          }
+      };
+      if (!hidden) read([](int, int) { return true; });
+      else read([&](int u, int at) { return found[u] && seen.sees(j0 + 16 * u + at); });
+    } else {
+      int64_t key_at[SUB], value_at[SUB][4];   // in bytes from the pool's head g; -1: nowhere, or not seen
+#pragma unroll
+      for (int u = 0; u < SUB; u++) {
+        const int j = j0 + 16 * u + m;
+        const uint32_t p = t.c.page(j);
+        const int32_t page = seen.sees(j) ? table[p] : -1;
+        const bool ok = (uint32_t)page < (uint32_t)t.c.pages;
+        key_at[u] = ok ? page * t.c.stride_p + (j - p * t.c.page.by) * t.c.stride_n : -1;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const int from = 4 * quarter + x;
+          value_at[u][x] = (int64_t)((uint64_t)(uint32_t)__shfl((int)(key_at[u] >> 32), from) << 32 | (uint32_t)__shfl((int)key_at[u], from));
+        }
+        hidden = hidden || __builtin_amdgcn_ballot_w64(!ok) != 0;
+      }
+      const auto read = [&](auto ok) {
+#pragma unroll
+        for (int u = 0; u < SUB; u++) {
+          const bool here = ok(key_at[u]);
+#pragma unroll
+          for (int s = 0; s < STEPS; s++) k[u][s] = here ? *reinterpret_cast<const u32x4_t*>(keys + key_at[u] + quarter * 16 + s * 64) : u32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; u++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            there[u][x] = ok(value_at[u][x]);
+#pragma unroll
+            for (int y = 0; y < VN; y++) v[u][x][y] = there[u][x] ? *reinterpret_cast<const VWord*>(values + value_at[u][x] + m * VB + y * 16) : VWord(0u);
+          }
+      };
+      if (!hidden) read([](int64_t) { return true; });
+      else read([](int64_t at) { return at >= 0; });
+    }
+    // S^T of the tile, in log2 units
+    f32x4_t x[SUB];
+#pragma unroll
+    for (int u = 0; u < SUB; u++) {
+      f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < STEPS; c++) {
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(number(k[u][c][e]), number(q[c][e]), s, 0, 0, 0);
+        } else {
+          s = mfma16<DT>(k[u][c], q[c], s);
+        }
+      }
+      x[u] = s * t.scale_log2;
+      if (hidden) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[u][e] = there[u][e] ? x[u][e] : -INFINITY;   // the entries of this lane's values are those of its scores
+      }
+      if (WEIGHTS && m < heads) *reinterpret_cast<f32x4_t*>(t.scores + (row0 + m) * t.row + j0 + 16 * u + 4 * quarter) = x[u];
+    }
+    float high = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
+    if constexpr (SUB == 2) high = fmaxf(high, fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    high = fmaxf(high, __shfl_xor(high, 16));
+    high = fmaxf(high, __shfl_xor(high, 32));
+    // The reference of the exponentials follows the maximum only in jumps of more than 8 (in log2 units): weights may then reach 2^8, which costs no precision,
+    // and the sums are scaled again only now and then
+    const float next = high > top + 8.f ? high : top;
+    const float ref = next == -INFINITY ? 0.f : next;   // a column that has seen nothing yet
+    if (__builtin_amdgcn_ballot_w64(next > top) != 0) {
+      const float by = __builtin_amdgcn_exp2f(top - ref);
+      sum *= by;
+#pragma unroll
+      for (int c = 0; c < C; c++) acc[c] *= by;
+    }
+    top = next;
+#pragma unroll
+    for (int u = 0; u < SUB; u++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        x[u][e] = __builtin_amdgcn_exp2f(x[u][e] - ref);
+        sum += x[u][e];
+      }
+    // O^T += V^T P^T
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int c = 0; c < C; c++) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(number(word<VW>(v[0][e][c / VW], c % VW)), x[0][e], acc[c], 0, 0, 0);
+    } else {
+      // weights are rounded to the type of the values, which are products' other factor: 2^-9 of a weight in bf16, as in attention over whole tensors
+      const u32x4_t p = {pack<DT>(x[0][0], x[0][1]), pack<DT>(x[0][2], x[0][3]), pack<DT>(x[SUB - 1][0], x[SUB - 1][1]), pack<DT>(x[SUB - 1][2], x[SUB - 1][3])};
+#pragma unroll
+      for (int c = 0; c < C; c += 2) {
+        const int w = c / 2;   // the word of channels c, c + 1
+        u32x4_t even, odd;
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          const uint32_t lo = word<VW>(v[y / 2][2 * (y % 2)][0], w), hi = word<VW>(v[y / 2][2 * (y % 2) + 1][0], w);
+          even[y] = __builtin_amdgcn_perm(hi, lo, 0x05040100), odd[y] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+        }
+        acc[c] = mfma16<DT>(even, p, acc[c]);
+        acc[c + 1] = mfma16<DT>(odd, p, acc[c + 1]);
+      }
+    }
+  }
+
+  // The waves' results on one maximum, joined in their order
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if (quarter == 0) tops[wave][m] = top;
+  __syncthreads();
+  float all = tops[0][m];
+#pragma unroll
+  for (int w = 1; w < kWaves; w++) all = fmaxf(all, tops[w][m]);
+  const float by = __builtin_amdgcn_exp2f(top - (all == -INFINITY ? 0.f : all));
+  if (quarter == 0) sums[wave][m] = sum * by;
+#pragma unroll
+  for (int c = 0; c < C; c++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) rows[wave][m][C * (4 * quarter + r) + c] = acc[c][r] * by;
+  __syncthreads();
+  for (int at = tid * 4; at < kColumns * D; at += kThreads * 4) {
+    const int h = at / D, c = at % D;
+    if (h >= heads) break;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) o += *reinterpret_cast<const f32x4_t*>(&rows[w][h][c]);
+    if (t.splits > 1) {
+      *reinterpret_cast<f32x4_t*>(t.part + ((int64_t)split * t.c.batch * t.heads_q + row0 + h) * D + c) = o;
+    } else {
+      float total = sums[0][h];
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) total += sums[w][h];
+      o *= total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;   // nothing seen: 0
+      char* const to = t.o + b * t.ob + (int64_t)(g * t.group + first_head + h) * t.oh + c * sizeof(T);
+      if constexpr (WIDE) *reinterpret_cast<f32x4_t*>(to) = o;
+      else *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack<DT>(o[0], o[1]), pack<DT>(o[2], o[3])};
+    }
+  }
+  if (tid < heads) {
+    float total = sums[0][tid], high = tops[0][tid];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) total += sums[w][tid], high = fmaxf(high, tops[w][tid]);
+    if (t.splits > 1 || WEIGHTS) t.stats[(int64_t)split * t.c.batch * t.heads_q + row0 + tid] = f32x2_t{high, total};
+    if (t.splits == 1) t.lse[row0 + tid] = total == 0.f ? -INFINITY : (high + __builtin_amdgcn_logf(total)) * kLn2;
+  }
+}
+
+// Maximum, in log2 units, and sum over the parts of a row
+__device__ __forceinline__ f32x2_t joined(const Token& t, int64_t row, int parts) {
+  const int64_t rows = (int64_t)t.c.batch * t.heads_q;
+  float high = -INFINITY, total = 0.f;
+  for (int i = 0; i < parts; i++) high = fmaxf(high, t.stats[i * rows + row][0]);
+  const float ref = high == -INFINITY ? 0.f : high;
+  for (int i = 0; i < parts; i++) {
+    const f32x2_t s = t.stats[i * rows + row];
+    total += s[1] * __builtin_amdgcn_exp2f(s[0] - ref);
+  }
+  return f32x2_t{high, total};
+}
+
+// O and L from the parts: a thread has four channels of a row
+template <int DT, int D>
+__device__ __forceinline__ void join_rows(const Token& t, int64_t id) {
+  constexpr bool WIDE = DT == FHOG_DTYPE_FP32;
+  const int64_t rows = (int64_t)t.c.batch * t.heads_q, row = id / (D / 4);
+  if (row >= rows) return;
+  const int c = (int)(id % (D / 4)) * 4, b = (int)(row / t.heads_q), h = (int)(row - (int64_t)b * t.heads_q);
+  const Seen<WIDE ? 16 : 32> seen(t.c.length(b), t.window, t.sinks);
+  const int parts = parts_of(seen.tiles, t);
+  const f32x2_t all = joined(t, row, parts);
+  const float ref = all[0] == -INFINITY ? 0.f : all[0];
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < parts; i++) o += *reinterpret_cast<const f32x4_t*>(t.part + (i * rows + row) * D + c) * __builtin_amdgcn_exp2f(t.stats[i * rows + row][0] - ref);
+  o *= all[1] > 0.f ? 1.f / all[1] : all[1] == 0.f ? 0.f : all[1];
+  char* const to = t.o + b * t.ob + h * t.oh + c * sizeof(typename Type<DT>::T);
+  if constexpr (WIDE) *reinterpret_cast<f32x4_t*>(to) = o;
+  else *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack<DT>(o[0], o[1]), pack<DT>(o[2], o[3])};
+  if (c == 0) t.lse[row] = all[1] == 0.f ? -INFINITY : (all[0] + __builtin_amdgcn_logf(all[1])) * kLn2;
+}
+
+constexpr int kEntries = 4 * kThreads;   // of the weights that a workgroup adds to
+
+// The weights of kEntries entries of a head of keys: what was kept of their scores, on the joined statistics
+template <int DT>
+__device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid) {
+  __shared__ float lse[kThreads];
+  const int blocks = (t.c.capacity + kEntries - 1) / kEntries;
+  const int64_t slice = id / blocks;
+  const int b = (int)(slice / t.c.heads_k), g = (int)(slice - (int64_t)b * t.c.heads_k), j0 = (int)(id - slice * blocks) * kEntries + tid;
+  const Seen<DT == FHOG_DTYPE_FP32 ? 16 : 32> seen(t.c.length(b), t.window, t.sinks);
+  const int parts = parts_of(seen.tiles, t);
+  const int64_t row0 = (int64_t)b * t.heads_q + g * t.group;
+  const float* const in = t.weights_in + b * t.wib + g * t.wih;
+  float* const out = t.weights_out + b * t.wob + g * t.woh;
+  float w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[i] = j0 + i * kThreads < t.c.capacity ? in[j0 + i * kThreads] : 0.f;
+  for (int h0 = 0; h0 < t.group; h0 += kThreads) {
+    const int heads = min(kThreads, t.group - h0);
+    __syncthreads();
+    if (tid < heads) {
+      const f32x2_t all = joined(t, row0 + h0 + tid, parts);
+      lse[tid] = all[1] == 0.f ? INFINITY : all[0] + __builtin_amdgcn_logf(all[1]);
+    }
+    __syncthreads();
+    for (int h = 0; h < heads; h++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int j = j0 + i * kThreads;
+        if (seen.sees(j)) w[i] += __builtin_amdgcn_exp2f(t.scores[(row0 + h0 + h) * t.row + j] - lse[h]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (j0 + i * kThreads < t.c.capacity) out[j0 + i * kThreads] = w[i];
+}
+
+// What is left after the parts, in one launch: workgroups that join rows, and those that add weights behind them
+template <int DT, int D>
+__global__ void __launch_bounds__(kThreads) join_parts(Token t, int row_blocks) {
+  if ((int)blockIdx.x < row_blocks) join_rows<DT, D>(t, (int64_t)blockIdx.x * kThreads + threadIdx.x);
+  else add_weights<DT>(t, (int64_t)blockIdx.x - row_blocks, threadIdx.x);
+}
+
+// How the tiles of a call are dealt out
+struct Plan {
+  int splits, least;
+  int64_t rows, row;   // batch * heads_q; scores of a row
+  size_t part_bytes, stats_bytes, score_bytes;
+  size_t bytes() const { return part_bytes + stats_bytes + score_bytes; }
+};
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+Plan plan_of(const fhog_paged_attn_args* a) {
+  Plan p;
+  const fhog_paged_cache& c = a->cache;
+  const int64_t tile = c.dtype == FHOG_DTYPE_FP32 ? 16 : 32, capacity = c.table_width * c.page;
+  int64_t most = capacity;   // entries that a token may see
+  if (a->window > 0 && a->window < capacity) most = std::min(capacity, a->window + std::min(a->sinks, capacity) + 2 * tile);
+  const int64_t tiles = (most + tile - 1) / tile, group = a->heads_q / c.heads_k, slices = c.batch * c.heads_k * ((group + kColumns - 1) / kColumns);
+  p.least = kWaves;
+  const int64_t wanted = (768 + slices - 1) / slices, possible = (tiles + p.least - 1) / p.least;
+  p.splits = (int)std::max<int64_t>(1, std::min({wanted, possible, (int64_t)256}));
+  p.rows = c.batch * a->heads_q, p.row = (capacity + 31) & ~(int64_t)31;
+  p.part_bytes = p.splits > 1 ? up16(sizeof(float) * p.splits * p.rows * c.d) : 0;
+  p.stats_bytes = p.splits > 1 || a->weights_out ? up16(sizeof(f32x2_t) * p.splits * p.rows) : 0;
+  p.score_bytes = a->weights_out ? sizeof(float) * p.rows * p.row : 0;
+  return p;
+}
+
+template <int DT, int D>
+hipError_t launch_d(const Token& t, const fhog_paged_attn_args* a, hipStream_t s) {
+  const dim3 grid((unsigned)t.splits, (unsigned)(t.c.heads_k * t.columns), (unsigned)t.c.batch);
+  const bool pages16 = t.c.page.by % 16 == 0;
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, t); };
+  if (t.weights_out) pages16 ? go(attend<DT, D, true, true>) : go(attend<DT, D, false, true>);
+  else pages16 ? go(attend<DT, D, true, false>) : go(attend<DT, D, false, false>);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || (t.splits == 1 && !t.weights_out)) return e;
+  const int64_t rows = t.splits > 1 ? ((int64_t)t.c.batch * t.heads_q * (D / 4) + kThreads - 1) / kThreads : 0;
+  const int64_t weights = t.weights_out ? (int64_t)t.c.batch * t.c.heads_k * ((t.c.capacity + kEntries - 1) / kEntries) : 0;
+  hipLaunchKernelGGL((join_parts<DT, D>), dim3((unsigned)(rows + weights)), dim3(kThreads), 0, s, t, (int)rows);
+  return hipGetLastError();
+}
+template <int DT>
+hipError_t launch_t(const Token& t, const fhog_paged_attn_args* a, hipStream_t s) {
+  switch (a->cache.d) {
+    case 32: return launch_d<DT, 32>(t, a, s);
+    case 64: return launch_d<DT, 64>(t, a, s);
+    default: return launch_d<DT, 128>(t, a, s);
+  }
+}
+
+}  // namespace
+
+size_t paged_attn_bytes(const fhog_paged_attn_args* a) { return plan_of(a).bytes(); }
+
+hipError_t launch_paged_attn(const fhog_paged_attn_args* a, hipStream_t s) {
+  const Plan p = plan_of(a);
+  const int es = a->cache.dtype == FHOG_DTYPE_FP32 ? 4 : 2;
+  Token t;
+  t.c = cache_of(a->cache);
+  t.q = (const char*)a->q, t.o = (char*)a->o, t.lse = a->lse, t.weights_in = a->weights_in, t.weights_out = a->weights_out;
+  t.qb = a->stride_qb * es, t.qh = a->stride_qh * es, t.ob = a->stride_ob * es, t.oh = a->stride_oh * es;
+  t.wib = a->stride_wib, t.wih = a->stride_wih, t.wob = a->stride_wob, t.woh = a->stride_woh;
+  t.heads_q = (int32_t)a->heads_q, t.group = (int32_t)(a->heads_q / a->cache.heads_k), t.columns = (t.group + kColumns - 1) / kColumns;
+  t.window = (int32_t)std::min<int64_t>(a->window, INT32_MAX), t.sinks = (int32_t)std::min<int64_t>(a->sinks, t.c.capacity);
+  t.splits = p.splits, t.least = p.least, t.scale_log2 = a->scale * kLog2e, t.row = p.row;
+  char* const ws = (char*)a->ws;
+  t.part = (float*)ws, t.stats = (f32x2_t*)(ws + p.part_bytes), t.scores = (float*)(ws + p.part_bytes + p.stats_bytes);
+  switch (a->cache.dtype) {
+    case FHOG_DTYPE_FP32: return launch_t<FHOG_DTYPE_FP32>(t, a, s);
+    case FHOG_DTYPE_FP16: return launch_t<FHOG_DTYPE_FP16>(t, a, s);
+    default: return launch_t<FHOG_DTYPE_BF16>(t, a, s);
+  }
+}
+
+}  // namespace fhog

@@ -437,6 +437,169 @@ std::optional<tensor_list> rotary(const Tensor& q, const std::optional<Tensor>& 
   return RotaryNode::apply(q, k, positions, turn);
 }
 
+// ---- a cache in pages -----------------------------------------------------------------------------------------------
+// What every tensor of these calls has to be: in the memory of one GPU, and neither a wrapper nor asking for a gradient, which is not formed
+bool usable(const Tensor& t, const Tensor& like) {
+  return t.defined() && !t.unsafeGetTensorImpl()->is_python_dispatch() && in_memory(t) && t.is_cuda() && t.device() == like.device() &&
+         !(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined();
+}
+bool usable(const std::optional<Tensor>& t, const Tensor& like) { return !t || usable(*t, like); }
+bool transformed() {
+  return at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+}
+
+// Stride along dimension i; a dimension of one is never stepped along, whatever it says
+int64_t step(const Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
+
+// A tensor whose rows are read 16 bytes at a time: as it lies if it can be, else packed
+Tensor rows16(const Tensor& t) {
+  bool fits = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); i++) fits = fits && step(t, i) % (16 / t.element_size()) == 0 && step(t, i) >= 0;
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+Tensor packed_rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+// What changed behind autograd's back counts as changed
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// The cache of a call; table and lengths as the library reads them
+struct Paged {
+  Tensor table, lengths;
+  fhog_paged_cache c = {};
+  bool set(const Tensor& keys, const Tensor& values, const Tensor& table_, const Tensor& lengths_) {
+    if (!usable(keys, keys) || !usable(values, keys) || !usable(table_, keys) || !usable(lengths_, keys) || transformed()) return false;
+    if (keys.dim() != 4 || values.sizes() != keys.sizes() || values.scalar_type() != keys.scalar_type() || keys.numel() == 0 || table_.dim() != 2 || lengths_.dim() != 1 ||
+        lengths_.size(0) != table_.size(0) || table_.scalar_type() != at::kInt || lengths_.scalar_type() != at::kInt || table_.size(1) < 1)
+      return false;
+    if (keys.stride(-1) != 1 || values.stride(-1) != 1) return false;
+    for (int64_t i = 0; i < 3; i++)
+      if (step(keys, i) != step(values, i)) return false;
+    table = packed_rows(table_), lengths = lengths_.contiguous();
+    c.keys = keys.data_ptr(), c.values = values.data_ptr(), c.table = (const int32_t*)table.data_ptr(), c.lengths = (const int32_t*)lengths.data_ptr();
+    c.batch = table.size(0), c.heads_k = keys.size(1), c.d = keys.size(3), c.pages = keys.size(0), c.page = keys.size(2), c.table_width = table.size(1);
+    c.stride_p = step(keys, 0), c.stride_h = step(keys, 1), c.stride_n = step(keys, 2), c.stride_tb = step(table, 0);
+    c.dtype = dtype_code(keys.scalar_type());
+    return c.dtype >= 0;
+  }
+};
+
+bool paged_append(const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const Tensor& k_, const Tensor& v_,
+                  const std::optional<Tensor>& counts_) {
+  Paged cache;
+  if (!usable(k_, keys) || !usable(v_, keys) || !usable(counts_, keys)) return false;
+  const c10::DeviceGuard guard(keys.device());
+  if (!cache.set(keys, values, table, lengths)) return false;
+  const at::NoGradGuard no_grad;   // behind the checks, which ask whether a gradient would be formed
+  const fhog_paged_cache& c = cache.c;
+  if (k_.dim() != 4 || k_.sizes() != v_.sizes() || k_.scalar_type() != keys.scalar_type() || v_.scalar_type() != keys.scalar_type() || k_.size(0) != c.batch ||
+      k_.size(1) != c.heads_k || k_.size(3) != c.d)
+    return false;
+  if (counts_ && (counts_->dim() != 1 || counts_->size(0) != c.batch || counts_->scalar_type() != at::kInt)) return false;
+  const Tensor k = rows16(k_), v = rows16(v_), counts = counts_ ? counts_->contiguous() : Tensor();
+  fhog_paged_append_args a = {};
+  a.cache = c, a.k = k.data_ptr(), a.v = v.data_ptr(), a.counts = counts.defined() ? (const int32_t*)counts.data_ptr() : nullptr, a.n = k.size(2);
+  a.stride_kb = step(k, 0), a.stride_kh = step(k, 1), a.stride_kn = step(k, 2), a.stride_vb = step(v, 0), a.stride_vh = step(v, 1), a.stride_vn = step(v, 2);
+  if (fhog_paged_append_validate(&a) != FHOG_OK) return false;
+  TORCH_CHECK(fhog_paged_append(&a, stream_of(keys)) == FHOG_OK, "fhog_paged_append: ", fhog_last_error());
+  changed(keys), changed(values);
+  return true;
+}
+
+// (B, H_k, entries) of fp32, last dimension side by side
+bool weights_of(const Tensor& w, const fhog_paged_cache& c) {
+  return w.dim() == 3 && w.scalar_type() == at::kFloat && w.size(0) == c.batch && w.size(1) == c.heads_k && w.size(2) == c.table_width * c.page;
+}
+
+std::optional<tensor_list> paged_attention(const Tensor& q_, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths,
+                                           std::optional<double> scale, int64_t window, int64_t sinks, const std::optional<Tensor>& weights_,
+                                           const std::optional<Tensor>& weights_out) {
+  Paged cache;
+  if (!usable(q_, keys) || !usable(weights_, keys) || !usable(weights_out, keys)) return std::nullopt;
+  const c10::DeviceGuard guard(keys.device());
+  if (!cache.set(keys, values, table, lengths)) return std::nullopt;
+  const at::NoGradGuard no_grad;
+  const fhog_paged_cache& c = cache.c;
+  if (q_.dim() != 4 || q_.scalar_type() != keys.scalar_type() || q_.size(0) != c.batch || q_.size(2) != 1 || q_.size(3) != c.d || q_.size(1) < 1) return std::nullopt;
+  if ((weights_ && !weights_of(*weights_, c)) || (weights_out && (!weights_ || !weights_of(*weights_out, c) || weights_out->stride(2) != 1))) return std::nullopt;
+  const Tensor q = rows16(q_);
+  fhog_paged_attn_args a = {};
+  a.cache = c, a.heads_q = q.size(1), a.stride_qb = step(q, 0), a.stride_qh = step(q, 1);
+  a.stride_ob = a.heads_q * c.d, a.stride_oh = c.d;
+  a.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)c.d)), a.window = window, a.sinks = sinks;
+  tensor_list out = {at::empty(q.sizes(), q.options()), at::empty({c.batch, a.heads_q, 1}, q.options().dtype(at::kFloat))};
+  a.q = q.data_ptr(), a.o = out[0].data_ptr(), a.lse = (float*)out[1].data_ptr();
+  Tensor weights;
+  if (weights_) {
+    weights = packed_rows(*weights_);
+    out.push_back(weights_out ? *weights_out : at::empty(weights.sizes(), weights.options()));
+    a.weights_in = (const float*)weights.data_ptr(), a.stride_wib = step(weights, 0), a.stride_wih = step(weights, 1);
+    a.weights_out = (float*)out[2].data_ptr(), a.stride_wob = step(out[2], 0), a.stride_woh = step(out[2], 1);
+  }
+  if (fhog_paged_attn_validate(&a) != FHOG_OK) return std::nullopt;
+  a.ws_bytes = (int64_t)fhog_paged_attn_workspace_bytes(&a);
+  Tensor ws;
+  if (a.ws_bytes > 0) ws = workspace(a.ws_bytes, q), a.ws = ws.data_ptr();
+  TORCH_CHECK(fhog_paged_attn(&a, stream_of(q)) == FHOG_OK, "fhog_paged_attn: ", fhog_last_error());
+  if (weights_out) changed(*weights_out);
+  return out;
+}
+
+std::optional<Tensor> key_weights(const Tensor& q_, const Tensor& k_, const Tensor& L, std::optional<double> scale, int causal, int64_t window, int64_t sinks,
+                                  const std::optional<Tensor>& lengths_) {
+  if (!usable(q_, q_) || !usable(k_, q_) || !usable(L, q_) || !usable(lengths_, q_) || transformed()) return std::nullopt;
+  if (q_.dim() != 4 || k_.dim() != 4 || k_.scalar_type() != q_.scalar_type() || k_.size(0) != q_.size(0) || k_.size(3) != q_.size(3) || !L.is_floating_point() ||
+      L.sizes() != q_.sizes().slice(0, 3) || !mask_applies(Mask{causal, window, sinks}, q_.size(2), k_.size(2)))
+    return std::nullopt;
+  if (lengths_ && (lengths_->dim() != 1 || lengths_->size(0) != q_.size(0) || lengths_->scalar_type() != at::kInt)) return std::nullopt;
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = rows16(q_), k = rows16(k_), lse = as_lse(L), lengths = lengths_ ? lengths_->contiguous() : Tensor();
+  fhog_key_weights_args a = {};
+  a.dtype = dtype_code(q.scalar_type());
+  if (a.dtype < 0) return std::nullopt;
+  a.batch = q.size(0), a.heads_q = q.size(1), a.heads_k = k.size(1), a.n_q = q.size(2), a.n_k = k.size(2), a.d = q.size(3);
+  a.stride_qb = step(q, 0), a.stride_qh = step(q, 1), a.stride_qn = step(q, 2), a.stride_kb = step(k, 0), a.stride_kh = step(k, 1), a.stride_kn = step(k, 2);
+  a.stride_oh = a.n_k, a.stride_ob = a.heads_k * a.n_k;
+  a.causal = causal, a.window = window, a.sinks = sinks, a.scale = (float)(scale ? *scale : scale_of(q));
+  const Tensor out = at::empty({a.batch, a.heads_k, a.n_k}, q.options().dtype(at::kFloat));
+  a.q = q.data_ptr(), a.k = k.data_ptr(), a.lse = (const float*)lse.data_ptr(), a.out = (float*)out.data_ptr();
+  a.lengths = lengths.defined() ? (const int32_t*)lengths.data_ptr() : nullptr;
+  if (fhog_key_weights_validate(&a) != FHOG_OK) return std::nullopt;
+  a.ws_bytes = (int64_t)fhog_key_weights_workspace_bytes(&a);
+  Tensor ws;
+  if (a.ws_bytes > 0) ws = workspace(a.ws_bytes, q), a.ws = ws.data_ptr();
+  TORCH_CHECK(fhog_key_weights(&a, stream_of(q)) == FHOG_OK, "fhog_key_weights: ", fhog_last_error());
+  return out;
+}
+
+// New lengths, the weights of what stays, and where it came from
+std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const Tensor& weights_,
+                                                              int64_t budget, const Tensor& into_, int64_t sinks, int64_t recent) {
+  Paged cache;
+  if (!usable(weights_, keys) || !usable(into_, keys)) return std::nullopt;
+  const c10::DeviceGuard guard(keys.device());
+  if (!cache.set(keys, values, table, lengths)) return std::nullopt;
+  const at::NoGradGuard no_grad;
+  const fhog_paged_cache& c = cache.c;
+  if (!weights_of(weights_, c) || into_.dim() != 2 || into_.scalar_type() != at::kInt || into_.size(0) != c.batch || budget < 1) return std::nullopt;
+  const Tensor weights = packed_rows(weights_), into = packed_rows(into_);
+  fhog_paged_evict_args a = {};
+  a.cache = c, a.weights = (const float*)weights.data_ptr(), a.stride_wb = step(weights, 0), a.stride_wh = step(weights, 1);
+  a.into = (const int32_t*)into.data_ptr(), a.stride_ib = step(into, 0), a.into_width = into.size(1);
+  a.budget = budget, a.sinks = sinks, a.recent = recent;
+  const auto ints = into.options();
+  // addresses of the outputs are looked at for NULL alone: their size is allocated once the call is known to be one
+  a.lengths_out = (int32_t*)keys.data_ptr(), a.kept = a.lengths_out, a.weights_out = (float*)a.kept;
+  if (fhog_paged_evict_validate(&a) != FHOG_OK) return std::nullopt;
+  const Tensor left = at::empty({c.batch}, ints), kept = at::empty({c.batch, c.heads_k, budget}, ints), out = at::empty({c.batch, c.heads_k, c.table_width * c.page}, weights.options());
+  a.lengths_out = (int32_t*)left.data_ptr(), a.kept = (int32_t*)kept.data_ptr(), a.weights_out = (float*)out.data_ptr();
+  TORCH_CHECK(fhog_paged_evict(&a, stream_of(keys)) == FHOG_OK, "fhog_paged_evict: ", fhog_last_error());
+  changed(keys), changed(values);
+  return std::make_tuple(left, out, kept);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_fhog_torch, m) {
@@ -460,4 +623,8 @@ PYBIND11_MODULE(_fhog_torch, m) {
   m.def("dispatches_to_python", [](const Tensor& t) { return t.unsafeGetTensorImpl()->is_python_dispatch(); }, free_lock);
   m.def("attention", &attention, free_lock);
   m.def("rotary", &rotary, free_lock);
+  m.def("paged_append", &paged_append, free_lock);
+  m.def("paged_attention", &paged_attention, free_lock);
+  m.def("key_weights", &key_weights, free_lock);
+  m.def("paged_evict", &paged_evict, free_lock);
 }

@@ -25,7 +25,7 @@ STATIC_WS_BYTES = 16 << 20   # of a default build; `lib().fhog_static_ws_bytes()
 ERROR_NAMES = {
     -1: "FHOG_E_NULL", -2: "FHOG_E_SHAPE", -3: "FHOG_E_DTYPE", -4: "FHOG_E_STRIDE", -5: "FHOG_E_ALIGN",
     -6: "FHOG_E_CAUSAL", -7: "FHOG_E_PASS", -8: "FHOG_E_LAUNCH", -9: "FHOG_E_SCALE", -10: "FHOG_E_IMPL",
-    -11: "FHOG_E_SCHEDULE", -12: "FHOG_E_ROTARY",
+    -11: "FHOG_E_SCHEDULE", -12: "FHOG_E_ROTARY", -13: "FHOG_E_PAGED",
 }
 
 
@@ -63,6 +63,52 @@ class RotaryArgs(Structure):
         ("stride_kon", c_int64), ("stride_pa", c_int64), ("stride_pb", c_int64), ("stride_pn", c_int64),
         ("theta", c_double), ("sections", c_int32 * 4), ("axes", c_int32), ("dtype", c_int32), ("position_type", c_int32), ("interleaved", c_int32),
         ("inverse", c_int32),
+    ]
+
+
+class PagedCacheArgs(Structure):
+    """Mirror of ``fhog_paged_cache``."""
+    _fields_ = [
+        ("keys", c_void_p), ("values", c_void_p), ("table", c_void_p), ("lengths", c_void_p),
+        ("batch", c_int64), ("heads_k", c_int64), ("d", c_int64), ("pages", c_int64), ("page", c_int64), ("table_width", c_int64),
+        ("stride_p", c_int64), ("stride_h", c_int64), ("stride_n", c_int64), ("stride_tb", c_int64), ("dtype", c_int32),
+    ]
+
+
+class PagedAppendArgs(Structure):
+    """Mirror of ``fhog_paged_append_args``."""
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("k", c_void_p), ("v", c_void_p), ("counts", c_void_p), ("n", c_int64),
+        ("stride_kb", c_int64), ("stride_kh", c_int64), ("stride_kn", c_int64), ("stride_vb", c_int64), ("stride_vh", c_int64), ("stride_vn", c_int64),
+    ]
+
+
+class PagedAttnArgs(Structure):
+    """Mirror of ``fhog_paged_attn_args``."""
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("q", c_void_p), ("o", c_void_p), ("lse", c_void_p), ("weights_in", c_void_p), ("weights_out", c_void_p), ("ws", c_void_p),
+        ("heads_q", c_int64), ("stride_qb", c_int64), ("stride_qh", c_int64), ("stride_ob", c_int64), ("stride_oh", c_int64),
+        ("stride_wib", c_int64), ("stride_wih", c_int64), ("stride_wob", c_int64), ("stride_woh", c_int64), ("window", c_int64), ("sinks", c_int64),
+        ("ws_bytes", c_int64), ("scale", c_float),
+    ]
+
+
+class KeyWeightsArgs(Structure):
+    """Mirror of ``fhog_key_weights_args``."""
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("lse", c_void_p), ("lengths", c_void_p), ("out", c_void_p), ("ws", c_void_p),
+        ("batch", c_int64), ("heads_q", c_int64), ("heads_k", c_int64), ("n_q", c_int64), ("n_k", c_int64), ("d", c_int64),
+        ("stride_qb", c_int64), ("stride_qh", c_int64), ("stride_qn", c_int64), ("stride_kb", c_int64), ("stride_kh", c_int64), ("stride_kn", c_int64),
+        ("stride_ob", c_int64), ("stride_oh", c_int64), ("window", c_int64), ("sinks", c_int64), ("ws_bytes", c_int64),
+        ("scale", c_float), ("dtype", c_int32), ("causal", c_int32),
+    ]
+
+
+class PagedEvictArgs(Structure):
+    """Mirror of ``fhog_paged_evict_args``."""
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("weights", c_void_p), ("into", c_void_p), ("lengths_out", c_void_p), ("kept", c_void_p), ("weights_out", c_void_p),
+        ("stride_wb", c_int64), ("stride_wh", c_int64), ("stride_ib", c_int64), ("into_width", c_int64), ("budget", c_int64), ("sinks", c_int64), ("recent", c_int64),
     ]
 
 
@@ -131,6 +177,16 @@ def lib() -> ctypes.CDLL:
     L.fhog_rotary_validate.argtypes = [POINTER(RotaryArgs)]
     L.fhog_rotary.restype = c_int
     L.fhog_rotary.argtypes = [POINTER(RotaryArgs), c_void_p]
+    for call, args in (("paged_append", PagedAppendArgs), ("paged_attn", PagedAttnArgs), ("key_weights", KeyWeightsArgs), ("paged_evict", PagedEvictArgs)):
+        size, validate, run = (getattr(L, f"fhog_{call}{x}") for x in ("_args_size", "_validate", ""))
+        size.restype, size.argtypes = c_size_t, []
+        validate.restype, validate.argtypes = c_int, [POINTER(args)]
+        run.restype, run.argtypes = c_int, [POINTER(args), c_void_p]
+        if size() != ctypes.sizeof(args):
+            raise RuntimeError(f"fhog_{call}_args layout differs between libfhog_hip.so and the ctypes mirror")
+    L.fhog_paged_attn_workspace_bytes.restype = L.fhog_key_weights_workspace_bytes.restype = c_size_t
+    L.fhog_paged_attn_workspace_bytes.argtypes = [POINTER(PagedAttnArgs)]
+    L.fhog_key_weights_workspace_bytes.argtypes = [POINTER(KeyWeightsArgs)]
     L.fhog_probe_mfma_rate.restype = c_int
     L.fhog_probe_mfma_rate.argtypes = [c_void_p, c_int, c_int, c_int, POINTER(ctypes.c_double), c_void_p]
     if L.fhog_attn_args_size() != ctypes.sizeof(AttnArgs):

@@ -50,6 +50,7 @@ extern "C" {
 #define FHOG_E_IMPL (-10)     /* unknown kernel family (fhog_bwdbwd_args.impl) */
 #define FHOG_E_SCHEDULE (-11) /* unknown pass schedule (fhog_bwdbwd_args.schedule), or one that does not know sinks */
 #define FHOG_E_ROTARY (-12)   /* axes, sections, base or type of the positions (fhog_rotary_args) */
+#define FHOG_E_PAGED (-13)    /* pages, table, budget or counts of a cache in pages (fhog_paged_cache and the calls on it) */
 
 /* pass ids for fhog_bwdbwd_pass */
 #define FHOG_PASS_D 0      /* d_i  = sum_c O_ic dO_ic                         (fhog/triton_bwdbwd.py:580)     */
@@ -329,6 +330,109 @@ int fhog_rotary_validate(const fhog_rotary_args* args);
 
 /* One launch; none where batch or n is 0. */
 int fhog_rotary(const fhog_rotary_args* args, void* hip_stream);
+
+/* ---- a cache of keys and values in pages ----------------------------------------------------------------------------
+ * Decoding token by token: keys and values of many sequences in pages of one pool, attention of one new token of each over its pages, the weights that the
+ * keys got, and the eviction of those that got least. No counterpart in the reference.
+ * Entry j of sequence b lies in slot j % page of page table[b][j / page], which all heads of keys share; a sequence has lengths[b] entries, the newest ones last, cut to
+ * 0 .. table_width * page. Lengths and table are read on the device when the kernels run, so that a captured graph follows them. A number in the table that is no page
+ * (below 0, or pages and more) holds no entries: what would be read there is not there, what would be written is dropped. What lies behind the last entry, in
+ * the pages and in other arrays, is neither read nor changed unless a call says so. Head h of heads_q queries belongs to head h / (heads_q / heads_k) of the keys.
+ * No call allocates, frees or synchronises; results do not depend on what else runs (no atomics on floats, partial results joined in a fixed order). */
+typedef struct fhog_paged_cache {
+  void* keys;             /* (pages, heads_k, page, d), last dimension contiguous */
+  void* values;           /* the same strides */
+  const int32_t* table;   /* (batch, table_width), rows stride_tb apart */
+  const int32_t* lengths; /* (batch), contiguous */
+  int64_t batch, heads_k, d, pages, page, table_width;
+  int64_t stride_p, stride_h, stride_n; /* of keys and values: pages, heads, entries; multiples of 16 bytes */
+  int64_t stride_tb;
+  int32_t dtype;          /* FHOG_DTYPE_* */
+} fhog_paged_cache;
+
+/* New entries: the last counts[b] of each sequence (cut to 0 .. n and to the sequence's length) are written from the first rows of k and v. Two sequences that
+   share a page must not both have new entries in the same slot. */
+typedef struct fhog_paged_append_args {
+  fhog_paged_cache cache;
+  const void* k;         /* (batch, heads_k, n, d) */
+  const void* v;         /* (batch, heads_k, n, d) */
+  const int32_t* counts; /* (batch), contiguous; NULL: n each */
+  int64_t n;
+  int64_t stride_kb, stride_kh, stride_kn, stride_vb, stride_vh, stride_vn; /* multiples of 16 bytes, 0 or negative too */
+} fhog_paged_append_args;
+
+size_t fhog_paged_append_args_size(void);
+int fhog_paged_append_validate(const fhog_paged_append_args* args); /* host-only */
+int fhog_paged_append(const fhog_paged_append_args* args, void* hip_stream);
+
+/* O = softmax(scale q K^T) V and L = logsumexp of the scaled scores of one token of each sequence over the entries that it sees: all, or with a window W > 0 the last
+   W and the first `sinks`. A sequence that sees none has O = 0 and L = -infinity.
+   weights_out, where given: weights_in (which may be the same array) plus, at every entry that is seen, sum over the heads of queries of a head of keys of
+   exp(scale q k - L); the other entries as they were. */
+typedef struct fhog_paged_attn_args {
+  fhog_paged_cache cache;
+  const void* q;           /* (batch, heads_q, d) */
+  void* o;                 /* (batch, heads_q, d) */
+  float* lse;              /* (batch, heads_q), contiguous */
+  const float* weights_in; /* (batch, heads_k, table_width * page), last dimension contiguous; NULL with weights_out NULL */
+  float* weights_out;
+  void* ws;                /* fhog_paged_attn_workspace_bytes, 16-byte aligned; may be NULL if that is 0 */
+  int64_t heads_q;
+  int64_t stride_qb, stride_qh, stride_ob, stride_oh;   /* multiples of 16 bytes */
+  int64_t stride_wib, stride_wih, stride_wob, stride_woh;
+  int64_t window, sinks;
+  int64_t ws_bytes;
+  float scale;
+} fhog_paged_attn_args;
+
+size_t fhog_paged_attn_args_size(void);
+int fhog_paged_attn_validate(const fhog_paged_attn_args* args); /* host-only; does not look at the workspace */
+size_t fhog_paged_attn_workspace_bytes(const fhog_paged_attn_args* args); /* 0 also if the arguments are not valid; host-only */
+int fhog_paged_attn(const fhog_paged_attn_args* args, void* hip_stream);
+
+/* out_gj = sum over the heads h of queries of head g of the keys, and over the queries i that see key j, of exp(scale q_hi . k_gj - lse_hi): the weight that each key got
+   in an attention call that lse is from. Masks as in fhog_attn_args (n_k >= n_q under FHOG_MASK_BOTTOM_RIGHT), sinks as above. A query whose lse is -infinity saw
+   nothing and gives nothing. lengths, where given (a causal mask only): keys of sequence b from lengths[b] on, and the queries in their places, are padding: the
+   former get 0, the latter give nothing, whatever they hold. */
+typedef struct fhog_key_weights_args {
+  const void* q;          /* (batch, heads_q, n_q, d) */
+  const void* k;          /* (batch, heads_k, n_k, d) */
+  const float* lse;       /* (batch, heads_q, n_q), contiguous */
+  const int32_t* lengths; /* (batch), contiguous, or NULL */
+  float* out;             /* (batch, heads_k, n_k), last dimension contiguous */
+  void* ws;               /* fhog_key_weights_workspace_bytes, 16-byte aligned; may be NULL if that is 0 */
+  int64_t batch, heads_q, heads_k, n_q, n_k, d;
+  int64_t stride_qb, stride_qh, stride_qn, stride_kb, stride_kh, stride_kn; /* multiples of 16 bytes */
+  int64_t stride_ob, stride_oh;
+  int64_t window, sinks;
+  int64_t ws_bytes;
+  float scale;
+  int32_t dtype, causal;
+} fhog_key_weights_args;
+
+size_t fhog_key_weights_args_size(void);
+int fhog_key_weights_validate(const fhog_key_weights_args* args); /* host-only; does not look at the workspace */
+size_t fhog_key_weights_workspace_bytes(const fhog_key_weights_args* args); /* 0 also if the arguments are not valid; host-only */
+int fhog_key_weights(const fhog_key_weights_args* args, void* hip_stream);
+
+/* Eviction, for each sequence and head of keys: of n = lengths[b] entries m = min(n, budget) stay: the first `sinks`, the last `recent`, and of the others those of the
+   largest weights, the lower index first among equal ones (0 and -0 are equal, a NaN ranks below every number). They are written, in their order, to the
+   entries 0 .. m - 1 of the pages that `into` names, which no sequence may be reading; the pages that they come from are not changed.
+   lengths_out[b] = m; kept[b][g][i] is where entry i came from, -1 from m on; weights_out holds the weights of what stayed, 0 from m on. */
+typedef struct fhog_paged_evict_args {
+  fhog_paged_cache cache;
+  const float* weights;  /* (batch, heads_k, table_width * page), last dimension contiguous */
+  const int32_t* into;   /* (batch, into_width), rows stride_ib apart; into_width * page >= min(budget, table_width * page) */
+  int32_t* lengths_out;  /* (batch) */
+  int32_t* kept;         /* (batch, heads_k, budget), contiguous */
+  float* weights_out;    /* (batch, heads_k, table_width * page), contiguous; not the array `weights` */
+  int64_t stride_wb, stride_wh, stride_ib, into_width;
+  int64_t budget, sinks, recent; /* sinks + recent <= budget */
+} fhog_paged_evict_args;
+
+size_t fhog_paged_evict_args_size(void);
+int fhog_paged_evict_validate(const fhog_paged_evict_args* args); /* host-only */
+int fhog_paged_evict(const fhog_paged_evict_args* args, void* hip_stream);
 
 /* Measurement aid (no counterpart in the reference): enqueue a loop of bf16 32x32x16 MFMAs on `blocks` workgroups of 8
    waves (one per CU fills the chip), `trips` x 32 MFMAs per wave. data_mode: 0 operands all zero; 1 random operands in
