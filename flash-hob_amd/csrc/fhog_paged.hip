@@ -1,6 +1,8 @@
 // New entries into a cache in pages, and the eviction of the entries of the least weight (include/fhog_hip.h).
 //
 // Both move rows: nothing is computed on them, and what bounds them is memory, every row in and out once, 16 bytes to a lane.
+#include <algorithm>
+
 #include "fhog_paged.h"
 
 namespace fhog {
@@ -8,6 +10,10 @@ namespace {
 
 using namespace paged;
 constexpr int kThreads = 256;
+// Rows go past the caches where they are written (a pool is larger than they are), and where they are read from it. us: 8 prompts of 4096 tokens, 8 heads, bf16, d = 128
+// (158 MB) 33.0 -> 28.6, with the new rows read past them too 30.4; 32 x 8 x 4096 rows moved (1.07 GB) 219 -> 203, with two rows to a thread on the way, four 212.
+__device__ __forceinline__ u32x4_t fetch_once(const char* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p)); }
+__device__ __forceinline__ void put(char* p, u32x4_t x) { __builtin_nontemporal_store(x, reinterpret_cast<u32x4_t*>(p)); }
 
 struct Append {
   Cache c;
@@ -36,8 +42,8 @@ __global__ void __launch_bounds__(kThreads) append_entries(Append a) {
   const int32_t page = a.c.table[b * a.c.stride_tb + at];
   if ((uint32_t)page >= (uint32_t)a.c.pages) return;
   const int64_t to = page * a.c.stride_p + h * a.c.stride_h + (j - at * a.c.page.by) * a.c.stride_n + chunk * 16;
-  *reinterpret_cast<u32x4_t*>(a.c.keys + to) = k;
-  *reinterpret_cast<u32x4_t*>(a.c.values + to) = v;
+  put(a.c.keys + to, k);
+  put(a.c.values + to, v);
 }
 
 // ---- eviction ---------------------------------------------------------------------------------------------------------
@@ -55,7 +61,9 @@ struct Evict {
   Divisor chunks;           // of a row
 };
 
-constexpr int kSelect = 1024, kWaves = kSelect / 64;
+constexpr int kSelect = 1024, kWaves = kSelect / 64, kHeld = 12288;   // kHeld: entries whose ranks are held in LDS
+constexpr int kCopies = 8, kDigits = 264;   // of the histogram; copies lie eight banks apart
+constexpr int kRowsEach = 2;   // chunks of keys and values that a thread moves
 
 // A number for each entry that grows with the order in which entries stay: what is protected first, then by weight, NaN last
 __device__ __forceinline__ uint32_t rank_of(float w, int j, int n, const Evict& e) {
@@ -65,11 +73,14 @@ __device__ __forceinline__ uint32_t rank_of(float w, int j, int n, const Evict& 
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Which entries of one sequence and head of keys stay. The rank of the last one that does is found digit by digit, eight bits at a time from the top: a histogram
-// of the digit over the entries whose higher digits are those found so far, and the digit at which the sum from above reaches what is still to be
-// found. Then the entries that stay are counted wave by wave, each wave a stretch of its own, and written to the places that the counts give.
+// Which entries of one sequence and head of keys stay. Each wave has a stretch of the entries. The rank of the last one that stays is found digit by digit, eight bits at a
+// time from the top: a histogram of the digit over the entries whose higher digits are those found so far, and the digit at which the sum from above reaches
+// what is still to be found. Then the entries that stay are counted, wave by wave, and written to the places that the counts give.
+// What bounds it: the waits between its passes. Ranks are formed once and held in LDS (us, 32 x 8 slices of 8192 | 4 x 4 of 1000: weights read anew in every pass 26.6 | 7.4, ranks in
+// registers 20.2 | 10.8, so TODO).
 __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
-  __shared__ uint32_t histogram[256];
+  extern __shared__ uint32_t held[];
+  __shared__ uint32_t histogram[kCopies][kDigits];   // a lane counts in copy lane % kCopies: the same digit of many lanes is not one address
   __shared__ uint32_t found[2];               // digits so far; how many of the entries of that rank stay
   __shared__ int counts[2][kWaves];           // entries of a wave's stretch above the rank, and of the rank itself
   const int b = blockIdx.x / e.c.heads_k, h = blockIdx.x - b * e.c.heads_k, tid = threadIdx.x, lane = tid & 63;
@@ -78,38 +89,40 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   const float* const w = e.weights + b * e.wb + h * e.wh;
   int32_t* const kept = e.kept + (int64_t)blockIdx.x * e.budget;
   float* const out = e.weights_out + (int64_t)blockIdx.x * e.c.capacity;
+  const int stretch = ((n + kWaves - 1) / kWaves + 63) & ~63, begin = min(n, wave * stretch), end = min(n, begin + stretch);
+  for (int j = tid; j < min(n, kHeld); j += kSelect) held[j] = rank_of(w[j], j, n, e);
+  // f(j, rank) for the wave's entries in order, 64 at a time; all lanes take part
+  const auto each = [&](auto f) {
+    for (int j = begin + lane; j - lane < end; j += 64) f(j, j >= end ? 0 : j < kHeld ? held[j] : rank_of(w[j], j, n, e));
+  };
   if (h == 0 && tid == 0) e.lengths_out[b] = m;
   for (int64_t i = m + tid; i < e.budget; i += kSelect) kept[i] = -1;
   for (int i = m + tid; i < e.c.capacity; i += kSelect) out[i] = 0.f;
   uint32_t rank = 0;
   int ties = n;
+  __syncthreads();
   if (m < n) {
     uint32_t above = 0;
     int need = m;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) histogram[tid] = 0;
+      for (int i = tid; i < kCopies * kDigits; i += kSelect) (&histogram[0][0])[i] = 0;
       __syncthreads();
-      for (int j0 = wave * 64; j0 < n; j0 += kSelect) {
-        const int j = j0 + lane;
-        const uint32_t r = j < n ? rank_of(w[j], j, n, e) : 0;
-        const bool in = j < n && (shift == 24 || r >> (shift + 8) == above);
+      each([&](int j, uint32_t r) {
         const uint32_t digit = r >> shift & 255;
-        const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-        if (who == 0) continue;
-        // one addition where all lanes have the same digit, as they do where many weights are equal
-        const uint32_t one = __builtin_amdgcn_readlane(digit, __builtin_ctzll(who));
-        if (__builtin_amdgcn_ballot_w64(in && digit != one) == 0) {
-          if (lane == 0) atomicAdd(&histogram[one], (uint32_t)__builtin_popcountll(who));
-        } else if (in) {
-          atomicAdd(&histogram[digit], 1u);
-        }
-      }
+        const bool in = j < end && (shift == 24 || r >> (shift + 8) == above);
+        if (in) atomicAdd(&histogram[lane % kCopies][digit], 1u);
+      });
       __syncthreads();
       if (wave == 0) {
         // lane l has the digits 4 l .. 4 l + 3; sum of the digits from there up
         uint32_t c[4], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) sum += c[i] = histogram[4 * lane + i];
+        for (int i = 0; i < 4; i++) {
+          c[i] = 0;
+#pragma unroll
+          for (int x = 0; x < kCopies; x++) c[i] += histogram[x][4 * lane + i];
+          sum += c[i];
+        }
         uint32_t up = sum;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -128,43 +141,46 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
     }
     rank = above, ties = need;
   }
-  const int stretch = ((n + kWaves - 1) / kWaves + 63) & ~63, begin = min(n, wave * stretch), end = min(n, begin + stretch);
   int over = 0, same = 0;
-  for (int j0 = begin; j0 < end; j0 += 64) {
-    const int j = j0 + lane;
-    const uint32_t r = j < end ? rank_of(w[j], j, n, e) : 0;
+  each([&](int j, uint32_t r) {
     over += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j < end && r > rank));
     same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j < end && r == rank));
-  }
+  });
   if (lane == 0) counts[0][wave] = over, counts[1][wave] = same;
   __syncthreads();
   over = same = 0;
   for (int i = 0; i < wave; i++) over += counts[0][i], same += counts[1][i];
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int j0 = begin; j0 < end; j0 += 64) {
-    const int j = j0 + lane;
-    const float x = j < end ? w[j] : 0.f;
-    const uint32_t r = j < end ? rank_of(x, j, n, e) : 0;
+  each([&](int j, uint32_t r) {
     const uint64_t o = __builtin_amdgcn_ballot_w64(j < end && r > rank), s = __builtin_amdgcn_ballot_w64(j < end && r == rank);
     const int same_before = same + __builtin_popcountll(s & below), at = over + __builtin_popcountll(o & below) + min(same_before, ties);
-    if (j < end && (r > rank || (r == rank && same_before < ties))) kept[at] = j, out[at] = x;
+    if (j < end && (r > rank || (r == rank && same_before < ties))) kept[at] = j, out[at] = w[j];
     over += __builtin_popcountll(o), same += __builtin_popcountll(s);
-  }
+  });
 }
 
-// The rows that stay, to their new places: a thread has one chunk of a key and of its value
+// The rows that stay, to their new places
 __global__ void __launch_bounds__(kThreads) move_entries(Evict e) {
   const int b = blockIdx.y / e.c.heads_k, h = blockIdx.y - b * e.c.heads_k;
-  const uint32_t id = blockIdx.x * kThreads + threadIdx.x, i = e.chunks(id), chunk = id - i * e.chunks.by;
-  if (i >= (uint32_t)min(e.c.length(b), e.rows)) return;
-  const uint32_t j = e.kept[(int64_t)blockIdx.y * e.budget + i], at = e.c.page(j), to = e.c.page(i);
-  const int32_t from_page = e.c.table[b * e.c.stride_tb + at], to_page = e.into[b * e.ib + to];
-  if ((uint32_t)from_page >= (uint32_t)e.c.pages || (uint32_t)to_page >= (uint32_t)e.c.pages) return;
-  const int64_t inside = h * e.c.stride_h + chunk * 16;
-  const int64_t src = from_page * e.c.stride_p + (j - at * e.c.page.by) * e.c.stride_n + inside, dst = to_page * e.c.stride_p + (i - to * e.c.page.by) * e.c.stride_n + inside;
-  const u32x4_t k = *reinterpret_cast<const u32x4_t*>(e.c.keys + src), v = *reinterpret_cast<const u32x4_t*>(e.c.values + src);
-  *reinterpret_cast<u32x4_t*>(e.c.keys + dst) = k;
-  *reinterpret_cast<u32x4_t*>(e.c.values + dst) = v;
+  const int rows = min(e.c.length(b), e.rows);
+  u32x4_t k[kRowsEach], v[kRowsEach];
+  int64_t dst[kRowsEach];
+#pragma unroll
+  for (int u = 0; u < kRowsEach; u++) {
+    dst[u] = -1;
+    const uint32_t id = (blockIdx.x * kRowsEach + u) * kThreads + threadIdx.x, i = e.chunks(id), chunk = id - i * e.chunks.by;
+    if (i >= (uint32_t)rows) continue;
+    const uint32_t j = e.kept[(int64_t)blockIdx.y * e.budget + i], at = e.c.page(j), to = e.c.page(i);
+    const int32_t from_page = e.c.table[b * e.c.stride_tb + at], to_page = e.into[b * e.ib + to];
+    if ((uint32_t)from_page >= (uint32_t)e.c.pages || (uint32_t)to_page >= (uint32_t)e.c.pages) continue;
+    const int64_t inside = h * e.c.stride_h + chunk * 16;
+    const int64_t src = from_page * e.c.stride_p + (j - at * e.c.page.by) * e.c.stride_n + inside;
+    dst[u] = to_page * e.c.stride_p + (i - to * e.c.page.by) * e.c.stride_n + inside;
+    k[u] = fetch_once(e.c.keys + src), v[u] = fetch_once(e.c.values + src);
+  }
+#pragma unroll
+  for (int u = 0; u < kRowsEach; u++)
+    if (dst[u] >= 0) put(e.c.keys + dst[u], k[u]), put(e.c.values + dst[u], v[u]);
 }
 
 uint32_t row_chunks(const fhog_paged_cache& c) { return (uint32_t)(c.d * (c.dtype == FHOG_DTYPE_FP32 ? 4 : 2) / 16); }
@@ -191,10 +207,10 @@ hipError_t launch_paged_evict(const fhog_paged_evict_args* a, hipStream_t s) {
   e.sinks = (int32_t)(a->sinks < e.c.capacity ? a->sinks : e.c.capacity), e.recent = (int32_t)(a->recent < e.c.capacity ? a->recent : e.c.capacity);
   e.into_width = (int32_t)a->into_width, e.chunks = Divisor(row_chunks(a->cache));
   const unsigned slices = (unsigned)(a->cache.batch * a->cache.heads_k);
-  hipLaunchKernelGGL(select_entries, dim3(slices), dim3(kSelect), 0, s, e);
+  hipLaunchKernelGGL(select_entries, dim3(slices), dim3(kSelect), std::min(e.c.capacity, kHeld) * sizeof(uint32_t), s, e);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || e.rows == 0) return err;
-  hipLaunchKernelGGL(move_entries, dim3((unsigned)(((int64_t)e.rows * e.chunks.by + kThreads - 1) / kThreads), slices), dim3(kThreads), 0, s, e);
+  hipLaunchKernelGGL(move_entries, dim3((unsigned)(((int64_t)e.rows * e.chunks.by + kThreads * kRowsEach - 1) / (kThreads * kRowsEach)), slices), dim3(kThreads), 0, s, e);
   return hipGetLastError();
 }
 

@@ -13,6 +13,7 @@
 // therefore loads the entries of its own group (l / 16), channels c (l % 16) .. + c - 1 with c = d / 16, which fills a row of a page with 16 lanes, and turns the
 // 8 x c block that it has in its own registers: product i of c takes channel c m + i as its row m, so the results of a lane are c consecutive channels.
 #include <algorithm>
+#include <type_traits>
 
 #include "fhog_paged.h"
 
@@ -74,6 +75,14 @@ __device__ __forceinline__ uint32_t word(const typename Words<4 * W>::type& v, i
   else return v[i];
 }
 
+// ONCE: past the caches, where nothing is read twice. TB/s of a loop of 16-byte loads over 2 GiB 6.2 -> 7.1; of rows of 256 bytes and more: rows of 128 bytes are read half
+// a line at a time, and lose what the first half brought.
+template <bool ONCE, typename V>
+__device__ __forceinline__ V fetch(const char* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  else return *reinterpret_cast<const V*>(p);
+}
+
 typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
 template <int DT>
 __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -91,13 +100,14 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 
 // PAGES16: pages of a multiple of 16 entries, so that 16 in a row share one. WEIGHTS: scores are kept.
 template <int DT, int D, bool PAGES16, bool WEIGHTS>
-__global__ void __launch_bounds__(kThreads) attend(Token t) {
+__global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32;
   typedef typename Type<DT>::T T;
   constexpr int TILE = WIDE ? 16 : 32, SUB = TILE / 16;   // entries of a tile; 16 at a time
   constexpr int STEPS = D * (int)sizeof(T) / 64;          // 16-byte pieces of a row that a lane has (four lanes to a row)
   constexpr int C = D / 16;                               // channels of a lane in V and O
   constexpr int VB = C * sizeof(T), VW = VB >= 16 ? 4 : VB / 4, VN = VB >= 16 ? VB / 16 : 1;   // bytes of them, words of a load, loads
+  constexpr bool WHOLE_LINES = D * (int)sizeof(T) >= 256;
   typedef typename Words<4 * VW>::type VWord;
   __shared__ float tops[kWaves][kColumns], sums[kWaves][kColumns];
   __shared__ float rows[kWaves][kColumns][D + 4];
@@ -131,78 +141,84 @@ __global__ void __launch_bounds__(kThreads) attend(Token t) {
   uint32_t value_off[4];
 #pragma unroll
   for (int x = 0; x < 4; x++) value_off[x] = (4 * quarter + x) * stride + m * VB;
-  for (int i = begin + wave; i < end; i += kWaves) {
-    const int j0 = seen.at(i);
-    u32x4_t k[SUB][STEPS];
-    VWord v[SUB][4][VN];
-    bool there[SUB][4];                 // whether the entries of this lane's values are there; `hidden`: some of the tile's are not, the same for the wave
-    bool hidden = !seen.whole(j0);
-    if constexpr (PAGES16) {
-      int64_t base[SUB];                // of 16 entries, from the pool's head g
-      bool found[SUB];
+  // Where the entries of a tile lie. `hidden`: some of them are not there or not seen, the same for the wave
+  struct Place {
+    int j0;
+    bool hidden;
+    int64_t at[SUB];   // in bytes from the pool's head g, -1: nowhere; of 16 entries in a row (PAGES16), else of entry m of 16, and of those that are seen alone
+  };
+  const auto locate = [&](int i) {
+    Place p;
+    p.j0 = seen.at(i), p.hidden = !seen.whole(p.j0);
 #pragma unroll
-      for (int u = 0; u < SUB; u++) {
-        const uint32_t j = j0 + 16 * u, p = __builtin_amdgcn_readfirstlane(t.c.page(j));
-        int32_t page = -1;
-        if ((int)j < seen.n) page = table[p];
+    for (int u = 0; u < SUB; u++) {
+      const int j = p.j0 + 16 * u + (PAGES16 ? 0 : m);
+      uint32_t index = t.c.page(j);
+      int32_t page = -1;
+      if constexpr (PAGES16) {
+        index = __builtin_amdgcn_readfirstlane(index);
+        if (j < seen.n) page = table[index];
         page = __builtin_amdgcn_readfirstlane(page);
-        found[u] = (uint32_t)page < (uint32_t)t.c.pages;
-        hidden = hidden || !found[u];
-        base[u] = page * t.c.stride_p + (j - p * t.c.page.by) * t.c.stride_n;
+      } else {
+        if (seen.sees(j)) page = table[index];
       }
-      const auto read = [&](auto sees) {
-#pragma unroll
-        for (int u = 0; u < SUB; u++) {
-          const bool ok = sees(u, m);
-#pragma unroll
-          for (int s = 0; s < STEPS; s++) k[u][s] = ok ? *reinterpret_cast<const u32x4_t*>(keys + base[u] + key_off + s * 64) : u32x4_t{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int u = 0; u < SUB; u++)
-#pragma unroll
-          for (int x = 0; x < 4; x++) {
-            there[u][x] = sees(u, 4 * quarter + x);
-#pragma unroll
-            for (int y = 0; y < VN; y++) v[u][x][y] = there[u][x] ? *reinterpret_cast<const VWord*>(values + base[u] + value_off[x] + y * 16) : VWord(0u);
-          }
-      };
-      if (!hidden) read([](int, int) { return true; });
-      else read([&](int u, int at) { return found[u] && seen.sees(j0 + 16 * u + at); });
+      const bool found = (uint32_t)page < (uint32_t)t.c.pages;
+      p.at[u] = found ? page * t.c.stride_p + (j - (int)(index * t.c.page.by)) * t.c.stride_n : -1;
+      p.hidden = p.hidden || (PAGES16 ? !found : __builtin_amdgcn_ballot_w64(!found) != 0);
+    }
+    return p;
+  };
+  // Whether entry `from` of 16 is there, and where; from: this lane's or another's
+  const auto entry = [&](const Place& p, int u, int from, int64_t& at) {
+    if constexpr (PAGES16) {
+      at = p.at[u];
+      return at >= 0 && seen.sees(p.j0 + 16 * u + from);
     } else {
-      int64_t key_at[SUB], value_at[SUB][4];   // in bytes from the pool's head g; -1: nowhere, or not seen
+      at = (int64_t)((uint64_t)(uint32_t)__shfl((int)(p.at[u] >> 32), from) << 32 | (uint32_t)__shfl((int)p.at[u], from));
+      return at >= 0;
+    }
+  };
+  u32x4_t k[SUB][STEPS];
+  VWord v[SUB][4][VN];
+  uint32_t there = 0;   // bit 4 u + x: value x of the lane's four of 16 entries is there; looked at where some are not
+  const auto load_keys = [&](const Place& p) {
+    const auto all = [&](auto guard) {
 #pragma unroll
       for (int u = 0; u < SUB; u++) {
-        const int j = j0 + 16 * u + m;
-        const uint32_t p = t.c.page(j);
-        const int32_t page = seen.sees(j) ? table[p] : -1;
-        const bool ok = (uint32_t)page < (uint32_t)t.c.pages;
-        key_at[u] = ok ? page * t.c.stride_p + (j - p * t.c.page.by) * t.c.stride_n : -1;
+        const char* const from = keys + p.at[u] + (PAGES16 ? key_off : quarter * 16);
+        const bool ok = !guard.value || (p.at[u] >= 0 && (!PAGES16 || seen.sees(p.j0 + 16 * u + m)));
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) k[u][s] = ok ? fetch<WHOLE_LINES, u32x4_t>(from + s * 64) : u32x4_t{0, 0, 0, 0};
+      }
+    };
+    if (p.hidden) all(std::true_type{});
+    else all(std::false_type{});
+  };
+  const auto load_values = [&](const Place& p) {
+    const auto all = [&](auto guard) {
+#pragma unroll
+      for (int u = 0; u < SUB; u++)
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-          const int from = 4 * quarter + x;
-          value_at[u][x] = (int64_t)((uint64_t)(uint32_t)__shfl((int)(key_at[u] >> 32), from) << 32 | (uint32_t)__shfl((int)key_at[u], from));
+          int64_t at;
+          const bool seen_here = entry(p, u, 4 * quarter + x, at), ok = !guard.value || seen_here;
+          if (guard.value) there = ok ? there | 1u << (4 * u + x) : there & ~(1u << (4 * u + x));
+          const char* const from = values + at + (PAGES16 ? value_off[x] : m * VB);
+#pragma unroll
+          for (int y = 0; y < VN; y++) v[u][x][y] = ok ? fetch<WHOLE_LINES, VWord>(from + y * 16) : VWord(0u);
         }
-        hidden = hidden || __builtin_amdgcn_ballot_w64(!ok) != 0;
-      }
-      const auto read = [&](auto ok) {
-#pragma unroll
-        for (int u = 0; u < SUB; u++) {
-          const bool here = ok(key_at[u]);
-#pragma unroll
-          for (int s = 0; s < STEPS; s++) k[u][s] = here ? *reinterpret_cast<const u32x4_t*>(keys + key_at[u] + quarter * 16 + s * 64) : u32x4_t{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int u = 0; u < SUB; u++)
-#pragma unroll
-          for (int x = 0; x < 4; x++) {
-            there[u][x] = ok(value_at[u][x]);
-#pragma unroll
-            for (int y = 0; y < VN; y++) v[u][x][y] = there[u][x] ? *reinterpret_cast<const VWord*>(values + value_at[u][x] + m * VB + y * 16) : VWord(0u);
-          }
-      };
-      if (!hidden) read([](int64_t) { return true; });
-      else read([](int64_t at) { return at >= 0; });
-    }
+    };
+    if (p.hidden) all(std::true_type{});
+    else all(std::false_type{});
+  };
+  // A tile's keys are asked for once those of the tile before have been multiplied, its values once those have: into the same registers, with the other half of
+  // a tile's work to hide behind. us, without -> so:
+  Place p;
+  if (begin + wave < end) p = locate(begin + wave), load_keys(p), load_values(p);
+  for (int i = begin + wave; i < end; i += kWaves) {
+    const int j0 = p.j0;
+    const bool hidden = p.hidden, more = i + kWaves < end;
+    if (more) p = locate(i + kWaves);
     // S^T of the tile, in log2 units
     f32x4_t x[SUB];
 #pragma unroll
@@ -220,10 +236,11 @@ __global__ void __launch_bounds__(kThreads) attend(Token t) {
       x[u] = s * t.scale_log2;
       if (hidden) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[u][e] = there[u][e] ? x[u][e] : -INFINITY;   // the entries of this lane's values are those of its scores
+        for (int e = 0; e < 4; e++) x[u][e] = there >> (4 * u + e) & 1 ? x[u][e] : -INFINITY;   // the entries of this lane's values are those of its scores
       }
       if (WEIGHTS && m < heads) *reinterpret_cast<f32x4_t*>(t.scores + (row0 + m) * t.row + j0 + 16 * u + 4 * quarter) = x[u];
     }
+    if (more) load_keys(p);
     float high = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
     if constexpr (SUB == 2) high = fmaxf(high, fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
     high = fmaxf(high, __shfl_xor(high, 16));
@@ -254,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) attend(Token t) {
         for (int c = 0; c < C; c++) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(number(word<VW>(v[0][e][c / VW], c % VW)), x[0][e], acc[c], 0, 0, 0);
     } else {
       // weights are rounded to the type of the values, which are products' other factor: 2^-9 of a weight in bf16, as in attention over whole tensors
-      const u32x4_t p = {pack<DT>(x[0][0], x[0][1]), pack<DT>(x[0][2], x[0][3]), pack<DT>(x[SUB - 1][0], x[SUB - 1][1]), pack<DT>(x[SUB - 1][2], x[SUB - 1][3])};
+      const u32x4_t weights = {pack<DT>(x[0][0], x[0][1]), pack<DT>(x[0][2], x[0][3]), pack<DT>(x[SUB - 1][0], x[SUB - 1][1]), pack<DT>(x[SUB - 1][2], x[SUB - 1][3])};
 #pragma unroll
       for (int c = 0; c < C; c += 2) {
         const int w = c / 2;   // the word of channels c, c + 1
@@ -264,10 +281,11 @@ __global__ void __launch_bounds__(kThreads) attend(Token t) {
           const uint32_t lo = word<VW>(v[y / 2][2 * (y % 2)][0], w), hi = word<VW>(v[y / 2][2 * (y % 2) + 1][0], w);
           even[y] = __builtin_amdgcn_perm(hi, lo, 0x05040100), odd[y] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
         }
-        acc[c] = mfma16<DT>(even, p, acc[c]);
-        acc[c + 1] = mfma16<DT>(odd, p, acc[c + 1]);
+        acc[c] = mfma16<DT>(even, weights, acc[c]);
+        acc[c + 1] = mfma16<DT>(odd, weights, acc[c + 1]);
       }
     }
+    if (more) load_values(p);
   }
 
   // The waves' results on one maximum, joined in their order
@@ -312,32 +330,43 @@ __global__ void __launch_bounds__(kThreads) attend(Token t) {
   }
 }
 
-// Maximum, in log2 units, and sum over the parts of a row
-__device__ __forceinline__ f32x2_t joined(const Token& t, int64_t row, int parts) {
+// Maximum, in log2 units, and sum over the parts of a row, by the lanes of a wave
+__device__ __forceinline__ f32x2_t joined(const Token& t, int64_t row, int parts, int lane) {
   const int64_t rows = (int64_t)t.c.batch * t.heads_q;
   float high = -INFINITY, total = 0.f;
-  for (int i = 0; i < parts; i++) high = fmaxf(high, t.stats[i * rows + row][0]);
+  for (int i = lane; i < parts; i += 64) high = fmaxf(high, t.stats[i * rows + row][0]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) high = fmaxf(high, __shfl_xor(high, d));
   const float ref = high == -INFINITY ? 0.f : high;
-  for (int i = 0; i < parts; i++) {
+  for (int i = lane; i < parts; i += 64) {
     const f32x2_t s = t.stats[i * rows + row];
     total += s[1] * __builtin_amdgcn_exp2f(s[0] - ref);
   }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
   return f32x2_t{high, total};
 }
 
-// O and L from the parts: a thread has four channels of a row
+// O and L of a row from its parts: a lane has four channels, groups of D / 4 lanes take the parts in turn. With one group and part after part 32 parts of 16 rows took
+// 21 us, each load waiting for the one before; so 5.
 template <int DT, int D>
-__device__ __forceinline__ void join_rows(const Token& t, int64_t id) {
+__device__ __forceinline__ void join_row(const Token& t, int64_t row, int tid) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32;
-  const int64_t rows = (int64_t)t.c.batch * t.heads_q, row = id / (D / 4);
-  if (row >= rows) return;
-  const int c = (int)(id % (D / 4)) * 4, b = (int)(row / t.heads_q), h = (int)(row - (int64_t)b * t.heads_q);
+  constexpr int LANES = D / 4, GROUPS = kThreads / LANES;
+  __shared__ f32x4_t sums[GROUPS][LANES];
+  const int64_t rows = (int64_t)t.c.batch * t.heads_q;
+  const int group = tid / LANES, c = tid % LANES * 4, b = (int)(row / t.heads_q), h = (int)(row - (int64_t)b * t.heads_q);
   const Seen<WIDE ? 16 : 32> seen(t.c.length(b), t.window, t.sinks);
   const int parts = parts_of(seen.tiles, t);
-  const f32x2_t all = joined(t, row, parts);
+  const f32x2_t all = joined(t, row, parts, tid & 63);   // every wave for itself
   const float ref = all[0] == -INFINITY ? 0.f : all[0];
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < parts; i++) o += *reinterpret_cast<const f32x4_t*>(t.part + (i * rows + row) * D + c) * __builtin_amdgcn_exp2f(t.stats[i * rows + row][0] - ref);
+#pragma unroll 4
+  for (int i = group; i < parts; i += GROUPS) o += *reinterpret_cast<const f32x4_t*>(t.part + (i * rows + row) * D + c) * __builtin_amdgcn_exp2f(t.stats[i * rows + row][0] - ref);
+  sums[group][tid % LANES] = o;
+  __syncthreads();
+  if (group != 0) return;
+  for (int i = 1; i < GROUPS; i++) o += sums[i][tid];
   o *= all[1] > 0.f ? 1.f / all[1] : all[1] == 0.f ? 0.f : all[1];
   char* const to = t.o + b * t.ob + h * t.oh + c * sizeof(typename Type<DT>::T);
   if constexpr (WIDE) *reinterpret_cast<f32x4_t*>(to) = o;
@@ -350,7 +379,8 @@ constexpr int kEntries = 4 * kThreads;   // of the weights that a workgroup adds
 // The weights of kEntries entries of a head of keys: what was kept of their scores, on the joined statistics
 template <int DT>
 __device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid) {
-  __shared__ float lse[kThreads];
+  constexpr int kHeads = 64, kGroup = 4;   // heads of queries at a time
+  __shared__ float lse[kHeads];
   const int blocks = (t.c.capacity + kEntries - 1) / kEntries;
   const int64_t slice = id / blocks;
   const int b = (int)(slice / t.c.heads_k), g = (int)(slice - (int64_t)b * t.c.heads_k), j0 = (int)(id - slice * blocks) * kEntries + tid;
@@ -362,20 +392,31 @@ __device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid)
   float w[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) w[i] = j0 + i * kThreads < t.c.capacity ? in[j0 + i * kThreads] : 0.f;
-  for (int h0 = 0; h0 < t.group; h0 += kThreads) {
-    const int heads = min(kThreads, t.group - h0);
+  const float* const scores = t.scores + row0 * t.row + j0;
+  float s[kGroup][4];
+  const auto load = [&](int h0) {   // of kGroup heads
+#pragma unroll
+    for (int h = 0; h < kGroup; h++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[h][i] = h0 + h < t.group && seen.sees(j0 + i * kThreads) ? scores[(h0 + h) * t.row + i * kThreads] : -INFINITY;
+  };
+  load(0);   // before the statistics, for which it does not have to wait
+  for (int h0 = 0; h0 < t.group; h0 += kHeads) {
+    const int heads = min(kHeads, t.group - h0);
     __syncthreads();
-    if (tid < heads) {
-      const f32x2_t all = joined(t, row0 + h0 + tid, parts);
-      lse[tid] = all[1] == 0.f ? INFINITY : all[0] + __builtin_amdgcn_logf(all[1]);
+    for (int h = tid >> 6; h < heads; h += kWaves) {
+      const f32x2_t all = joined(t, row0 + h0 + h, parts, tid & 63);
+      if ((tid & 63) == 0) lse[h] = all[1] == 0.f ? INFINITY : all[0] + __builtin_amdgcn_logf(all[1]);
     }
     __syncthreads();
-    for (int h = 0; h < heads; h++)
+    for (int h1 = 0; h1 < heads; h1 += kGroup) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int j = j0 + i * kThreads;
-        if (seen.sees(j)) w[i] += __builtin_amdgcn_exp2f(t.scores[(row0 + h0 + h) * t.row + j] - lse[h]);
-      }
+      for (int h = 0; h < kGroup; h++)
+        if (h1 + h < heads)
+#pragma unroll
+          for (int i = 0; i < 4; i++) w[i] += s[h][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[h][i] - lse[h1 + h]);
+      load(h0 + h1 + kGroup);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; i++)
@@ -384,9 +425,9 @@ __device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid)
 
 // What is left after the parts, in one launch: workgroups that join rows, and those that add weights behind them
 template <int DT, int D>
-__global__ void __launch_bounds__(kThreads) join_parts(Token t, int row_blocks) {
-  if ((int)blockIdx.x < row_blocks) join_rows<DT, D>(t, (int64_t)blockIdx.x * kThreads + threadIdx.x);
-  else add_weights<DT>(t, (int64_t)blockIdx.x - row_blocks, threadIdx.x);
+__global__ void __launch_bounds__(kThreads) join_parts(Token t, int rows) {
+  if ((int)blockIdx.x < rows) join_row<DT, D>(t, blockIdx.x, threadIdx.x);
+  else add_weights<DT>(t, (int64_t)blockIdx.x - rows, threadIdx.x);
 }
 
 // How the tiles of a call are dealt out
@@ -406,9 +447,13 @@ Plan plan_of(const fhog_paged_attn_args* a) {
   int64_t most = capacity;   // entries that a token may see
   if (a->window > 0 && a->window < capacity) most = std::min(capacity, a->window + std::min(a->sinks, capacity) + 2 * tile);
   const int64_t tiles = (most + tile - 1) / tile, group = a->heads_q / c.heads_k, slices = c.batch * c.heads_k * ((group + kColumns - 1) / kColumns);
-  p.least = kWaves;
-  const int64_t wanted = (768 + slices - 1) / slices, possible = (tiles + p.least - 1) / p.least;
-  p.splits = (int)std::max<int64_t>(1, std::min({wanted, possible, (int64_t)256}));
+  // Two workgroups to a CU, and where that many are there, nothing to join. us at 256 | 384 | 512 workgroups to a CU and more, bf16, d = 128, 8 heads of keys:
+  // TODO
+  int64_t least = (tiles * slices + 511) / 512;
+  least = std::max<int64_t>(kWaves, (least + kWaves - 1) / kWaves * kWaves);
+  if (tiles <= 16) least = 16;
+  p.least = (int)least;
+  p.splits = (int)((tiles + least - 1) / least);
   p.rows = c.batch * a->heads_q, p.row = (capacity + 31) & ~(int64_t)31;
   p.part_bytes = p.splits > 1 ? up16(sizeof(float) * p.splits * p.rows * c.d) : 0;
   p.stats_bytes = p.splits > 1 || a->weights_out ? up16(sizeof(f32x2_t) * p.splits * p.rows) : 0;
@@ -425,7 +470,7 @@ hipError_t launch_d(const Token& t, const fhog_paged_attn_args* a, hipStream_t s
   else pages16 ? go(attend<DT, D, true, false>) : go(attend<DT, D, false, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (t.splits == 1 && !t.weights_out)) return e;
-  const int64_t rows = t.splits > 1 ? ((int64_t)t.c.batch * t.heads_q * (D / 4) + kThreads - 1) / kThreads : 0;
+  const int64_t rows = t.splits > 1 ? (int64_t)t.c.batch * t.heads_q : 0;
   const int64_t weights = t.weights_out ? (int64_t)t.c.batch * t.c.heads_k * ((t.c.capacity + kEntries - 1) / kEntries) : 0;
   hipLaunchKernelGGL((join_parts<DT, D>), dim3((unsigned)(rows + weights)), dim3(kThreads), 0, s, t, (int)rows);
   return hipGetLastError();
