@@ -10,16 +10,22 @@
 // workgroup would go through are cut into pieces of equal length, one to a workgroup, where there are several they leave partial sums, which a second kernel
 // adds in their order: a causal mask leaves the first keys many times the work of the last, and a sink all of it.
 //
-// What bounds it: vector instructions, three of them and an exponential to 2 d flop of a pair.
+// What bounds it: the instructions of a SIMD. A block of 32 x 32 pairs takes d / 16 matrix instructions of 32 cycles and 48 vector instructions, 16 of them exponentials at half
+// rate: 256 cycles each at d = 128, which run side by side two thirds of the time. bf16, 16 heads x 16384 causal, four to one of keys, d = 128: 637 us, 864 TFLOP/s, 73 % of
+// what a large library product of bf16 matrices reaches here, which takes no exponentials.
 #include <algorithm>
+#include <type_traits>
 
-#include "fhog_bf16_util.h"
+#include "fhog_small.h"
 
 namespace fhog {
 using namespace bf16k;
 namespace {
 
 constexpr int kThreads = 256, kRows = 64;   // queries of a stage
+// Stages in LDS: the one that is read, the one after it, which has landed so that its statistics can be made ready, and those that are on their way
+template <int BYTES>
+constexpr int kRing = BYTES > 256 ? 3 : 4;
 
 struct Weigh {
   const char* q;
@@ -34,6 +40,9 @@ struct Weigh {
   int32_t tiles, pieces, chunk;               // of keys; pieces of a tile of keys at most; stages of a piece
   float scale_log2;
 };
+
+// Pieces into which the stages of a tile of keys go: as few as hold `chunk` each at most, the same number in every kernel
+__device__ __forceinline__ int pieces_of(int steps, const Weigh& w) { return (steps + w.chunk - 1) / w.chunk; }
 
 // Which queries see a key
 struct Queries {
@@ -74,6 +83,13 @@ struct Type<FHOG_DTYPE_FP32> {
 // The bits of a vector's element as a number; handed over by value: of an element itself __builtin_bit_cast takes the vector's first
 __device__ __forceinline__ float number(uint32_t bits) { return __builtin_bit_cast(float, bits); }
 
+// All loads but the last N of this wave have landed
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(N < 64, "a counter of six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // rows of BYTES bytes in LDS: chunk ch of row r lies at ch ^ swizzle(r), so that the 16-byte reads of a column of rows meet no bank twice
 template <int BYTES>
 __device__ __forceinline__ int swizzle(int r) {
@@ -84,21 +100,26 @@ template <int DT, int D, int NK>
 __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32, F16 = DT == FHOG_DTYPE_FP16;
   constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), CHUNKS = BYTES / 16, PER_LOAD = 64 / CHUNKS, LOADS = kRows / PER_LOAD / 4;
-  constexpr int TILE = kRows * BYTES, STAGE = TILE + kRows * 4, KEYS = 128 * NK, STEPS = CHUNKS / 2;
+  constexpr int TILE = kRows * BYTES, STAGE = TILE + kRows * 4, RING = kRing<BYTES>, KEYS = 128 * NK, STEPS = CHUNKS / 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
-  const int tile = blockIdx.x / w.pieces, piece = blockIdx.x - tile * w.pieces, g = blockIdx.y, b = blockIdx.z;
+  // Workgroup ids go round the eight XCDs: one piece of every tile after the other, so that those that have no such piece are spread over them, each piece beginning a
+  // tile further on, so that those of a tile are too. (Tile after tile, 64 tiles of 16 pieces left half of the XCDs idle: us, 16 x 16384 causal, d = 128 1082, so 650.)
+  const int piece = blockIdx.x / w.tiles, g = blockIdx.y, b = blockIdx.z;
+  int tile = blockIdx.x - piece * w.tiles + piece % w.tiles;
+  if (tile >= w.tiles) tile -= w.tiles;
   const Queries geo(w, b);
   const int k0 = tile * KEYS, kw = k0 + 32 * NK * wave;
   int begin, end;
   geo.stages(k0, KEYS, begin, end);
-  const int each = end - begin, steps = w.group * each, from = piece * w.chunk, to = min(steps, from + w.chunk);
-  if (w.pieces > 1 && from >= steps) return;
+  const int each = end - begin, steps = w.group * each, pieces = pieces_of(steps, w);
+  if (piece >= max(pieces, w.pieces == 1 ? 1 : 0)) return;
+  const int from = piece * w.chunk, to = min(steps, from + w.chunk);
 
   u32x4_t key[NK][STEPS];
   int lo[NK], hi[NK];                              // queries that see this lane's keys
-  int whole_lo[NK], whole_hi[NK], any_lo[NK], any_hi[NK];   // ... all of the wave's 32, and some of them
+  int any_lo = INT32_MAX, any_hi = -1, whole_lo = 0, whole_hi = INT32_MAX;   // ... some of the wave's, and all of them
 #pragma unroll
   for (int x = 0; x < NK; x++) {
     const int j0 = kw + 32 * x, j = j0 + n, last = min(j0 + 31, geo.n_k - 1);
@@ -106,10 +127,11 @@ __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
 #pragma unroll
     for (int s = 0; s < STEPS; s++) key[x][s] = geo.n_k > 0 ? *reinterpret_cast<const u32x4_t*>(row + 32 * s) : u32x4_t{0, 0, 0, 0};
     lo[x] = geo.first(j), hi[x] = j < geo.n_k ? geo.last(j) : -1;
-    any_lo[x] = geo.first(j0), any_hi[x] = j0 >= geo.n_k ? -1 : j0 < geo.sinks ? geo.n_q - 1 : geo.last(last);
-    whole_lo[x] = geo.first(j0 + 31), whole_hi[x] = j0 + 31 >= geo.n_k ? -1 : geo.last(max(j0, min(geo.sinks, j0 + 31)));
+    any_lo = min(any_lo, geo.first(j0)), any_hi = max(any_hi, j0 >= geo.n_k ? -1 : j0 < geo.sinks ? geo.n_q - 1 : geo.last(last));
+    whole_lo = max(whole_lo, geo.first(j0 + 31)), whole_hi = min(whole_hi, j0 + 31 >= geo.n_k ? -1 : geo.last(max(j0, min(geo.sinks, j0 + 31))));
   }
   float sum[NK] = {};
+  wait_vm0();   // the keys are there: said once here, or the compiler waits for them, and for the staging loads under way, in every tile
 
   // staging: straight into LDS, 1 KiB to an instruction; rows past the end are copies of the last
   uint32_t off[LOADS];
@@ -120,89 +142,140 @@ __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
 #pragma unroll
   for (int u = 0; u < LOADS; u++) off[u] = offset(u, kRows);
   const uint32_t ring = lds_addr(smem);
-  float stat = 0.f;
-  int head = 0, t = begin;   // of the stage that is issued next
-  if (each > 0) head = from / each, t = begin + from - head * each;
-  const auto issue = [&](int slot) {
-    const int64_t row = ((int64_t)b * w.heads_q + g * w.group + head);
-    const char* const src = w.q + b * w.qb + (int64_t)(g * w.group + head) * w.qh + (int64_t)t * kRows * w.qn;
-    const int valid = geo.n_q - t * kRows;
-    if (tid < kRows) stat = *(global_f32_ptr)(w.lse + row * w.n_q + min(t * kRows + tid, geo.n_q - 1));
-#pragma unroll
-    for (int u = 0; u < LOADS; u++)
-      Dma<64>::issue_one(ring + slot * STAGE + (wave + 4 * u) * 1024, valid >= kRows ? off[u] : offset(u, valid), (const __bf16*)src);
-    if (++t == end) t = begin, head++;
-  };
-  // A query that saw nothing has no weights to give: exp(s - infinity)
-  const auto publish = [&](int slot) {
-    if (tid < kRows) reinterpret_cast<float*>(smem + slot * STAGE + TILE)[tid] = stat == -INFINITY ? INFINITY : stat * kLog2e;
-  };
-  if (from < to) {
-    issue(0);
-    wait_vm0();
-    publish(0);
+  int t = begin;            // of the stage that is issued next; its queries, its statistics, and where it goes
+  const int64_t row0 = (int64_t)b * w.heads_q + g * w.group, stage_bytes = kRows * w.qn;
+  const char* src = w.q + b * w.qb + (int64_t)g * w.group * w.qh + begin * stage_bytes;
+  const float* lse = w.lse + row0 * w.n_q + begin * kRows;
+  uint32_t into = ring;
+  if (each > 0) {
+    const int head = from / each;
+    t = begin + from - head * each, src += head * w.qh + (t - begin) * stage_bytes, lse += (int64_t)head * w.n_q + (t - begin) * kRows;
   }
+  const int64_t back = w.qh - (each - 1) * stage_bytes, lse_back = w.n_q - (int64_t)(each - 1) * kRows;   // to the first stage of the next head
+  // Every wave asks for the statistics too, to the same place: then each has as many loads of a stage under way, and can wait for all but the last stages'
+  constexpr int MINE = LOADS + 1;
+  const auto issue = [&] {
+    const int valid = geo.n_q - t * kRows;
+    if (valid >= kRows) {
+      smallk::stage_words(into + TILE, lse + lane);
+#pragma unroll
+      for (int u = 0; u < LOADS; u++) Dma<64>::issue_one(into + (wave + 4 * u) * 1024, off[u], (const __bf16*)src);
+    } else {
+      keep_branch();
+      smallk::stage_words(into + TILE, lse + min(lane, valid - 1));
+#pragma unroll
+      for (int u = 0; u < LOADS; u++) Dma<64>::issue_one(into + (wave + 4 * u) * 1024, offset(u, valid), (const __bf16*)src);
+    }
+    into = into == ring + (RING - 1) * STAGE ? ring : into + STAGE;
+    if (++t == end) t = begin, src += back, lse += lse_back;
+    else src += stage_bytes, lse += kRows;
+  };
+  // L in log2 units. A query that saw nothing has no weights to give: exp(s - infinity)
+  const auto make_ready = [&](char* stage) {
+    float* const at = reinterpret_cast<float*>(stage + TILE) + lane;
+    const float l = *at;
+    *at = l == -INFINITY ? INFINITY : l * kLog2e;
+  };
+  for (int i = 0; i < RING - 1 && from + i < to; i++) issue();
   dma_wait();
   __syncthreads();
+  if (from < to && wave == 0) make_ready(smem);
+  char* stage = smem;
+  __syncthreads();
   int now = each > 0 ? begin + from % each : 0;
+  // Two tiles of 32 queries are on the way at a time, each in registers of its own: while one is multiplied, the exponentials of the one before are taken behind its
+  // matrix instructions, a few behind each, so that neither kind waits for the other. us, 16 x 16384 causal, d = 128: one tile at a time 760, so 690; the scalars of a stage carried along instead of
+  // formed anew 660 -> 637.
+  f32x16_t scores[2][NK];
+  f32x4_t stats[2][4];      // L of the lane's 16 queries: 8 g + 4 h + e
+  int waiting = -1;         // the tile whose exponentials are still to be taken; the same for the wave
+  float part[NK][2];        // sums of a tile
+  // a slice of the exponentials of a tile
+  const auto some = [&](int t, int c, int x) {
+#pragma unroll
+    for (int r = c * 16 / STEPS; r < (c + 1) * 16 / STEPS; r++) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[t][x][r], w.scale_log2, -stats[t][r / 4][r % 4]));
+      part[x][r % 2] = r < 2 ? p : part[x][r % 2] + p;
+    }
+  };
+  // sums of tiles, then of their sums: a sum over many queries is rounded once for each tile, not for each query
+  const auto add = [&] {
+#pragma unroll
+    for (int x = 0; x < NK; x++) sum[x] += part[x][0] + part[x][1];
+  };
+  const auto rest = [&](int t) {
+#pragma unroll
+    for (int c = 0; c < STEPS; c++)
+#pragma unroll
+      for (int x = 0; x < NK; x++) some(t, c, x);
+    add();
+  };
   for (int step = from; step < to; step++) {
-    const int slot = (step - from) & 1;
-    if (step + 1 < to) issue(slot ^ 1);
-    const char* const stage = smem + slot * STAGE;
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
+    const bool more = step + RING - 1 < to;
+    if (more) issue();
+    char* const after = stage == smem + (RING - 1) * STAGE ? smem : stage + STAGE;
+    if (step + 1 < to && wave == (step & 3)) make_ready(after);
+    const auto tile_of = [&](auto which) {
+      constexpr int u = decltype(which)::value;
       const int i0 = now * kRows + 32 * u;
-      bool dead = true;
+      if (i0 > any_hi || i0 + 31 < any_lo) return;   // no query of the tile sees a key of this wave
+      if (waiting == u) rest(u);
+      const auto multiply = [&](auto beside) {
+        constexpr int AHEAD = STEPS < 3 ? STEPS : 3;
+        const char* const row = stage + (32 * u + n) * BYTES;
+        u32x4_t a[AHEAD];
+        const auto read = [&](int c) { a[c % AHEAD] = *reinterpret_cast<const u32x4_t*>(row + (((2 * c + h) ^ swizzle<BYTES>(n)) << 4)); };
 #pragma unroll
-      for (int x = 0; x < NK; x++) dead = dead && (i0 > any_hi[x] || i0 + 31 < any_lo[x]);
-      if (dead) continue;   // no query of the tile sees a key of this wave
-      f32x16_t s[NK];
+        for (int c = 0; c < AHEAD - 1; c++) read(c);
 #pragma unroll
-      for (int x = 0; x < NK; x++) s[x] = f32x16_t{0};
+        for (int e = 0; e < 4; e++) stats[u][e] = *reinterpret_cast<const f32x4_t*>(stage + TILE + (32 * u + 8 * e + 4 * h) * 4);
 #pragma unroll
-      for (int c = 0; c < STEPS; c++) {
-        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(stage + (32 * u + n) * BYTES + (((2 * c + h) ^ swizzle<BYTES>(32 * u + n)) << 4));
+        for (int c = 0; c < STEPS; c++) {
+          if (c + AHEAD - 1 < STEPS) read(c + AHEAD - 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int x = 0; x < NK; x++) {
-          if constexpr (WIDE) {
+          for (int x = 0; x < NK; x++) {
+            if (c == 0) scores[u][x] = f32x16_t{0};
+            if constexpr (WIDE) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(number(a[e]), number(key[x][c][e]), s[x], 0, 0, 0);
-          } else {
-            s[x] = mfma<F16>(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, key[x][c]), s[x]);
+              for (int e = 0; e < 4; e++) scores[u][x] = __builtin_amdgcn_mfma_f32_32x32x2f32(number(a[c % AHEAD][e]), number(key[x][c][e]), scores[u][x], 0, 0, 0);
+            } else {
+              scores[u][x] = mfma<F16>(__builtin_bit_cast(bf16x8_t, a[c % AHEAD]), __builtin_bit_cast(bf16x8_t, key[x][c]), scores[u][x]);
+            }
+            if (beside.value) some(u ^ 1, c, x);
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
-      }
-      f32x4_t l[4];   // of the lane's 16 queries: 8 g + 4 h + e
-#pragma unroll
-      for (int e = 0; e < 4; e++) l[e] = *reinterpret_cast<const f32x4_t*>(stage + TILE + (32 * u + 8 * e + 4 * h) * 4);
+        if (beside.value) add();
+      };
+      if (waiting == (u ^ 1)) multiply(std::true_type{});
+      else multiply(std::false_type{});
+      waiting = u;
+      if (i0 >= whole_lo && i0 + 31 <= whole_hi) return;
+      // some queries do not see some keys: at once, with a look at each
+      keep_branch();
+      waiting = -1;
 #pragma unroll
       for (int x = 0; x < NK; x++) {
+        float all = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], w.scale_log2, -l[r / 4][r % 4]));
-        if (i0 < whole_lo[x] || i0 + 31 > whole_hi[x]) {   // the same for the wave
-          keep_branch();
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const int i = i0 + 8 * (r / 4) + 4 * h + r % 4;
-            s[x][r] = i >= lo[x] && i <= hi[x] ? s[x][r] : 0.f;
-          }
+        for (int r = 0; r < 16; r++) {
+          const int i = i0 + 8 * (r / 4) + 4 * h + r % 4;
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[u][x][r], w.scale_log2, -stats[u][r / 4][r % 4]));
+          all += i >= lo[x] && i <= hi[x] ? p : 0.f;
         }
-        // in pairs: a sum over many tiles loses a rounding for each tile, not for each query
-#pragma unroll
-        for (int d = 8; d; d /= 2)
-#pragma unroll
-          for (int r = 0; r < d; r++) s[x][r] += s[x][r + d];
-        sum[x] += s[x][0];
+        sum[x] += all;
       }
-    }
+    };
+    tile_of(Slot<0>{}), tile_of(Slot<1>{});
     if (++now == end) now = begin;
-    if (step + 1 < to) {
-      wait_vm0();
-      publish(slot ^ 1);
-    }
-    dma_wait();
+    stage = after;
+    if (more) wait_vm<(RING - 3) * MINE>();   // the stage after the next one has landed
+    else dma_wait();
     __syncthreads();
   }
+  if (waiting == 0) rest(0);
+  if (waiting == 1) rest(1);
 #pragma unroll
   for (int x = 0; x < NK; x++) {
     const float total = sum[x] + __shfl_xor(sum[x], 32);
@@ -220,7 +293,7 @@ __global__ void __launch_bounds__(kThreads) add_pieces(Weigh w) {
   const Queries geo(w, b);
   int begin, end;
   geo.stages(j / KEYS * KEYS, KEYS, begin, end);
-  const int pieces = (w.group * (end - begin) + w.chunk - 1) / w.chunk;
+  const int pieces = pieces_of(w.group * (end - begin), w);
   const int64_t slice = (int64_t)w.heads_k * w.batch * w.n_k;
   const float* const part = w.part + ((int64_t)b * w.heads_k + g) * w.n_k + j;
   float sum = 0.f;
@@ -237,28 +310,41 @@ struct Plan {
 
 Plan plan_of(const fhog_key_weights_args* a) {
   Plan p;
-  const int64_t slices = a->batch * a->heads_k, group = a->heads_q / a->heads_k;
-  const int64_t window = a->causal != FHOG_MASK_NONE && a->window > 0 ? std::min(a->window, a->n_k) : a->n_k;
-  p.nk = a->dtype == FHOG_DTYPE_FP32 ? 1 : 2;
-  const int64_t keys = 128 * p.nk;
-  p.tiles = (a->n_k + keys - 1) / keys;
-  // stages of the tile of keys with the most, and about how many there are in all
-  const int64_t all = (a->n_q + kRows - 1) / kRows, most = a->sinks > 0 || window >= a->n_k ? all : std::min(all, (window + keys) / kRows + 2);
-  const int64_t mean = a->causal == FHOG_MASK_NONE ? all : std::min(most, (a->n_q < a->n_k ? all : all / 2 + 1));
-  const int64_t total = mean * group * p.tiles * slices;
-  const int64_t chunk = std::max<int64_t>(8, (total + 1535) / 1536);
+  const int64_t slices = a->batch * a->heads_k, group = a->heads_q / a->heads_k, all = (a->n_q + kRows - 1) / kRows;
+  const bool banded = a->causal != FHOG_MASK_NONE && a->window > 0 && a->window < a->n_q;
+  // stages of a tile of keys in one head of queries: those of the tile with the most, and about those of all of them together
+  const auto stages = [&](int64_t keys, int64_t& most, int64_t& total) {
+    p.tiles = (a->n_k + keys - 1) / keys;
+    const int64_t band = banded ? std::min(all, (a->window + keys) / kRows + 2) : all;
+    most = a->sinks > 0 ? all : band;
+    const int64_t seen = a->causal == FHOG_MASK_NONE ? a->n_k : a->n_k - a->n_q / 2;   // keys of a query, about, without a window
+    total = std::max(p.tiles, banded ? std::min(p.tiles, (a->n_q + a->window + keys - 1) / keys) * band : all * ((seen + keys - 1) / keys));
+  };
+  // 64 keys to a wave where there is work for it: half the reads of LDS, but fewer waves and coarser masks. us, 32 | 64 keys, bf16: d = 128 causal 16 heads x 16384
+  // 728 | 638, 32 x 4096 127 | 110, window 4096 of 16 x 16384 340 | 303, window 1024 167 | 180, 8 x 512 11 | 15; d = 64, whose waves have fewer matrix instructions to hide
+  // behind, 16 x 16384 422 | 491, 32 x 2048 32 | 42
+  int64_t most, total;
+  p.nk = 2, stages(256, most, total);
+  if (a->dtype == FHOG_DTYPE_FP32 || a->d != 128 || (banded && a->window < 2048) || total * group * slices < 4096) p.nk = 1, stages(128, most, total);
+  // Two workgroups to a CU as long as that leaves pieces worth their beginning, and short enough to even out the end of the launch. us, at most 16 | 24 | 32 | 40 stages:
+  // 16 x 16384 d = 128 650 | 640 | 638 | 634, d = 64 444 | 427 | 422 | 428; at least 6 | 8: 16 x 3000 60 | 47, 8 x 512 12.6 | 11.3
+  int64_t chunk = std::min<int64_t>(32, std::max<int64_t>(a->dtype == FHOG_DTYPE_FP32 ? 3 : 8, (total * group * slices + 1023) / 1024));
+  if (banded) {   // most tiles have as many stages: cut them evenly (us, fp16 48 x 1537, window 400: 32 -> 28)
+    const int64_t mine = group * std::min(all, (a->window + 128 * p.nk) / kRows + 2), n = std::max<int64_t>(1, (mine + chunk / 2) / chunk);
+    chunk = (mine + n - 1) / n;
+  }
   p.pieces = (int)std::max<int64_t>(1, (most * group + chunk - 1) / chunk);
-  p.chunk = p.pieces == 1 ? (int)(most * group) : (int)chunk;
+  p.chunk = (int)std::max(chunk, p.pieces == 1 ? most * group : 0);
   p.bytes = p.pieces > 1 ? sizeof(float) * p.pieces * slices * a->n_k : 0;
   return p;
 }
 
 template <int DT, int D, int NK>
 hipError_t launch_d(const Weigh& w, hipStream_t s) {
-  constexpr int STAGE = kRows * D * (int)sizeof(typename Type<DT>::T) + kRows * 4;
-  const hipError_t e = allow_dynamic_lds<weigh<DT, D, NK>>(2 * STAGE);
+  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), STAGE = kRows * BYTES + kRows * 4, LDS = kRing<BYTES> * STAGE;
+  const hipError_t e = allow_dynamic_lds<weigh<DT, D, NK>>(LDS);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((weigh<DT, D, NK>), dim3((unsigned)(w.tiles * w.pieces), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), 2 * STAGE, s, w);
+  hipLaunchKernelGGL((weigh<DT, D, NK>), dim3((unsigned)(w.tiles * w.pieces), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), LDS, s, w);
   if (w.pieces > 1) hipLaunchKernelGGL((add_pieces<128 * NK>), dim3((unsigned)((w.n_k + kThreads - 1) / kThreads), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), 0, s, w);
   return hipGetLastError();
 }
@@ -284,11 +370,9 @@ hipError_t launch_key_weights(const fhog_key_weights_args* a, hipStream_t s) {
   w.window = a->window > 0 && a->window < w.n_q + (int64_t)w.n_k ? (int32_t)a->window : w.n_q + w.n_k;
   w.sinks = (int32_t)std::min<int64_t>(a->sinks, a->n_k);
   w.tiles = (int32_t)p.tiles, w.pieces = p.pieces, w.chunk = p.chunk, w.scale_log2 = a->scale * kLog2e;
-  switch (a->dtype) {
-    case FHOG_DTYPE_FP32: return launch_t<FHOG_DTYPE_FP32, 1>(w, a->d, s);
-    case FHOG_DTYPE_FP16: return launch_t<FHOG_DTYPE_FP16, 2>(w, a->d, s);
-    default: return launch_t<FHOG_DTYPE_BF16, 2>(w, a->d, s);
-  }
+  if (a->dtype == FHOG_DTYPE_FP32) return launch_t<FHOG_DTYPE_FP32, 1>(w, a->d, s);
+  if (a->dtype == FHOG_DTYPE_FP16) return p.nk == 1 ? launch_t<FHOG_DTYPE_FP16, 1>(w, a->d, s) : launch_t<FHOG_DTYPE_FP16, 2>(w, a->d, s);
+  return p.nk == 1 ? launch_t<FHOG_DTYPE_BF16, 1>(w, a->d, s) : launch_t<FHOG_DTYPE_BF16, 2>(w, a->d, s);
 }
 
 }  // namespace fhog

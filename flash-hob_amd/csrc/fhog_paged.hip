@@ -76,8 +76,8 @@ __device__ __forceinline__ uint32_t rank_of(float w, int j, int n, const Evict& 
 // Which entries of one sequence and head of keys stay. Each wave has a stretch of the entries. The rank of the last one that stays is found digit by digit, eight bits at a
 // time from the top: a histogram of the digit over the entries whose higher digits are those found so far, and the digit at which the sum from above reaches
 // what is still to be found. Then the entries that stay are counted, wave by wave, and written to the places that the counts give.
-// What bounds it: the waits between its passes. Ranks are formed once and held in LDS (us, 32 x 8 slices of 8192 | 4 x 4 of 1000: weights read anew in every pass 26.6 | 7.4, ranks in
-// registers 20.2 | 10.8, so TODO).
+// What bounds it: the waits between its passes. us, 32 x 8 slices of 8192 | 4 x 4 of 1000: weights read anew in every pass 26.6 | 7.4, ranks formed once and kept in registers
+// 20.2 | 10.8, in LDS 22.7 | 7.6, and there with a histogram of eight copies 19.8 | 7.7.
 __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   extern __shared__ uint32_t held[];
   __shared__ uint32_t histogram[kCopies][kDigits];   // a lane counts in copy lane % kCopies: the same digit of many lanes is not one address
