@@ -75,8 +75,8 @@ __device__ __forceinline__ uint32_t word(const typename Words<4 * W>::type& v, i
   else return v[i];
 }
 
-// ONCE: past the caches, where nothing is read twice. TB/s of a loop of 16-byte loads over 2 GiB 6.2 -> 7.1; of rows of 256 bytes and more: rows of 128 bytes are read half
-// a line at a time, and lose what the first half brought.
+// ONCE: past the caches. TB/s of a loop of 16-byte loads over 2 GiB 6.2 -> 7.1; us, d = 128, bf16, 8 heads of keys 32 x 16384 326 -> 302, 64 x 2048 93 -> 84. For rows of 256 bytes
+// and more (rows of 128 are read half a line at a time: d = 64, 24 x 700 15 -> 17) that one workgroup alone reads (64 heads of queries to 2 of keys, 32 x 16384: 113, else 150).
 template <bool ONCE, typename V>
 __device__ __forceinline__ V fetch(const char* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
@@ -98,23 +98,31 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, pair{(T)lo, (T)hi});
 }
 
-// PAGES16: pages of a multiple of 16 entries, so that 16 in a row share one. WEIGHTS: scores are kept.
-template <int DT, int D, bool PAGES16, bool WEIGHTS>
+// Entries of a tile
+template <int DT>
+constexpr int kTile = DT == FHOG_DTYPE_FP32 ? 16 : 32;
+int tile_of(int dtype) { return dtype == FHOG_DTYPE_FP32 ? kTile<FHOG_DTYPE_FP32> : kTile<FHOG_DTYPE_BF16>; }
+
+// PAGES16: pages of a multiple of 16 entries, so that 16 in a row share one. WEIGHTS: scores are kept. ONCE: as in fetch.
+template <int DT, int D, bool PAGES16, bool WEIGHTS, bool ONCE>
 __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32;
   typedef typename Type<DT>::T T;
-  constexpr int TILE = WIDE ? 16 : 32, SUB = TILE / 16;   // entries of a tile; 16 at a time
+  constexpr int TILE = kTile<DT>, SUB = TILE / 16;     // entries of a tile; 16 at a time
   constexpr int STEPS = D * (int)sizeof(T) / 64;          // 16-byte pieces of a row that a lane has (four lanes to a row)
   constexpr int C = D / 16;                               // channels of a lane in V and O
   constexpr int VB = C * sizeof(T), VW = VB >= 16 ? 4 : VB / 4, VN = VB >= 16 ? VB / 16 : 1;   // bytes of them, words of a load, loads
-  constexpr bool WHOLE_LINES = D * (int)sizeof(T) >= 256;
   typedef typename Words<4 * VW>::type VWord;
   __shared__ float tops[kWaves][kColumns], sums[kWaves][kColumns];
   __shared__ float rows[kWaves][kColumns][D + 4];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, quarter = lane >> 4;
-  const int split = blockIdx.x, b = blockIdx.z, g = blockIdx.y / t.columns, first_head = (blockIdx.y - g * t.columns) * kColumns;
+  // Workgroups of the same entries, for other heads of queries, come eight ids apart: on the same XCD, where the second one finds what the first one read
+  const uint32_t turn = blockIdx.x / (8 * t.columns), inside = blockIdx.x - turn * (8 * t.columns), unit = 8 * turn + (inside & 7);
+  const uint32_t slice = unit / t.splits;
+  if (slice >= (uint32_t)(t.c.batch * t.c.heads_k)) return;
+  const int split = unit - slice * t.splits, b = slice / t.c.heads_k, g = slice - b * t.c.heads_k, first_head = (inside >> 3) * kColumns;
   const int heads = min(kColumns, t.group - first_head);
   const int64_t row0 = (int64_t)b * t.heads_q + g * t.group + first_head;   // of (batch * heads_q)
   const Seen<TILE> seen(t.c.length(b), t.window, t.sinks);
@@ -188,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
         const char* const from = keys + p.at[u] + (PAGES16 ? key_off : quarter * 16);
         const bool ok = !guard.value || (p.at[u] >= 0 && (!PAGES16 || seen.sees(p.j0 + 16 * u + m)));
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) k[u][s] = ok ? fetch<WHOLE_LINES, u32x4_t>(from + s * 64) : u32x4_t{0, 0, 0, 0};
+        for (int s = 0; s < STEPS; s++) k[u][s] = ok ? fetch<ONCE, u32x4_t>(from + s * 64) : u32x4_t{0, 0, 0, 0};
       }
     };
     if (p.hidden) all(std::true_type{});
@@ -205,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
           if (guard.value) there = ok ? there | 1u << (4 * u + x) : there & ~(1u << (4 * u + x));
           const char* const from = values + at + (PAGES16 ? value_off[x] : m * VB);
 #pragma unroll
-          for (int y = 0; y < VN; y++) v[u][x][y] = ok ? fetch<WHOLE_LINES, VWord>(from + y * 16) : VWord(0u);
+          for (int y = 0; y < VN; y++) v[u][x][y] = ok ? fetch<ONCE, VWord>(from + y * 16) : VWord(0u);
         }
     };
     if (p.hidden) all(std::true_type{});
@@ -241,8 +249,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
       if (WEIGHTS && m < heads) *reinterpret_cast<f32x4_t*>(t.scores + (row0 + m) * t.row + j0 + 16 * u + 4 * quarter) = x[u];
     }
     if (more) load_keys(p);
-    float high = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
-    if constexpr (SUB == 2) high = fmaxf(high, fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    float high = x[0][0];
+#pragma unroll
+    for (int u = 0; u < SUB; u++) high = fmaxf(fmaxf(high, fmaxf(x[u][0], x[u][1])), fmaxf(x[u][2], x[u][3]));
     high = fmaxf(high, __shfl_xor(high, 16));
     high = fmaxf(high, __shfl_xor(high, 32));
     // The reference of the exponentials follows the maximum only in jumps of more than 8 (in log2 units): weights may then reach 2^8, which costs no precision,
@@ -266,23 +275,28 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
     // O^T += V^T P^T
     if constexpr (WIDE) {
 #pragma unroll
-      for (int e = 0; e < 4; e++)
+      for (int u = 0; u < SUB; u++)
 #pragma unroll
-        for (int c = 0; c < C; c++) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(number(word<VW>(v[0][e][c / VW], c % VW)), x[0][e], acc[c], 0, 0, 0);
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int c = 0; c < C; c++) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(number(word<VW>(v[u][e][c / VW], c % VW)), x[u][e], acc[c], 0, 0, 0);
     } else {
-      // weights are rounded to the type of the values, which are products' other factor: 2^-9 of a weight in bf16, as in attention over whole tensors
-      const u32x4_t weights = {pack<DT>(x[0][0], x[0][1]), pack<DT>(x[0][2], x[0][3]), pack<DT>(x[SUB - 1][0], x[SUB - 1][1]), pack<DT>(x[SUB - 1][2], x[SUB - 1][3])};
 #pragma unroll
-      for (int c = 0; c < C; c += 2) {
-        const int w = c / 2;   // the word of channels c, c + 1
-        u32x4_t even, odd;
+      for (int u = 0; u < SUB; u += 2) {
+        // weights are rounded to the type of the values, which are products' other factor: 2^-9 of a weight in bf16, as in attention over whole tensors
+        const u32x4_t weights = {pack<DT>(x[u][0], x[u][1]), pack<DT>(x[u][2], x[u][3]), pack<DT>(x[u + 1][0], x[u + 1][1]), pack<DT>(x[u + 1][2], x[u + 1][3])};
 #pragma unroll
-        for (int y = 0; y < 4; y++) {
-          const uint32_t lo = word<VW>(v[y / 2][2 * (y % 2)][0], w), hi = word<VW>(v[y / 2][2 * (y % 2) + 1][0], w);
-          even[y] = __builtin_amdgcn_perm(hi, lo, 0x05040100), odd[y] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+        for (int c = 0; c < C; c += 2) {
+          const int w = c / 2;   // the word of channels c, c + 1
+          u32x4_t even, odd;
+#pragma unroll
+          for (int y = 0; y < 4; y++) {
+            const uint32_t lo = word<VW>(v[u + y / 2][2 * (y % 2)][0], w), hi = word<VW>(v[u + y / 2][2 * (y % 2) + 1][0], w);
+            even[y] = __builtin_amdgcn_perm(hi, lo, 0x05040100), odd[y] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+          }
+          acc[c] = mfma16<DT>(even, weights, acc[c]);
+          acc[c + 1] = mfma16<DT>(odd, weights, acc[c + 1]);
         }
-        acc[c] = mfma16<DT>(even, weights, acc[c]);
-        acc[c + 1] = mfma16<DT>(odd, weights, acc[c + 1]);
       }
     }
     if (more) load_values(p);
@@ -356,7 +370,7 @@ __device__ __forceinline__ void join_row(const Token& t, int64_t row, int tid) {
   __shared__ f32x4_t sums[GROUPS][LANES];
   const int64_t rows = (int64_t)t.c.batch * t.heads_q;
   const int group = tid / LANES, c = tid % LANES * 4, b = (int)(row / t.heads_q), h = (int)(row - (int64_t)b * t.heads_q);
-  const Seen<WIDE ? 16 : 32> seen(t.c.length(b), t.window, t.sinks);
+  const Seen<kTile<DT>> seen(t.c.length(b), t.window, t.sinks);
   const int parts = parts_of(seen.tiles, t);
   const f32x2_t all = joined(t, row, parts, tid & 63);   // every wave for itself
   const float ref = all[0] == -INFINITY ? 0.f : all[0];
@@ -384,7 +398,7 @@ __device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid)
   const int blocks = (t.c.capacity + kEntries - 1) / kEntries;
   const int64_t slice = id / blocks;
   const int b = (int)(slice / t.c.heads_k), g = (int)(slice - (int64_t)b * t.c.heads_k), j0 = (int)(id - slice * blocks) * kEntries + tid;
-  const Seen<DT == FHOG_DTYPE_FP32 ? 16 : 32> seen(t.c.length(b), t.window, t.sinks);
+  const Seen<kTile<DT>> seen(t.c.length(b), t.window, t.sinks);
   const int parts = parts_of(seen.tiles, t);
   const int64_t row0 = (int64_t)b * t.heads_q + g * t.group;
   const float* const in = t.weights_in + b * t.wib + g * t.wih;
@@ -443,7 +457,7 @@ size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 Plan plan_of(const fhog_paged_attn_args* a) {
   Plan p;
   const fhog_paged_cache& c = a->cache;
-  const int64_t tile = c.dtype == FHOG_DTYPE_FP32 ? 16 : 32, capacity = c.table_width * c.page;
+  const int64_t tile = tile_of(c.dtype), capacity = c.table_width * c.page;
   int64_t most = capacity;   // entries that a token may see
   if (a->window > 0 && a->window < capacity) most = std::min(capacity, a->window + std::min(a->sinks, capacity) + 2 * tile);
   const int64_t tiles = (most + tile - 1) / tile, group = a->heads_q / c.heads_k, slices = c.batch * c.heads_k * ((group + kColumns - 1) / kColumns);
@@ -451,10 +465,10 @@ Plan plan_of(const fhog_paged_attn_args* a) {
   // 8 x 4096 28.2 | 29.4 | 29.0, 64 x 2048 84.5 | 90.5 | 90.6, 32 x 16384 of ragged lengths 302 | 300 | 303. Up to 512 entries stay in one workgroup (1 x 300: 11.6 -> 9.0).
   int64_t least = (tiles * slices + 511) / 512;
   least = std::max<int64_t>(kWaves, (least + kWaves - 1) / kWaves * kWaves);
-  if (tiles <= 16) least = 16;
+  if (tiles * tile <= 512) least = tiles;
   p.least = (int)least;
   p.splits = (int)((tiles + least - 1) / least);
-  p.rows = c.batch * a->heads_q, p.row = (capacity + 31) & ~(int64_t)31;
+  p.rows = c.batch * a->heads_q, p.row = (capacity + tile - 1) / tile * tile;
   p.part_bytes = p.splits > 1 ? up16(sizeof(float) * p.splits * p.rows * c.d) : 0;
   p.stats_bytes = p.splits > 1 || a->weights_out ? up16(sizeof(f32x2_t) * p.splits * p.rows) : 0;
   p.score_bytes = a->weights_out ? sizeof(float) * p.rows * p.row : 0;
@@ -463,11 +477,18 @@ Plan plan_of(const fhog_paged_attn_args* a) {
 
 template <int DT, int D>
 hipError_t launch_d(const Token& t, const fhog_paged_attn_args* a, hipStream_t s) {
-  const dim3 grid((unsigned)t.splits, (unsigned)(t.c.heads_k * t.columns), (unsigned)t.c.batch);
+  const int64_t units = (int64_t)t.splits * t.c.heads_k * t.c.batch;
+  const dim3 grid((unsigned)((units + 7) / 8 * 8 * t.columns));
   const bool pages16 = t.c.page.by % 16 == 0;
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, t); };
-  if (t.weights_out) pages16 ? go(attend<DT, D, true, true>) : go(attend<DT, D, false, true>);
-  else pages16 ? go(attend<DT, D, true, false>) : go(attend<DT, D, false, false>);
+  const auto pick = [&](auto once) {
+    constexpr bool ONCE = decltype(once)::value;
+    if (t.weights_out) pages16 ? go(attend<DT, D, true, true, ONCE>) : go(attend<DT, D, false, true, ONCE>);
+    else pages16 ? go(attend<DT, D, true, false, ONCE>) : go(attend<DT, D, false, false, ONCE>);
+  };
+  constexpr bool WHOLE_LINES = D * sizeof(typename Type<DT>::T) >= 256;
+  if (WHOLE_LINES && t.columns == 1) pick(std::bool_constant<WHOLE_LINES>{});
+  else pick(std::false_type{});
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (t.splits == 1 && !t.weights_out)) return e;
   const int64_t rows = t.splits > 1 ? (int64_t)t.c.batch * t.heads_q : 0;
