@@ -512,6 +512,17 @@ bool weights_of(const Tensor& w, const fhog_paged_cache& c) {
   return w.dim() == 3 && w.scalar_type() == at::kFloat && w.size(0) == c.batch && w.size(1) == c.heads_k && w.size(2) == c.table_width * c.page;
 }
 
+// Whether two of them lie apart, or are one and the same
+bool apart_or_same(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || (a.data_ptr() == b.data_ptr() && step(a, 0) == step(b, 0) && step(a, 1) == step(b, 1) && step(a, 2) == step(b, 2))) return true;
+  const auto last = [](const Tensor& t) {
+    const char* p = (const char*)t.data_ptr();
+    for (int64_t i = 0; i < t.dim(); i++) p += (t.size(i) - 1) * t.stride(i) * t.element_size();
+    return p;
+  };
+  return last(a) < (const char*)b.data_ptr() || last(b) < (const char*)a.data_ptr();
+}
+
 std::optional<tensor_list> paged_attention(const Tensor& q_, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths,
                                            std::optional<double> scale, int64_t window, int64_t sinks, const std::optional<Tensor>& weights_,
                                            const std::optional<Tensor>& weights_out) {
@@ -522,7 +533,7 @@ std::optional<tensor_list> paged_attention(const Tensor& q_, const Tensor& keys,
   const at::NoGradGuard no_grad;
   const fhog_paged_cache& c = cache.c;
   if (q_.dim() != 4 || q_.scalar_type() != keys.scalar_type() || q_.size(0) != c.batch || q_.size(2) != 1 || q_.size(3) != c.d || q_.size(1) < 1) return std::nullopt;
-  if ((weights_ && !weights_of(*weights_, c)) || (weights_out && (!weights_ || !weights_of(*weights_out, c) || weights_out->stride(2) != 1))) return std::nullopt;
+  if ((weights_ && !weights_of(*weights_, c)) || (weights_out && (!weights_ || !weights_of(*weights_out, c) || weights_out->stride(2) != 1 || !apart_or_same(*weights_, *weights_out)))) return std::nullopt;
   const Tensor q = rows16(q_);
   fhog_paged_attn_args a = {};
   a.cache = c, a.heads_q = q.size(1), a.stride_qb = step(q, 0), a.stride_qh = step(q, 1);
@@ -623,6 +634,8 @@ PYBIND11_MODULE(_fhog_torch, m) {
   m.def("dispatches_to_python", [](const Tensor& t) { return t.unsafeGetTensorImpl()->is_python_dispatch(); }, free_lock);
   m.def("attention", &attention, free_lock);
   m.def("rotary", &rotary, free_lock);
+  m.def("transformed", &transformed, free_lock);
+  m.def("apart_or_same", &apart_or_same, free_lock);
   m.def("paged_append", &paged_append, free_lock);
   m.def("paged_attention", &paged_attention, free_lock);
   m.def("key_weights", &key_weights, free_lock);

@@ -18,7 +18,7 @@ from .bwdbwd import _MAX_WINDOW, mask_code, native_mask, native_sinks, sinks_cod
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class PagedCache:
     """Keys and values of many sequences in pages of one pool.
 
@@ -88,7 +88,9 @@ def _check_cache(cache, written: bool = False) -> Tuple[int, int, int, int, int]
 
 def _refused(what: str):
     """The error for a call that passed the checks above and that the library still does not take; its own message says why."""
-    return ValueError(f"{what}: {_lib.lib().fhog_last_error().decode() or 'not under torch.jit.trace or torch.func transforms'}")
+    if _lib.torch_ext().transformed():
+        return ValueError(f"{what} does not run under torch.jit.trace or torch.func transforms")
+    return ValueError(f"{what}: {_lib.lib().fhog_last_error().decode()}")
 
 
 def paged_append(cache: PagedCache, k, v, *, counts=None) -> None:
@@ -135,7 +137,7 @@ def paged_attention(q, cache: PagedCache, scale: Optional[float] = None, *, wind
         window, sinks: only the last ``window`` entries and the first ``sinks`` are seen.
         weights: (B, H_k, P * page) fp32. What each entry weighed is added up: the result is ``(O, L, W)`` with W = ``weights`` plus, at every entry that is seen, the sum
             over its heads of queries of ``exp(score - L)``.
-        weights_out: where W is written, e.g. ``weights`` itself; None = a new tensor.
+        weights_out: where W is written: ``weights`` itself, or a tensor that lies apart from it; None = a new tensor.
 
     A sequence without entries (or whose table names no page) has O = 0 and L = -inf.
     """
@@ -159,6 +161,8 @@ def paged_attention(q, cache: PagedCache, scale: Optional[float] = None, *, wind
         _check_shape(name, t, (B, H_k, P * page), torch.float32)
     if weights_out is not None and weights_out.stride(-1) != 1:
         raise ValueError(f"weights_out has strides {weights_out.stride()}: the last dimension has to be contiguous")
+    if weights_out is not None and not _lib.torch_ext().apart_or_same(weights, weights_out):
+        raise ValueError("weights_out overlaps with weights: give the same tensor, or one that lies apart from it")
     if scale is not None and not isinstance(scale, (int, float)):
         raise TypeError(f"scale must be a number, got {type(scale).__name__}")
     raise _refused("paged_attention")

@@ -516,3 +516,58 @@ def test_two_streams_and_the_same_bits_again():
         for g, x in zip(got, want):
             for y in g:
                 assert all(torch.equal(a, b) for a, b in zip(y, x))
+
+
+def test_weights_that_overlap_are_refused():
+    import fhog
+    c = Case(torch.bfloat16, 2, 64, 16, [40, 20], seed=18)
+    q, n = c.normal(2, 4, 1, 64), c.table.shape[1] * 16
+    both = torch.rand(2, 2, 2 * n + 3).cuda()
+    w, shifted, behind = both[..., :n], both[..., 1:n + 1], both[..., n:2 * n]
+    with pytest.raises(ValueError, match="overlaps"):
+        fhog.paged_attention(q, c.cache(), weights=w, weights_out=shifted)
+    with pytest.raises(ValueError, match="overlaps"):     # rows of one between the other's
+        fhog.paged_attention(q, c.cache(), weights=w, weights_out=behind)
+    want = fhog.paged_attention(q, c.cache(), weights=w)[2]
+    apart = torch.rand(2, 2, 2, n).cuda()
+    apart[0] = w
+    assert torch.equal(fhog.paged_attention(q, c.cache(), weights=apart[0], weights_out=apart[1])[2], want)
+    assert torch.equal(fhog.paged_attention(q, c.cache(), weights=w, weights_out=w)[2], want) and torch.equal(w, want)
+
+
+def test_no_sequences():
+    import fhog
+    c = Case(torch.float16, 2, 64, 16, [40], seed=19)
+    none = fhog.PagedCache(c.keys, c.values, c.table[:0], c.n[:0])
+    w = torch.zeros(0, 2, c.table.shape[1] * 16).cuda()
+    o, lse, new = fhog.paged_attention(c.normal(0, 4, 1, 64), none, weights=w)
+    assert o.shape == (0, 4, 1, 64) and lse.shape == (0, 4, 1) and new.shape == w.shape
+    left, new, kept = fhog.paged_evict(none, w, 5, c.table[:0])
+    assert left.lengths.shape == (0,) and new.shape == w.shape and kept.shape == (0, 2, 5)
+
+
+def test_under_transforms():
+    """torch.func and torch.jit.trace are refused by name, whatever the error before was."""
+    import fhog
+    c = Case(torch.float32, 2, 64, 16, [40, 20], seed=20)
+    q = c.normal(3, 2, 4, 1, 64)
+    with pytest.raises(ValueError, match="scale"):
+        fhog.paged_attention(q[0], c.cache(), NAN)
+    with pytest.raises(ValueError, match="torch.func"):
+        torch.func.vmap(lambda x: fhog.paged_attention(x, c.cache())[0])(q)
+    with pytest.raises(ValueError, match="torch.jit.trace"):
+        torch.jit.trace(lambda x: fhog.paged_attention(x, c.cache())[0], (q[0],))
+    with torch.inference_mode():
+        assert torch.equal(fhog.paged_attention(q[0], c.cache())[0], fhog.paged_attention(q[0].clone(), c.cache())[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [1, 5, 16, 17, 33])
+def test_groups_in_parts(dtype, group):
+    """Heads of queries in several workgroups, sequences in several parts, parts that a ragged batch leaves empty, and the weights of all of it."""
+    import fhog
+    c = Case(dtype, 2, 128, 32, [2500, 700, 40, 0, 1], seed=21)
+    q = c.normal(5, 2 * group, 1, 128)
+    w = torch.rand(5, 2, c.table.shape[1] * 32).cuda()
+    o, lse, new = fhog.paged_attention(q, c.cache(), weights=w)
+    _check_attention(c, q, o, lse, weights=w, new=new)
