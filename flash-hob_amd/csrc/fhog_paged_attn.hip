@@ -35,16 +35,15 @@ struct Token {
   int64_t wib, wih, wob, woh;
   int32_t heads_q, group, columns; // group: heads of queries of a head of keys; columns: workgroups that they take
   int32_t window, sinks;
-  int32_t splits, least;           // workgroups to a sequence and head of keys, at most; tiles to one of them, at least
+  int32_t units, slots;            // workgroups to a head of keys and 16 of its heads of queries: about, and at most
+  int32_t dealt;                   // the tiles of all sequences are dealt out over them (Deal); else a workgroup has a sequence
   float scale_log2;
-  float* part;                     // [split][batch * heads_q][d]
-  f32x2_t* stats;                  // [split][batch * heads_q]: maximum in log2 units, sum
+  float* part;                     // [slot][16][d]
+  f32x2_t* stats;                  // [slot][16]: maximum in log2 units, sum
+  f32x2_t* whole;                  // [batch * heads_q]: the same of rows that one workgroup had for itself
   float* scores;                   // [batch * heads_q][row]: scores in log2 units of the entries that are seen
   int64_t row;
 };
-
-// Parts into which the tiles of a sequence go: as many as leave each `least`, the same number in every kernel
-__device__ __forceinline__ int parts_of(int tiles, const Token& t) { return min(t.splits, (tiles + t.least - 1) / t.least); }
 
 template <int DT>
 struct Type;   // by FHOG_DTYPE_*
@@ -103,6 +102,69 @@ template <int DT>
 constexpr int kTile = DT == FHOG_DTYPE_FP32 ? 16 : 32;
 int tile_of(int dtype) { return dtype == FHOG_DTYPE_FP32 ? kTile<FHOG_DTYPE_FP32> : kTile<FHOG_DTYPE_BF16>; }
 
+// Sum over the lanes up to this one, in registers
+__device__ __forceinline__ int scan(int x) {
+  const auto add = [&](auto control, auto mask) { x += __builtin_amdgcn_update_dpp(0, x, control.value, mask.value, 0xf, false); };
+  const auto all = std::integral_constant<int, 0xf>{};
+  add(std::integral_constant<int, 0x111>{}, all), add(std::integral_constant<int, 0x112>{}, all);   // the lanes 1, 2, 4 and 8 before it in its row of 16
+  add(std::integral_constant<int, 0x114>{}, all), add(std::integral_constant<int, 0x118>{}, all);
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});                   // the last of the row before, into rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});                   // lane 31, into rows 2 and 3
+  return x;
+}
+
+// How the tiles of all sequences are dealt out over about t.units workgroups (dealt): a sequence goes to as many as its share of all tiles comes to, rounded, and one at least. So a long
+// sequence among short ones has many, whatever the table has room for. By a wave, lane b of each 64 sequences. Else every sequence has one workgroup.
+template <int TILE>
+struct Deal {
+  const Token& t;
+  int lane, share = 1;   // tiles of a workgroup, about
+  int n0;                // tiles of this lane's sequence of the first 64
+  __device__ __forceinline__ int tiles(int b) const { return b < t.c.batch ? Seen<TILE>(t.c.length(b), t.window, t.sinks).tiles : 0; }
+  __device__ __forceinline__ int mine(int b) const { return b == 0 ? n0 : tiles(b + lane); }
+  __device__ __forceinline__ int parts(int n) const { return n == 0 ? 0 : max(1, (n + share / 2) / share); }
+  __device__ __forceinline__ static int last(int x) { return __builtin_amdgcn_readlane(x, 63); }
+  __device__ __forceinline__ Deal(const Token& t_, int lane_) : t(t_), lane(lane_) {
+    n0 = tiles(lane);
+    int total = last(scan(n0));
+    for (int b = 64; b < t.c.batch; b += 64) total += last(scan(tiles(b + lane)));
+    share = max(kWaves, (total + t.units - 1) / t.units);
+  }
+  // The sequence that workgroup `unit` has a part of, -1 if none; the part, and how many there are
+  __device__ __forceinline__ int find(int unit, int& part, int& count) const {
+    for (int b = 0, before = 0; b < t.c.batch; b += 64) {
+      const int n = parts(mine(b)), upto = scan(n);
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(before + upto > unit);
+      if (hit != 0) {
+        const int l = __builtin_ctzll(hit);
+        count = __builtin_amdgcn_readlane(n, l);
+        part = unit - (before + __builtin_amdgcn_readlane(upto, l) - count);
+        return b + l;
+      }
+      before += last(upto);
+    }
+    return -1;
+  }
+  // The first workgroup of sequence b, and how many it has
+  __device__ __forceinline__ int first(int b, int& count) const {
+    int before = 0;
+    for (int i = 0; i + 64 <= b; i += 64) before += last(scan(parts(mine(i))));
+    const int n = parts(mine(b & ~63)), upto = scan(n);
+    count = __builtin_amdgcn_readlane(n, b & 63);
+    return before + __builtin_amdgcn_readlane(upto, b & 63) - count;
+  }
+};
+
+// Where the parts of a sequence lie: in the slots of its workgroups
+template <int TILE>
+struct Shares {
+  int first = 0, parts = 1;
+  __device__ __forceinline__ Shares(const Token& t, int b, int lane) {
+    if (t.dealt) first = Deal<TILE>(t, lane).first(__builtin_amdgcn_readfirstlane(b), parts);
+  }
+  __device__ __forceinline__ int64_t slot(const Token& t, int column, int part) const { return (int64_t)column * t.slots + min(first + part, t.slots - 1); }
+};
+
 // PAGES16: pages of a multiple of 16 entries, so that 16 in a row share one. WEIGHTS: scores are kept. ONCE: as in fetch.
 template <int DT, int D, bool PAGES16, bool WEIGHTS, bool ONCE>
 __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
@@ -120,15 +182,38 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
   const int m = lane & 15, quarter = lane >> 4;
   // Workgroups of the same entries, for other heads of queries, come eight ids apart: on the same XCD, where the second one finds what the first one read
   const uint32_t turn = blockIdx.x / (8 * t.columns), inside = blockIdx.x - turn * (8 * t.columns), unit = 8 * turn + (inside & 7);
-  const uint32_t slice = unit / t.splits;
-  if (slice >= (uint32_t)(t.c.batch * t.c.heads_k)) return;
-  const int split = unit - slice * t.splits, b = slice / t.c.heads_k, g = slice - b * t.c.heads_k, first_head = (inside >> 3) * kColumns;
+  const int own = unit / t.c.heads_k, g = unit - own * t.c.heads_k;   // those that there is nothing for come last
+  if (own >= t.slots) return;
+  const int column = g * t.columns + (inside >> 3), first_head = (inside >> 3) * kColumns;
   const int heads = min(kColumns, t.group - first_head);
-  const int64_t row0 = (int64_t)b * t.heads_q + g * t.group + first_head;   // of (batch * heads_q)
-  const Seen<TILE> seen(t.c.length(b), t.window, t.sinks);
-  const int parts = parts_of(seen.tiles, t);
-  if (split >= max(parts, 1)) return;
+  const char* const keys = t.c.keys + (int64_t)g * t.c.stride_h;
+  const char* const values = t.c.values + (int64_t)g * t.c.stride_h;
+  // a lane's bytes from the first of 16 entries that lie in a row
+  const uint32_t stride = (uint32_t)t.c.stride_n, key_off = m * stride + quarter * 16;
+  uint32_t value_off[4];
+#pragma unroll
+  for (int x = 0; x < 4; x++) value_off[x] = (4 * quarter + x) * stride + m * VB;
 
+  // The first wave finds out what there is to do and says so: lengths that someone changes meanwhile make wrong results, but no waves that disagree on them at a barrier
+  __shared__ int task[4];   // sequence, its entries, the tiles of this workgroup: the first one, and the one behind the last
+  __shared__ bool task_shared;
+  if (wave == 0) {
+    int b = own, part = 0, parts = 1;
+    if (t.dealt) b = Deal<TILE>(t, lane).find(own, part, parts);
+    if (lane == 0) {
+      const int n = b < 0 ? 0 : t.c.length(b);
+      const int64_t tiles = Seen<TILE>(n, t.window, t.sinks).tiles;
+      task[0] = b, task[1] = n, task[2] = (int)(tiles * part / parts), task[3] = (int)(tiles * (part + 1) / parts), task_shared = parts > 1;
+    }
+  }
+  __syncthreads();
+  const auto told = [&](int i) { return __builtin_amdgcn_readfirstlane(task[i]); };
+  const int b = told(0), begin = told(2), end = told(3);
+  if (b < 0) return;
+  const bool shared = task_shared;
+  const int64_t slot = (int64_t)column * t.slots + own;
+  const int64_t row0 = (int64_t)b * t.heads_q + g * t.group + first_head;   // of (batch * heads_q)
+  const Seen<TILE> seen(told(1), t.window, t.sinks);
   u32x4_t q[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; s++) {
@@ -140,15 +225,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
 #pragma unroll
   for (int i = 0; i < C; i++) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  const int begin = parts ? (int)((int64_t)seen.tiles * split / parts) : 0, end = parts ? (int)((int64_t)seen.tiles * (split + 1) / parts) : 0;
   const int32_t* const table = t.c.table + b * t.c.stride_tb;
-  const char* const keys = t.c.keys + (int64_t)g * t.c.stride_h;
-  const char* const values = t.c.values + (int64_t)g * t.c.stride_h;
-  // a lane's bytes from the first of 16 entries that lie in a row
-  const uint32_t stride = (uint32_t)t.c.stride_n, key_off = m * stride + quarter * 16;
-  uint32_t value_off[4];
-#pragma unroll
-  for (int x = 0; x < 4; x++) value_off[x] = (4 * quarter + x) * stride + m * VB;
   // Where the entries of a tile lie. `hidden`: some of them are not there or not seen, the same for the wave
   struct Place {
     int j0;
@@ -323,8 +400,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; w++) o += *reinterpret_cast<const f32x4_t*>(&rows[w][h][c]);
-    if (t.splits > 1) {
-      *reinterpret_cast<f32x4_t*>(t.part + ((int64_t)split * t.c.batch * t.heads_q + row0 + h) * D + c) = o;
+    if (shared) {
+      *reinterpret_cast<f32x4_t*>(t.part + (slot * kColumns + h) * D + c) = o;
     } else {
       float total = sums[0][h];
 #pragma unroll
@@ -339,21 +416,25 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
     float total = sums[0][tid], high = tops[0][tid];
 #pragma unroll
     for (int w = 1; w < kWaves; w++) total += sums[w][tid], high = fmaxf(high, tops[w][tid]);
-    if (t.splits > 1 || WEIGHTS) t.stats[(int64_t)split * t.c.batch * t.heads_q + row0 + tid] = f32x2_t{high, total};
-    if (t.splits == 1) t.lse[row0 + tid] = total == 0.f ? -INFINITY : (high + __builtin_amdgcn_logf(total)) * kLn2;
+    if (shared) {
+      t.stats[slot * kColumns + tid] = f32x2_t{high, total};
+    } else {
+      if (WEIGHTS) t.whole[row0 + tid] = f32x2_t{high, total};
+      t.lse[row0 + tid] = total == 0.f ? -INFINITY : (high + __builtin_amdgcn_logf(total)) * kLn2;
+    }
   }
 }
 
-// Maximum, in log2 units, and sum over the parts of a row, by the lanes of a wave
-__device__ __forceinline__ f32x2_t joined(const Token& t, int64_t row, int parts, int lane) {
-  const int64_t rows = (int64_t)t.c.batch * t.heads_q;
+// Maximum, in log2 units, and sum over the parts of head `head` of a column, by the lanes of a wave
+template <int TILE>
+__device__ __forceinline__ f32x2_t joined(const Token& t, const Shares<TILE>& of, int column, int head, int lane) {
   float high = -INFINITY, total = 0.f;
-  for (int i = lane; i < parts; i += 64) high = fmaxf(high, t.stats[i * rows + row][0]);
+  for (int i = lane; i < of.parts; i += 64) high = fmaxf(high, t.stats[of.slot(t, column, i) * kColumns + head][0]);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) high = fmaxf(high, __shfl_xor(high, d));
   const float ref = high == -INFINITY ? 0.f : high;
-  for (int i = lane; i < parts; i += 64) {
-    const f32x2_t s = t.stats[i * rows + row];
+  for (int i = lane; i < of.parts; i += 64) {
+    const f32x2_t s = t.stats[of.slot(t, column, i) * kColumns + head];
     total += s[1] * __builtin_amdgcn_exp2f(s[0] - ref);
   }
 #pragma unroll
@@ -361,22 +442,28 @@ __device__ __forceinline__ f32x2_t joined(const Token& t, int64_t row, int parts
   return f32x2_t{high, total};
 }
 
-// O and L of a row from its parts: a lane has four channels, groups of D / 4 lanes take the parts in turn. With one group and part after part 32 parts of 16 rows took
-// 21 us, each load waiting for the one before; so 5.
+// O and L of a row that several workgroups have shared: a lane has four channels, groups of D / 4 lanes take the parts in turn. (With one group and part after part 32 parts of 16
+// rows took 21 us, each load waiting for the one before; so 4.) Rows of sequences without entries, which no workgroup had.
 template <int DT, int D>
 __device__ __forceinline__ void join_row(const Token& t, int64_t row, int tid) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32;
   constexpr int LANES = D / 4, GROUPS = kThreads / LANES;
   __shared__ f32x4_t sums[GROUPS][LANES];
-  const int64_t rows = (int64_t)t.c.batch * t.heads_q;
   const int group = tid / LANES, c = tid % LANES * 4, b = (int)(row / t.heads_q), h = (int)(row - (int64_t)b * t.heads_q);
-  const Seen<kTile<DT>> seen(t.c.length(b), t.window, t.sinks);
-  const int parts = parts_of(seen.tiles, t);
-  const f32x2_t all = joined(t, row, parts, tid & 63);   // every wave for itself
+  __shared__ int parts;   // as the first wave has them: all waves are to agree on whether there is something to do
+  const Shares<kTile<DT>> of(t, b, tid & 63);
+  if (tid == 0) parts = of.parts;
+  __syncthreads();
+  if (parts == 1) return;
+  const int g = h / t.group, inside = h - g * t.group, column = g * t.columns + inside / kColumns, head = inside % kColumns;
+  const f32x2_t all = joined(t, of, column, head, tid & 63);   // every wave for itself
   const float ref = all[0] == -INFINITY ? 0.f : all[0];
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = group; i < parts; i += GROUPS) o += *reinterpret_cast<const f32x4_t*>(t.part + (i * rows + row) * D + c) * __builtin_amdgcn_exp2f(t.stats[i * rows + row][0] - ref);
+  for (int i = group; i < of.parts; i += GROUPS) {
+    const int64_t at = of.slot(t, column, i) * kColumns + head;
+    o += *reinterpret_cast<const f32x4_t*>(t.part + at * D + c) * __builtin_amdgcn_exp2f(t.stats[at][0] - ref);
+  }
   sums[group][tid % LANES] = o;
   __syncthreads();
   if (group != 0) return;
@@ -399,7 +486,6 @@ __device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid)
   const int64_t slice = id / blocks;
   const int b = (int)(slice / t.c.heads_k), g = (int)(slice - (int64_t)b * t.c.heads_k), j0 = (int)(id - slice * blocks) * kEntries + tid;
   const Seen<kTile<DT>> seen(t.c.length(b), t.window, t.sinks);
-  const int parts = parts_of(seen.tiles, t);
   const int64_t row0 = (int64_t)b * t.heads_q + g * t.group;
   const float* const in = t.weights_in + b * t.wib + g * t.wih;
   float* const out = t.weights_out + b * t.wob + g * t.woh;
@@ -415,11 +501,12 @@ __device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid)
       for (int i = 0; i < 4; i++) s[h][i] = h0 + h < t.group && seen.sees(j0 + i * kThreads) ? scores[(h0 + h) * t.row + i * kThreads] : -INFINITY;
   };
   load(0);   // before the statistics, for which it does not have to wait
+  const Shares<kTile<DT>> of(t, b, tid & 63);
   for (int h0 = 0; h0 < t.group; h0 += kHeads) {
     const int heads = min(kHeads, t.group - h0);
     __syncthreads();
     for (int h = tid >> 6; h < heads; h += kWaves) {
-      const f32x2_t all = joined(t, row0 + h0 + h, parts, tid & 63);
+      const f32x2_t all = of.parts > 1 ? joined(t, of, g * t.columns + (h0 + h) / kColumns, (h0 + h) % kColumns, tid & 63) : seen.tiles ? t.whole[row0 + h0 + h] : f32x2_t{0.f, 0.f};
       if ((tid & 63) == 0) lse[h] = all[1] == 0.f ? INFINITY : all[0] + __builtin_amdgcn_logf(all[1]);
     }
     __syncthreads();
@@ -444,12 +531,13 @@ __global__ void __launch_bounds__(kThreads) join_parts(Token t, int rows) {
   else add_weights<DT>(t, (int64_t)blockIdx.x - rows, threadIdx.x);
 }
 
-// How the tiles of a call are dealt out
+// How the tiles of a call are dealt out, and what that leaves in the workspace
 struct Plan {
-  int splits, least;
-  int64_t rows, row;   // batch * heads_q; scores of a row
-  size_t part_bytes, stats_bytes, score_bytes;
-  size_t bytes() const { return part_bytes + stats_bytes + score_bytes; }
+  int units, slots;
+  bool dealt;
+  int64_t row;   // scores of a row
+  size_t part_bytes, stats_bytes, whole_bytes, score_bytes;
+  size_t bytes() const { return part_bytes + stats_bytes + whole_bytes + score_bytes; }
 };
 
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
@@ -460,24 +548,26 @@ Plan plan_of(const fhog_paged_attn_args* a) {
   const int64_t tile = tile_of(c.dtype), capacity = c.table_width * c.page;
   int64_t most = capacity;   // entries that a token may see
   if (a->window > 0 && a->window < capacity) most = std::min(capacity, a->window + std::min(a->sinks, capacity) + 2 * tile);
-  const int64_t tiles = (most + tile - 1) / tile, group = a->heads_q / c.heads_k, slices = c.batch * c.heads_k * ((group + kColumns - 1) / kColumns);
-  // Two workgroups to a CU, as few as keep memory busy: what is split has to be joined. us at 512 | 768 | 1024 workgroups, bf16, d = 128, 8 heads of keys: 1 x 32768 28.5 | 31.0 | 30.5,
-  // 8 x 4096 28.2 | 29.4 | 29.0, 64 x 2048 84.5 | 90.5 | 90.6, 32 x 16384 of ragged lengths 302 | 300 | 303. Up to 512 entries stay in one workgroup (1 x 300: 11.6 -> 9.0).
-  int64_t least = (tiles * slices + 511) / 512;
-  least = std::max<int64_t>(kWaves, (least + kWaves - 1) / kWaves * kWaves);
-  if (tiles * tile <= 512) least = tiles;
-  p.least = (int)least;
-  p.splits = (int)((tiles + least - 1) / least);
-  p.rows = c.batch * a->heads_q, p.row = (capacity + tile - 1) / tile * tile;
-  p.part_bytes = p.splits > 1 ? up16(sizeof(float) * p.splits * p.rows * c.d) : 0;
-  p.stats_bytes = p.splits > 1 || a->weights_out ? up16(sizeof(f32x2_t) * p.splits * p.rows) : 0;
-  p.score_bytes = a->weights_out ? sizeof(float) * p.rows * p.row : 0;
+  const int64_t tiles = (most + tile - 1) / tile, group = a->heads_q / c.heads_k, columns = c.heads_k * ((group + kColumns - 1) / kColumns), slices = c.batch * columns;
+  // Two workgroups to a CU, as few as keep memory busy: what is split has to be joined. us at 512 | 768 | 1024 workgroups, bf16, d = 128, 8 heads of keys, when each sequence had
+  // as many parts as the longest would need: 1 x 32768 28.5 | 31.0 | 30.5, 8 x 4096 28.2 | 29.4 | 29.0, 64 x 2048 84.5 | 90.5 | 90.6. Dealt out by their lengths: 16384 beside 31 of 500
+  // 138 -> 30, beside 63 of 100 240 -> 30, 8192 and 300 in turn 136 -> 99; 8 x 4096 28.5 -> 29.2, 1 x 4096 12.1 -> 13.0, which is what finding out costs. So not where
+  // up to 512 entries are seen (1 x 300 11.6 -> 9.4), or where there are workgroups enough without, of sequences too short to leave much of the GPU idle at the end.
+  p.dealt = most > 512 && c.batch <= 512 && (slices < 512 || most >= 4096) && tiles * c.batch < ((int64_t)1 << 30);
+  p.units = (int)(p.dealt ? std::max<int64_t>(1, std::min(512 / columns, (tiles * c.batch + kWaves - 1) / kWaves)) : c.batch);
+  p.slots = (int)(p.dealt ? p.units + c.batch : c.batch);   // a part is rounded up by less than one for each sequence
+  p.row = (capacity + tile - 1) / tile * tile;
+  const int64_t slots = p.slots * columns, rows = c.batch * a->heads_q;
+  p.part_bytes = p.dealt ? sizeof(float) * slots * kColumns * c.d : 0;
+  p.stats_bytes = p.dealt ? sizeof(f32x2_t) * slots * kColumns : 0;
+  p.whole_bytes = a->weights_out ? up16(sizeof(f32x2_t) * rows) : 0;
+  p.score_bytes = a->weights_out ? sizeof(float) * rows * p.row : 0;
   return p;
 }
 
 template <int DT, int D>
 hipError_t launch_d(const Token& t, const fhog_paged_attn_args* a, hipStream_t s) {
-  const int64_t units = (int64_t)t.splits * t.c.heads_k * t.c.batch;
+  const int64_t units = (int64_t)t.slots * t.c.heads_k;
   const dim3 grid((unsigned)((units + 7) / 8 * 8 * t.columns));
   const bool pages16 = t.c.page.by % 16 == 0;
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, t); };
@@ -490,8 +580,8 @@ hipError_t launch_d(const Token& t, const fhog_paged_attn_args* a, hipStream_t s
   if (WHOLE_LINES && t.columns == 1) pick(std::bool_constant<WHOLE_LINES>{});
   else pick(std::false_type{});
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || (t.splits == 1 && !t.weights_out)) return e;
-  const int64_t rows = t.splits > 1 ? (int64_t)t.c.batch * t.heads_q : 0;
+  if (e != hipSuccess || (!t.dealt && !t.weights_out)) return e;
+  const int64_t rows = t.dealt ? (int64_t)t.c.batch * t.heads_q : 0;
   const int64_t weights = t.weights_out ? (int64_t)t.c.batch * t.c.heads_k * ((t.c.capacity + kEntries - 1) / kEntries) : 0;
   hipLaunchKernelGGL((join_parts<DT, D>), dim3((unsigned)(rows + weights)), dim3(kThreads), 0, s, t, (int)rows);
   return hipGetLastError();
@@ -519,9 +609,10 @@ hipError_t launch_paged_attn(const fhog_paged_attn_args* a, hipStream_t s) {
   t.wib = a->stride_wib, t.wih = a->stride_wih, t.wob = a->stride_wob, t.woh = a->stride_woh;
   t.heads_q = (int32_t)a->heads_q, t.group = (int32_t)(a->heads_q / a->cache.heads_k), t.columns = (t.group + kColumns - 1) / kColumns;
   t.window = (int32_t)std::min<int64_t>(a->window, INT32_MAX), t.sinks = (int32_t)std::min<int64_t>(a->sinks, t.c.capacity);
-  t.splits = p.splits, t.least = p.least, t.scale_log2 = a->scale * kLog2e, t.row = p.row;
+  t.units = p.units, t.slots = p.slots, t.dealt = p.dealt, t.scale_log2 = a->scale * kLog2e, t.row = p.row;
   char* const ws = (char*)a->ws;
-  t.part = (float*)ws, t.stats = (f32x2_t*)(ws + p.part_bytes), t.scores = (float*)(ws + p.part_bytes + p.stats_bytes);
+  t.part = (float*)ws, t.stats = (f32x2_t*)(ws + p.part_bytes);
+  t.whole = (f32x2_t*)(ws + p.part_bytes + p.stats_bytes), t.scores = (float*)(ws + p.part_bytes + p.stats_bytes + p.whole_bytes);
   switch (a->cache.dtype) {
     case FHOG_DTYPE_FP32: return launch_t<FHOG_DTYPE_FP32>(t, a, s);
     case FHOG_DTYPE_FP16: return launch_t<FHOG_DTYPE_FP16>(t, a, s);
