@@ -73,11 +73,37 @@ __device__ __forceinline__ uint32_t rank_of(float w, int j, int n, const Evict& 
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Rows that stay, to their new places: the chunks of 16 bytes `id` and, kRowsEach - 1 times more, `step` further on, of the keys and values of m rows
+__device__ __forceinline__ void move_chunks(const Evict& e, int b, int h, const int32_t* kept, int m, uint32_t id, uint32_t step) {
+  u32x4_t k[kRowsEach], v[kRowsEach];
+  int64_t dst[kRowsEach];
+#pragma unroll
+  for (int u = 0; u < kRowsEach; u++, id += step) {
+    dst[u] = -1;
+    const uint32_t i = e.chunks(id), chunk = id - i * e.chunks.by;
+    if (i >= (uint32_t)m) continue;
+    const uint32_t j = kept[i];
+    if (j >= (uint32_t)e.c.capacity) continue;   // lengths that someone has changed meanwhile
+    const uint32_t at = e.c.page(j), to = e.c.page(i);
+    const int32_t from_page = e.c.table[b * e.c.stride_tb + at], to_page = e.into[b * e.ib + to];
+    if ((uint32_t)from_page >= (uint32_t)e.c.pages || (uint32_t)to_page >= (uint32_t)e.c.pages) continue;
+    const int64_t inside = h * e.c.stride_h + chunk * 16;
+    const int64_t src = from_page * e.c.stride_p + (j - at * e.c.page.by) * e.c.stride_n + inside;
+    dst[u] = to_page * e.c.stride_p + (i - to * e.c.page.by) * e.c.stride_n + inside;
+    k[u] = fetch_once(e.c.keys + src), v[u] = fetch_once(e.c.values + src);
+  }
+#pragma unroll
+  for (int u = 0; u < kRowsEach; u++)
+    if (dst[u] >= 0) put(e.c.keys + dst[u], k[u]), put(e.c.values + dst[u], v[u]);
+}
+
 // Which entries of one sequence and head of keys stay. Each wave has a stretch of the entries. The rank of the last one that stays is found digit by digit, eight bits at a
 // time from the top: a histogram of the digit over the entries whose higher digits are those found so far, and the digit at which the sum from above reaches
 // what is still to be found. Then the entries that stay are counted, wave by wave, and written to the places that the counts give.
 // What bounds it: the waits between its passes. us, 32 x 8 slices of 8192 | 4 x 4 of 1000: weights read anew in every pass 26.6 | 7.4, ranks formed once and kept in registers
 // 20.2 | 10.8, in LDS 22.7 | 7.6, and there with a histogram of eight copies 19.8 | 7.7.
+// MOVE: and are moved by the same workgroup.
+template <bool MOVE>
 __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   extern __shared__ uint32_t held[];
   __shared__ uint32_t histogram[kCopies][kDigits];   // a lane counts in copy lane % kCopies: the same digit of many lanes is not one address
@@ -157,30 +183,15 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
     if (j < end && (r > rank || (r == rank && same_before < ties))) kept[at] = j, out[at] = w[j];
     over += __builtin_popcountll(o), same += __builtin_popcountll(s);
   });
+  if constexpr (MOVE) {
+    __syncthreads();   // all of `kept` is there
+    for (uint32_t id = tid; id < (uint32_t)m * e.chunks.by; id += kRowsEach * kSelect) move_chunks(e, b, h, kept, m, id, kSelect);
+  }
 }
 
-// The rows that stay, to their new places
 __global__ void __launch_bounds__(kThreads) move_entries(Evict e) {
   const int b = blockIdx.y / e.c.heads_k, h = blockIdx.y - b * e.c.heads_k;
-  const int rows = min(e.c.length(b), e.rows);
-  u32x4_t k[kRowsEach], v[kRowsEach];
-  int64_t dst[kRowsEach];
-#pragma unroll
-  for (int u = 0; u < kRowsEach; u++) {
-    dst[u] = -1;
-    const uint32_t id = (blockIdx.x * kRowsEach + u) * kThreads + threadIdx.x, i = e.chunks(id), chunk = id - i * e.chunks.by;
-    if (i >= (uint32_t)rows) continue;
-    const uint32_t j = e.kept[(int64_t)blockIdx.y * e.budget + i], at = e.c.page(j), to = e.c.page(i);
-    const int32_t from_page = e.c.table[b * e.c.stride_tb + at], to_page = e.into[b * e.ib + to];
-    if ((uint32_t)from_page >= (uint32_t)e.c.pages || (uint32_t)to_page >= (uint32_t)e.c.pages) continue;
-    const int64_t inside = h * e.c.stride_h + chunk * 16;
-    const int64_t src = from_page * e.c.stride_p + (j - at * e.c.page.by) * e.c.stride_n + inside;
-    dst[u] = to_page * e.c.stride_p + (i - to * e.c.page.by) * e.c.stride_n + inside;
-    k[u] = fetch_once(e.c.keys + src), v[u] = fetch_once(e.c.values + src);
-  }
-#pragma unroll
-  for (int u = 0; u < kRowsEach; u++)
-    if (dst[u] >= 0) put(e.c.keys + dst[u], k[u]), put(e.c.values + dst[u], v[u]);
+  move_chunks(e, b, h, e.kept + (int64_t)blockIdx.y * e.budget, min(e.c.length(b), e.rows), blockIdx.x * kRowsEach * kThreads + threadIdx.x, kThreads);
 }
 
 uint32_t row_chunks(const fhog_paged_cache& c) { return (uint32_t)(c.d * (c.dtype == FHOG_DTYPE_FP32 ? 4 : 2) / 16); }
@@ -207,9 +218,16 @@ hipError_t launch_paged_evict(const fhog_paged_evict_args* a, hipStream_t s) {
   e.sinks = (int32_t)(a->sinks < e.c.capacity ? a->sinks : e.c.capacity), e.recent = (int32_t)(a->recent < e.c.capacity ? a->recent : e.c.capacity);
   e.into_width = (int32_t)a->into_width, e.chunks = Divisor(row_chunks(a->cache));
   const unsigned slices = (unsigned)(a->cache.batch * a->cache.heads_k);
-  hipLaunchKernelGGL(select_entries, dim3(slices), dim3(kSelect), std::min(e.c.capacity, kHeld) * sizeof(uint32_t), s, e);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess || e.rows == 0) return err;
+  const size_t lds = std::min(e.c.capacity, kHeld) * sizeof(uint32_t);
+  // In one launch up to 96 KiB of rows to a slice. us, one launch | two: 4 x 4 slices of 301 rows, d = 64 (77 KB) 11.3 | 12.9, 32 x 8 of 500, d = 64 (128 KB) 22.2 | 23.2,
+  // 8 of 500, d = 128 (256 KB) 19.0 | 12.8
+  if ((int64_t)e.rows * e.chunks.by * 32 <= 96 << 10) {
+    hipLaunchKernelGGL(select_entries<true>, dim3(slices), dim3(kSelect), lds, s, e);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(select_entries<false>, dim3(slices), dim3(kSelect), lds, s, e);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
   hipLaunchKernelGGL(move_entries, dim3((unsigned)(((int64_t)e.rows * e.chunks.by + kThreads * kRowsEach - 1) / (kThreads * kRowsEach)), slices), dim3(kThreads), 0, s, e);
   return hipGetLastError();
 }

@@ -551,9 +551,11 @@ Plan plan_of(const fhog_paged_attn_args* a) {
   const int64_t tiles = (most + tile - 1) / tile, group = a->heads_q / c.heads_k, columns = c.heads_k * ((group + kColumns - 1) / kColumns), slices = c.batch * columns;
   // Two workgroups to a CU, as few as keep memory busy: what is split has to be joined. us at 512 | 768 | 1024 workgroups, bf16, d = 128, 8 heads of keys, when each sequence had
   // as many parts as the longest would need: 1 x 32768 28.5 | 31.0 | 30.5, 8 x 4096 28.2 | 29.4 | 29.0, 64 x 2048 84.5 | 90.5 | 90.6. Dealt out by their lengths: 16384 beside 31 of 500
-  // 138 -> 30, beside 63 of 100 240 -> 30, 8192 and 300 in turn 136 -> 99; 8 x 4096 28.5 -> 29.2, 1 x 4096 12.1 -> 13.0, which is what finding out costs. So not where
-  // up to 512 entries are seen (1 x 300 11.6 -> 9.4), or where there are workgroups enough without, of sequences too short to leave much of the GPU idle at the end.
-  p.dealt = most > 512 && c.batch <= 512 && (slices < 512 || most >= 4096) && tiles * c.batch < ((int64_t)1 << 30);
+  // 138 -> 30, beside 63 of 100 240 -> 30, 8192 and 300 in turn 136 -> 99; 8 x 4096 28.5 -> 29.2, 1 x 4096 12.1 -> 13.0, which is what finding out costs. So not where one workgroup
+  // reads up to 256 KiB, 512 where every CU has one (dealt out | not, 8 sequences of 600 d = 128 14.6 | 16.4, d = 64 11.9 | 9.7, 1 x 300 11.6 | 9.4; 32 of 1000 d = 128 29.9 | 25.8,
+  // d = 64 19.1 | 13.8), or where there are two to a CU, of sequences too short to leave much of the GPU idle at the end.
+  const int64_t bytes = most * 2 * c.d * (c.dtype == FHOG_DTYPE_FP32 ? 4 : 2);
+  p.dealt = bytes > (slices < 256 ? 256 << 10 : 512 << 10) && c.batch <= 512 && (slices < 512 || bytes >= 2 << 20) && tiles * c.batch < ((int64_t)1 << 30);
   p.units = (int)(p.dealt ? std::max<int64_t>(1, std::min(512 / columns, (tiles * c.batch + kWaves - 1) / kWaves)) : c.batch);
   p.slots = (int)(p.dealt ? p.units + c.batch : c.batch);   // a part is rounded up by less than one for each sequence
   p.row = (capacity + tile - 1) / tile * tile;

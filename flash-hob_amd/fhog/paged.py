@@ -86,10 +86,13 @@ def _check_cache(cache, written: bool = False) -> Tuple[int, int, int, int, int]
     return table.shape[0], H_k, d, table.shape[1], page
 
 
+def _not_transformed(what: str) -> None:
+    if _lib.torch_ext().transformed():
+        raise ValueError(f"{what} does not run under torch.jit.trace or torch.func transforms")
+
+
 def _refused(what: str):
     """The error for a call that passed the checks above and that the library still does not take; its own message says why."""
-    if _lib.torch_ext().transformed():
-        return ValueError(f"{what} does not run under torch.jit.trace or torch.func transforms")
     return ValueError(f"{what}: {_lib.lib().fhog_last_error().decode()}")
 
 
@@ -110,6 +113,7 @@ def paged_append(cache: PagedCache, k, v, *, counts=None) -> None:
         done = False
     if done:
         return
+    _not_transformed("paged_append")
     B, H_k, d, _, _ = _check_cache(cache, written=True)
     _check_tensors(cache.keys, ("counts",), k=k, v=v, counts=counts)
     if k.dim() != 4:
@@ -150,6 +154,7 @@ def paged_attention(q, cache: PagedCache, scale: Optional[float] = None, *, wind
         res = None
     if res is not None:
         return res
+    _not_transformed("paged_attention")
     B, H_k, d, P, page = _check_cache(cache)
     _check_tensors(cache.keys, ("weights", "weights_out"), q=q, weights=weights, weights_out=weights_out)
     if q.dim() != 4 or q.shape[1] < 1 or q.shape[1] % H_k:
@@ -184,6 +189,7 @@ def key_weights(q, k, L, scale: Optional[float] = None, causal=False, *, window:
         res = None
     if res is not None:
         return res
+    _not_transformed("key_weights")
     if not isinstance(q, torch.Tensor):
         raise TypeError(f"q must be a torch.Tensor, got {type(q).__name__}")
     _check_tensors(q, ("lengths",), q=q, k=k, L=L, lengths=lengths)
@@ -232,6 +238,7 @@ def paged_evict(cache: PagedCache, weights, budget: int, into, *, sinks: int = 0
     if res is not None:
         lengths, new, kept = res
         return PagedCache(cache.keys, cache.values, into, lengths), new, kept
+    _not_transformed("paged_evict")
     B, H_k, _, P, page = _check_cache(cache, written=True)
     _check_tensors(cache.keys, weights=weights, into=into)
     _check_shape("weights", weights, (B, H_k, P * page), torch.float32)
