@@ -11,7 +11,7 @@
 // adds in their order: a causal mask leaves the first keys many times the work of the last, and a sink all of it.
 //
 // What bounds it: the instructions of a SIMD. A block of 32 x 32 pairs takes d / 16 matrix instructions of 32 cycles and 48 vector instructions, 16 of them exponentials at half
-// rate: 256 cycles each at d = 128, which run side by side two thirds of the time. bf16, 16 heads x 16384 causal, four to one of keys, d = 128: 637 us, 864 TFLOP/s, 73 % of
+// rate: 256 cycles each at d = 128, which run side by side two thirds of the time. bf16, 16 heads x 16384 causal, four to one of keys, d = 128: 619 us, 888 TFLOP/s, 75 % of
 // what a large library product of bf16 matrices reaches here, which takes no exponentials.
 #include <algorithm>
 #include <type_traits>
@@ -23,9 +23,10 @@ using namespace bf16k;
 namespace {
 
 constexpr int kThreads = 256, kRows = 64;   // queries of a stage
-// Stages in LDS: the one that is read, the one after it, which has landed so that its statistics can be made ready, and those that are on their way
-template <int BYTES>
-constexpr int kRing = BYTES > 256 ? 3 : 4;
+// Stages in LDS: the one that is read, the one after it, which has landed so that its statistics can be made ready, and those that are on their way: two with 64 keys to a wave, one
+// with 32, which leaves room for three workgroups (us, 16 x 16384, window 1024, d = 128 168 -> 146; 16 x 2048 31 -> 28)
+template <int BYTES, int NK>
+constexpr int kRing = BYTES > 256 || NK == 1 ? 3 : 4;
 
 struct Weigh {
   const char* q;
@@ -100,7 +101,7 @@ template <int DT, int D, int NK>
 __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32, F16 = DT == FHOG_DTYPE_FP16;
   constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), CHUNKS = BYTES / 16, PER_LOAD = 64 / CHUNKS, LOADS = kRows / PER_LOAD / 4;
-  constexpr int TILE = kRows * BYTES, STAGE = TILE + kRows * 4, RING = kRing<BYTES>, KEYS = 128 * NK, STEPS = CHUNKS / 2;
+  constexpr int TILE = kRows * BYTES, STAGE = TILE + kRows * 4, RING = kRing<BYTES, NK>, KEYS = 128 * NK, STEPS = CHUNKS / 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
@@ -131,8 +132,6 @@ __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
     whole_lo = max(whole_lo, geo.first(j0 + 31)), whole_hi = min(whole_hi, j0 + 31 >= geo.n_k ? -1 : geo.last(max(j0, min(geo.sinks, j0 + 31))));
   }
   float sum[NK] = {};
-  wait_vm0();   // the keys are there: said once here, or the compiler waits for them, and for the staging loads under way, in every tile
-
   // staging: straight into LDS, 1 KiB to an instruction; rows past the end are copies of the last
   uint32_t off[LOADS];
   const auto offset = [&](int u, int valid) {
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
     *at = l == -INFINITY ? INFINITY : l * kLog2e;
   };
   for (int i = 0; i < RING - 1 && from + i < to; i++) issue();
-  dma_wait();
+  wait_vm0();   // the keys and the first stages; with the builtin, or the compiler waits for the keys, and for the stages under way, in every tile
   __syncthreads();
   if (from < to && wave == 0) make_ready(smem);
   char* stage = smem;
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
   int now = each > 0 ? begin + from % each : 0;
   // Two tiles of 32 queries are on the way at a time, each in registers of its own: while one is multiplied, the exponentials of the one before are taken behind its
   // matrix instructions, a few behind each, so that neither kind waits for the other. us, 16 x 16384 causal, d = 128: one tile at a time 760, so 690; the scalars of a stage carried along instead of
-  // formed anew 660 -> 637.
+  // formed anew 660 -> 637, the keys asked for together with the first stages 637 -> 619.
   f32x16_t scores[2][NK];
   f32x4_t stats[2][4];      // L of the lane's 16 queries: 8 g + 4 h + e
   int waiting = -1;         // the tile whose exponentials are still to be taken; the same for the wave
@@ -321,11 +320,11 @@ Plan plan_of(const fhog_key_weights_args* a) {
     total = std::max(p.tiles, banded ? std::min(p.tiles, (a->n_q + a->window + keys - 1) / keys) * band : all * ((seen + keys - 1) / keys));
   };
   // 64 keys to a wave where there is work for it: half the reads of LDS, but fewer waves and coarser masks. us, 32 | 64 keys, bf16: d = 128 causal 16 heads x 16384
-  // 728 | 638, 32 x 4096 127 | 110, window 4096 of 16 x 16384 340 | 303, window 1024 167 | 180, 8 x 512 11 | 15; d = 64, whose waves have fewer matrix instructions to hide
-  // behind, 16 x 16384 422 | 491, 32 x 2048 32 | 42
+  // 639 | 618, 32 x 4096 120 | 110, 16 x 3000 39 | 47, 128 x 64 queries of 8192 keys 29 | 36, window 4096 of 16 x 16384 297 | 295, window 1024 146 | 180, 8 x 512 11 | 15; d = 64, whose
+  // waves have fewer matrix instructions to hide behind, 16 x 16384 422 | 491, 32 x 2048 31 | 42
   int64_t most, total;
   p.nk = 2, stages(256, most, total);
-  if (a->dtype == FHOG_DTYPE_FP32 || a->d != 128 || (banded && a->window < 2048) || total * group * slices < 4096) p.nk = 1, stages(128, most, total);
+  if (a->dtype == FHOG_DTYPE_FP32 || a->d != 128 || (banded && a->window < 2048) || total * group * slices < 8192) p.nk = 1, stages(128, most, total);
   // Two workgroups to a CU as long as that leaves pieces worth their beginning, and short enough to even out the end of the launch. us, at most 16 | 24 | 32 | 40 stages:
   // 16 x 16384 d = 128 650 | 640 | 638 | 634, d = 64 444 | 427 | 422 | 428; at least 6 | 8: 16 x 3000 60 | 47, 8 x 512 12.6 | 11.3
   int64_t chunk = std::min<int64_t>(32, std::max<int64_t>(a->dtype == FHOG_DTYPE_FP32 ? 3 : 8, (total * group * slices + 1023) / 1024));
@@ -341,7 +340,7 @@ Plan plan_of(const fhog_key_weights_args* a) {
 
 template <int DT, int D, int NK>
 hipError_t launch_d(const Weigh& w, hipStream_t s) {
-  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), STAGE = kRows * BYTES + kRows * 4, LDS = kRing<BYTES> * STAGE;
+  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), STAGE = kRows * BYTES + kRows * 4, LDS = kRing<BYTES, NK> * STAGE;
   const hipError_t e = allow_dynamic_lds<weigh<DT, D, NK>>(LDS);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((weigh<DT, D, NK>), dim3((unsigned)(w.tiles * w.pieces), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), LDS, s, w);
