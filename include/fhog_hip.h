@@ -351,7 +351,7 @@ typedef struct fhog_paged_cache {
 } fhog_paged_cache;
 
 /* New entries: the last counts[b] of each sequence (cut to 0 .. n and to the sequence's length) are written from the first rows of k and v. Two sequences that
-   share a page must not both have new entries in the same slot. */
+   share a page must not both have new entries in the same slot, and k and v must not lie in the pages that are written. */
 typedef struct fhog_paged_append_args {
   fhog_paged_cache cache;
   const void* k;         /* (batch, heads_k, n, d) */
@@ -367,7 +367,7 @@ int fhog_paged_append(const fhog_paged_append_args* args, void* hip_stream);
 
 /* O = softmax(scale q K^T) V and L = logsumexp of the scaled scores of one token of each sequence over the entries that it sees: all, or with a window W > 0 the last
    W and the first `sinks`. A sequence that sees none has O = 0 and L = -infinity.
-   weights_out, where given: weights_in (which may be the same array) plus, at every entry that is seen, sum over the heads of queries of a head of keys of
+   weights_out, where given: weights_in (the same array, or one that lies apart) plus, at every entry that is seen, sum over the heads of queries of a head of keys of
    exp(scale q k - L); the other entries as they were. */
 typedef struct fhog_paged_attn_args {
   fhog_paged_cache cache;

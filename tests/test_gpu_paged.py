@@ -571,3 +571,54 @@ def test_groups_in_parts(dtype, group):
     w = torch.rand(5, 2, c.table.shape[1] * 32).cuda()
     o, lse, new = fhog.paged_attention(q, c.cache(), weights=w)
     _check_attention(c, q, o, lse, weights=w, new=new)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B, longest, H, H_k, d", [(70, 2500, 2, 1, 64), (130, 1500, 3, 1, 128), (200, 3000, 1, 1, 64), (530, 1100, 1, 1, 32), (64, 1700, 70, 1, 64), (65, 1300, 4, 4, 128)])
+def test_large_ragged_batches(dtype, B, longest, H, H_k, d):
+    """Tiles dealt out over more sequences than a wave has lanes, some long among many short ones and some of none; and more sequences than are dealt out."""
+    import fhog
+    lengths = [longest if b % 23 == 5 else 0 if b % 11 == 3 else (b * 37) % 90 for b in range(B)]
+    c = Case(dtype, H_k, d, 16, lengths, seed=22)
+    q = c.normal(B, H, 1, d)
+    w = torch.rand(B, H_k, c.table.shape[1] * 16).cuda()
+    o, lse, new = fhog.paged_attention(q, c.cache(), weights=w)
+    plain = fhog.paged_attention(q, c.cache())
+    assert torch.equal(plain[0], o) and torch.equal(plain[1], lse)
+    _check_attention(c, q, o, lse, weights=w, new=new)
+    # a sequence by itself, dealt out otherwise: the same to rounding
+    b = next(b for b in range(B) if lengths[b] == longest)
+    alone = fhog.PagedCache(c.keys, c.values, c.table[b:b + 1], c.n[b:b + 1])
+    one = fhog.paged_attention(q[b:b + 1], alone)
+    assert (one[1] - lse[b:b + 1]).abs().max() <= 1e-4
+
+
+@pytest.mark.parametrize("rows", [40, 700])
+def test_a_captured_eviction(rows):
+    """Selection and copy in a graph, in one launch and in two; replayed over other weights, lengths and pages."""
+    import fhog
+    c = Case(torch.bfloat16, 2, 128, 16, [1500, 900, 20], seed=23, spare=300)
+    free = [p for p in range(c.keys.shape[0]) if p not in c.table.flatten().tolist()]
+    P = -(-rows // 16)
+    into = torch.tensor([free[i * P:(i + 1) * P] for i in range(3)], dtype=torch.int32).cuda()
+    w = torch.rand(3, 2, c.table.shape[1] * 16, device="cuda")
+    cache = c.cache()
+    fhog.paged_evict(cache, w, rows, into, sinks=2, recent=9)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        left, new, kept = fhog.paged_evict(cache, w, rows, into, sinks=2, recent=9)
+    for i in range(4):
+        w.copy_(torch.rand(w.shape, generator=c.g))
+        c.n.sub_(7)
+        into.copy_(into.roll(1, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (left.lengths, new, kept, c.keys, c.values)]
+        eager = fhog.paged_evict(cache, w, rows, into, sinks=2, recent=9)
+        for a, b in zip(got, (eager[0].lengths, eager[1], eager[2], c.keys, c.values)):
+            assert torch.equal(a.view(torch.int16) if a.dtype == torch.bfloat16 else a, b.view(torch.int16) if b.dtype == torch.bfloat16 else b), i
+        for b, n in enumerate(c.n.tolist()):
+            for h in range(2):
+                n = max(0, n)   # a length below zero is none
+                assert kept[b, h].tolist()[:min(n, rows)] == _stays(w[b, h].tolist(), n, rows, 2, 9)
