@@ -11,10 +11,9 @@
 // adds in their order: a causal mask leaves the first keys many times the work of the last, and a sink all of it.
 //
 // What bounds it: the instructions of a SIMD. A block of 32 x 32 pairs takes d / 16 matrix instructions of 32 cycles and 48 vector instructions, 16 of them exponentials at half
-// rate: 256 cycles each at d = 128, which run side by side two thirds of the time. bf16, 16 heads x 16384 causal, four to one of keys, d = 128: 619 us, 888 TFLOP/s, 75 % of
-// what a large library product of bf16 matrices reaches here, which takes no exponentials.
+// rate: 256 cycles each at d = 128. The matrix instructions of one wave run beside the exponentials of another: three workgroups to a CU, four below d = 128. bf16, 16 heads x 16384
+// causal, four to one of keys, d = 128: 534 us, 1030 TFLOP/s, 87 % of what a large library product of bf16 matrices reaches here, which takes no exponentials.
 #include <algorithm>
-#include <type_traits>
 
 #include "fhog_small.h"
 
@@ -23,10 +22,8 @@ using namespace bf16k;
 namespace {
 
 constexpr int kThreads = 256, kRows = 64;   // queries of a stage
-// Stages in LDS: the one that is read, the one after it, which has landed so that its statistics can be made ready, and those that are on their way: two with 64 keys to a wave, one
-// with 32, which leaves room for three workgroups (us, 16 x 16384, window 1024, d = 128 168 -> 146; 16 x 2048 31 -> 28)
-template <int BYTES, int NK>
-constexpr int kRing = BYTES > 256 || NK == 1 ? 3 : 4;
+// Stages in LDS: the one that is read, the one after it, which has landed so that its statistics can be made ready, and one that is on its way
+constexpr int kRing = 3;
 
 struct Weigh {
   const char* q;
@@ -84,24 +81,22 @@ struct Type<FHOG_DTYPE_FP32> {
 // The bits of a vector's element as a number; handed over by value: of an element itself __builtin_bit_cast takes the vector's first
 __device__ __forceinline__ float number(uint32_t bits) { return __builtin_bit_cast(float, bits); }
 
-// All loads but the last N of this wave have landed
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  static_assert(N < 64, "a counter of six bits");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
 // rows of BYTES bytes in LDS: chunk ch of row r lies at ch ^ swizzle(r), so that the 16-byte reads of a column of rows meet no bank twice
 template <int BYTES>
 __device__ __forceinline__ int swizzle(int r) {
   return swz<(BYTES > 256 ? 128 : BYTES / 2)>(r);
 }
 
+// Workgroups of a CU that the registers are to leave room for; the stages in LDS do, where the keys are of 16 bits. us, 16 x 16384 causal, 64 keys to a wave: d = 128 with two
+// workgroups 605, with three 538, with two that take the exponentials of one tile of queries behind the matrix products of the next 619; d = 64 with three 368, with four 355
+template <int DT, int D>
+constexpr int kWorkgroups = D == 128 ? (DT == FHOG_DTYPE_FP32 ? 2 : 3) : DT == FHOG_DTYPE_FP32 ? 3 : 4;
+
 template <int DT, int D, int NK>
-__global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
+__global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32, F16 = DT == FHOG_DTYPE_FP16;
   constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), CHUNKS = BYTES / 16, PER_LOAD = 64 / CHUNKS, LOADS = kRows / PER_LOAD / 4;
-  constexpr int TILE = kRows * BYTES, STAGE = TILE + kRows * 4, RING = kRing<BYTES, NK>, KEYS = 128 * NK, STEPS = CHUNKS / 2;
+  constexpr int TILE = kRows * BYTES, STAGE = TILE + kRows * 4, KEYS = 128 * NK, STEPS = CHUNKS / 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
@@ -151,21 +146,19 @@ __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
     t = begin + from - head * each, src += head * w.qh + (t - begin) * stage_bytes, lse += (int64_t)head * w.n_q + (t - begin) * kRows;
   }
   const int64_t back = w.qh - (each - 1) * stage_bytes, lse_back = w.n_q - (int64_t)(each - 1) * kRows;   // to the first stage of the next head
-  // Every wave asks for the statistics too, to the same place: then each has as many loads of a stage under way, and can wait for all but the last stages'
-  constexpr int MINE = LOADS + 1;
   const auto issue = [&] {
     const int valid = geo.n_q - t * kRows;
     if (valid >= kRows) {
-      smallk::stage_words(into + TILE, lse + lane);
+      if (wave == 3) smallk::stage_words(into + TILE, lse + lane);
 #pragma unroll
       for (int u = 0; u < LOADS; u++) Dma<64>::issue_one(into + (wave + 4 * u) * 1024, off[u], (const __bf16*)src);
     } else {
       keep_branch();
-      smallk::stage_words(into + TILE, lse + min(lane, valid - 1));
+      if (wave == 3) smallk::stage_words(into + TILE, lse + min(lane, valid - 1));
 #pragma unroll
       for (int u = 0; u < LOADS; u++) Dma<64>::issue_one(into + (wave + 4 * u) * 1024, offset(u, valid), (const __bf16*)src);
     }
-    into = into == ring + (RING - 1) * STAGE ? ring : into + STAGE;
+    into = into == ring + (kRing - 1) * STAGE ? ring : into + STAGE;
     if (++t == end) t = begin, src += back, lse += lse_back;
     else src += stage_bytes, lse += kRows;
   };
@@ -175,106 +168,78 @@ __global__ void __launch_bounds__(kThreads, 2) weigh(Weigh w) {
     const float l = *at;
     *at = l == -INFINITY ? INFINITY : l * kLog2e;
   };
-  for (int i = 0; i < RING - 1 && from + i < to; i++) issue();
+  for (int i = 0; i < kRing - 1 && from + i < to; i++) issue();
   wait_vm0();   // the keys and the first stages; with the builtin, or the compiler waits for the keys, and for the stages under way, in every tile
   __syncthreads();
   if (from < to && wave == 0) make_ready(smem);
   char* stage = smem;
   __syncthreads();
   int now = each > 0 ? begin + from % each : 0;
-  // Two tiles of 32 queries are on the way at a time, each in registers of its own: while one is multiplied, the exponentials of the one before are taken behind its
-  // matrix instructions, a few behind each, so that neither kind waits for the other. us, 16 x 16384 causal, d = 128: one tile at a time 760, so 690; the scalars of a stage carried along instead of
-  // formed anew 660 -> 637, the keys asked for together with the first stages 637 -> 619.
-  f32x16_t scores[2][NK];
-  f32x4_t stats[2][4];      // L of the lane's 16 queries: 8 g + 4 h + e
-  int waiting = -1;         // the tile whose exponentials are still to be taken; the same for the wave
-  float part[NK][2];        // sums of a tile
-  // a slice of the exponentials of a tile
-  const auto some = [&](int t, int c, int x) {
-#pragma unroll
-    for (int r = c * 16 / STEPS; r < (c + 1) * 16 / STEPS; r++) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[t][x][r], w.scale_log2, -stats[t][r / 4][r % 4]));
-      part[x][r % 2] = r < 2 ? p : part[x][r % 2] + p;
-    }
-  };
-  // sums of tiles, then of their sums: a sum over many queries is rounded once for each tile, not for each query
-  const auto add = [&] {
-#pragma unroll
-    for (int x = 0; x < NK; x++) sum[x] += part[x][0] + part[x][1];
-  };
-  const auto rest = [&](int t) {
-#pragma unroll
-    for (int c = 0; c < STEPS; c++)
-#pragma unroll
-      for (int x = 0; x < NK; x++) some(t, c, x);
-    add();
-  };
   for (int step = from; step < to; step++) {
-    const bool more = step + RING - 1 < to;
+    const bool more = step + kRing - 1 < to;
     if (more) issue();
-    char* const after = stage == smem + (RING - 1) * STAGE ? smem : stage + STAGE;
+    char* const after = stage == smem + (kRing - 1) * STAGE ? smem : stage + STAGE;
     if (step + 1 < to && wave == (step & 3)) make_ready(after);
-    const auto tile_of = [&](auto which) {
-      constexpr int u = decltype(which)::value;
+#pragma unroll
+    for (int u = 0; u < kRows / 32; u++) {
       const int i0 = now * kRows + 32 * u;
-      if (i0 > any_hi || i0 + 31 < any_lo) return;   // no query of the tile sees a key of this wave
-      if (waiting == u) rest(u);
-      const auto multiply = [&](auto beside) {
-        constexpr int AHEAD = STEPS < 3 ? STEPS : 3;
-        const char* const row = stage + (32 * u + n) * BYTES;
-        u32x4_t a[AHEAD];
-        const auto read = [&](int c) { a[c % AHEAD] = *reinterpret_cast<const u32x4_t*>(row + (((2 * c + h) ^ swizzle<BYTES>(n)) << 4)); };
+      if (i0 > any_hi || i0 + 31 < any_lo) continue;   // no query of the tile sees a key of this wave
+      constexpr int AHEAD = STEPS < 3 ? STEPS : 3;
+      const char* const row = stage + (32 * u + n) * BYTES;
+      u32x4_t a[AHEAD];
+      const auto read = [&](int c) { a[c % AHEAD] = *reinterpret_cast<const u32x4_t*>(row + (((2 * c + h) ^ swizzle<BYTES>(n)) << 4)); };
 #pragma unroll
-        for (int c = 0; c < AHEAD - 1; c++) read(c);
+      for (int c = 0; c < AHEAD - 1; c++) read(c);
+      f32x16_t scores[NK];
 #pragma unroll
-        for (int e = 0; e < 4; e++) stats[u][e] = *reinterpret_cast<const f32x4_t*>(stage + TILE + (32 * u + 8 * e + 4 * h) * 4);
+      for (int c = 0; c < STEPS; c++) {
+        if (c + AHEAD - 1 < STEPS) read(c + AHEAD - 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < STEPS; c++) {
-          if (c + AHEAD - 1 < STEPS) read(c + AHEAD - 1);
-          __builtin_amdgcn_sched_barrier(0);
+        for (int x = 0; x < NK; x++) {
+          if (c == 0) scores[x] = f32x16_t{0};
+          if constexpr (WIDE) {
 #pragma unroll
-          for (int x = 0; x < NK; x++) {
-            if (c == 0) scores[u][x] = f32x16_t{0};
-            if constexpr (WIDE) {
-#pragma unroll
-              for (int e = 0; e < 4; e++) scores[u][x] = __builtin_amdgcn_mfma_f32_32x32x2f32(number(a[c % AHEAD][e]), number(key[x][c][e]), scores[u][x], 0, 0, 0);
-            } else {
-              scores[u][x] = mfma<F16>(__builtin_bit_cast(bf16x8_t, a[c % AHEAD]), __builtin_bit_cast(bf16x8_t, key[x][c]), scores[u][x]);
-            }
-            if (beside.value) some(u ^ 1, c, x);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int e = 0; e < 4; e++) scores[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(number(a[c % AHEAD][e]), number(key[x][c][e]), scores[x], 0, 0, 0);
+          } else {
+            scores[x] = mfma<F16>(__builtin_bit_cast(bf16x8_t, a[c % AHEAD]), __builtin_bit_cast(bf16x8_t, key[x][c]), scores[x]);
           }
         }
-        if (beside.value) add();
-      };
-      if (waiting == (u ^ 1)) multiply(std::true_type{});
-      else multiply(std::false_type{});
-      waiting = u;
-      if (i0 >= whole_lo && i0 + 31 <= whole_hi) return;
-      // some queries do not see some keys: at once, with a look at each
-      keep_branch();
-      waiting = -1;
-#pragma unroll
-      for (int x = 0; x < NK; x++) {
-        float all = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int i = i0 + 8 * (r / 4) + 4 * h + r % 4;
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[u][x][r], w.scale_log2, -stats[u][r / 4][r % 4]));
-          all += i >= lo[x] && i <= hi[x] ? p : 0.f;
-        }
-        sum[x] += all;
+        __builtin_amdgcn_sched_barrier(0);
       }
-    };
-    tile_of(Slot<0>{}), tile_of(Slot<1>{});
+      f32x4_t stats[4];   // L of the lane's 16 queries: 8 g + 4 h + e
+#pragma unroll
+      for (int e = 0; e < 4; e++) stats[e] = *reinterpret_cast<const f32x4_t*>(stage + TILE + (32 * u + 8 * e + 4 * h) * 4);
+      const auto weight = [&](int x, int r) { return __builtin_amdgcn_exp2f(__builtin_fmaf(scores[x][r], w.scale_log2, -stats[r / 4][r % 4])); };
+      // sums of tiles, then of their sums: a sum over many queries is rounded once for each tile, not for each query
+      if (i0 >= whole_lo && i0 + 31 <= whole_hi) {
+#pragma unroll
+        for (int x = 0; x < NK; x++) {
+          float part[2] = {weight(x, 0), weight(x, 1)};
+#pragma unroll
+          for (int r = 2; r < 16; r++) part[r % 2] += weight(x, r);
+          sum[x] += part[0] + part[1];
+        }
+      } else {   // some queries do not see some keys
+        keep_branch();
+#pragma unroll
+        for (int x = 0; x < NK; x++) {
+          float all = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int i = i0 + 8 * (r / 4) + 4 * h + r % 4;
+            const float p = weight(x, r);
+            all += i >= lo[x] && i <= hi[x] ? p : 0.f;
+          }
+          sum[x] += all;
+        }
+      }
+    }
     if (++now == end) now = begin;
     stage = after;
-    if (more) wait_vm<(RING - 3) * MINE>();   // the stage after the next one has landed
-    else dma_wait();
+    dma_wait();   // the stage after the next one has landed
     __syncthreads();
   }
-  if (waiting == 0) rest(0);
-  if (waiting == 1) rest(1);
 #pragma unroll
   for (int x = 0; x < NK; x++) {
     const float total = sum[x] + __shfl_xor(sum[x], 32);
@@ -296,7 +261,13 @@ __global__ void __launch_bounds__(kThreads) add_pieces(Weigh w) {
   const int64_t slice = (int64_t)w.heads_k * w.batch * w.n_k;
   const float* const part = w.part + ((int64_t)b * w.heads_k + g) * w.n_k + j;
   float sum = 0.f;
-  for (int i = 0; i < pieces; i++) sum += part[i * slice];
+  for (int i = 0; i < pieces; i += 8) {   // eight on their way at a time, added in their order
+    float of[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) of[e] = i + e < pieces ? part[(i + e) * slice] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum += of[e];
+  }
   w.out[b * w.ob + g * w.oh + j] = sum;
 }
 
@@ -319,16 +290,18 @@ Plan plan_of(const fhog_key_weights_args* a) {
     const int64_t seen = a->causal == FHOG_MASK_NONE ? a->n_k : a->n_k - a->n_q / 2;   // keys of a query, about, without a window
     total = std::max(p.tiles, banded ? std::min(p.tiles, (a->n_q + a->window + keys - 1) / keys) * band : all * ((seen + keys - 1) / keys));
   };
-  // 64 keys to a wave where there is work for it: half the reads of LDS, but fewer waves and coarser masks. us, 32 | 64 keys, bf16: d = 128 causal 16 heads x 16384
-  // 639 | 618, 32 x 4096 120 | 110, 16 x 3000 39 | 47, 128 x 64 queries of 8192 keys 29 | 36, window 4096 of 16 x 16384 297 | 295, window 1024 146 | 180, 8 x 512 11 | 15; d = 64, whose
-  // waves have fewer matrix instructions to hide behind, 16 x 16384 422 | 491, 32 x 2048 31 | 42
+  // 64 keys to a wave where there is work for it: half the reads of LDS, but fewer workgroups and coarser masks. us, 32 | 64 keys, bf16, heads x length: d = 128 causal 16 x 16384
+  // 631 | 534, 16 x 8192 179 | 153, 32 x 4096 99 | 86, 64 x 2048 56.7 | 59.7, 16 x 3000 36.8 | 39.2, 8 x 512 10.8 | 18.1, window 2048 of 16 x 16384 175 | 159, window 1024 134 | 140;
+  // d = 64 16 x 16384 386 | 354, 32 x 4096 67 | 62, 32 x 2048 25.5 | 33.4, window 2048 112 | 110; d = 32 16 x 16384 295 | 290, 16 x 8192 98 | 91
   int64_t most, total;
   p.nk = 2, stages(256, most, total);
-  if (a->dtype == FHOG_DTYPE_FP32 || a->d != 128 || (banded && a->window < 2048) || total * group * slices < 8192) p.nk = 1, stages(128, most, total);
-  // Two workgroups to a CU as long as that leaves pieces worth their beginning, and short enough to even out the end of the launch. us, at most 16 | 24 | 32 | 40 stages:
-  // 16 x 16384 d = 128 650 | 640 | 638 | 634, d = 64 444 | 427 | 422 | 428; at least 6 | 8: 16 x 3000 60 | 47, 8 x 512 12.6 | 11.3
-  int64_t chunk = std::min<int64_t>(32, std::max<int64_t>(a->dtype == FHOG_DTYPE_FP32 ? 3 : 8, (total * group * slices + 1023) / 1024));
-  if (banded) {   // most tiles have as many stages: cut them evenly (us, fp16 48 x 1537, window 400: 32 -> 28)
+  if (a->dtype == FHOG_DTYPE_FP32 || (banded && a->window < 2048) || total * group * slices < 12288) p.nk = 1, stages(128, most, total);
+  // Eight pieces to a CU, as long as that leaves pieces worth their beginning, and short enough to even out the end of the launch. us, at most 16 | 24 | 32 | 48 | 64 stages, 32 keys to
+  // a wave, 16 x 16384: d = 128 651 | 642 | 628 | 650 | 660, d = 64 399 | 394 | 391 | 410 | 418; four | eight pieces to a CU, 64 keys to a wave: 16 x 8192 172 | 154; at least 6 | 8 stages:
+  // 16 x 3000 39.1 | 36.9, 8 x 512 12.0 | 10.8 (which then needs no second kernel); of a band, whose tiles have few, 5 | 8: fp16 48 x 1537, window 400, d = 64 22.4 | 26.3
+  const int64_t least = a->dtype == FHOG_DTYPE_FP32 ? 3 : p.nk == 1 && banded ? 5 : 8;
+  int64_t chunk = std::min<int64_t>(32, std::max(least, (total * group * slices + 2047) / 2048));
+  if (banded) {   // most tiles have as many stages: cut them evenly, not into full pieces and a short one
     const int64_t mine = group * std::min(all, (a->window + 128 * p.nk) / kRows + 2), n = std::max<int64_t>(1, (mine + chunk / 2) / chunk);
     chunk = (mine + n - 1) / n;
   }
@@ -340,7 +313,7 @@ Plan plan_of(const fhog_key_weights_args* a) {
 
 template <int DT, int D, int NK>
 hipError_t launch_d(const Weigh& w, hipStream_t s) {
-  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), STAGE = kRows * BYTES + kRows * 4, LDS = kRing<BYTES, NK> * STAGE;
+  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), STAGE = kRows * BYTES + kRows * 4, LDS = kRing * STAGE;
   const hipError_t e = allow_dynamic_lds<weigh<DT, D, NK>>(LDS);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((weigh<DT, D, NK>), dim3((unsigned)(w.tiles * w.pieces), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), LDS, s, w);
