@@ -396,6 +396,8 @@ int validate_paged_attn(const fhog_paged_attn_args* a) {
   if (const int rc = check_pointer("lse", a->lse, false)) return rc;
   if (!a->weights_in != !a->weights_out) return fail(FHOG_E_NULL, "one of weights_in and weights_out is NULL");
   if (!a->weights_out) return FHOG_OK;
+  if (c.batch * a->heads_q + c.batch * c.heads_k * ((capacity + 1023) / 1024) >= 1 << 24)   // workgroups of the launch that adds them
+    return fail(FHOG_E_SHAPE, "weights of more than about 2^34 entries, of all sequences and heads of keys together, are not supported");
   if (const int rc = check_pointer("weights_in", a->weights_in, false)) return rc;
   if (const int rc = check_pointer("weights_out", a->weights_out, false)) return rc;
   if (!rows_apart(c.batch, c.heads_k, 1, capacity, a->stride_wob, a->stride_woh, 0)) return fail(FHOG_E_STRIDE, "rows of an output overlap");

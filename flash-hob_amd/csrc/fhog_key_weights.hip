@@ -162,11 +162,13 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
     if (++t == end) t = begin, src += back, lse += lse_back;
     else src += stage_bytes, lse += kRows;
   };
-  // L in log2 units. A query that saw nothing has no weights to give: exp(s - infinity)
+  // L in log2 units. A query that saw nothing has no weights to give, whatever it holds: it becomes 0, exp(0 - infinity)
   const auto make_ready = [&](char* stage) {
     float* const at = reinterpret_cast<float*>(stage + TILE) + lane;
     const float l = *at;
     *at = l == -INFINITY ? INFINITY : l * kLog2e;
+    for (uint64_t empty = __builtin_amdgcn_ballot_w64(l == -INFINITY); empty != 0; empty &= empty - 1)
+      for (int c = lane; c < BYTES / 4; c += 64) reinterpret_cast<uint32_t*>(stage + __builtin_ctzll(empty) * BYTES)[c] = 0;
   };
   for (int i = 0; i < kRing - 1 && from + i < to; i++) issue();
   wait_vm0();   // the keys and the first stages; with the builtin, or the compiler waits for the keys, and for the stages under way, in every tile
@@ -271,6 +273,9 @@ __global__ void __launch_bounds__(kThreads) add_pieces(Weigh w) {
   w.out[b * w.ob + g * w.oh + j] = sum;
 }
 
+// Pieces at most: a workspace of that many rows like the result's, whatever the length (one head in four of keys, 131072 tokens: 134 MB to 4 heads of keys), and a grid of 2^23 workgroups
+constexpr int64_t kPieces = 64;
+
 // Keys of a workgroup and how the queries of one are cut
 struct Plan {
   int nk, pieces, chunk;
@@ -305,6 +310,7 @@ Plan plan_of(const fhog_key_weights_args* a) {
     const int64_t mine = group * std::min(all, (a->window + 128 * p.nk) / kRows + 2), n = std::max<int64_t>(1, (mine + chunk / 2) / chunk);
     chunk = (mine + n - 1) / n;
   }
+  chunk = std::max(chunk, (most * group + kPieces - 1) / kPieces);
   p.pieces = (int)std::max<int64_t>(1, (most * group + chunk - 1) / chunk);
   p.chunk = (int)std::max(chunk, p.pieces == 1 ? most * group : 0);
   p.bytes = p.pieces > 1 ? sizeof(float) * p.pieces * slices * a->n_k : 0;

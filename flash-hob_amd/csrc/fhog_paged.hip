@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   each([&](int j, uint32_t r) {
     const uint64_t o = __builtin_amdgcn_ballot_w64(j < end && r > rank), s = __builtin_amdgcn_ballot_w64(j < end && r == rank);
     const int same_before = same + __builtin_popcountll(s & below), at = over + __builtin_popcountll(o & below) + min(same_before, ties);
-    if (j < end && (r > rank || (r == rank && same_before < ties))) kept[at] = j, out[at] = w[j];
+    if (j < end && at < m && (r > rank || (r == rank && same_before < ties))) kept[at] = j, out[at] = w[j];   // at >= m: of lengths that someone has changed meanwhile
     over += __builtin_popcountll(o), same += __builtin_popcountll(s);
   });
   if constexpr (MOVE) {

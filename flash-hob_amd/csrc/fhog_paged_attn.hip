@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
     } else {
 #pragma unroll
       for (int u = 0; u < SUB; u += 2) {
-        // weights are rounded to the type of the values, which are products' other factor: 2^-9 of a weight in bf16, as in attention over whole tensors
+        // weights are rounded to the type of the values, which are products' other factor: up to 2^-8 of a weight in bf16 and 2^-11 in fp16, as in attention over whole tensors
         const u32x4_t weights = {pack<DT>(x[u][0], x[u][1]), pack<DT>(x[u][2], x[u][3]), pack<DT>(x[u + 1][0], x[u + 1][1]), pack<DT>(x[u + 1][2], x[u + 1][3])};
 #pragma unroll
         for (int c = 0; c < C; c += 2) {

@@ -103,7 +103,7 @@ def paged_append(cache: PagedCache, k, v, *, counts=None) -> None:
         k, v: (B, H_k, N, d), the dtype of the cache, any strides. A token each, or prompts.
         counts: (B,) int32, how many of the N tokens sequence b has, the first ones; the others are padding. None: all. A sequence never gets more entries than it is long.
 
-    Sequences that share pages must not both write to the same entry of one.
+    Sequences that share pages must not both write to the same entry of one, and ``k`` and ``v`` must not lie where entries are written.
     """
     if not isinstance(cache, PagedCache):
         _check_cache(cache)

@@ -132,6 +132,33 @@ def test_queries_that_saw_nothing_and_hidden_infinities():
     assert got[0, 0, :101].isnan().all() and torch.equal(got[0, 0, 101:], base[0, 0, 101:])
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("causal, window, sinks", [(True, None, 0), (True, 2500, 3), (False, None, 0)])
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_long_prompts_of_many_heads(dtype, causal, window, sinks, d):
+    """Enough work for 64 keys to a wave, with a ragged end; against fp64."""
+    import fhog
+    q, k, lse = _make(dtype, 1, 32, 8, 4001, 4001, d, causal, window, sinks, seed=11)
+    got = fhog.key_weights(q, k, lse, None, causal, window=window, sinks=sinks)
+    _check(got, q, k, lse, causal, window, sinks)
+    assert torch.equal(fhog.key_weights(q, k, lse, None, causal, window=window, sinks=sinks), got)
+
+
+@pytest.mark.parametrize("hidden", [NAN, math.inf])
+@pytest.mark.parametrize("dtype, n, H", [(torch.bfloat16, 300, 2), (torch.float16, 300, 2), (torch.float32, 300, 2), (torch.bfloat16, 4001, 32)])
+def test_what_a_query_that_saw_nothing_holds_does_not_matter(dtype, n, H, hidden):
+    """L = -inf takes a query out, also one that is NaN or infinite, and also where every query of its tile would see every key."""
+    import fhog
+    q, k, lse = _make(dtype, 1, H, H // 2, n, n, 64, False, None, 0, seed=12)
+    out = torch.zeros(n, dtype=torch.bool, device="cuda")
+    out[5], out[64:200:3], out[n - 1] = True, True, True
+    lse[..., out] = -math.inf
+    base = fhog.key_weights(q, k, lse)
+    _check(base, q, k, lse, False, None, 0)
+    q[..., out, :] = hidden
+    assert torch.equal(fhog.key_weights(q, k, lse), base)
+
+
 def test_refusals():
     import fhog
     q, k, lse = _make(torch.bfloat16, 2, 4, 2, 40, 60, 64, "bottom_right", None, 0)

@@ -85,6 +85,8 @@ OWN = {
                    (dict(lse=0), -1, "'lse'"), (dict(weights_in=0), -1, "weights"), (dict(weights_out=0), -1, "weights"), (dict(weights_in=0, weights_out=0), 0, ""),
                    (dict(weights_out=2), -5, "weights_out"), (dict(stride_woh=79), -4, "overlap"), (dict(stride_wih=0, stride_wib=0), 0, ""),
                    (dict(cache_batch=30000, cache_page=2 ** 15, cache_table_width=2 ** 15, cache_stride_h=2 ** 21, cache_stride_p=2 ** 22, stride_wob=2 ** 32, stride_woh=2 ** 30), -2, "2^40"),
+                   (dict(cache_batch=200, cache_table_width=2 ** 22, stride_wob=2 ** 31, stride_woh=2 ** 30), -2, "2^34"),
+                   (dict(cache_batch=200, cache_table_width=2 ** 22, weights_in=0, weights_out=0), 0, ""),
                    (dict(cache_values=0x10000), 0, ""), (dict(window=5, sinks=2 ** 40), 0, "")],
     "key_weights": [(dict(dtype=9), -3, "dtype"), (dict(d=256), -2, "head dim"), (dict(batch=-1), -2, "sequences"), (dict(batch=65536), -2, "sequences"), (dict(heads_k=0), -2, "heads"),
                     (dict(heads_k=3), -2, "heads"), (dict(n_q=0), -2, "n_q"), (dict(n_k=2 ** 24 + 1), -2, "n_k"), (dict(n_q=300), -6, "bottom-right"), (dict(causal=1), -6, "top-left"),
@@ -141,6 +143,18 @@ def test_workspaces(L):
                 setattr(args, n, v)
             assert getattr(L, f"fhog_{name}")(ctypes.byref(args), None) == code and word in L.fhog_last_error().decode()
             args.ws, args.ws_bytes = kept
+
+
+@pytest.mark.parametrize("change", [{}, dict(sinks=4), dict(window=1024), dict(window=1024, sinks=4), dict(window=100000, sinks=4), dict(causal=0)])
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n", [30000, 2 ** 17, 2 ** 20, 2 ** 24])
+def test_the_workspace_of_long_prompts_is_bounded(L, n, dtype, change):
+    """64 rows like the result's at most: partial sums do not grow with the square of the length."""
+    a = _args("key_weights", batch=1, heads_q=16, heads_k=2, n_q=n, n_k=n, dtype=dtype, causal=1, stride_qh=64 * n, stride_kh=64 * n, stride_oh=n, stride_ob=2 * n)
+    for name, v in change.items():
+        setattr(a, name, v)
+    assert L.fhog_key_weights_validate(ctypes.byref(a)) == 0
+    assert 0 <= L.fhog_key_weights_workspace_bytes(ctypes.byref(a)) <= 64 * 4 * 2 * n
 
 
 def _cache(**kw):
