@@ -144,6 +144,19 @@ def test_long_prompts_of_many_heads(dtype, causal, window, sinks, d):
     assert torch.equal(fhog.key_weights(q, k, lse, None, causal, window=window, sinks=sinks), got)
 
 
+@pytest.mark.parametrize("causal, n_q", [(True, 4001), ("bottom_right", 3500)])
+@pytest.mark.parametrize("lengths", [[4001, 1234], [0, 5000], [600, 513]])
+def test_long_padded_prompts(lengths, causal, n_q):
+    """As above, padded: what lies in the padding counts for nothing."""
+    import fhog
+    q, k, lse = _make(torch.bfloat16, 2, 16, 4, n_q, 4001, 64, causal, None, 0, seed=13)
+    off = 4001 - n_q if causal == "bottom_right" else 0
+    for b, m in enumerate(lengths):
+        q[b, :, max(0, m - off):], k[b, :, m:], lse[b, :, max(0, m - off):] = NAN, NAN, NAN
+    got = fhog.key_weights(q, k, lse, None, causal, lengths=torch.tensor(lengths, dtype=torch.int32).cuda())
+    _check(got, q, k, lse, causal, None, 0, lengths=lengths)
+
+
 @pytest.mark.parametrize("hidden", [NAN, math.inf])
 @pytest.mark.parametrize("dtype, n, H", [(torch.bfloat16, 300, 2), (torch.float16, 300, 2), (torch.float32, 300, 2), (torch.bfloat16, 4001, 32)])
 def test_what_a_query_that_saw_nothing_holds_does_not_matter(dtype, n, H, hidden):
