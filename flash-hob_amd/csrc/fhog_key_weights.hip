@@ -21,7 +21,10 @@ namespace fhog {
 using namespace bf16k;
 namespace {
 
-constexpr int kThreads = 256, kRows = 64;   // queries of a stage
+constexpr int kThreads = 256;
+// Queries of a stage. Rows of 512 bytes in stages of 64 leave room in LDS for one workgroup, of 32 for three: fp32, d = 128, us 16 x 8192 1642 -> 1120 (122 TFLOP/s of the 154 that a
+// large library product reaches), 8 x 2048 74 -> 59, 16 x 4096, window 512 130 -> 103
+constexpr int rows_of(int bytes) { return bytes > 256 ? 32 : 64; }
 // Stages in LDS: the one that is read, the one after it, which has landed so that its statistics can be made ready, and one that is on its way
 constexpr int kRing = 3;
 
@@ -53,12 +56,13 @@ struct Queries {
   }
   __device__ __forceinline__ int first(int j) const { return causal ? max(0, j - off) : 0; }
   __device__ __forceinline__ int last(int j) const { return causal && j >= sinks && j - off < n_q - window ? j - off + window - 1 : n_q - 1; }
-  // stages of 64 queries of which some see some of the keys [j, j + n)
+  // stages of ROWS queries of which some see some of the keys [j, j + n)
+  template <int ROWS>
   __device__ __forceinline__ void stages(int j, int n, int& begin, int& end) const {
     begin = end = 0;
     if (j >= n_k || n_q == 0) return;
     const int to = j < sinks ? n_q - 1 : last(min(j + n, n_k) - 1);
-    begin = first(j) / kRows, end = max(begin, to / kRows + 1);
+    begin = first(j) / ROWS, end = max(begin, to / ROWS + 1);
     if (first(j) >= n_q) end = begin;
   }
 };
@@ -87,16 +91,16 @@ __device__ __forceinline__ int swizzle(int r) {
   return swz<(BYTES > 256 ? 128 : BYTES / 2)>(r);
 }
 
-// Workgroups of a CU that the registers are to leave room for; the stages in LDS do, where the keys are of 16 bits. us, 16 x 16384 causal, 64 keys to a wave: d = 128 with two
+// Workgroups of a CU that the registers are to leave room for; the stages in LDS do. us, 16 x 16384 causal, 64 keys to a wave: d = 128 with two
 // workgroups 605, with three 538, with two that take the exponentials of one tile of queries behind the matrix products of the next 619; d = 64 with three 368, with four 355
 template <int DT, int D>
-constexpr int kWorkgroups = D == 128 ? (DT == FHOG_DTYPE_FP32 ? 2 : 3) : DT == FHOG_DTYPE_FP32 ? 3 : 4;
+constexpr int kWorkgroups = D == 128 || DT == FHOG_DTYPE_FP32 ? 3 : 4;
 
 template <int DT, int D, int NK>
 __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32, F16 = DT == FHOG_DTYPE_FP16;
-  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), CHUNKS = BYTES / 16, PER_LOAD = 64 / CHUNKS, LOADS = kRows / PER_LOAD / 4;
-  constexpr int TILE = kRows * BYTES, STAGE = TILE + kRows * 4, KEYS = 128 * NK, STEPS = CHUNKS / 2;
+  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), CHUNKS = BYTES / 16, PER_LOAD = 64 / CHUNKS, ROWS = rows_of(BYTES), LOADS = ROWS / PER_LOAD / 4;
+  constexpr int TILE = ROWS * BYTES, STAGE = TILE + 256, KEYS = 128 * NK, STEPS = CHUNKS / 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
@@ -108,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
   const Queries geo(w, b);
   const int k0 = tile * KEYS, kw = k0 + 32 * NK * wave;
   int begin, end;
-  geo.stages(k0, KEYS, begin, end);
+  geo.template stages<ROWS>(k0, KEYS, begin, end);
   const int each = end - begin, steps = w.group * each, pieces = pieces_of(steps, w);
   if (piece >= max(pieces, w.pieces == 1 ? 1 : 0)) return;
   const int from = piece * w.chunk, to = min(steps, from + w.chunk);
@@ -134,40 +138,40 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
     return (uint32_t)(min(r, valid - 1) * (uint32_t)w.qn) + (uint32_t)((pc ^ swizzle<BYTES>(r)) << 4);
   };
 #pragma unroll
-  for (int u = 0; u < LOADS; u++) off[u] = offset(u, kRows);
+  for (int u = 0; u < LOADS; u++) off[u] = offset(u, ROWS);
   const uint32_t ring = lds_addr(smem);
   int t = begin;            // of the stage that is issued next; its queries, its statistics, and where it goes
-  const int64_t row0 = (int64_t)b * w.heads_q + g * w.group, stage_bytes = kRows * w.qn;
+  const int64_t row0 = (int64_t)b * w.heads_q + g * w.group, stage_bytes = ROWS * w.qn;
   const char* src = w.q + b * w.qb + (int64_t)g * w.group * w.qh + begin * stage_bytes;
-  const float* lse = w.lse + row0 * w.n_q + begin * kRows;
+  const float* lse = w.lse + row0 * w.n_q + begin * ROWS;
   uint32_t into = ring;
   if (each > 0) {
     const int head = from / each;
-    t = begin + from - head * each, src += head * w.qh + (t - begin) * stage_bytes, lse += (int64_t)head * w.n_q + (t - begin) * kRows;
+    t = begin + from - head * each, src += head * w.qh + (t - begin) * stage_bytes, lse += (int64_t)head * w.n_q + (t - begin) * ROWS;
   }
-  const int64_t back = w.qh - (each - 1) * stage_bytes, lse_back = w.n_q - (int64_t)(each - 1) * kRows;   // to the first stage of the next head
+  const int64_t back = w.qh - (each - 1) * stage_bytes, lse_back = w.n_q - (int64_t)(each - 1) * ROWS;   // to the first stage of the next head
   const auto issue = [&] {
-    const int valid = geo.n_q - t * kRows;
-    if (valid >= kRows) {
-      if (wave == 3) smallk::stage_words(into + TILE, lse + lane);
+    const int valid = geo.n_q - t * ROWS;
+    if (valid >= ROWS) {
+      if (wave == 3) smallk::stage_words(into + TILE, lse + lane % ROWS);
 #pragma unroll
       for (int u = 0; u < LOADS; u++) Dma<64>::issue_one(into + (wave + 4 * u) * 1024, off[u], (const __bf16*)src);
     } else {
       keep_branch();
-      if (wave == 3) smallk::stage_words(into + TILE, lse + min(lane, valid - 1));
+      if (wave == 3) smallk::stage_words(into + TILE, lse + min(lane % ROWS, valid - 1));
 #pragma unroll
       for (int u = 0; u < LOADS; u++) Dma<64>::issue_one(into + (wave + 4 * u) * 1024, offset(u, valid), (const __bf16*)src);
     }
     into = into == ring + (kRing - 1) * STAGE ? ring : into + STAGE;
     if (++t == end) t = begin, src += back, lse += lse_back;
-    else src += stage_bytes, lse += kRows;
+    else src += stage_bytes, lse += ROWS;
   };
   // L in log2 units. A query that saw nothing has no weights to give, whatever it holds: it becomes 0, exp(0 - infinity)
   const auto make_ready = [&](char* stage) {
     float* const at = reinterpret_cast<float*>(stage + TILE) + lane;
     const float l = *at;
     *at = l == -INFINITY ? INFINITY : l * kLog2e;
-    for (uint64_t empty = __builtin_amdgcn_ballot_w64(l == -INFINITY); empty != 0; empty &= empty - 1)
+    for (uint64_t empty = __builtin_amdgcn_ballot_w64(lane < ROWS && l == -INFINITY); empty != 0; empty &= empty - 1)
       for (int c = lane; c < BYTES / 4; c += 64) reinterpret_cast<uint32_t*>(stage + __builtin_ctzll(empty) * BYTES)[c] = 0;
   };
   for (int i = 0; i < kRing - 1 && from + i < to; i++) issue();
@@ -183,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
     char* const after = stage == smem + (kRing - 1) * STAGE ? smem : stage + STAGE;
     if (step + 1 < to && wave == (step & 3)) make_ready(after);
 #pragma unroll
-    for (int u = 0; u < kRows / 32; u++) {
-      const int i0 = now * kRows + 32 * u;
+    for (int u = 0; u < ROWS / 32; u++) {
+      const int i0 = now * ROWS + 32 * u;
       if (i0 > any_hi || i0 + 31 < any_lo) continue;   // no query of the tile sees a key of this wave
       constexpr int AHEAD = STEPS < 3 ? STEPS : 3;
       const char* const row = stage + (32 * u + n) * BYTES;
@@ -252,13 +256,13 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
   }
 }
 
-template <int KEYS>
+template <int KEYS, int ROWS>
 __global__ void __launch_bounds__(kThreads) add_pieces(Weigh w) {
   const int j = blockIdx.x * kThreads + threadIdx.x, g = blockIdx.y, b = blockIdx.z;
   if (j >= w.n_k) return;
   const Queries geo(w, b);
   int begin, end;
-  geo.stages(j / KEYS * KEYS, KEYS, begin, end);
+  geo.template stages<ROWS>(j / KEYS * KEYS, KEYS, begin, end);
   const int pieces = pieces_of(w.group * (end - begin), w);
   const int64_t slice = (int64_t)w.heads_k * w.batch * w.n_k;
   const float* const part = w.part + ((int64_t)b * w.heads_k + g) * w.n_k + j;
@@ -285,12 +289,12 @@ struct Plan {
 
 Plan plan_of(const fhog_key_weights_args* a) {
   Plan p;
-  const int64_t slices = a->batch * a->heads_k, group = a->heads_q / a->heads_k, all = (a->n_q + kRows - 1) / kRows;
+  const int64_t slices = a->batch * a->heads_k, group = a->heads_q / a->heads_k, rows = rows_of((int)a->d * (a->dtype == FHOG_DTYPE_FP32 ? 4 : 2)), all = (a->n_q + rows - 1) / rows;
   const bool banded = a->causal != FHOG_MASK_NONE && a->window > 0 && a->window < a->n_q;
   // stages of a tile of keys in one head of queries: those of the tile with the most, and about those of all of them together
   const auto stages = [&](int64_t keys, int64_t& most, int64_t& total) {
     p.tiles = (a->n_k + keys - 1) / keys;
-    const int64_t band = banded ? std::min(all, (a->window + keys) / kRows + 2) : all;
+    const int64_t band = banded ? std::min(all, (a->window + keys) / rows + 2) : all;
     most = a->sinks > 0 ? all : band;
     const int64_t seen = a->causal == FHOG_MASK_NONE ? a->n_k : a->n_k - a->n_q / 2;   // keys of a query, about, without a window
     total = std::max(p.tiles, banded ? std::min(p.tiles, (a->n_q + a->window + keys - 1) / keys) * band : all * ((seen + keys - 1) / keys));
@@ -307,7 +311,7 @@ Plan plan_of(const fhog_key_weights_args* a) {
   const int64_t least = a->dtype == FHOG_DTYPE_FP32 ? 3 : p.nk == 1 && banded ? 5 : 8;
   int64_t chunk = std::min<int64_t>(32, std::max(least, (total * group * slices + 2047) / 2048));
   if (banded) {   // most tiles have as many stages: cut them evenly, not into full pieces and a short one
-    const int64_t mine = group * std::min(all, (a->window + 128 * p.nk) / kRows + 2), n = std::max<int64_t>(1, (mine + chunk / 2) / chunk);
+    const int64_t mine = group * std::min(all, (a->window + 128 * p.nk) / rows + 2), n = std::max<int64_t>(1, (mine + chunk / 2) / chunk);
     chunk = (mine + n - 1) / n;
   }
   chunk = std::max(chunk, (most * group + kPieces - 1) / kPieces);
@@ -319,11 +323,11 @@ Plan plan_of(const fhog_key_weights_args* a) {
 
 template <int DT, int D, int NK>
 hipError_t launch_d(const Weigh& w, hipStream_t s) {
-  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), STAGE = kRows * BYTES + kRows * 4, LDS = kRing * STAGE;
+  constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), ROWS = rows_of(BYTES), STAGE = ROWS * BYTES + 256, LDS = kRing * STAGE;
   const hipError_t e = allow_dynamic_lds<weigh<DT, D, NK>>(LDS);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((weigh<DT, D, NK>), dim3((unsigned)(w.tiles * w.pieces), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), LDS, s, w);
-  if (w.pieces > 1) hipLaunchKernelGGL((add_pieces<128 * NK>), dim3((unsigned)((w.n_k + kThreads - 1) / kThreads), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), 0, s, w);
+  if (w.pieces > 1) hipLaunchKernelGGL((add_pieces<128 * NK, ROWS>), dim3((unsigned)((w.n_k + kThreads - 1) / kThreads), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), 0, s, w);
   return hipGetLastError();
 }
 template <int DT, int NK>

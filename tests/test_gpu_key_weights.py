@@ -144,12 +144,13 @@ def test_long_prompts_of_many_heads(dtype, causal, window, sinks, d):
     assert torch.equal(fhog.key_weights(q, k, lse, None, causal, window=window, sinks=sinks), got)
 
 
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 64), (torch.float32, 128)])
 @pytest.mark.parametrize("causal, n_q", [(True, 4001), ("bottom_right", 3500)])
 @pytest.mark.parametrize("lengths", [[4001, 1234], [0, 5000], [600, 513]])
-def test_long_padded_prompts(lengths, causal, n_q):
+def test_long_padded_prompts(lengths, causal, n_q, dtype, d):
     """As above, padded: what lies in the padding counts for nothing."""
     import fhog
-    q, k, lse = _make(torch.bfloat16, 2, 16, 4, n_q, 4001, 64, causal, None, 0, seed=13)
+    q, k, lse = _make(dtype, 2, 16, 4, n_q, 4001, d, causal, None, 0, seed=13)
     off = 4001 - n_q if causal == "bottom_right" else 0
     for b, m in enumerate(lengths):
         q[b, :, max(0, m - off):], k[b, :, m:], lse[b, :, max(0, m - off):] = NAN, NAN, NAN
@@ -158,11 +159,11 @@ def test_long_padded_prompts(lengths, causal, n_q):
 
 
 @pytest.mark.parametrize("hidden", [NAN, math.inf])
-@pytest.mark.parametrize("dtype, n, H", [(torch.bfloat16, 300, 2), (torch.float16, 300, 2), (torch.float32, 300, 2), (torch.bfloat16, 4001, 32)])
-def test_what_a_query_that_saw_nothing_holds_does_not_matter(dtype, n, H, hidden):
+@pytest.mark.parametrize("dtype, n, H, d", [(torch.bfloat16, 300, 2, 64), (torch.float16, 300, 2, 32), (torch.float32, 300, 2, 64), (torch.float32, 300, 2, 128), (torch.bfloat16, 4001, 32, 64)])
+def test_what_a_query_that_saw_nothing_holds_does_not_matter(dtype, n, H, d, hidden):
     """L = -inf takes a query out, also one that is NaN or infinite, and also where every query of its tile would see every key."""
     import fhog
-    q, k, lse = _make(dtype, 1, H, H // 2, n, n, 64, False, None, 0, seed=12)
+    q, k, lse = _make(dtype, 1, H, H // 2, n, n, d, False, None, 0, seed=12)
     out = torch.zeros(n, dtype=torch.bool, device="cuda")
     out[5], out[64:200:3], out[n - 1] = True, True, True
     lse[..., out] = -math.inf
