@@ -1,5 +1,7 @@
 // What the kernels on a cache in pages share: where an entry lies, and which tiles of its entries a token sees.
 #pragma once
+#include <type_traits>
+
 #include "fhog_common.h"
 
 namespace fhog {
@@ -38,6 +40,17 @@ inline Cache cache_of(const fhog_paged_cache& c) {
   r.page = Divisor((uint32_t)c.page);
   r.pages = (int32_t)c.pages, r.width = (int32_t)c.table_width, r.capacity = (int32_t)(c.table_width * c.page), r.heads_k = (int32_t)c.heads_k, r.batch = (int32_t)c.batch;
   return r;
+}
+
+// Sum over the lanes up to this one, in registers
+__device__ __forceinline__ int scan(int x) {
+  const auto add = [&](auto control, auto mask) { x += __builtin_amdgcn_update_dpp(0, x, control.value, mask.value, 0xf, false); };
+  const auto all = std::integral_constant<int, 0xf>{};
+  add(std::integral_constant<int, 0x111>{}, all), add(std::integral_constant<int, 0x112>{}, all);   // the lanes 1, 2, 4 and 8 before it in its row of 16
+  add(std::integral_constant<int, 0x114>{}, all), add(std::integral_constant<int, 0x118>{}, all);
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});                   // the last of the row before, into rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});                   // lane 31, into rows 2 and 3
+  return x;
 }
 
 // The tiles of T entries of which a token sees some, in a row: those of the sinks that lie before its window, then the window's

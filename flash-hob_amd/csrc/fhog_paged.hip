@@ -101,13 +101,14 @@ __device__ __forceinline__ void move_chunks(const Evict& e, int b, int h, const 
 // time from the top: a histogram of the digit over the entries whose higher digits are those found so far, and the digit at which the sum from above reaches
 // what is still to be found. Then the entries that stay are counted, wave by wave, and written to the places that the counts give.
 // What bounds it: the waits between its passes. us, 32 x 8 slices of 8192 | 4 x 4 of 1000: weights read anew in every pass 26.6 | 7.4, ranks formed once and kept in registers
-// 20.2 | 10.8, in LDS 22.7 | 7.6, and there with a histogram of eight copies 19.8 | 7.7.
+// 20.2 | 10.8, in LDS 22.7 | 7.6, and there with a histogram of eight copies 19.8 | 7.7. The wave that sums a histogram clears it for the next pass, and digits that stay all together end the
+// search: the whole call 230.6 -> 228.8 | 11.4 -> 10.0.
 // MOVE: and are moved by the same workgroup.
 template <bool MOVE>
 __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   extern __shared__ uint32_t held[];
-  __shared__ uint32_t histogram[kCopies][kDigits];   // a lane counts in copy lane % kCopies: the same digit of many lanes is not one address
-  __shared__ uint32_t found[2];               // digits so far; how many of the entries of that rank stay
+  __shared__ __attribute__((aligned(16))) uint32_t histogram[kCopies][kDigits];   // a lane counts in copy lane % kCopies: the same digit of many lanes is not one address
+  __shared__ uint32_t found[3];               // digits so far; how many of the entries of these digits stay, and whether all do
   __shared__ int counts[2][kWaves];           // entries of a wave's stretch above the rank, and of the rank itself
   const int b = blockIdx.x / e.c.heads_k, h = blockIdx.x - b * e.c.heads_k, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   const auto each = [&](auto f) {
     for (int j = begin + lane; j - lane < end; j += 64) f(j, j >= end ? 0 : j < kHeld ? held[j] : rank_of(w[j], j, n, e));
   };
+  for (int i = tid; i < kCopies * kDigits; i += kSelect) (&histogram[0][0])[i] = 0;
   if (h == 0 && tid == 0) e.lengths_out[b] = m;
   for (int64_t i = m + tid; i < e.budget; i += kSelect) kept[i] = -1;
   for (int i = m + tid; i < e.c.capacity; i += kSelect) out[i] = 0.f;
@@ -130,9 +132,7 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   if (m < n) {
     uint32_t above = 0;
     int need = m;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < kCopies * kDigits; i += kSelect) (&histogram[0][0])[i] = 0;
-      __syncthreads();
+    for (int shift = 24;; shift -= 8) {
       each([&](int j, uint32_t r) {
         const uint32_t digit = r >> shift & 255;
         const bool in = j < end && (shift == 24 || r >> (shift + 8) == above);
@@ -141,31 +141,32 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
       __syncthreads();
       if (wave == 0) {
         // lane l has the digits 4 l .. 4 l + 3; sum of the digits from there up
-        uint32_t c[4], sum = 0;
+        u32x4_t c = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          c[i] = 0;
-#pragma unroll
-          for (int x = 0; x < kCopies; x++) c[i] += histogram[x][4 * lane + i];
-          sum += c[i];
+        for (int x = 0; x < kCopies; x++) {
+          u32x4_t& counted = *reinterpret_cast<u32x4_t*>(&histogram[x][4 * lane]);
+          c += counted, counted = u32x4_t{0, 0, 0, 0};   // for the next pass
         }
-        uint32_t up = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const uint32_t other = __shfl_down(up, d);
-          up += lane + d < 64 ? other : 0;
-        }
-        uint32_t over = up - sum;   // entries of higher digits than this lane's
+        const uint32_t sum = c[0] + c[1] + c[2] + c[3], upto = scan((int)sum);
+        uint32_t over = __builtin_amdgcn_readlane(upto, 63) - upto;   // entries of higher digits than this lane's
+        const uint32_t up = over + sum;
         if (over < (uint32_t)need && up >= (uint32_t)need) {   // one lane alone
           int i = 3;
           while (over + c[i] < (uint32_t)need) over += c[i], i--;
-          found[0] = above << 8 | (4 * lane + i), found[1] = need - over;
+          found[0] = above << 8 | (4 * lane + i), found[1] = need - over, found[2] = c[i] == need - over;
         }
       }
       __syncthreads();
       above = found[0], need = (int)found[1];
+      if (found[2]) {   // all of these digits, and of higher ones
+        rank = above << shift;
+        break;
+      }
+      if (shift == 0) {
+        rank = above, ties = need;
+        break;
+      }
     }
-    rank = above, ties = need;
   }
   int over = 0, same = 0;
   each([&](int j, uint32_t r) {

@@ -102,17 +102,6 @@ template <int DT>
 constexpr int kTile = DT == FHOG_DTYPE_FP32 ? 16 : 32;
 int tile_of(int dtype) { return dtype == FHOG_DTYPE_FP32 ? kTile<FHOG_DTYPE_FP32> : kTile<FHOG_DTYPE_BF16>; }
 
-// Sum over the lanes up to this one, in registers
-__device__ __forceinline__ int scan(int x) {
-  const auto add = [&](auto control, auto mask) { x += __builtin_amdgcn_update_dpp(0, x, control.value, mask.value, 0xf, false); };
-  const auto all = std::integral_constant<int, 0xf>{};
-  add(std::integral_constant<int, 0x111>{}, all), add(std::integral_constant<int, 0x112>{}, all);   // the lanes 1, 2, 4 and 8 before it in its row of 16
-  add(std::integral_constant<int, 0x114>{}, all), add(std::integral_constant<int, 0x118>{}, all);
-  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});                   // the last of the row before, into rows 1 and 3
-  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});                   // lane 31, into rows 2 and 3
-  return x;
-}
-
 // How the tiles of all sequences are dealt out over about t.units workgroups (dealt): a sequence goes to as many as its share of all tiles comes to, rounded, and one at least. So a long
 // sequence among short ones has many, whatever the table has room for. By a wave, lane b of each 64 sequences. Else every sequence has one workgroup.
 template <int TILE>
