@@ -324,8 +324,7 @@ Plan plan_of(const fhog_key_weights_args* a) {
 template <int DT, int D, int NK>
 hipError_t launch_d(const Weigh& w, hipStream_t s) {
   constexpr int BYTES = D * (int)sizeof(typename Type<DT>::T), ROWS = rows_of(BYTES), STAGE = ROWS * BYTES + 256, LDS = kRing * STAGE;
-  const hipError_t e = allow_dynamic_lds<weigh<DT, D, NK>>(LDS);
-  if (e != hipSuccess) return e;
+  static_assert(LDS <= 64 << 10, "what a launch may ask for without further ado");
   hipLaunchKernelGGL((weigh<DT, D, NK>), dim3((unsigned)(w.tiles * w.pieces), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), LDS, s, w);
   if (w.pieces > 1) hipLaunchKernelGGL((add_pieces<128 * NK, ROWS>), dim3((unsigned)((w.n_k + kThreads - 1) / kThreads), (unsigned)w.heads_k, (unsigned)w.batch), dim3(kThreads), 0, s, w);
   return hipGetLastError();
