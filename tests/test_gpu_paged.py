@@ -593,6 +593,21 @@ def test_large_ragged_batches(dtype, B, longest, H, H_k, d):
     assert (one[1] - lse[b:b + 1]).abs().max() <= 1e-4
 
 
+@pytest.mark.parametrize("H", [8, 32])
+def test_a_table_as_wide_as_sequences_may_become(H):
+    """Tiles are dealt out over more workgroups than run at a time where a cache may be that large; a table cut to what is in use gives the same to rounding."""
+    import fhog
+    lengths = [2600 if b % 7 == 1 else 1 if b % 5 == 2 else 300 + 61 * b for b in range(32)]
+    c = Case(torch.bfloat16, 8, 128, 16, lengths, seed=26)
+    q = c.normal(32, H, 1, 128)
+    o, lse = fhog.paged_attention(q, c.cache())
+    _check_attention(c, q, o, lse)
+    wide = fhog.PagedCache(c.keys, c.values, torch.cat([c.table, torch.full((32, 1024 - c.table.shape[1]), -1, dtype=torch.int32, device="cuda")], 1), c.n)
+    o2, lse2 = fhog.paged_attention(q, wide)
+    _check_attention(c, q, o2, lse2)
+    assert (lse2 - lse).abs().max() <= 1e-4
+
+
 @pytest.mark.parametrize("rows", [40, 700])
 def test_a_captured_eviction(rows):
     """Selection and copy in a graph, in one launch and in two; replayed over other weights, lengths and pages."""
