@@ -43,7 +43,7 @@ struct Weigh {
 };
 
 // Pieces into which the stages of a tile of keys go: as few as hold `chunk` each at most, the same number in every kernel
-__device__ __forceinline__ int pieces_of(int steps, const Weigh& w) { return (steps + w.chunk - 1) / w.chunk; }
+__device__ __forceinline__ int pieces_of(int steps, const Weigh& w) { return steps == 0 ? 0 : (steps - 1) / w.chunk + 1; }
 
 // Which queries see a key
 struct Queries {
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
   geo.template stages<ROWS>(k0, KEYS, begin, end);
   const int each = end - begin, steps = w.group * each, pieces = pieces_of(steps, w);
   if (piece >= max(pieces, w.pieces == 1 ? 1 : 0)) return;
-  const int from = piece * w.chunk, to = min(steps, from + w.chunk);
+  const int from = piece * w.chunk, to = from + min(steps - from, w.chunk);
 
   u32x4_t key[NK][STEPS];
   int lo[NK], hi[NK];                              // queries that see this lane's keys
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) add_pieces(Weigh w) {
   w.out[b * w.ob + g * w.oh + j] = sum;
 }
 
-// Pieces at most: a workspace of that many rows like the result's, whatever the length (one head in four of keys, 131072 tokens: 134 MB to 4 heads of keys), and a grid of 2^23 workgroups
+// Pieces at most: a workspace of that many rows like the result's, whatever the length (131072 tokens, 4 heads of keys: 134 MB), and a grid of 2^23 workgroups
 constexpr int64_t kPieces = 64;
 
 // Keys of a workgroup and how the queries of one are cut
