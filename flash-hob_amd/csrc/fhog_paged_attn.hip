@@ -96,6 +96,20 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   typedef T pair __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, pair{(T)lo, (T)hi});
 }
+// Two weights, not negative, cut to the type, and what that leaves of them. The rest of a weight that is not 0 is not 0 either, or infinite values would turn into NaN
+template <int DT>
+__device__ __forceinline__ u32x2_t cut(float lo, float hi) {
+  if constexpr (DT == FHOG_DTYPE_FP16) {
+    const auto first = __builtin_amdgcn_cvt_pkrtz(lo, hi);
+    const auto rest = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)first[0], -1.f, lo), __builtin_fmaf((float)first[1], -1.f, hi));
+    const uint32_t bits = __builtin_bit_cast(uint32_t, first), not0 = (bits + 0x7fff7fffu) >> 15 & 0x00010001u;
+    return u32x2_t{bits, __builtin_bit_cast(uint32_t, rest) | not0};
+  } else {
+    const uint32_t a = __builtin_bit_cast(uint32_t, lo), b = __builtin_bit_cast(uint32_t, hi);
+    const auto left = [](float x, uint32_t bits) { return __builtin_fmaf(x, 1.f + 0x1p-22f, -number(bits & 0xffff0000u)); };
+    return u32x2_t{__builtin_amdgcn_perm(b, a, 0x07060302), pack<DT>(left(lo, a), left(hi, b))};
+  }
+}
 
 // Entries of a tile
 template <int DT>
@@ -349,8 +363,15 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
     } else {
 #pragma unroll
       for (int u = 0; u < SUB; u += 2) {
-        // weights are rounded to the type of the values, which are products' other factor: up to 2^-8 of a weight in bf16 and 2^-11 in fp16, as in attention over whole tensors
-        const u32x4_t weights = {pack<DT>(x[u][0], x[u][1]), pack<DT>(x[u][2], x[u][3]), pack<DT>(x[u + 1][0], x[u + 1][1]), pack<DT>(x[u + 1][2], x[u + 1][3])};
+        // The products' other factor, the values, has 16 bits, so a weight enters in two terms of its type, what it is cut to and what that leaves: off by 2^-15 of a weight in
+        // bf16 and 2^-19 in fp16 (and 2^-24 of the reference's), where one term is by 2^-8 and 2^-11. The matrix pipe has little else to do: us, one
+        // term | two: bf16, d = 128 32 x 16384 291 | 291, 64 x 2048 84.5 | 84.4, d = 32 32 x 8192 56.2 | 56.3; fp16, d = 64, window 700 of 24 x 3001, where its latency shows, 13.9 | 14.5
+        u32x4_t weights, rest;
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          const u32x2_t both = cut<DT>(x[u + y / 2][2 * (y % 2)], x[u + y / 2][2 * (y % 2) + 1]);
+          weights[y] = both[0], rest[y] = both[1];
+        }
 #pragma unroll
         for (int c = 0; c < C; c += 2) {
           const int w = c / 2;   // the word of channels c, c + 1
@@ -360,8 +381,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
             const uint32_t lo = word<VW>(v[u + y / 2][2 * (y % 2)][0], w), hi = word<VW>(v[u + y / 2][2 * (y % 2) + 1][0], w);
             even[y] = __builtin_amdgcn_perm(hi, lo, 0x05040100), odd[y] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
           }
-          acc[c] = mfma16<DT>(even, weights, acc[c]);
-          acc[c + 1] = mfma16<DT>(odd, weights, acc[c + 1]);
+          acc[c] = mfma16<DT>(even, rest, mfma16<DT>(even, weights, acc[c]));
+          acc[c + 1] = mfma16<DT>(odd, rest, mfma16<DT>(odd, weights, acc[c + 1]));
         }
       }
     }

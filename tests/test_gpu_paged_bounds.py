@@ -1,0 +1,42 @@
+"""GPU tier: the calls on a cache in pages held to what the documents promise beyond the formulas: how exact sums are, rows that have no place, workspaces.
+
+Bounds are those of the tests of attention over pages: D = 2^-24 (d + 8) scale |q|.|k| + 2^-21 for a score, E = 2 D + (n + 8) 2^-24 for a weight."""
+import math
+
+import pytest
+import torch
+
+from gpu_util import require_gpu
+from test_gpu_paged import Case
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+NAN = float("nan")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    require_gpu()
+
+
+@pytest.mark.parametrize("dtype, two", [(torch.bfloat16, 2.0 ** -15 + 2.0 ** -22), (torch.float16, 2.0 ** -19)])
+@pytest.mark.parametrize("H, H_k, d, page, lengths", [(4, 2, 128, 64, [700, 33]), (2, 1, 64, 24, [300, 1]), (16, 1, 32, 16, [2000, 5]), (8, 8, 128, 16, [4000, 90])])
+def test_weights_are_not_rounded_to_the_values_type(H, H_k, d, page, lengths, dtype, two):
+    """A weight enters its product with a value in two terms of the type, the second one what the first, cut, leaves: 2^-7 of it in bf16, rounded by 2^-8 of that, and 2^-22; 2^-10 in
+    fp16, cut by 2^-10 of that, and as much again where its last bit is set. fp16: 2^-24 of the largest at least."""
+    import fhog
+    c = Case(dtype, H_k, d, page, lengths, seed=31)
+    q = c.normal(len(lengths), H, 1, d)
+    o = fhog.paged_attention(q, c.cache())[0].cpu().double()
+    h, q64 = torch.finfo(dtype).eps / 2, q.cpu().double()
+    for b, n in enumerate(lengths):
+        for head in range(H):
+            k, v = (t[head // (H // H_k)].double() for t in c.rows[b])
+            x = q64[b, head, 0]
+            p = torch.softmax(d ** -0.5 * (k @ x), 0)
+            D = 2.0 ** -24 * (d + 8) * d ** -0.5 * (k.abs() @ x.abs()) + 2.0 ** -21
+            E = 2 * D.max() + (n + 8) * 2.0 ** -24
+            want = p @ v
+            bound = (two + E + n * 2.0 ** -24) * (p @ v.abs()) + h * want.abs() * 1.01 + (n * 2.0 ** -24 * v.abs().max() if dtype == torch.float16 else 0)
+            err = (o[b, head, 0] - want).abs()
+            assert (err <= bound).all(), (b, head, (err / bound).max().item())
