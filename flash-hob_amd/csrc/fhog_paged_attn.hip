@@ -111,6 +111,11 @@ __device__ __forceinline__ u32x2_t cut(float lo, float hi) {
   }
 }
 
+// What weights of fp16 are multiplied by on their way into the product: with references within 2^4 of the maximum they reach 2^15 there, and the steps of 2^-24 that fp16 has at its lower end
+// are 2^-35 of the largest weight, not 2^-24. Without it many weak entries vanished beside a strong one: of 8192 that each weigh e^-17.4 of it a fourth of their sum.
+template <int DT>
+constexpr float kLift = DT == FHOG_DTYPE_FP16 ? 2048.f : 1.f;
+
 // Entries of a tile
 template <int DT>
 constexpr int kTile = DT == FHOG_DTYPE_FP32 ? 16 : 32;
@@ -174,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
   constexpr bool WIDE = DT == FHOG_DTYPE_FP32;
   typedef typename Type<DT>::T T;
   constexpr int TILE = kTile<DT>, SUB = TILE / 16;     // entries of a tile; 16 at a time
+  constexpr float JUMP = DT == FHOG_DTYPE_FP16 ? 4.f : 8.f;
   constexpr int STEPS = D * (int)sizeof(T) / 64;          // 16-byte pieces of a row that a lane has (four lanes to a row)
   constexpr int C = D / 16;                               // channels of a lane in V and O
   constexpr int VB = C * sizeof(T), VW = VB >= 16 ? 4 : VB / 4, VN = VB >= 16 ? VB / 16 : 1;   // bytes of them, words of a load, loads
@@ -334,9 +340,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
     for (int u = 0; u < SUB; u++) high = fmaxf(fmaxf(high, fmaxf(x[u][0], x[u][1])), fmaxf(x[u][2], x[u][3]));
     high = fmaxf(high, __shfl_xor(high, 16));
     high = fmaxf(high, __shfl_xor(high, 32));
-    // The reference of the exponentials follows the maximum only in jumps of more than 8 (in log2 units): weights may then reach 2^8, which costs no precision,
+    // The reference of the exponentials follows the maximum only in jumps of more than 8 (in log2 units; fp16: kLift): weights may then reach 2^8, which costs no precision,
     // and the sums are scaled again only now and then
-    const float next = high > top + 8.f ? high : top;
+    const float next = high > top + JUMP ? high : top;
     const float ref = next == -INFINITY ? 0.f : next;   // a column that has seen nothing yet
     if (__builtin_amdgcn_ballot_w64(next > top) != 0) {
       const float by = __builtin_amdgcn_exp2f(top - ref);
@@ -364,12 +370,12 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
 #pragma unroll
       for (int u = 0; u < SUB; u += 2) {
         // The products' other factor, the values, has 16 bits, so a weight enters in two terms of its type, what it is cut to and what that leaves: off by 2^-15 of a weight in
-        // bf16 and 2^-19 in fp16 (and 2^-24 of the reference's), where one term is by 2^-8 and 2^-11. The matrix pipe has little else to do: us, one
+        // bf16 and 2^-19 in fp16 (and 2^-35 of the largest), where one term is by 2^-8 and 2^-11. The matrix pipe has little else to do: us, one
         // term | two: bf16, d = 128 32 x 16384 291 | 291, 64 x 2048 84.5 | 84.4, d = 32 32 x 8192 56.2 | 56.3; fp16, d = 64, window 700 of 24 x 3001, where its latency shows, 13.9 | 14.5
         u32x4_t weights, rest;
 #pragma unroll
         for (int y = 0; y < 4; y++) {
-          const u32x2_t both = cut<DT>(x[u + y / 2][2 * (y % 2)], x[u + y / 2][2 * (y % 2) + 1]);
+          const u32x2_t both = cut<DT>(x[u + y / 2][2 * (y % 2)] * kLift<DT>, x[u + y / 2][2 * (y % 2) + 1] * kLift<DT>);
           weights[y] = both[0], rest[y] = both[1];
         }
 #pragma unroll
@@ -402,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend(Token t) {
 #pragma unroll
   for (int c = 0; c < C; c++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) rows[wave][m][C * (4 * quarter + r) + c] = acc[c][r] * by;
+    for (int r = 0; r < 4; r++) rows[wave][m][C * (4 * quarter + r) + c] = acc[c][r] * (by / kLift<DT>);
   __syncthreads();
   for (int at = tid * 4; at < kColumns * D; at += kThreads * 4) {
     const int h = at / D, c = at % D;

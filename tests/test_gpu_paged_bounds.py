@@ -40,3 +40,29 @@ def test_weights_are_not_rounded_to_the_values_type(H, H_k, d, page, lengths, dt
             bound = (two + E + n * 2.0 ** -24) * (p @ v.abs()) + h * want.abs() * 1.01 + (n * 2.0 ** -24 * v.abs().max() if dtype == torch.float16 else 0)
             err = (o[b, head, 0] - want).abs()
             assert (err <= bound).all(), (b, head, (err / bound).max().item())
+
+
+@pytest.mark.parametrize("gap", [10.0, 16.0, 17.2, 17.4, 20.0])
+@pytest.mark.parametrize("dtype, two", [(torch.bfloat16, 2.0 ** -15 + 2.0 ** -22), (torch.float16, 2.0 ** -19), (torch.float32, 0.0)])
+@pytest.mark.parametrize("n, where", [(8192, 0), (8192, 5000), (40000, 39999), (200, 3)])
+def test_weak_entries_beside_a_strong_one(n, where, dtype, two, gap):
+    """One entry of value 0 that outweighs each of the others by e^gap: O is what the others' values come to, all of them together. As above; in fp16 the smallest step is 2^-35 of the
+    largest weight, in two terms half of it and one more."""
+    import fhog
+    d, page = 64, 64
+    pages = -(-n // page)
+    q = torch.zeros(1, 1, 1, d, dtype=dtype)
+    q[..., 0], q[..., 1] = 8.0, 1.0
+    keys = torch.zeros(pages * page, d, dtype=dtype)
+    keys[where, 0], keys[:, 1] = gap, (torch.arange(pages * page) % 7).to(dtype) / 8      # scores gap and 0, and a little of their own
+    values = (1 + (torch.arange(pages * page)[:, None] * 3 + torch.arange(d)) % 5 / 4).to(dtype)
+    values[where] = 0
+    cache = fhog.PagedCache(*(t.view(pages, 1, page, d).cuda() for t in (keys, values)), torch.arange(pages, dtype=torch.int32).cuda()[None], torch.tensor([n], dtype=torch.int32).cuda())
+    o = fhog.paged_attention(q.cuda(), cache)[0][0, 0, 0].cpu().double()
+    k, v, x = keys[:n].double(), values[:n].double(), q[0, 0, 0].double()
+    p = torch.softmax(d ** -0.5 * (k @ x), 0)
+    E = 2 * (2.0 ** -24 * (d + 8) * d ** -0.5 * (k.abs() @ x.abs()).max() + 2.0 ** -21) + (n + 8) * 2.0 ** -24
+    want, h = p @ v, torch.finfo(dtype).eps / 2
+    # below its normal numbers fp16 has steps of 2^-24, O too
+    bound = (two + E + n * 2.0 ** -24) * (p @ v.abs()) + h * want.abs() * 1.01 + ((1.5 * n * 2.0 ** -35 * v.abs().max() + 2.0 ** -25) if dtype == torch.float16 else 0)
+    assert ((o - want).abs() <= bound).all(), ((o - want).abs() / bound).max().item()
