@@ -34,11 +34,13 @@ __global__ void __launch_bounds__(kThreads) append_entries(Append a) {
   uint32_t row = a.tokens(rest);
   const int t = (int)(rest - row * a.tokens.by);
   const uint32_t b = a.heads(row), h = row - b * a.heads.by;
-  const int n = a.c.length(b), count = min(a.counts ? max(0, a.counts[b]) : (int)a.tokens.by, min((int)a.tokens.by, n));
+  const int n = max(0, a.c.lengths[b]), count = min(a.counts ? max(0, a.counts[b]) : (int)a.tokens.by, min((int)a.tokens.by, n));
   if (t >= count) return;
+  const uint32_t j = n - count + t;
+  if (j >= (uint32_t)a.c.capacity) return;   // a length beyond the table: what has no place is dropped, and the entries that the table has room for stay
   const u32x4_t k = *reinterpret_cast<const u32x4_t*>(a.k + b * a.kb + h * a.kh + t * a.kn + chunk * 16);
   const u32x4_t v = *reinterpret_cast<const u32x4_t*>(a.v + b * a.vb + h * a.vh + t * a.vn + chunk * 16);
-  const uint32_t j = n - count + t, at = a.c.page(j);
+  const uint32_t at = a.c.page(j);
   const int32_t page = a.c.table[b * a.c.stride_tb + at];
   if ((uint32_t)page >= (uint32_t)a.c.pages) return;
   const int64_t to = page * a.c.stride_p + h * a.c.stride_h + (j - at * a.c.page.by) * a.c.stride_n + chunk * 16;

@@ -103,6 +103,8 @@ def paged_append(cache: PagedCache, k, v, *, counts=None) -> None:
         k, v: (B, H_k, N, d), the dtype of the cache, any strides. A token each, or prompts.
         counts: (B,) int32, how many of the N tokens sequence b has, the first ones; the others are padding. None: all. A sequence never gets more entries than it is long.
 
+    Tokens that the table has no room for (a length beyond ``P * page``) are dropped, and the entries before them stay as they were.
+
     Sequences that share pages must not both write to the same entry of one, and ``k`` and ``v`` must not lie where entries are written.
     """
     if not isinstance(cache, PagedCache):

@@ -350,8 +350,8 @@ typedef struct fhog_paged_cache {
   int32_t dtype;          /* FHOG_DTYPE_* */
 } fhog_paged_cache;
 
-/* New entries: the last counts[b] of each sequence (cut to 0 .. n and to the sequence's length) are written from the first rows of k and v. Two sequences that
-   share a page must not both have new entries in the same slot, and k and v must not lie in the pages that are written. */
+/* New entries: the last counts[b] of each sequence (cut to 0 .. n and to lengths[b]) are written from the first rows of k and v. Here lengths[b] is taken as it is, also beyond
+   table_width * page: rows whose entries the table has no room for are dropped, the entries before them are left as they were. Two sequences that share a page must not both have new entries in the same slot, and k and v must not lie in the pages that are written. */
 typedef struct fhog_paged_append_args {
   fhog_paged_cache cache;
   const void* k;         /* (batch, heads_k, n, d) */

@@ -66,3 +66,26 @@ def test_weak_entries_beside_a_strong_one(n, where, dtype, two, gap):
     # below its normal numbers fp16 has steps of 2^-24, O too
     bound = (two + E + n * 2.0 ** -24) * (p @ v.abs()) + h * want.abs() * 1.01 + ((1.5 * n * 2.0 ** -35 * v.abs().max() + 2.0 ** -25) if dtype == torch.float16 else 0)
     assert ((o - want).abs() <= bound).all(), ((o - want).abs() / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page, N, lengths, counts", [(16, 1, [48, 49, 47, 2 ** 31 - 1], None), (16, 10, [48, 51, 58, 1000], None), (24, 30, [49, 72, 73, 90], [10, 1, 30, 18]),
+                                                      (1, 4, [4, 5, 6, 8], None), (100, 300, [300, 301, 4, 599], [300, 300, 0, 300])])
+def test_append_beyond_the_table(dtype, page, N, lengths, counts):
+    """What the table has no room for is dropped; no entry that was there is written over."""
+    import fhog
+    P = {16: 3, 24: 3, 1: 5, 100: 3}[page]
+    c = Case(dtype, 2, 64, page, [P * page] * len(lengths), seed=32)
+    k, v = c.normal(len(lengths), 2, N, 64), c.normal(len(lengths), 2, N, 64)
+    want = [t.clone() for t in (c.keys, c.values)]
+    for b, n in enumerate(lengths):
+        m = min(N if counts is None else counts[b], N, n)
+        for t in range(m):
+            j = n - m + t
+            if j < P * page:
+                for pool, new in zip(want, (k, v)):
+                    pool[int(c.table[b, j // page]), :, j % page] = new[b, :, t]
+    c.n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    fhog.paged_append(c.cache(), k, v, counts=None if counts is None else torch.tensor(counts, dtype=torch.int32).cuda())
+    for got, w in zip((c.keys, c.values), want):
+        assert torch.equal(got.view(torch.uint8), w.view(torch.uint8))
