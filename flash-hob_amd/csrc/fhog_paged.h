@@ -67,6 +67,15 @@ struct Seen {
     tiles = all - skip;
   }
   __device__ __forceinline__ int at(int i) const { return (i < first ? i : i + skip) * T; }
+  // Where an entry that is seen comes among those of these tiles
+  __device__ __forceinline__ int place(int j) const { return j < first * T ? j : j - skip * T; }
+  // Tiles at most, whatever the length: the window's begin and end inside a tile
+  __host__ __device__ static int64_t most(int64_t capacity, int64_t window, int64_t sinks) {
+    const int64_t all = (capacity + T - 1) / T;
+    if (window <= 0 || window >= capacity) return all;
+    const int64_t sunk = sinks < capacity ? sinks : capacity, some = (sunk + T - 1) / T + (window + T - 2) / T + 1;
+    return some < all ? some : all;
+  }
   __device__ __forceinline__ bool sees(int j) const { return j < n && (j >= lo || j < sinks); }
   __device__ __forceinline__ bool whole(int j0) const { return j0 + T <= n && (j0 >= lo || j0 + T <= sinks); }
 };

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from gpu_util import require_gpu
-from test_gpu_paged import Case
+from test_gpu_paged import Case, _check_attention
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -89,3 +89,20 @@ def test_append_beyond_the_table(dtype, page, N, lengths, counts):
     fhog.paged_append(c.cache(), k, v, counts=None if counts is None else torch.tensor(counts, dtype=torch.int32).cuda())
     for got, w in zip((c.keys, c.values), want):
         assert torch.equal(got.view(torch.uint8), w.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H, H_k, d, page, lengths, window, sinks", [
+    (8, 2, 64, 16, [3000, 1, 700, 33, 0, 705, 2999], 700, 4), (4, 4, 128, 24, [2500, 90, 64, 65], 33, 100), (34, 2, 64, 16, [2000, 40], 1, 0), (2, 1, 128, 32, [1500, 1000], 64, 64),
+    (2, 1, 32, 1, [300, 31], 32, 33), (16, 1, 128, 64, [4000, 2100], 2047, 31), (6, 3, 64, 100, [1999, 1000], 1000, 1999), (2, 2, 128, 256, [16000, 50], 8000, 65)])
+def test_weights_under_a_window_of_a_wide_table(H, H_k, d, page, lengths, window, sinks, dtype):
+    """Scores are kept for the entries that are seen, wherever window and sinks begin and end in tiles; tables as wide as the longest sequence, and far wider."""
+    import fhog
+    for width in (None, 4 * -(-max(lengths) // page)):
+        c = Case(dtype, H_k, d, page, lengths, seed=33, width=width)
+        q = c.normal(len(lengths), H, 1, d)
+        w = torch.rand(len(lengths), H_k, c.table.shape[1] * page, generator=c.g).cuda()
+        o, lse, new = fhog.paged_attention(q, c.cache(), window=window, sinks=sinks, weights=w)
+        plain = fhog.paged_attention(q, c.cache(), window=window, sinks=sinks)
+        assert torch.equal(plain[0], o) and torch.equal(plain[1], lse)
+        _check_attention(c, q, o, lse, window=window, sinks=sinks, weights=w, new=new)
