@@ -114,23 +114,29 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   __shared__ int counts[2][kWaves];           // entries of a wave's stretch above the rank, and of the rank itself
   const int b = blockIdx.x / e.c.heads_k, h = blockIdx.x - b * e.c.heads_k, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = e.c.length(b), m = (int)min((int64_t)n, e.budget);
+  // The first wave says how many entries there are, behind the barrier that there is in any case: lengths that someone changes meanwhile make wrong results, but no waves that disagree at a barrier
+  __shared__ int entries;
   const float* const w = e.weights + b * e.wb + h * e.wh;
   int32_t* const kept = e.kept + (int64_t)blockIdx.x * e.budget;
   float* const out = e.weights_out + (int64_t)blockIdx.x * e.c.capacity;
+  {
+    const int n = e.c.length(b);
+    if (tid == 0) entries = n;
+    for (int j = tid; j < min(n, kHeld); j += kSelect) held[j] = rank_of(w[j], j, n, e);
+  }
+  for (int i = tid; i < kCopies * kDigits; i += kSelect) (&histogram[0][0])[i] = 0;
+  __syncthreads();
+  const int n = __builtin_amdgcn_readfirstlane(entries), m = (int)min((int64_t)n, e.budget);
   const int stretch = ((n + kWaves - 1) / kWaves + 63) & ~63, begin = min(n, wave * stretch), end = min(n, begin + stretch);
-  for (int j = tid; j < min(n, kHeld); j += kSelect) held[j] = rank_of(w[j], j, n, e);
   // f(j, rank) for the wave's entries in order, 64 at a time; all lanes take part
   const auto each = [&](auto f) {
     for (int j = begin + lane; j - lane < end; j += 64) f(j, j >= end ? 0 : j < kHeld ? held[j] : rank_of(w[j], j, n, e));
   };
-  for (int i = tid; i < kCopies * kDigits; i += kSelect) (&histogram[0][0])[i] = 0;
   if (h == 0 && tid == 0) e.lengths_out[b] = m;
   for (int64_t i = m + tid; i < e.budget; i += kSelect) kept[i] = -1;
   for (int i = m + tid; i < e.c.capacity; i += kSelect) out[i] = 0.f;
   uint32_t rank = 0;
   int ties = n;
-  __syncthreads();
   if (m < n) {
     uint32_t above = 0;
     int need = m;

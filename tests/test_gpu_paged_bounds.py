@@ -106,3 +106,27 @@ def test_weights_under_a_window_of_a_wide_table(H, H_k, d, page, lengths, window
         plain = fhog.paged_attention(q, c.cache(), window=window, sinks=sinks)
         assert torch.equal(plain[0], o) and torch.equal(plain[1], lse)
         _check_attention(c, q, o, lse, window=window, sinks=sinks, weights=w, new=new)
+
+
+@pytest.mark.parametrize("budget", [40, 1500])
+def test_an_eviction_whose_lengths_change_meanwhile_ends(budget):
+    """Its waves go by one number of entries, whichever it is. What comes out then is anyone's guess; calls before and after are right."""
+    import fhog
+    c = Case(torch.bfloat16, 2, 64, 16, [3000, 2000, 900], seed=34, spare=300)
+    free = [p for p in range(c.keys.shape[0]) if p not in c.table.flatten().tolist()]
+    into = torch.tensor([free[i * 95:(i + 1) * 95] for i in range(3)], dtype=torch.int32).cuda()
+    w = torch.rand(3, 2, c.table.shape[1] * 16, device="cuda")
+    want = fhog.paged_evict(c.cache(), w, budget, into)
+    before = c.n.clone()
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for i in range(20):
+        with torch.cuda.stream(streams[0]):
+            for n in (0, 17, 3000, 30):
+                c.n.fill_(n)
+        with torch.cuda.stream(streams[1]):
+            fhog.paged_evict(c.cache(), w, budget, into)
+    torch.cuda.synchronize()
+    c.n.copy_(before)
+    got = fhog.paged_evict(c.cache(), w, budget, into)
+    assert all(torch.equal(a, b) for a, b in zip((got[0].lengths, *got[1:]), (want[0].lengths, *want[1:])))
