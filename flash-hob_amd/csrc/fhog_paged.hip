@@ -67,13 +67,17 @@ constexpr int kSelect = 1024, kWaves = kSelect / 64, kHeld = 12288;   // kHeld: 
 constexpr int kCopies = 8, kDigits = 264;   // of the histogram; copies lie eight banks apart
 constexpr int kRowsEach = 2;   // chunks of keys and values that a thread moves
 
-// A number for each entry that grows with the order in which entries stay: what is protected first, then by weight, NaN last
+// A number for each entry that grows with the order in which entries stay: what is protected first, then by weight, NaN last; 0 is for those that are not there
 __device__ __forceinline__ uint32_t rank_of(float w, int j, int n, const Evict& e) {
   if (j < e.sinks || j >= n - e.recent) return 0xffffffffu;
-  if (w != w) return 0;
+  if (w != w) return 1;
   const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.f);   // -0 becomes 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+
+// Whether a number in a table names a page
+__device__ __forceinline__ bool names(int32_t page, const Cache& c) { return (uint32_t)page < (uint32_t)c.pages; }
+__device__ __forceinline__ int pages_of(int n, const Cache& c) { return n > 0 ? (int)c.page(n - 1) + 1 : 0; }
 
 // Rows that stay, to their new places: the chunks of 16 bytes `id` and, kRowsEach - 1 times more, `step` further on, of the keys and values of m rows
 __device__ __forceinline__ void move_chunks(const Evict& e, int b, int h, const int32_t* kept, int m, uint32_t id, uint32_t step) {
@@ -85,10 +89,10 @@ __device__ __forceinline__ void move_chunks(const Evict& e, int b, int h, const 
     const uint32_t i = e.chunks(id), chunk = id - i * e.chunks.by;
     if (i >= (uint32_t)m) continue;
     const uint32_t j = kept[i];
-    if (j >= (uint32_t)e.c.capacity) continue;   // lengths that someone has changed meanwhile
+    if (j >= (uint32_t)e.c.capacity) continue;   // -1, or lengths that someone has changed meanwhile
     const uint32_t at = e.c.page(j), to = e.c.page(i);
     const int32_t from_page = e.c.table[b * e.c.stride_tb + at], to_page = e.into[b * e.ib + to];
-    if ((uint32_t)from_page >= (uint32_t)e.c.pages || (uint32_t)to_page >= (uint32_t)e.c.pages) continue;
+    if (!names(from_page, e.c) || !names(to_page, e.c)) continue;
     const int64_t inside = h * e.c.stride_h + chunk * 16;
     const int64_t src = from_page * e.c.stride_p + (j - at * e.c.page.by) * e.c.stride_n + inside;
     dst[u] = to_page * e.c.stride_p + (i - to * e.c.page.by) * e.c.stride_n + inside;
@@ -105,45 +109,84 @@ __device__ __forceinline__ void move_chunks(const Evict& e, int b, int h, const 
 // What bounds it: the waits between its passes. us, 32 x 8 slices of 8192 | 4 x 4 of 1000: weights read anew in every pass 26.6 | 7.4, ranks formed once and kept in registers
 // 20.2 | 10.8, in LDS 22.7 | 7.6, and there with a histogram of eight copies 19.8 | 7.7. The wave that sums a histogram clears it for the next pass, and digits that stay all together end the
 // search: the whole call 230.6 -> 228.8 | 11.4 -> 10.0.
+// Entries whose page is none are not there: they do not stay. Places whose page in `into` is none are passed over: there `kept` names entries that are not there, as far as there are any, so that
+// an entry of nothing never comes to lie in a page that is read. The tables are looked at page by page beside the first pass, and entry by entry only where a page is missing: 0.3 us
+// of 10 (4 x 4 of 1000), none of 228.
 // MOVE: and are moved by the same workgroup.
 template <bool MOVE>
 __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
   extern __shared__ uint32_t held[];
   __shared__ __attribute__((aligned(16))) uint32_t histogram[kCopies][kDigits];   // a lane counts in copy lane % kCopies: the same digit of many lanes is not one address
   __shared__ uint32_t found[3];               // digits so far; how many of the entries of these digits stay, and whether all do
-  __shared__ int counts[2][kWaves];           // entries of a wave's stretch above the rank, and of the rank itself
+  __shared__ int counts[3][kWaves];           // entries of a wave's stretch above the rank, of the rank itself, and those that are not there
   const int b = blockIdx.x / e.c.heads_k, h = blockIdx.x - b * e.c.heads_k, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ int with[3 * kWaves];            // by wave: whether pages lack; entries that are there, and places
   // The first wave says how many entries there are, behind the barrier that there is in any case: lengths that someone changes meanwhile make wrong results, but no waves that disagree at a barrier
   __shared__ int entries;
   const float* const w = e.weights + b * e.wb + h * e.wh;
+  const int32_t* const table = e.c.table + b * e.c.stride_tb;
+  const int32_t* const into = e.into + b * e.ib;
   int32_t* const kept = e.kept + (int64_t)blockIdx.x * e.budget;
   float* const out = e.weights_out + (int64_t)blockIdx.x * e.c.capacity;
+  const int32_t first_into = tid < pages_of(e.rows, e.c) ? into[tid] : 0;   // pages of the tables are asked for ahead of the weights, and looked at behind them
   {
     const int n = e.c.length(b);
     if (tid == 0) entries = n;
+    const int32_t first = tid < pages_of(n, e.c) ? table[tid] : 0;
     for (int j = tid; j < min(n, kHeld); j += kSelect) held[j] = rank_of(w[j], j, n, e);
+    const auto lacks = [&](const int32_t* pages, int32_t first, int n) {   // a page of n entries, in this wave's share
+      bool none = !names(first, e.c);
+      for (int i = tid + kSelect; i < pages_of(n, e.c); i += kSelect) none = none || !names(pages[i], e.c);
+      return __builtin_amdgcn_ballot_w64(none) != 0;
+    };
+    const int lack = (lacks(table, first, n) ? 1 : 0) | (lacks(into, first_into, e.rows) ? 2 : 0);
+    if (lane == 0) with[wave] = lack;
   }
   for (int i = tid; i < kCopies * kDigits; i += kSelect) (&histogram[0][0])[i] = 0;
   __syncthreads();
-  const int n = __builtin_amdgcn_readfirstlane(entries), m = (int)min((int64_t)n, e.budget);
+  const int n = __builtin_amdgcn_readfirstlane(entries), lack = with[lane % kWaves];
+  const bool gaps = __builtin_amdgcn_ballot_w64(lack & 1) != 0, closed = __builtin_amdgcn_ballot_w64(lack & 2) != 0;
+  int here = n, open = e.rows;   // entries that are there, and places
+  if (gaps || closed) {
+    const auto share = [&](const int32_t* pages, int n) {
+      int sum = 0;
+      for (int i = tid; i < pages_of(n, e.c); i += kSelect)
+        if (names(pages[i], e.c)) sum += min((int)e.c.page.by, n - i * (int)e.c.page.by);
+      return scan(sum);
+    };
+    const int some_here = share(table, n), some_open = share(into, e.rows);
+    if (lane == 63) with[kWaves + wave] = some_here, with[2 * kWaves + wave] = some_open;
+    if (gaps)
+      for (int j = tid; j < min(n, kHeld); j += kSelect)
+        if (!names(table[e.c.page(j)], e.c)) held[j] = 0;
+    __syncthreads();
+    const int upto = scan(lane < 2 * kWaves ? with[kWaves + lane] : 0);
+    here = __builtin_amdgcn_readlane(upto, kWaves - 1), open = __builtin_amdgcn_readlane(upto, 2 * kWaves - 1) - here;
+  }
+  const int m = min(here, open);
   const int stretch = ((n + kWaves - 1) / kWaves + 63) & ~63, begin = min(n, wave * stretch), end = min(n, begin + stretch);
   // f(j, rank) for the wave's entries in order, 64 at a time; all lanes take part
   const auto each = [&](auto f) {
-    for (int j = begin + lane; j - lane < end; j += 64) f(j, j >= end ? 0 : j < kHeld ? held[j] : rank_of(w[j], j, n, e));
+    int j = begin + lane;
+    for (; j - lane < min(end, kHeld); j += 64) f(j, j < end ? held[j] : 0);
+    for (; j - lane < end; j += 64) f(j, j >= end || (gaps && !names(table[e.c.page(j)], e.c)) ? 0 : rank_of(w[j], j, n, e));
   };
-  if (h == 0 && tid == 0) e.lengths_out[b] = m;
-  for (int64_t i = m + tid; i < e.budget; i += kSelect) kept[i] = -1;
-  for (int i = m + tid; i < e.c.capacity; i += kSelect) out[i] = 0.f;
+  if (!closed) {
+    if (h == 0 && tid == 0) e.lengths_out[b] = m;
+    for (int64_t i = m + tid; i < e.budget; i += kSelect) kept[i] = -1;
+    for (int i = m + tid; i < e.c.capacity; i += kSelect) out[i] = 0.f;
+  }
   uint32_t rank = 0;
-  int ties = n;
-  if (m < n) {
+  int ties = 0;
+  if (0 < m && m < here) {
+    ties = n;
     uint32_t above = 0;
     int need = m;
     for (int shift = 24;; shift -= 8) {
       each([&](int j, uint32_t r) {
         const uint32_t digit = r >> shift & 255;
-        const bool in = j < end && (shift == 24 || r >> (shift + 8) == above);
+        const bool in = r != 0 && (shift == 24 || r >> (shift + 8) == above);
         if (in) atomicAdd(&histogram[lane % kCopies][digit], 1u);
       });
       __syncthreads();
@@ -176,31 +219,72 @@ __global__ void __launch_bounds__(kSelect) select_entries(Evict e) {
       }
     }
   }
-  int over = 0, same = 0;
+  int over = 0, same = 0, gone = 0;
   each([&](int j, uint32_t r) {
     over += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j < end && r > rank));
     same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j < end && r == rank));
+    if (closed) gone += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j < end && r == 0));
   });
-  if (lane == 0) counts[0][wave] = over, counts[1][wave] = same;
+  if (lane == 0) counts[0][wave] = over, counts[1][wave] = same, counts[2][wave] = gone;
   __syncthreads();
-  over = same = 0;
-  for (int i = 0; i < wave; i++) over += counts[0][i], same += counts[1][i];
+  over = same = gone = 0;
+  for (int i = 0; i < wave; i++) over += counts[0][i], same += counts[1][i], gone += counts[2][i];
   const uint64_t below = ((uint64_t)1 << lane) - 1;
+  const auto list = [&](int i, int j) { out[i] = __builtin_bit_cast(float, j); };   // closed: what stays in order, and behind it what is not there, until places are dealt out
+  const auto listed = [&](int i) { return __builtin_bit_cast(int, out[i]); };
   each([&](int j, uint32_t r) {
     const uint64_t o = __builtin_amdgcn_ballot_w64(j < end && r > rank), s = __builtin_amdgcn_ballot_w64(j < end && r == rank);
     const int same_before = same + __builtin_popcountll(s & below), at = over + __builtin_popcountll(o & below) + min(same_before, ties);
-    if (j < end && at < m && (r > rank || (r == rank && same_before < ties))) kept[at] = j, out[at] = w[j];   // at >= m: of lengths that someone has changed meanwhile
+    if (j < end && at < m && (r > rank || (r == rank && same_before < ties))) {   // at >= m: of lengths that someone has changed meanwhile
+      if (closed) list(at, j);
+      else kept[at] = j, out[at] = w[j];
+    }
     over += __builtin_popcountll(o), same += __builtin_popcountll(s);
+    if (closed) {
+      const uint64_t g = __builtin_amdgcn_ballot_w64(j < end && r == 0);
+      const int to = here + gone + __builtin_popcountll(g & below);
+      if (j < end && r == 0 && to < n) list(to, j);
+      gone += __builtin_popcountll(g);
+    }
   });
+  int length = m;
+  if (closed) {
+    const int part = ((e.rows + kWaves - 1) / kWaves + 63) & ~63, first = min(e.rows, wave * part), last = min(e.rows, first + part);
+    const auto open_at = [&](int i) { return i < last && names(into[e.c.page(i)], e.c); };
+    int before = 0;   // open places
+    for (int i = first + lane; i - lane < last; i += 64) before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(open_at(i)));
+    __syncthreads();   // the list is there, and the counts have been read
+    if (lane == 0) counts[0][wave] = before;
+    if (tid == 0) entries = 0;
+    __syncthreads();
+    before = 0;
+    for (int i = 0; i < wave; i++) before += counts[0][i];
+    for (int i = first + lane; i - lane < last; i += 64) {
+      const bool is = open_at(i);
+      const uint64_t o = __builtin_amdgcn_ballot_w64(is);
+      const int k = before + __builtin_popcountll(o & below);   // open places in front of it; i - k closed ones
+      if (i < last) kept[i] = k >= m ? -1 : is ? listed(k) : i - k < n - here ? listed(here + i - k) : -1;
+      if (is && k == m - 1) entries = i + 1;
+      before += __builtin_popcountll(o);
+    }
+    for (int64_t i = e.rows + tid; i < e.budget; i += kSelect) kept[i] = -1;
+    __syncthreads();   // the list has been read
+    length = entries;
+    if (h == 0 && tid == 0) e.lengths_out[b] = length;
+    for (int i = tid; i < e.c.capacity; i += kSelect) {
+      const int j = i < length && names(into[e.c.page(i)], e.c) ? kept[i] : -1;
+      out[i] = (uint32_t)j < (uint32_t)n ? w[j] : 0.f;
+    }
+  }
   if constexpr (MOVE) {
     __syncthreads();   // all of `kept` is there
-    for (uint32_t id = tid; id < (uint32_t)m * e.chunks.by; id += kRowsEach * kSelect) move_chunks(e, b, h, kept, m, id, kSelect);
+    for (uint32_t id = tid; id < (uint32_t)length * e.chunks.by; id += kRowsEach * kSelect) move_chunks(e, b, h, kept, length, id, kSelect);
   }
 }
 
 __global__ void __launch_bounds__(kThreads) move_entries(Evict e) {
   const int b = blockIdx.y / e.c.heads_k, h = blockIdx.y - b * e.c.heads_k;
-  move_chunks(e, b, h, e.kept + (int64_t)blockIdx.y * e.budget, min(e.c.length(b), e.rows), blockIdx.x * kRowsEach * kThreads + threadIdx.x, kThreads);
+  move_chunks(e, b, h, e.kept + (int64_t)blockIdx.y * e.budget, e.rows, blockIdx.x * kRowsEach * kThreads + threadIdx.x, kThreads);
 }
 
 uint32_t row_chunks(const fhog_paged_cache& c) { return (uint32_t)(c.d * (c.dtype == FHOG_DTYPE_FP32 ? 4 : 2) / 16); }

@@ -223,13 +223,17 @@ def paged_evict(cache: PagedCache, weights, budget: int, into, *, sinks: int = 0
     What stays is copied to the pages that ``into`` names, (B, P') int32 with room for it, which no sequence may be reading: neither the cache's own pages nor each other's.
     The cache's pages stay as they are, so that pages which sequences share can be read on, and can be handed out again afterwards.
 
+    Entries whose number in the table is no page are not there and never stay (``sinks`` and ``recent`` count from the ends of the sequence all the same); what stays closes up, so that the new lengths
+    count entries that are there. Places whose number in ``into`` is no page are passed over.
+
     Args:
         weights: (B, H_k, P * page) fp32, as :func:`paged_attention` adds them up.
         budget: entries that may stay, 1 or more, at least ``sinks + recent``.
 
     Returns:
         ``(left, weights, kept)``: the :class:`PagedCache` of what stayed (keys and values the same tensors, table ``into``, new lengths); its weights, shaped like
-        ``weights``, 0 behind the last entry; and (B, H_k, budget) int32, where in the cache each entry came from, -1 behind the last one.
+        ``weights``, 0 where there is no entry; and (B, H_k, budget) int32, where in the cache each entry came from, -1 behind the last one (at places that are passed over: entries that are
+        not there, as far as there are any, else -1).
     """
     if not isinstance(cache, PagedCache):
         _check_cache(cache)

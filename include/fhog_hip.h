@@ -415,10 +415,12 @@ int fhog_key_weights_validate(const fhog_key_weights_args* args); /* host-only; 
 size_t fhog_key_weights_workspace_bytes(const fhog_key_weights_args* args); /* 0 also if the arguments are not valid; host-only */
 int fhog_key_weights(const fhog_key_weights_args* args, void* hip_stream);
 
-/* Eviction, for each sequence and head of keys: of n = lengths[b] entries m = min(n, budget) stay: the first `sinks`, the last `recent`, and of the others those of the
-   largest weights, the lower index first among equal ones (0 and -0 are equal, a NaN ranks below every number). They are written, in their order, to the
-   entries 0 .. m - 1 of the pages that `into` names, which no sequence may be reading; the pages that they come from are not changed.
-   lengths_out[b] = m; kept[b][g][i] is where entry i came from, -1 from m on; weights_out holds the weights of what stayed, 0 from m on. */
+/* Eviction, for each sequence and head of keys: of the n entries that are there m stay, which is n or, if that is less, the number of places for them: the first `sinks`, the last
+   `recent`, and of the others those of the largest weights, the lower index first among equal ones (0 and -0 are equal, a NaN ranks below every number). They are written, in their order, to the
+   places 0, 1, .. of the pages that `into` names, which no sequence may be reading; the pages that they come from are not changed.
+   Entries whose number in the table is no page are not there: they do not stay, wherever they are. There are min(budget, table_width * page) places, less those whose number in `into` is no page,
+   which are passed over. lengths_out[b] is the last place of an entry and one more (m, if no place is passed over); kept[b][g][i] is where the entry of place i came from, -1 behind the last one; at places
+   that are passed over it names the entries that are not there, in their order, and -1 once there are no more. weights_out holds the weights of what stayed, 0 at other places. */
 typedef struct fhog_paged_evict_args {
   fhog_paged_cache cache;
   const float* weights;  /* (batch, heads_k, table_width * page), last dimension contiguous */

@@ -130,3 +130,86 @@ def test_an_eviction_whose_lengths_change_meanwhile_ends(budget):
     c.n.copy_(before)
     got = fhog.paged_evict(c.cache(), w, budget, into)
     assert all(torch.equal(a, b) for a, b in zip((got[0].lengths, *got[1:]), (want[0].lengths, *want[1:])))
+
+
+def _check_evict(c, w, budget, sinks, recent, bad, bad_into, seed):
+    """bad: (sequence, page of its table) that is none; bad_into: (sequence, page of `into`). Attention over what is left, and one more eviction of that."""
+    import fhog
+    B, page, H_k = len(c.lengths), c.page, c.H_k
+    C = c.table.shape[1] * page
+    rows = min(budget, C)
+    P = -(-rows // page)
+    for i, (b, x) in enumerate(bad):
+        c.table[b, x] = [-1, 10 ** 9, -2 ** 31][i % 3]
+    first = c.keys.shape[0]
+    junk = torch.randn(B * P, *c.keys.shape[1:], generator=torch.Generator().manual_seed(seed)).to(c.dtype).cuda()     # what others left in the pages of `into`
+    keys, values = torch.cat([c.keys, junk]), torch.cat([c.values, -junk])
+    into = (first + torch.randperm(B * P, generator=c.g)).int().view(B, P).cuda()
+    for i, (b, x) in enumerate(bad_into):
+        into[b, x] = [keys.shape[0], -1][i % 2]
+    want = [keys.clone(), values.clone()]
+    left, new, kept = fhog.paged_evict(fhog.PagedCache(keys, values, c.table, c.n), w, budget, into, sinks=sinks, recent=recent)
+    rows_left, gone = [], []
+    for b, n in enumerate(c.lengths):
+        there = [j for j in range(n) if (b, j // page) not in bad]
+        missing = [j for j in range(n) if (b, j // page) in bad]
+        places = [i for i in range(rows) if (b, i // page) not in bad_into]
+        m = min(len(there), len(places))
+        length = places[m - 1] + 1 if m else 0
+        assert int(left.lengths[b]) == length
+        passed = [i for i in range(length) if (b, i // page) in bad_into]
+        gone += [(b, i) for i in passed]
+        new_rows = [torch.zeros(H_k, length, c.d, dtype=c.dtype) for _ in range(2)]
+        for h in range(H_k):
+            weights = w[b, h].tolist()
+            safe = [j for j in there if j < sinks or j >= n - recent]
+            rest = sorted(set(there) - set(safe), key=lambda j: (weights[j] != weights[j], -weights[j] if weights[j] == weights[j] else 0.0, j))
+            at = sorted((safe + rest)[:m])
+            expected = [-1] * budget
+            for i, j in zip(places, at):
+                expected[i] = j
+                for pool, row, out in zip(want, c.rows[b], new_rows):
+                    pool[int(into[b, i // page]), h, i % page] = row[h, j].cuda()
+                    out[h, i] = row[h, j]
+            for i, j in zip(passed, missing):
+                expected[i] = j
+            assert kept[b, h].tolist() == expected
+            stays = torch.zeros(C)
+            for i, j in zip(places, at):
+                stays[i] = weights[j]
+            assert torch.equal(new[b, h].cpu().view(torch.int32), stays.view(torch.int32))
+        rows_left.append(new_rows)
+    for got, x in zip((keys, values), want):
+        assert torch.equal(got.view(torch.uint8), x.view(torch.uint8))
+    q = c.normal(B, 2 * H_k, 1, c.d)
+    o, lse = fhog.paged_attention(q, left)
+    c.rows, c.lengths = rows_left, left.lengths.tolist()
+    _check_attention(c, q, o, lse, gone=set(gone))
+
+
+MISSING = [  # H_k, d, page, lengths, budget, sinks, recent, bad, bad_into
+    (2, 64, 16, [100, 40, 41], 40, 3, 5, [(0, 0), (0, 6), (1, 1)], []), (1, 32, 8, [30], 20, 0, 0, [(0, 1)], [(0, 1)]), (2, 32, 8, [70, 64, 9], 200, 4, 4, [(0, 2), (0, 8), (1, 0), (2, 0), (2, 1)], []),
+    (1, 128, 24, [300, 299], 100, 4, 20, [(0, 0), (0, 12), (1, 5)], [(0, 0), (1, 2)]), (2, 64, 16, [100, 100, 10], 64, 10, 40, [], [(0, 0), (0, 1), (1, 3), (2, 0)]),
+    (1, 32, 1, [50, 20], 13, 6, 7, [(0, i) for i in range(0, 50, 3)] + [(1, i) for i in range(12)], [(0, 2), (0, 3), (1, 0)]), (2, 64, 16, [60, 33], 40, 0, 0, [(0, i) for i in range(4)], []),
+    (2, 64, 16, [60, 33], 40, 2, 3, [(1, 1)], [(0, 0), (0, 1), (0, 2)]), (1, 128, 64, [5000, 2000], 1500, 4, 64, [(0, 3), (0, 77), (0, 78), (1, 0)], [(0, 1), (0, 23), (1, 22)]),
+    (1, 32, 100, [20000, 13000], 9000, 4, 1000, [(0, 130), (0, 150), (0, 199), (1, 125), (0, 2)], [(1, 4)]), (1, 32, 16, [15000], 20000, 0, 0, [(0, 900)], [(0, 0), (0, 930)])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["random", "nan", "tiny", "equal"])
+@pytest.mark.parametrize("H_k, d, page, lengths, budget, sinks, recent, bad, bad_into", MISSING)
+def test_what_is_not_there_does_not_stay(H_k, d, page, lengths, budget, sinks, recent, bad, bad_into, kind, dtype):
+    """Entries without a page, protected ones too and where all entries stay, never come to lie in a page that is read; places without a page lose no entry."""
+    if dtype != torch.bfloat16 and kind != "random":
+        pytest.skip("the selection does not know types")
+    c = Case(dtype, H_k, d, page, lengths, seed=35, width=-(-max(lengths) // page) + 1)
+    w = torch.randn(len(lengths), H_k, c.table.shape[1] * page, generator=c.g).mul(2).exp()
+    if kind == "nan":
+        w[torch.rand(w.shape, generator=c.g) < 0.6] = NAN
+    elif kind == "tiny":
+        w = -w * 2.0 ** 100                 # negative, some of them -inf
+    elif kind == "equal":
+        w[:] = 0
+    for b, x in bad:
+        w[b, :, x * page:(x + 1) * page] = 1e30 if kind == "random" else 0.0
+    _check_evict(c, w.cuda(), budget, sinks, recent, set(bad), set(bad_into), 36)
