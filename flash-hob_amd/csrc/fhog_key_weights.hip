@@ -246,6 +246,55 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
     dma_wait();   // the stage after the next one has landed
     __syncthreads();
   }
+  // A query that saw nothing is 0 in LDS, which makes NaN of keys that are infinite or NaN. So where a sum is NaN the wave forms it once more, straight from memory and from the queries that
+  // saw something alone; it stays NaN if one of these sees such a key. (Looked at in the loop, in place of this, L cost all calls 1 to 6 %.)
+  bool nan = false;
+#pragma unroll
+  for (int x = 0; x < NK; x++) nan = nan || sum[x] != sum[x];
+  if (__builtin_amdgcn_ballot_w64(nan) != 0) {
+    float anew[NK] = {};
+    int at = lane;
+    asm volatile("" : "+v"(at));   // what follows is formed here, and not held in registers through the loop above
+    const int n = at & 31, h = at >> 5;
+    int head = from / each;
+    now = begin + from - head * each;
+#pragma unroll 1
+    for (int step = from; step < to; step++) {
+      const char* const rows = w.q + b * w.qb + (int64_t)(g * w.group + head) * w.qh + 16 * h;
+      const float* const L = w.lse + (row0 + head) * w.n_q;
+#pragma unroll 1
+      for (int i0 = now * ROWS; i0 < (now + 1) * ROWS; i0 += 32) {
+        if (i0 > any_hi || i0 + 31 < any_lo) continue;
+        const char* const row = rows + min(i0 + n, geo.n_q - 1) * w.qn;
+#pragma unroll
+        for (int x = 0; x < NK; x++) {
+          const char* const keys = w.k + b * w.kb + g * w.kh + (int64_t)min(kw + 32 * x + n, geo.n_k - 1) * w.kn + 16 * h;
+          f32x16_t scores = {0};
+#pragma unroll
+          for (int c = 0; c < STEPS; c++) {
+            __builtin_amdgcn_sched_barrier(0);   // one load after the other: registers are the loop's above
+            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(row + 32 * c), of = *reinterpret_cast<const u32x4_t*>(keys + 32 * c);
+            if constexpr (WIDE) {
+#pragma unroll
+              for (int e = 0; e < 4; e++) scores = __builtin_amdgcn_mfma_f32_32x32x2f32(number(a[e]), number(of[e]), scores, 0, 0, 0);
+            } else {
+              scores = mfma<F16>(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, of), scores);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            __builtin_amdgcn_sched_barrier(0);
+            const int i = i0 + 8 * (r / 4) + 4 * h + r % 4;
+            const float l = L[min(i, geo.n_q - 1)], p = __builtin_amdgcn_exp2f(__builtin_fmaf(scores[r], w.scale_log2, -(l * kLog2e)));
+            anew[x] += i >= lo[x] && i <= hi[x] && l != -INFINITY ? p : 0.f;
+          }
+        }
+      }
+      if (++now == end) now = begin, head++;
+    }
+#pragma unroll
+    for (int x = 0; x < NK; x++) sum[x] = sum[x] != sum[x] ? anew[x] : sum[x];
+  }
 #pragma unroll
   for (int x = 0; x < NK; x++) {
     const float total = sum[x] + __shfl_xor(sum[x], 32);

@@ -213,3 +213,35 @@ def test_what_is_not_there_does_not_stay(H_k, d, page, lengths, budget, sinks, r
     for b, x in bad:
         w[b, :, x * page:(x + 1) * page] = 1e30 if kind == "random" else 0.0
     _check_evict(c, w.cuda(), budget, sinks, recent, set(bad), set(bad_into), 36)
+
+
+# ---- weights of a prompt's keys ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hidden", [NAN, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype, n, H, d", [(torch.bfloat16, 300, 2, 64), (torch.float16, 300, 2, 32), (torch.float16, 300, 4, 128), (torch.float32, 300, 2, 64), (torch.float32, 300, 2, 128),
+                                            (torch.bfloat16, 4001, 32, 64), (torch.bfloat16, 4001, 32, 128)])
+@pytest.mark.parametrize("causal, window", [(False, None), (True, None), (True, 70)])
+def test_queries_that_saw_nothing_give_nothing_to_odd_keys(causal, window, dtype, n, H, d, hidden):
+    """Keys that are NaN or infinite: NaN from the queries that see them, nothing from those whose L is -inf; the other keys' weights stay as they were, bit by bit, where their tile of keys is
+    another one, and to rounding beside them."""
+    import fhog
+    g = torch.Generator(device="cuda").manual_seed(37)
+    q, k = (torch.randn(1, h, n, d, generator=g, device="cuda").to(dtype) for h in (H, H // 2))
+    i, j = torch.arange(n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+    seen = torch.ones(n, n, dtype=torch.bool, device="cuda") if not causal else (j <= i) & (i - j < (window or n))
+    s = torch.matmul(q.float(), k.float().repeat_interleave(2, 1).transpose(-1, -2).contiguous()) * d ** -0.5
+    lse = s.masked_fill(~seen, -math.inf).logsumexp(-1)
+    del s
+    lse[:, :, n - 60:] = -math.inf                       # padding at the end, and heads apart
+    lse[:, 1, 100:200] = -math.inf
+    base = fhog.key_weights(q, k, lse, None, causal, window=window)
+    odd = [n - 1, n - 33, n - 60]                        # seen by those alone where the mask is causal
+    k[:, :, odd, 5] = hidden
+    k[:, 0, 70] = hidden                                 # and one that others see
+    got = fhog.key_weights(q, k, lse, None, causal, window=window)
+    if causal:
+        assert (got[:, :, odd] == 0).all()
+    else:
+        assert not got[:, :, odd].isfinite().all()
+    assert got[0, 0, 70].isnan() and torch.equal(got[0, 1, 70], base[0, 1, 70]) if H == 4 else got[0, 0, 70].isnan()
+    rest = [x for x in range(n) if x not in (70, *odd)]
+    assert torch.equal(got[..., rest], base[..., rest])
