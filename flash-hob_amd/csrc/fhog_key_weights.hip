@@ -48,9 +48,10 @@ __device__ __forceinline__ int pieces_of(int steps, const Weigh& w) { return ste
 // Which queries see a key
 struct Queries {
   int n_q, n_k, off, window, sinks, causal;
-  __device__ __forceinline__ Queries(const Weigh& w, int b) : n_q(w.n_q), n_k(w.n_k), off(w.off), window(w.window), sinks(w.sinks), causal(w.causal) {
-    if (w.lengths) {   // padding is as if it were not there
-      n_k = max(0, min(w.lengths[b], n_k));
+  // length: of the sequence, where there are lengths; padding is as if it were not there
+  __device__ __forceinline__ Queries(const Weigh& w, int length) : n_q(w.n_q), n_k(w.n_k), off(w.off), window(w.window), sinks(w.sinks), causal(w.causal) {
+    if (w.lengths) {
+      n_k = max(0, min(length, n_k));
       n_q = max(0, min(n_k - off, n_q));
     }
   }
@@ -109,7 +110,14 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
   const int piece = blockIdx.x / w.tiles, g = blockIdx.y, b = blockIdx.z;
   int tile = blockIdx.x - piece * w.tiles + piece % w.tiles;
   if (tile >= w.tiles) tile -= w.tiles;
-  const Queries geo(w, b);
+  int length = 0;
+  if (w.lengths) {   // one thread reads it: lengths that someone changes meanwhile make wrong results, but no waves that disagree at a barrier
+    __shared__ int read;
+    if (tid == 0) read = w.lengths[b];
+    __syncthreads();
+    length = __builtin_amdgcn_readfirstlane(read);
+  }
+  const Queries geo(w, length);
   const int k0 = tile * KEYS, kw = k0 + 32 * NK * wave;
   int begin, end;
   geo.template stages<ROWS>(k0, KEYS, begin, end);
@@ -309,7 +317,7 @@ template <int KEYS, int ROWS>
 __global__ void __launch_bounds__(kThreads) add_pieces(Weigh w) {
   const int j = blockIdx.x * kThreads + threadIdx.x, g = blockIdx.y, b = blockIdx.z;
   if (j >= w.n_k) return;
-  const Queries geo(w, b);
+  const Queries geo(w, w.lengths ? w.lengths[b] : 0);
   int begin, end;
   geo.template stages<ROWS>(j / KEYS * KEYS, KEYS, begin, end);
   const int pieces = pieces_of(w.group * (end - begin), w);

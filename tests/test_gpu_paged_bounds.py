@@ -245,3 +245,26 @@ def test_queries_that_saw_nothing_give_nothing_to_odd_keys(causal, window, dtype
     assert got[0, 0, 70].isnan() and torch.equal(got[0, 1, 70], base[0, 1, 70]) if H == 4 else got[0, 0, 70].isnan()
     rest = [x for x in range(n) if x not in (70, *odd)]
     assert torch.equal(got[..., rest], base[..., rest])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_whose_lengths_change_meanwhile_end(dtype):
+    """The waves of a workgroup go by one length, whichever it is. What comes out then is anyone's guess; calls before and after are right."""
+    import fhog
+    g = torch.Generator(device="cuda").manual_seed(38)
+    n = 2500
+    q, k = (torch.randn(2, h, n, 64, generator=g, device="cuda").to(dtype) for h in (8, 2))
+    lse = torch.rand(2, 8, n, generator=g, device="cuda") + 9
+    lengths = torch.tensor([2400, 1300], dtype=torch.int32, device="cuda")
+    want, before = fhog.key_weights(q, k, lse, None, True, lengths=lengths), lengths.clone()
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for i in range(20):
+        with torch.cuda.stream(streams[0]):
+            for m in (0, 700, 2500, 64):
+                lengths.fill_(m)
+        with torch.cuda.stream(streams[1]):
+            fhog.key_weights(q, k, lse, None, True, lengths=lengths)
+    torch.cuda.synchronize()
+    lengths.copy_(before)
+    assert torch.equal(fhog.key_weights(q, k, lse, None, True, lengths=lengths), want)
