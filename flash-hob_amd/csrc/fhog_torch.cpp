@@ -439,13 +439,21 @@ std::optional<tensor_list> rotary(const Tensor& q, const std::optional<Tensor>& 
 
 // ---- a cache in pages -----------------------------------------------------------------------------------------------
 // What every tensor of these calls has to be: in the memory of one GPU, and neither a wrapper nor asking for a gradient, which is not formed
+bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
 bool usable(const Tensor& t, const Tensor& like) {
   return t.defined() && !t.unsafeGetTensorImpl()->is_python_dispatch() && in_memory(t) && t.is_cuda() && t.device() == like.device() &&
-         !(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined();
+         !(t.requires_grad() && at::GradMode::is_enabled()) && !dual(t);
 }
 bool usable(const std::optional<Tensor>& t, const Tensor& like) { return !t || usable(*t, like); }
 bool transformed() {
   return at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+}
+
+// Whether the library refused the last call here, on this thread; else it was declined before the library was asked
+thread_local bool library_refused = false;
+bool valid(int code) {
+  library_refused = code != FHOG_OK;
+  return !library_refused;
 }
 
 // Stride along dimension i; a dimension of one is never stepped along, whatever it says
@@ -487,6 +495,7 @@ struct Paged {
 
 bool paged_append(const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const Tensor& k_, const Tensor& v_,
                   const std::optional<Tensor>& counts_) {
+  library_refused = false;
   Paged cache;
   if (!usable(k_, keys) || !usable(v_, keys) || !usable(counts_, keys)) return false;
   const c10::DeviceGuard guard(keys.device());
@@ -501,7 +510,7 @@ bool paged_append(const Tensor& keys, const Tensor& values, const Tensor& table,
   fhog_paged_append_args a = {};
   a.cache = c, a.k = k.data_ptr(), a.v = v.data_ptr(), a.counts = counts.defined() ? (const int32_t*)counts.data_ptr() : nullptr, a.n = k.size(2);
   a.stride_kb = step(k, 0), a.stride_kh = step(k, 1), a.stride_kn = step(k, 2), a.stride_vb = step(v, 0), a.stride_vh = step(v, 1), a.stride_vn = step(v, 2);
-  if (fhog_paged_append_validate(&a) != FHOG_OK) return false;
+  if (!valid(fhog_paged_append_validate(&a))) return false;
   TORCH_CHECK(fhog_paged_append(&a, stream_of(keys)) == FHOG_OK, "fhog_paged_append: ", fhog_last_error());
   changed(keys), changed(values);
   return true;
@@ -526,6 +535,7 @@ bool apart_or_same(const Tensor& a, const Tensor& b) {
 std::optional<tensor_list> paged_attention(const Tensor& q_, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths,
                                            std::optional<double> scale, int64_t window, int64_t sinks, const std::optional<Tensor>& weights_,
                                            const std::optional<Tensor>& weights_out) {
+  library_refused = false;
   Paged cache;
   if (!usable(q_, keys) || !usable(weights_, keys) || !usable(weights_out, keys)) return std::nullopt;
   const c10::DeviceGuard guard(keys.device());
@@ -548,7 +558,7 @@ std::optional<tensor_list> paged_attention(const Tensor& q_, const Tensor& keys,
     a.weights_in = (const float*)weights.data_ptr(), a.stride_wib = step(weights, 0), a.stride_wih = step(weights, 1);
     a.weights_out = (float*)out[2].data_ptr(), a.stride_wob = step(out[2], 0), a.stride_woh = step(out[2], 1);
   }
-  if (fhog_paged_attn_validate(&a) != FHOG_OK) return std::nullopt;
+  if (!valid(fhog_paged_attn_validate(&a))) return std::nullopt;
   a.ws_bytes = (int64_t)fhog_paged_attn_workspace_bytes(&a);
   Tensor ws;
   if (a.ws_bytes > 0) ws = workspace(a.ws_bytes, q), a.ws = ws.data_ptr();
@@ -559,6 +569,7 @@ std::optional<tensor_list> paged_attention(const Tensor& q_, const Tensor& keys,
 
 std::optional<Tensor> key_weights(const Tensor& q_, const Tensor& k_, const Tensor& L, std::optional<double> scale, int causal, int64_t window, int64_t sinks,
                                   const std::optional<Tensor>& lengths_) {
+  library_refused = false;
   if (!usable(q_, q_) || !usable(k_, q_) || !usable(L, q_) || !usable(lengths_, q_) || transformed()) return std::nullopt;
   if (q_.dim() != 4 || k_.dim() != 4 || k_.scalar_type() != q_.scalar_type() || k_.size(0) != q_.size(0) || k_.size(3) != q_.size(3) || !L.is_floating_point() ||
       L.sizes() != q_.sizes().slice(0, 3) || !mask_applies(Mask{causal, window, sinks}, q_.size(2), k_.size(2)))
@@ -577,7 +588,7 @@ std::optional<Tensor> key_weights(const Tensor& q_, const Tensor& k_, const Tens
   const Tensor out = at::empty({a.batch, a.heads_k, a.n_k}, q.options().dtype(at::kFloat));
   a.q = q.data_ptr(), a.k = k.data_ptr(), a.lse = (const float*)lse.data_ptr(), a.out = (float*)out.data_ptr();
   a.lengths = lengths.defined() ? (const int32_t*)lengths.data_ptr() : nullptr;
-  if (fhog_key_weights_validate(&a) != FHOG_OK) return std::nullopt;
+  if (!valid(fhog_key_weights_validate(&a))) return std::nullopt;
   a.ws_bytes = (int64_t)fhog_key_weights_workspace_bytes(&a);
   Tensor ws;
   if (a.ws_bytes > 0) ws = workspace(a.ws_bytes, q), a.ws = ws.data_ptr();
@@ -588,6 +599,7 @@ std::optional<Tensor> key_weights(const Tensor& q_, const Tensor& k_, const Tens
 // New lengths, the weights of what stays, and where it came from
 std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const Tensor& weights_,
                                                               int64_t budget, const Tensor& into_, int64_t sinks, int64_t recent) {
+  library_refused = false;
   Paged cache;
   if (!usable(weights_, keys) || !usable(into_, keys)) return std::nullopt;
   const c10::DeviceGuard guard(keys.device());
@@ -603,7 +615,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(const Tensor& keys
   const auto ints = into.options();
   // addresses of the outputs are looked at for NULL alone: their size is allocated once the call is known to be one
   a.lengths_out = (int32_t*)keys.data_ptr(), a.kept = a.lengths_out, a.weights_out = (float*)a.kept;
-  if (fhog_paged_evict_validate(&a) != FHOG_OK) return std::nullopt;
+  if (!valid(fhog_paged_evict_validate(&a))) return std::nullopt;
   const Tensor left = at::empty({c.batch}, ints), kept = at::empty({c.batch, c.heads_k, budget}, ints), out = at::empty({c.batch, c.heads_k, c.table_width * c.page}, weights.options());
   a.lengths_out = (int32_t*)left.data_ptr(), a.kept = (int32_t*)kept.data_ptr(), a.weights_out = (float*)out.data_ptr();
   TORCH_CHECK(fhog_paged_evict(&a, stream_of(keys)) == FHOG_OK, "fhog_paged_evict: ", fhog_last_error());
@@ -635,6 +647,9 @@ PYBIND11_MODULE(_fhog_torch, m) {
   m.def("attention", &attention, free_lock);
   m.def("rotary", &rotary, free_lock);
   m.def("transformed", &transformed, free_lock);
+  m.def("dual", &dual, free_lock);
+  m.def("library_refused", [] { return library_refused; }, free_lock);
+  m.def("not_called", [] { library_refused = false; }, free_lock);   // after arguments that fit no call here
   m.def("apart_or_same", &apart_or_same, free_lock);
   m.def("paged_append", &paged_append, free_lock);
   m.def("paged_attention", &paged_attention, free_lock);

@@ -52,6 +52,11 @@ def _check_tensors(like, optional=(), **tensors) -> None:
         if t is not None and (not t.is_cuda or t.device != like.device):
             raise ValueError(f"{name} is on {t.device}: this runs on the GPU only, on one device (there is no CPU path)")
     _lib.check_memory(**tensors)
+    for name, t in tensors.items():
+        if t is not None and _lib.torch_ext().dual(t):
+            raise ValueError(f"{name} is a dual tensor of forward mode: no derivative is formed here")
+        if t is not None and _lib.torch_ext().dispatches_to_python(t):
+            raise ValueError(f"{name} is a {type(t).__name__}, which dispatches to Python: plain tensors are expected")
 
 
 def _check_shape(name, t, shape, dtype) -> None:
@@ -75,6 +80,9 @@ def _check_cache(cache, written: bool = False) -> Tuple[int, int, int, int, int]
     if min(keys.shape) < 1 or d not in (32, 64, 128):
         raise ValueError(f"keys of shape {tuple(keys.shape)} not supported (d 32, 64 or 128, one page, head and entry or more)")
     _check_shape("values", cache.values, keys.shape, keys.dtype)
+    for name, t in (("keys", keys), ("values", cache.values)):
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name} have strides {t.stride()}: the last dimension has to be contiguous")
     if any(n > 1 and a != b for n, a, b in zip(keys.shape, keys.stride(), cache.values.stride())):
         raise ValueError(f"values have strides {cache.values.stride()}, expected {keys.stride()} like keys")
     if table.dim() != 2 or table.dtype != torch.int32 or table.shape[1] < 1:
@@ -92,8 +100,8 @@ def _not_transformed(what: str) -> None:
 
 
 def _refused(what: str):
-    """The error for a call that passed the checks above and that the library still does not take; its own message says why."""
-    return ValueError(f"{what}: {_lib.lib().fhog_last_error().decode()}")
+    """The error for a call that passed the checks above and was declined all the same: by the library, whose message says why, or before it was asked."""
+    return ValueError(f"{what}: {_lib.lib().fhog_last_error().decode() if _lib.torch_ext().library_refused() else 'these arguments are not supported'}")
 
 
 def paged_append(cache: PagedCache, k, v, *, counts=None) -> None:
@@ -112,6 +120,7 @@ def paged_append(cache: PagedCache, k, v, *, counts=None) -> None:
     try:
         done = _lib.torch_ext().paged_append(cache.keys, cache.values, cache.table, cache.lengths, k, v, counts)
     except TypeError:   # not tensors: named below
+        _lib.torch_ext().not_called()
         done = False
     if done:
         return
@@ -153,6 +162,7 @@ def paged_attention(q, cache: PagedCache, scale: Optional[float] = None, *, wind
     try:
         res = _lib.torch_ext().paged_attention(q, cache.keys, cache.values, cache.table, cache.lengths, scale, w, s, weights, weights_out)
     except TypeError:   # not tensors or numbers: named below
+        _lib.torch_ext().not_called()
         res = None
     if res is not None:
         return res
@@ -188,6 +198,7 @@ def key_weights(q, k, L, scale: Optional[float] = None, causal=False, *, window:
     try:
         res = _lib.torch_ext().key_weights(q, k, L, scale, *native_mask(causal, window), native_sinks(sinks), lengths)
     except TypeError:   # not tensors or numbers: named below
+        _lib.torch_ext().not_called()
         res = None
     if res is not None:
         return res
@@ -240,6 +251,7 @@ def paged_evict(cache: PagedCache, weights, budget: int, into, *, sinks: int = 0
     try:
         res = _lib.torch_ext().paged_evict(cache.keys, cache.values, cache.table, cache.lengths, weights, budget, into, sinks, recent)
     except TypeError:   # not tensors or numbers: named below
+        _lib.torch_ext().not_called()
         res = None
     if res is not None:
         lengths, new, kept = res

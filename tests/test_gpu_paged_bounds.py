@@ -268,3 +268,46 @@ def test_weights_whose_lengths_change_meanwhile_end(dtype):
     torch.cuda.synchronize()
     lengths.copy_(before)
     assert torch.equal(fhog.key_weights(q, k, lse, None, True, lengths=lengths), want)
+
+
+# ---- refusals -----------------------------------------------------------------------------------------------------------------
+class _Wrapped(torch.Tensor):
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, strides=t.stride(), dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError
+
+
+def test_refusals_say_what_they_are_about():
+    """Rows that are not contiguous, dual tensors, wrappers: named, whatever the library said to a call before."""
+    import torch.autograd.forward_ad as fwAD
+
+    import fhog
+    c = Case(torch.float32, 2, 64, 16, [40, 20], seed=39)
+    q, kv, w = c.normal(2, 4, 1, 64), c.normal(2, 2, 3, 64), torch.zeros(2, 2, c.table.shape[1] * 16).cuda()
+    cache, into = c.cache(), torch.tensor([[4, 5], [6, 7]], dtype=torch.int32).cuda()
+    apart = [torch.zeros(*t.shape[:3], 128, device="cuda")[..., ::2] for t in (c.keys, c.values)]
+    x, lse = c.normal(1, 2, 9, 64), torch.zeros(1, 2, 9).cuda()
+
+    def refused(word, *calls):
+        for call in calls:
+            with pytest.raises(ValueError, match="scale is not finite"):
+                fhog.paged_attention(q, cache, NAN)
+            with pytest.raises(ValueError, match=word):
+                call()
+
+    far = fhog.PagedCache(*apart, c.table, c.n)
+    refused("contiguous", lambda: fhog.paged_attention(q, far), lambda: fhog.paged_append(far, kv, kv), lambda: fhog.paged_evict(far, w, 20, into))
+    refused("not supported", lambda: fhog.paged_evict(cache, w, 2 ** 70, torch.zeros(2, 3, dtype=torch.int32).cuda()))
+    with fwAD.dual_level():
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))  # noqa: E731
+        duals = fhog.PagedCache(dual(c.keys), c.values, c.table, c.n)
+        refused("q is a dual", lambda: fhog.paged_attention(dual(q), cache), lambda: fhog.key_weights(dual(x), x, lse))
+        refused("k is a dual", lambda: fhog.paged_append(cache, dual(kv), kv), lambda: fhog.key_weights(x, dual(x), lse))
+        refused("weights is a dual", lambda: fhog.paged_attention(q, cache, weights=dual(w)), lambda: fhog.paged_evict(cache, dual(w), 20, into))
+        refused("keys is a dual", lambda: fhog.paged_attention(q, duals), lambda: fhog.paged_append(duals, kv, kv), lambda: fhog.paged_evict(duals, w, 20, into))
+    refused("no memory|dispatches to Python", lambda: fhog.paged_attention(_Wrapped(q), cache), lambda: fhog.paged_append(cache, kv, _Wrapped(kv)), lambda: fhog.key_weights(x, x, _Wrapped(lse)),
+            lambda: fhog.paged_evict(cache, _Wrapped(w), 20, into))
