@@ -244,7 +244,8 @@ def paged_evict(cache: PagedCache, weights, budget: int, into, *, sinks: int = 0
     Returns:
         ``(left, weights, kept)``: the :class:`PagedCache` of what stayed (keys and values the same tensors, table ``into``, new lengths); its weights, shaped like
         ``weights``, 0 where there is no entry; and (B, H_k, budget) int32, where in the cache each entry came from, -1 behind the last one (at places that are passed over: entries that are
-        not there, as far as there are any, else -1).
+        not there, as far as there are any, else -1). Calls on ``left`` take weights of its own P' * page entries: where ``into`` is not as wide as the table, cut them, or pad them with
+        zeros: ``torch.nn.functional.pad(weights, (0, into.shape[1] * page - weights.shape[-1]))`` does either.
     """
     if not isinstance(cache, PagedCache):
         _check_cache(cache)

@@ -215,6 +215,46 @@ def test_what_is_not_there_does_not_stay(H_k, d, page, lengths, budget, sinks, r
     _check_evict(c, w.cuda(), budget, sinks, recent, set(bad), set(bad_into), 36)
 
 
+@pytest.mark.parametrize("width", [4, 7, 12, 30])
+def test_from_one_eviction_to_the_next(width):
+    """Into tables that are narrower than the cache's, as wide, and wider: weights cut or padded as documented, tokens appended, weights added up, and evicted again."""
+    import fhog
+    page, budget, lengths, sinks, recent = 16, 60, [100, 190, 45], 2, 10
+    c = Case(torch.float32, 2, 64, page, lengths, seed=40, width=12, spare=300)
+    free = [p for p in range(c.keys.shape[0]) if p not in c.table.flatten().tolist()]
+    rows = [[[(c.rows[b][0][h, j], c.rows[b][1][h, j]) for j in range(n)] for h in range(2)] for b, n in enumerate(lengths)]
+    cache, w = c.cache(), torch.rand(3, 2, 12 * page, generator=c.g).cuda()
+    for turn in range(3):
+        into = torch.tensor([[free.pop() for _ in range(width)] for _ in range(3)], dtype=torch.int32).cuda()
+        old = w.cpu()
+        cache, w, kept = fhog.paged_evict(cache, w, budget, into, sinks=sinks, recent=recent)
+        w = torch.nn.functional.pad(w, (0, into.shape[1] * page - w.shape[-1]))
+        assert w.shape == (3, 2, width * page)
+        for b in range(3):
+            for h in range(2):
+                n = len(rows[b][h])
+                at = [j for j in kept[b, h].tolist() if j >= 0]
+                safe = [j for j in range(n) if n <= budget or j < sinks or j >= n - recent]
+                rest = sorted(set(range(n)) - set(safe), key=lambda j: (-float(old[b, h, j]), j))
+                assert at == sorted((safe + rest)[:min(n, budget)])
+                rows[b][h] = [rows[b][h][j] for j in at]
+                assert torch.equal(w[b, h, :len(at)].cpu(), old[b, h, at])
+        for token in range(3):
+            q, k, v = c.normal(3, 4, 1, 64), c.normal(3, 2, 1, 64), c.normal(3, 2, 1, 64)
+            cache.lengths.add_(1)
+            fhog.paged_append(cache, k, v)
+            before = w.cpu().double()
+            o, lse = fhog.paged_attention(q, cache, weights=w, weights_out=w)[:2]
+            for b in range(3):
+                for h in range(2):
+                    rows[b][h].append((k[b, h, 0].cpu(), v[b, h, 0].cpu()))
+                    K, V = (torch.stack([e[i] for e in rows[b][h]]).double() for i in (0, 1))
+                    p = torch.softmax(q[b, 2 * h:2 * h + 2, 0].cpu().double() @ K.T / 8, 1)
+                    n = len(rows[b][h])
+                    assert (o[b, 2 * h:2 * h + 2, 0].cpu().double() - p @ V).abs().max() <= 1e-5 * V.abs().max()
+                    assert (w[b, h, :n].cpu().double() - before[b, h, :n] - p.sum(0)).abs().max() <= 1e-5 and (w[b, h, n:] == 0).all()
+
+
 # ---- weights of a prompt's keys ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("hidden", [NAN, math.inf, -math.inf])
 @pytest.mark.parametrize("dtype, n, H, d", [(torch.bfloat16, 300, 2, 64), (torch.float16, 300, 2, 32), (torch.float16, 300, 4, 128), (torch.float32, 300, 2, 64), (torch.float32, 300, 2, 128),
