@@ -351,6 +351,7 @@ int validate_cache(const fhog_paged_cache& c, bool written) {
     return fail(FHOG_E_PAGED, "pages of %lld entries, %lld to a sequence: expected 1 or more of each, and 2^30 entries or fewer of a sequence", (long long)c.page, (long long)c.table_width);
   if (const int rc = check_strides("keys", c.dtype, {c.pages, c.heads_k, c.page}, {c.stride_p, c.stride_h, c.stride_n})) return rc;
   if (c.page > 1 && (c.stride_n < c.d || c.stride_n > kMaxRowStride)) return fail(FHOG_E_STRIDE, "entries of a page have to lie d to 2^24 elements apart (got %lld)", (long long)c.stride_n);
+  if ((c.pages > 1 && c.stride_p < 0) || (c.heads_k > 1 && c.stride_h < 0)) return fail(FHOG_E_STRIDE, "strides of pages and heads of keys must not be negative");
   if (!rows_apart(c.pages, c.heads_k, c.page, c.d, c.stride_p, c.stride_h, c.stride_n)) return fail(FHOG_E_STRIDE, "entries of the pages overlap");
   if (c.batch == 0) return FHOG_OK;
   for (const auto& x : {std::make_pair("keys", c.keys), std::make_pair("values", c.values)})

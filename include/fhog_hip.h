@@ -345,7 +345,7 @@ typedef struct fhog_paged_cache {
   const int32_t* table;   /* (batch, table_width), rows stride_tb apart */
   const int32_t* lengths; /* (batch), contiguous */
   int64_t batch, heads_k, d, pages, page, table_width;
-  int64_t stride_p, stride_h, stride_n; /* of keys and values: pages, heads, entries; multiples of 16 bytes */
+  int64_t stride_p, stride_h, stride_n; /* of keys and values: pages, heads, entries; multiples of 16 bytes, not negative */
   int64_t stride_tb;
   int32_t dtype;          /* FHOG_DTYPE_* */
 } fhog_paged_cache;

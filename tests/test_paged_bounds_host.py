@@ -20,3 +20,13 @@ def test_the_workspace_under_a_window_does_not_grow_with_the_table(L, window, si
     a.weights_in = a.weights_out = 0
     scores = need[2] - L.fhog_paged_attn_workspace_bytes(ctypes.byref(a))
     assert 64 * 64 * 4 * (window + sinks) <= scores <= 64 * 64 * 4 * (window + sinks + 4 * 32) + 64 * 64 * 8 + 16
+
+
+@pytest.mark.parametrize("call", ["paged_append", "paged_attn", "paged_evict"])
+@pytest.mark.parametrize("change", [dict(cache_stride_p=-2 * 16 * 64), dict(cache_stride_h=-16 * 64)])
+def test_pages_and_heads_that_lie_backwards_are_refused(L, call, change):  # noqa: F811
+    """Offsets below zero stand for entries that are not there."""
+    a = _args(call, **change)
+    assert getattr(L, f"fhog_{call}_validate")(ctypes.byref(a)) == -4 and "negative" in L.fhog_last_error().decode()
+    one = {"cache_stride_p": "cache_pages", "cache_stride_h": "cache_heads_k"}[next(iter(change))]
+    assert getattr(L, f"fhog_{call}_validate")(ctypes.byref(_args(call, **change, **{one: 1}))) == 0     # a dimension of one is never stepped along
