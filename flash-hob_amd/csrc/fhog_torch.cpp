@@ -607,6 +607,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(const Tensor& keys
   const at::NoGradGuard no_grad;
   const fhog_paged_cache& c = cache.c;
   if (!weights_of(weights_, c) || into_.dim() != 2 || into_.scalar_type() != at::kInt || into_.size(0) != c.batch || budget < 1) return std::nullopt;
+  if (c.batch > 0 && into_.data_ptr() == table.data_ptr()) return std::nullopt;   // before they are packed, which would hide it
   const Tensor weights = packed_rows(weights_), into = packed_rows(into_);
   fhog_paged_evict_args a = {};
   a.cache = c, a.weights = (const float*)weights.data_ptr(), a.stride_wb = step(weights, 0), a.stride_wh = step(weights, 1);

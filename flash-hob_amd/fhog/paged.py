@@ -268,6 +268,8 @@ def paged_evict(cache: PagedCache, weights, budget: int, into, *, sinks: int = 0
         raise ValueError(f"sinks ({sinks}) and recent ({recent}) are more than the budget ({budget})")
     if into.dim() != 2 or into.dtype != torch.int32 or into.shape[0] != B:
         raise (TypeError if into.dtype != torch.int32 else ValueError)(f"into: expected a ({B}, P') tensor of torch.int32, got {tuple(into.shape)} of {into.dtype}")
+    if B > 0 and into.data_ptr() == cache.table.data_ptr():
+        raise ValueError("into is the table of the cache: entries would be written over others that are still to be read")
     if into.shape[1] * page < min(budget, P * page):
         raise ValueError(f"into has {into.shape[1]} pages of {page} entries: expected room for {min(budget, P * page)}")
     raise _refused("paged_evict")

@@ -351,3 +351,16 @@ def test_refusals_say_what_they_are_about():
         refused("keys is a dual", lambda: fhog.paged_attention(q, duals), lambda: fhog.paged_append(duals, kv, kv), lambda: fhog.paged_evict(duals, w, 20, into))
     refused("no memory|dispatches to Python", lambda: fhog.paged_attention(_Wrapped(q), cache), lambda: fhog.paged_append(cache, kv, _Wrapped(kv)), lambda: fhog.key_weights(x, x, _Wrapped(lse)),
             lambda: fhog.paged_evict(cache, _Wrapped(w), 20, into))
+
+
+def test_the_caches_own_table_is_refused_however_it_lies():
+    """Also where table and `into` are one tensor that is packed on the way to the library, twice."""
+    import fhog
+    c = Case(torch.bfloat16, 2, 64, 16, [40, 20], seed=41)
+    w = torch.zeros(2, 2, c.table.shape[1] * 16).cuda()
+    for table in (c.table, c.table.t().contiguous().t(), torch.stack([c.table, c.table], 2)[..., 0]):
+        cache, before = fhog.PagedCache(c.keys, c.values, table, c.n), c.keys.clone()
+        for into in (table, table[:, :2]):
+            with pytest.raises(ValueError, match="table of the cache"):
+                fhog.paged_evict(cache, w, 20, into)
+        assert torch.equal(c.keys.view(torch.int16), before.view(torch.int16))
