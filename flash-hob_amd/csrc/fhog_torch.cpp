@@ -459,10 +459,11 @@ bool valid(int code) {
 // Stride along dimension i; a dimension of one is never stepped along, whatever it says
 int64_t step(const Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
 
-// A tensor whose rows are read 16 bytes at a time: as it lies if it can be, else packed
-Tensor rows16(const Tensor& t) {
+// A tensor whose rows are read 16 bytes at a time: as it lies if it can be, else packed; rows at most `apart` elements apart
+Tensor rows16(const Tensor& t, int64_t apart = INT64_MAX) {
   bool fits = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); i++) fits = fits && step(t, i) % (16 / t.element_size()) == 0 && step(t, i) >= 0;
+  fits = fits && step(t, t.dim() - 2) <= apart;
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 Tensor packed_rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
@@ -577,7 +578,7 @@ std::optional<Tensor> key_weights(const Tensor& q_, const Tensor& k_, const Tens
   if (lengths_ && (lengths_->dim() != 1 || lengths_->size(0) != q_.size(0) || lengths_->scalar_type() != at::kInt)) return std::nullopt;
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(q_.device());
-  const Tensor q = rows16(q_), k = rows16(k_), lse = as_lse(L), lengths = lengths_ ? lengths_->contiguous() : Tensor();
+  const Tensor q = rows16(q_, 1 << 24), k = rows16(k_, 1 << 24), lse = as_lse(L), lengths = lengths_ ? lengths_->contiguous() : Tensor();
   fhog_key_weights_args a = {};
   a.dtype = dtype_code(q.scalar_type());
   if (a.dtype < 0) return std::nullopt;

@@ -310,6 +310,18 @@ def test_weights_whose_lengths_change_meanwhile_end(dtype):
     assert torch.equal(fhog.key_weights(q, k, lse, None, True, lengths=lengths), want)
 
 
+def test_rows_that_lie_far_apart():
+    """Queries and keys of any strides: rows more than 2^24 elements apart are packed."""
+    import fhog
+    g = torch.Generator(device="cuda").manual_seed(42)
+    q, k = (torch.randn(1, h, 3, 64, generator=g, device="cuda").bfloat16() for h in (2, 1))
+    lse = torch.rand(1, 2, 3, device="cuda") + 1
+    want = fhog.key_weights(q, k, lse, None, True)
+    far = [torch.empty(3 * (2 ** 24 + 64), dtype=torch.bfloat16, device="cuda").as_strided(t.shape, (64, 64, 2 ** 24 + 64, 1)).copy_(t) for t in (q, k)]
+    for x in ((far[0], k), (q, far[1]), far):
+        assert torch.equal(fhog.key_weights(*x, lse, None, True), want)
+
+
 # ---- refusals -----------------------------------------------------------------------------------------------------------------
 class _Wrapped(torch.Tensor):
     @staticmethod
