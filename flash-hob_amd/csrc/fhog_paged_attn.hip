@@ -533,7 +533,7 @@ __device__ __forceinline__ void add_weights(const Token& t, int64_t id, int tid)
       for (int h = 0; h < kGroup; h++)
         if (h1 + h < heads)
 #pragma unroll
-          for (int i = 0; i < 4; i++) w[i] += s[h][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[h][i] - lse[h1 + h]);
+          for (int i = 0; i < 4; i++) w[i] = s[h][i] == -INFINITY ? w[i] : w[i] + __builtin_amdgcn_exp2f(s[h][i] - lse[h1 + h]);   // else as it was, also -0
       load(h0 + h1 + kGroup);
     }
   }

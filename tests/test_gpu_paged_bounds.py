@@ -215,6 +215,21 @@ def test_what_is_not_there_does_not_stay(H_k, d, page, lengths, budget, sinks, r
     _check_evict(c, w.cuda(), budget, sinks, recent, set(bad), set(bad_into), 36)
 
 
+@pytest.mark.parametrize("window", [None, 20])
+def test_weights_of_entries_that_are_not_seen_stay_bit_by_bit(window):
+    """Also -0 and NaN."""
+    import fhog
+    c = Case(torch.bfloat16, 2, 64, 16, [100, 40, 0], seed=43)
+    q = c.normal(3, 4, 1, 64)
+    w = torch.full((3, 2, c.table.shape[1] * 16), -0.0)
+    w[:, :, ::3] = torch.tensor([0x7fc12345], dtype=torch.int32).view(torch.float32)
+    w = w.cuda()
+    new = fhog.paged_attention(q, c.cache(), weights=w, window=window)[2]
+    for b, n in enumerate(c.lengths):
+        rest = [j for j in range(w.shape[2]) if j >= n or (window and j < n - window)]
+        assert torch.equal(new[b][:, rest].view(torch.int32), w[b][:, rest].view(torch.int32))
+
+
 @pytest.mark.parametrize("width", [4, 7, 12, 30])
 def test_from_one_eviction_to_the_next(width):
     """Into tables that are narrower than the cache's, as wide, and wider: weights cut or padded as documented, tokens appended, weights added up, and evicted again."""
