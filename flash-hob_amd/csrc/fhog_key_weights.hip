@@ -12,7 +12,7 @@
 //
 // What bounds it: the instructions of a SIMD. A block of 32 x 32 pairs takes d / 16 matrix instructions of 32 cycles and 48 vector instructions, 16 of them exponentials at half
 // rate: 256 cycles each at d = 128. The matrix instructions of one wave run beside the exponentials of another: three workgroups to a CU, four below d = 128. bf16, 16 heads x 16384
-// causal, four to one of keys, d = 128: 534 us, 1030 TFLOP/s, 87 % of what a large library product of bf16 matrices reaches here, which takes no exponentials.
+// causal, four to one of keys, d = 128: 540 us (557 on another card), 1020 TFLOP/s, 86 % of what a large library product of bf16 matrices reaches here, which takes no exponentials.
 #include <algorithm>
 
 #include "fhog_small.h"
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, (kWorkgroups<DT, D>)) weigh(Weigh w)
     if (++t == end) t = begin, src += back, lse += lse_back;
     else src += stage_bytes, lse += ROWS;
   };
-  // L in log2 units. A query that saw nothing has no weights to give, whatever it holds: it becomes 0, exp(0 - infinity)
+  // L in log2 units: it and the score are rounded there apart, 1.5e-7 of the weights (5e-8 if their difference were, which takes an instruction more to a score). A query that saw nothing has no weights to give, whatever it holds: it becomes 0, exp(0 - infinity)
   const auto make_ready = [&](char* stage) {
     float* const at = reinterpret_cast<float*>(stage + TILE) + lane;
     const float l = *at;
@@ -364,7 +364,9 @@ Plan plan_of(const fhog_key_weights_args* a) {
   if (a->dtype == FHOG_DTYPE_FP32 || (banded && a->window < 2048) || total * group * slices < 12288) p.nk = 1, stages(128, most, total);
   // Eight pieces to a CU, as long as that leaves pieces worth their beginning, and short enough to even out the end of the launch. us, at most 16 | 24 | 32 | 48 | 64 stages, 32 keys to
   // a wave, 16 x 16384: d = 128 651 | 642 | 628 | 650 | 660, d = 64 399 | 394 | 391 | 410 | 418; four | eight pieces to a CU, 64 keys to a wave: 16 x 8192 172 | 154; at least 6 | 8 stages:
-  // 16 x 3000 39.1 | 36.9, 8 x 512 12.0 | 10.8 (which then needs no second kernel); of a band, whose tiles have few, 5 | 8: fp16 48 x 1537, window 400, d = 64 22.4 | 26.3
+  // 16 x 3000 39.1 | 36.9, 8 x 512 12.0 | 10.8 (which then needs no second kernel); of a band, whose tiles have few, 3 | 5 | 8: fp16 48 x 1537, window 400, d = 64 23.0 | 22.3 | 26.1, bf16 64 x 1000,
+  // window 128 17.9 | 17.5 | 21.0, 32 x 2048, window 512 24.0 | 23.0 | 23.6, d = 128 8 x 3000, window 1000 19.1 | 18.3 | 20.1, 16 x 4096, window 256 30.1 | 28.5 | 26.8; of fp32, whose stages take
+  // eight times as long, 3 | 5 | 8: d = 64 16 x 2048 56.5 | 65.7 | 60.6, 8 x 4096 106 | 116 | 130, 8 x 512 14.5 | 19.7 | 24.2, 64 x 300 19.5 | 17.5 | 17.5, d = 128 32 x 1024 59 | 67 | 67, d = 32 4 x 3000 26 | 32 | 36
   const int64_t least = a->dtype == FHOG_DTYPE_FP32 ? 3 : p.nk == 1 && banded ? 5 : 8;
   int64_t chunk = std::min<int64_t>(32, std::max(least, (total * group * slices + 2047) / 2048));
   if (banded) {   // most tiles have as many stages: cut them evenly, not into full pieces and a short one

@@ -27,7 +27,7 @@ struct Cache {
   int64_t stride_p, stride_h, stride_n;   // in bytes
   int64_t stride_tb;
   Divisor page;
-  int32_t pages, width, capacity, heads_k, batch;
+  int32_t pages, capacity, heads_k, batch;
   // entries of sequence b
   __device__ __forceinline__ int length(int b) const { return max(0, min(lengths[b], capacity)); }
 };
@@ -38,7 +38,7 @@ inline Cache cache_of(const fhog_paged_cache& c) {
   r.keys = (char*)c.keys, r.values = (char*)c.values, r.table = c.table, r.lengths = c.lengths;
   r.stride_p = c.stride_p * es, r.stride_h = c.stride_h * es, r.stride_n = c.stride_n * es, r.stride_tb = c.stride_tb;
   r.page = Divisor((uint32_t)c.page);
-  r.pages = (int32_t)c.pages, r.width = (int32_t)c.table_width, r.capacity = (int32_t)(c.table_width * c.page), r.heads_k = (int32_t)c.heads_k, r.batch = (int32_t)c.batch;
+  r.pages = (int32_t)c.pages, r.capacity = (int32_t)(c.table_width * c.page), r.heads_k = (int32_t)c.heads_k, r.batch = (int32_t)c.batch;
   return r;
 }
 

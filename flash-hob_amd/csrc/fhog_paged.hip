@@ -59,7 +59,7 @@ struct Evict {
   int64_t wb, wh, ib;
   int64_t budget;
   int32_t rows;             // rows that may stay: min(budget, capacity)
-  int32_t sinks, recent, into_width;
+  int32_t sinks, recent;
   Divisor chunks;           // of a row
 };
 
@@ -309,11 +309,11 @@ hipError_t launch_paged_evict(const fhog_paged_evict_args* a, hipStream_t s) {
   e.rows = (int32_t)(a->budget < e.c.capacity ? a->budget : e.c.capacity);
   // beyond the capacity all entries are protected either way
   e.sinks = (int32_t)(a->sinks < e.c.capacity ? a->sinks : e.c.capacity), e.recent = (int32_t)(a->recent < e.c.capacity ? a->recent : e.c.capacity);
-  e.into_width = (int32_t)a->into_width, e.chunks = Divisor(row_chunks(a->cache));
+  e.chunks = Divisor(row_chunks(a->cache));
   const unsigned slices = (unsigned)(a->cache.batch * a->cache.heads_k);
   const size_t lds = std::min(e.c.capacity, kHeld) * sizeof(uint32_t);
-  // In one launch up to 96 KiB of rows to a slice. us, one launch | two: 4 x 4 slices of 301 rows, d = 64 (77 KB) 11.3 | 12.9, 32 x 8 of 500, d = 64 (128 KB) 22.2 | 23.2,
-  // 8 of 500, d = 128 (256 KB) 19.0 | 12.8
+  // In one launch up to 96 KiB of rows to a slice, where that is nowhere slower. us, one launch | two, d = 64, slices of 64 | 98 | 128 | 179 KB: 16 slices 10.0 | 12.9, 11.0 | 12.9, 12.2 | 13.0, 15.0 | 13.0;
+  // 64 10.2 | 12.8, 12.8 | 12.8, 15.4 | 13.5, 19.4 | 15.0; 128 11.4 | 13.2, 14.3 | 14.4, 17.7 | 16.1, 22.0 | 19.4; 256 13.2 | 15.8, 17.1 | 19.2, 21.4 | 23.0, 27.0 | 28.7
   if ((int64_t)e.rows * e.chunks.by * 32 <= 96 << 10) {
     hipLaunchKernelGGL(select_entries<true>, dim3(slices), dim3(kSelect), lds, s, e);
     return hipGetLastError();

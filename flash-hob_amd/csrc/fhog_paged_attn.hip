@@ -4,8 +4,9 @@
 //
 // over the entries j that the token sees; g: the head of keys that head h of queries belongs to.
 //
-// What bounds it: memory, every key and value once (4 flop to a byte with one head of queries to one of keys, 64 with 16). So nothing goes through LDS: a wave takes
-// tiles of its own, keys and values straight into the registers that the matrix instructions read, and the waves meet only at the end.
+// What bounds it: memory, every key and value once (4 flop to a byte with one head of queries to one of keys, 64 with 16). So no key and no value goes through LDS: a wave takes
+// tiles of its own, straight into the registers that the matrix instructions read. The waves meet twice: behind the first one's finding out what there is to do (the lengths of all sequences, where
+// tiles are dealt out: 12.1 -> 13.0 us for one sequence of 4096), and at the end.
 //
 // A tile is 32 entries (16 of fp32). The heads of queries of a head of keys are the columns, up to 16 of them; more take workgroups of their own. S^T = K Q^T
 // with 16x16 products: lane l has row l % 16 of K, 16 bytes at a time, and gets column l % 16 of S^T, entries 4 (l / 16) + 0..3 of each 16. These are, with
@@ -590,7 +591,7 @@ Plan plan_of(const fhog_paged_attn_args* a) {
 }
 
 template <int DT, int D>
-hipError_t launch_d(const Token& t, const fhog_paged_attn_args* a, hipStream_t s) {
+hipError_t launch_d(const Token& t, hipStream_t s) {
   const int64_t units = (int64_t)t.slots * t.c.heads_k;
   const dim3 grid((unsigned)((units + 7) / 8 * 8 * t.columns));
   const bool pages16 = t.c.page.by % 16 == 0;
@@ -611,11 +612,11 @@ hipError_t launch_d(const Token& t, const fhog_paged_attn_args* a, hipStream_t s
   return hipGetLastError();
 }
 template <int DT>
-hipError_t launch_t(const Token& t, const fhog_paged_attn_args* a, hipStream_t s) {
-  switch (a->cache.d) {
-    case 32: return launch_d<DT, 32>(t, a, s);
-    case 64: return launch_d<DT, 64>(t, a, s);
-    default: return launch_d<DT, 128>(t, a, s);
+hipError_t launch_t(const Token& t, int64_t d, hipStream_t s) {
+  switch (d) {
+    case 32: return launch_d<DT, 32>(t, s);
+    case 64: return launch_d<DT, 64>(t, s);
+    default: return launch_d<DT, 128>(t, s);
   }
 }
 
@@ -638,9 +639,9 @@ hipError_t launch_paged_attn(const fhog_paged_attn_args* a, hipStream_t s) {
   t.part = (float*)ws, t.stats = (f32x2_t*)(ws + p.part_bytes);
   t.whole = (f32x2_t*)(ws + p.part_bytes + p.stats_bytes), t.scores = (float*)(ws + p.part_bytes + p.stats_bytes + p.whole_bytes);
   switch (a->cache.dtype) {
-    case FHOG_DTYPE_FP32: return launch_t<FHOG_DTYPE_FP32>(t, a, s);
-    case FHOG_DTYPE_FP16: return launch_t<FHOG_DTYPE_FP16>(t, a, s);
-    default: return launch_t<FHOG_DTYPE_BF16>(t, a, s);
+    case FHOG_DTYPE_FP32: return launch_t<FHOG_DTYPE_FP32>(t, a->cache.d, s);
+    case FHOG_DTYPE_FP16: return launch_t<FHOG_DTYPE_FP16>(t, a->cache.d, s);
+    default: return launch_t<FHOG_DTYPE_BF16>(t, a->cache.d, s);
   }
 }
 

@@ -152,7 +152,7 @@ def paged_attention(q, cache: PagedCache, scale: Optional[float] = None, *, wind
         window, sinks: only the last ``window`` entries and the first ``sinks`` are seen.
         weights: (B, H_k, P * page) fp32. What each entry weighed is added up: the result is ``(O, L, W)`` with W = ``weights`` plus, at every entry that is seen, the sum
             over its heads of queries of ``exp(score - L)``.
-        weights_out: where W is written: ``weights`` itself, or a tensor that lies apart from it; None = a new tensor.
+        weights_out: where W is written: ``weights`` itself, or a tensor whose memory, from its first element to its last, lies apart from that of ``weights``; None = a new tensor.
 
     A sequence without entries (or whose table names no page) has O = 0 and L = -inf.
     """
@@ -235,7 +235,7 @@ def paged_evict(cache: PagedCache, weights, budget: int, into, *, sinks: int = 0
     The cache's pages stay as they are, so that pages which sequences share can be read on, and can be handed out again afterwards.
 
     Entries whose number in the table is no page are not there and never stay (``sinks`` and ``recent`` count from the ends of the sequence all the same); what stays closes up, so that the new lengths
-    count entries that are there. Places whose number in ``into`` is no page are passed over.
+    count entries that are there. They go to the places 0 .. min(budget, P * page) - 1 of ``into``; those whose number there is no page are passed over, and fewer entries stay.
 
     Args:
         weights: (B, H_k, P * page) fp32, as :func:`paged_attention` adds them up.

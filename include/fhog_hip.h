@@ -367,7 +367,7 @@ int fhog_paged_append(const fhog_paged_append_args* args, void* hip_stream);
 
 /* O = softmax(scale q K^T) V and L = logsumexp of the scaled scores of one token of each sequence over the entries that it sees: all, or with a window W > 0 the last
    W and the first `sinks`. A sequence that sees none has O = 0 and L = -infinity.
-   weights_out, where given: weights_in (the same array, or one that lies apart) plus, at every entry that is seen, sum over the heads of queries of a head of keys of
+   weights_out, where given: weights_in (the same array, or one whose memory lies apart from first element to last) plus, at every entry that is seen, sum over the heads of queries of a head of keys of
    exp(scale q k - L); the other entries as they were. */
 typedef struct fhog_paged_attn_args {
   fhog_paged_cache cache;
